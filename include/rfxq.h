@@ -39,6 +39,7 @@ extern "C" {
 #define RFXQ_TYPE_Q8_1 9
 #define RFXQ_TYPE_Q4_K 12
 #define RFXQ_TYPE_Q6_K 14
+#define RFXQ_TYPE_BF16 30
 
 /*
  * A quantized-resident weight: `Weight { data: WeightData::Quant { ty, arena,
@@ -373,6 +374,77 @@ int rfxq_moe_ffn_grouped_device(const float* x, uint32_t rows, uint32_t hidden, 
                                 uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
                                 const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out,
                                 hipStream_t stream);
+
+/* ---- grouped rows, products with half-typed stacks, adapters --------------- */
+
+/* Rows of a device matrix: row r starts at data + r * stride elements. */
+typedef struct rfxq_rows {
+    void* data;
+    uint32_t type;   /* RFXQ_TYPE_F32, RFXQ_TYPE_F16 or RFXQ_TYPE_BF16 */
+    uint32_t rows;
+    uint64_t stride; /* elements between rows, at least the row's columns */
+} rfxq_rows;
+
+/* Rows grouped by an id: the experts a router chose (rfxq_moe_route_device's
+ * idx), the adapter that each row's request asked for. With key_i = ids[i], or
+ * `groups` for an id outside [0, groups) (a row in no group):
+ *   offsets[g] = the number of rows with key < g, g = 0..groups
+ *   order      = the rows by (key, row): group g's rows in their order are
+ *                order[offsets[g]] .. order[offsets[g + 1] - 1]; rows in no group last.
+ * ids and order: n values, offsets: groups + 1, all in device memory; order must
+ * not overlap ids. 1 <= groups <= 1024; n up to 2^24; n = 0 clears the offsets
+ * (ids and order may then be NULL). One launch, no workspace, no host
+ * synchronisation: it can be captured. The reference groups on the host
+ * (src/model/dense.rs:1523-1546). */
+int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order,
+                    hipStream_t stream);
+
+/* Products of grouped rows with a stack of matrices that a GGUF file keeps in F16
+ * or BF16 ([in, out, expert_count]; a 2-D weight is a stack of one): for every
+ * place p < rows with offsets[g] <= p < offsets[g + 1]
+ *   y[dst][n] = sum_k x[src][k] W_g[n][k]
+ *   src = x_index ? x_index[p] / x_div : p,   dst = y_index ? y_index[p] : p
+ * offsets (expert_count + 1 values, rising from 0), x_index and y_index (rows values)
+ * are device memory, as rfxq_group_rows writes them: an expert layer's gate and
+ * up products pass x_index = order and x_div = top_k (pair p belongs to token
+ * order[p] / top_k), its down product y_index = order. Rows that no place
+ * names, and places in no group, with an index out of range or behind
+ * x->rows, leave y as it was; a destination named twice holds one of its results.
+ * x: f32, or the weights' type; y: f32, or the weights' type (its rows must not
+ * overlap x). Accumulation is f32, each result is rounded once; f32 activations
+ * keep f32 accuracy (they are split into 2 (F16) or 3 (BF16) pieces of the
+ * weights' type in the workspace; a weight that is infinite gives a result that is
+ * not finite, of either kind). Any in_features, stride and alignment of whole
+ * elements; rows of x and W that start at multiples of 16 bytes (in_features and
+ * strides multiples of 8) are faster. `workspace`: rfxq_grouped_gemm_workspace_size
+ * bytes, 16-byte aligned, or NULL for the library's own (see rfxq_gemm). The
+ * counterpart of rfxq_expert_gemm for all experts at once
+ * (src/model/dense.rs:1086-1115, 1531-1548). */
+int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
+                      const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
+                      void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+/* 0 unless x_type is RFXQ_TYPE_F32 (or the weight or type has no product). */
+uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows, uint32_t x_type);
+
+/* Low-rank adapters of many requests beside a projection that all rows share:
+ * for the rows r = order[p] (NULL: p) of group g, offsets[g] <= p < offsets[g + 1],
+ *   out[r] = y[r] + scales[g] * B_g (A_g x[r])
+ * over the first ranks[g] rows of A_g and columns of B_g; rows in no group:
+ * out[r] = y[r]. y is what the shared projection gave (rfxq_gemm, rfxq_gemv_rows);
+ * out may be y. a: a stack [in, rank, adapters], b: a stack [rank, out, adapters],
+ * of one type (F32, F16 or BF16), such as a pool whose places hold adapters of up
+ * to `rank`; what lies past an adapter's own rank is not used. ranks (values
+ * clamped to [0, rank]; NULL: all of it) and scales (NULL: 1): device memory,
+ * a value per adapter. offsets and order as rfxq_group_rows writes them from the
+ * rows' adapter ids, once for all projections of a step; order lists every row
+ * of x once (a row that it does not list keeps what out held). x, y and out have
+ * one type: f32 (any adapters), or the adapters' F16 / BF16; as many rows each.
+ * A x is kept in f32, accumulation is f32, each result is rounded once.
+ * `workspace` as for rfxq_grouped_gemm. No counterpart in the reference. */
+int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b, const int32_t* ranks,
+                  const float* scales, const int32_t* offsets, const int32_t* order, const rfxq_rows* y,
+                  const rfxq_rows* out, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
+uint64_t rfxq_lora_add_workspace_size(const rfxq_weight* a, uint32_t rows);
 
 /* ---- GGUF files (the on-disk path) ---------------------------------------- */
 

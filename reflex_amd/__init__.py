@@ -1,4 +1,5 @@
-"""reflex_amd: MI355X-native GGUF quantized-matmul path (Q4_K / Q6_K / Q8_0).
+"""reflex_amd: MI355X-native GGUF quantized-matmul path (Q4_K / Q6_K / Q8_0), with products of
+grouped rows and half-typed stacks (F16 / BF16 experts) and low-rank adapters beside it.
 
 The compute lives in ``librfxq.so`` (HIP C++ host code + an embedded gfx950
 code object, see ``build.py``); its C ABI is ``include/rfxq.h``. This package
@@ -34,6 +35,13 @@ class RfxqGemvItem(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("w", ctypes.POINTER(RfxqWeight)), ("y", ctypes.c_void_p)]
 
 
+class RfxqRows(ctypes.Structure):
+    """``rfxq_rows`` (include/rfxq.h)."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("type", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("stride", ctypes.c_uint64)]
+
+
 class RfxqOptions(ctypes.Structure):
     """``rfxq_options`` (include/rfxq.h)."""
 
@@ -56,6 +64,7 @@ class RfxqGemmPolicy(ctypes.Structure):
 # name -> (restype, argtypes); every symbol declared in include/rfxq.h
 _P, _U32, _U64, _I = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int
 _WP = ctypes.POINTER(RfxqWeight)
+_RP = ctypes.POINTER(RfxqRows)
 SIGNATURES = {
     "rfxq_last_error": (ctypes.c_char_p, []),
     "rfxq_last_error_code": (_I, []),
@@ -115,6 +124,11 @@ SIGNATURES = {
     "rfxq_gemm_gate_up_silu_workspace_size": (_U64, [_WP, _U32]),
     "rfxq_gemm_q8_1_batch": (_I, [_P, _U32, _U32, _P]),
     "rfxq_gemm_q8_1_plan_create": (_I, [_P, _U32, _U32, _I, ctypes.POINTER(_P)]),
+    "rfxq_group_rows": (_I, [_P, _U32, _U32, _P, _P, _P]),
+    "rfxq_grouped_gemm": (_I, [_RP, _WP, _P, _U32, _P, _U32, _P, _RP, _P, _U64, _P]),
+    "rfxq_grouped_gemm_workspace_size": (_U64, [_WP, _U32, _U32]),
+    "rfxq_lora_add": (_I, [_RP, _WP, _WP, _P, _P, _P, _P, _RP, _RP, _P, _U64, _P]),
+    "rfxq_lora_add_workspace_size": (_U64, [_WP, _U32]),
 }
 
 

@@ -3,8 +3,10 @@
 Steps (the counterpart of the reference's build.rs:199-252 + src/aot.rs, which
 run nvcc per .cu file and embed the images as bytes):
   1. hipcc --offload-arch=gfx950 --cuda-device-only --no-gpu-bundle-output
-     compiles csrc/kernels.hip to a raw code object (_build/rfxq_gfx950.co).
-  2. An assembler stub .incbin's that file into .rodata (_build/embed.o).
+     compiles csrc/kernels.hip (the quantized path) and csrc/half.hip (grouped
+     rows, half-typed stacks, adapters) side by side to raw code objects
+     (_build/rfxq_gfx950.co, _build/half_gfx950.co).
+  2. An assembler stub .incbin's those files into .rodata (_build/embed.o).
   3. hipcc compiles csrc/scratch.hip (host code plus the fixed device scratch
      array of rfxq_gemm_no_alloc) to an ordinary object.
   4. The host C++ (csrc/rfxq.cpp, no device code) is linked with them against
@@ -15,6 +17,7 @@ Run: python -m reflex_amd.build
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -25,6 +28,8 @@ BUILD = os.path.join(HERE, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 LIB = os.path.join(HERE, "librfxq.so")
 ARCH = "gfx950"
+# device sources and the symbols their images are embedded under
+IMAGES = [("kernels", "rfxq_code_object"), ("half", "rfxq_half_code_object")]
 
 DEVICE_FLAGS = [
     "-O3", "-std=c++17", f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output",
@@ -47,22 +52,30 @@ def _run(cmd: list[str], verbose: bool) -> None:
 
 def build(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
-    co = os.path.join(BUILD, f"rfxq_{ARCH}.co")
-    _run([os.path.join(ROCM, "bin", "hipcc"), *DEVICE_FLAGS, "-c", os.path.join(CSRC, "kernels.hip"), "-o", co],
-         verbose)
+    cos = {}
+    with concurrent.futures.ThreadPoolExecutor() as pool:
+        jobs = []
+        for source, symbol in IMAGES:
+            co = os.path.join(BUILD, f"{'rfxq' if source == 'kernels' else source}_{ARCH}.co")
+            cos[symbol] = co
+            jobs.append(pool.submit(_run, [os.path.join(ROCM, "bin", "hipcc"), *DEVICE_FLAGS, "-c",
+                                           os.path.join(CSRC, f"{source}.hip"), "-o", co], verbose))
+        for j in jobs:
+            j.result()
     embed_s = os.path.join(BUILD, "embed.S")
     with open(embed_s, "w") as f:
-        f.write(
-            "    .section .rodata\n"
-            "    .p2align 12\n"
-            "    .globl rfxq_code_object\n"
-            "rfxq_code_object:\n"
-            f"    .incbin \"{co}\"\n"
-            "    .globl rfxq_code_object_end\n"
-            "rfxq_code_object_end:\n"
-            "    .byte 0\n"
-            "    .section .note.GNU-stack,\"\",@progbits\n"
-        )
+        f.write("    .section .rodata\n")
+        for symbol, co in cos.items():
+            f.write(
+                "    .p2align 12\n"
+                f"    .globl {symbol}\n"
+                f"{symbol}:\n"
+                f"    .incbin \"{co}\"\n"
+                f"    .globl {symbol}_end\n"
+                f"{symbol}_end:\n"
+                "    .byte 0\n"
+            )
+        f.write("    .section .note.GNU-stack,\"\",@progbits\n")
     embed_o = os.path.join(BUILD, "embed.o")
     _run(["gcc", "-c", embed_s, "-o", embed_o], verbose)
     # the fixed scratch array of rfxq_gemm_no_alloc: host + gfx950 device code

@@ -1,0 +1,348 @@
+// Host side of the entry points on grouped rows: rfxq_group_rows,
+// rfxq_grouped_gemm and rfxq_lora_add (kernels: rows.hpp, grouped.hpp,
+// lora.hpp). Included by rfxq.cpp, whose errors, contexts, launches and
+// workspaces it uses.
+#pragma once
+
+namespace {
+
+constexpr uint32_t kMaxGroups = 1024;         // rows.hpp
+constexpr uint32_t kMaxGroupRows = 1u << 24;  // rows of rfxq_group_rows
+constexpr uint32_t kGroupThreads = 1024;      // of its workgroups, 1 to 4 rows each
+
+// Mirrors of the device structs.
+struct GroupRowsArgs {
+    const int32_t* ids;
+    int32_t* offsets;
+    int32_t* order;
+    uint32_t n, groups, rounds, pad;
+};
+static_assert(sizeof(GroupRowsArgs) == 40, "GroupRowsArgs layout");
+
+struct GroupedArgs {
+    const void* x;
+    const void* w;
+    void* y;
+    const int32_t* offsets;
+    const int32_t* x_index;
+    const int32_t* y_index;
+    const int32_t* x_exp;
+    uint64_t ldx, ldy, plane, w_stride;
+    uint32_t rows, x_rows, y_rows, x_div;
+    uint32_t k, n, groups, pieces;
+    uint32_t y_f32, tiles_m, tiles_n, sm, sn, pad;
+};
+static_assert(sizeof(GroupedArgs) == 144, "GroupedArgs layout");
+
+struct SplitArgs {
+    const float* x;
+    void* out;
+    int32_t* exp;
+    uint64_t ldx, plane;
+    uint32_t rows, k, ldo, pad;
+};
+static_assert(sizeof(SplitArgs) == 56, "SplitArgs layout");
+
+struct LoraArgs {
+    const void* x;
+    const void* a;
+    const void* b;
+    const int32_t* ranks;
+    const float* scales;
+    const int32_t* offsets;
+    const int32_t* order;
+    const void* y;
+    void* out;
+    float* v;
+    uint64_t ldx, ldy, ldo;
+    uint32_t rows, x_rows, k, n;
+    uint32_t rank, ldv, groups, splits;
+    uint32_t k_split, tiles, tiles_n, vec;
+};
+static_assert(sizeof(LoraArgs) == 152, "LoraArgs layout");
+
+bool float_type(uint32_t ty) { return ty == RFXQ_TYPE_F32 || ty == RFXQ_TYPE_F16 || ty == RFXQ_TYPE_BF16; }
+bool half_type(uint32_t ty) { return ty == RFXQ_TYPE_F16 || ty == RFXQ_TYPE_BF16; }
+uint32_t elem_bytes(uint32_t ty) { return ty == RFXQ_TYPE_F32 ? 4u : 2u; }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16u == 0; }
+
+// A stack of float matrices: [in, out] or [in, out, count].
+int check_stack(const rfxq_weight* w, bool f32_too, const char* what) {
+    if (!w) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight is NULL", what);
+    if (!half_type(w->ggml_type) && !(f32_too && w->ggml_type == RFXQ_TYPE_F32))
+        return fail(RFXQ_ERR_GGUF, "%s: ggml_type=%u (%sF16 or BF16 stacks)", what, w->ggml_type,
+                    f32_too ? "F32, " : "");
+    if (w->in_features == 0 || w->out_features == 0)
+        return fail(RFXQ_ERR_OTHER, "%s: shape [%u, %u]", what, w->in_features, w->out_features);
+    if (w->expert_count > kMaxGroups)
+        return fail(RFXQ_ERR_OTHER, "%s: expert_count=%u (at most %u)", what, w->expert_count, kMaxGroups);
+    const unsigned __int128 need = (unsigned __int128)std::max(w->expert_count, 1u) * w->out_features *
+                                   w->in_features * elem_bytes(w->ggml_type);
+    if (w->len < need)
+        return fail(RFXQ_ERR_OTHER, "%s: weight of %llu bytes, shape [%u, %u, %u] needs %llu", what,
+                    (unsigned long long)w->len, w->in_features, w->out_features, std::max(w->expert_count, 1u),
+                    (unsigned long long)need);
+    if (!w->data) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight data is NULL", what);
+    if (reinterpret_cast<uintptr_t>(w->data) % elem_bytes(w->ggml_type))
+        return fail(RFXQ_ERR_OTHER, "%s: weight data at %p is not %u-byte aligned", what, w->data,
+                    elem_bytes(w->ggml_type));
+    return RFXQ_OK;
+}
+
+int check_rows(const rfxq_rows* r, uint32_t columns, const char* what, const char* name) {
+    if (!r) return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s is NULL", what, name);
+    if (!float_type(r->type)) return fail(RFXQ_ERR_GGUF, "%s: %s of type %u (F32, F16 or BF16)", what, name, r->type);
+    if (r->rows == 0) return RFXQ_OK;
+    if (!r->data) return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s data is NULL", what, name);
+    if (r->rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "%s: %u rows of %s", what, r->rows, name);
+    if (r->stride < columns || r->stride > (1ull << 40))
+        return fail(RFXQ_ERR_OTHER, "%s: %s stride=%llu (at least %u columns)", what, name,
+                    (unsigned long long)r->stride, columns);
+    if (reinterpret_cast<uintptr_t>(r->data) % elem_bytes(r->type))
+        return fail(RFXQ_ERR_OTHER, "%s: %s at %p is not %u-byte aligned", what, name, r->data, elem_bytes(r->type));
+    return RFXQ_OK;
+}
+
+// bytes from a matrix's first element to its last
+uint64_t rows_span(const rfxq_rows* r, uint32_t columns) {
+    return r->rows ? ((uint64_t)(r->rows - 1u) * r->stride + columns) * elem_bytes(r->type) : 0;
+}
+
+// caller's workspace, or the library's own
+int take_workspace(Ctx* c, void* ws, uint64_t have, uint64_t need, hipStream_t stream, const char* what, void** out) {
+    if (!ws) return need ? ctx_workspace(c, need, out, stream) : RFXQ_OK;
+    if (have < need)
+        return fail(RFXQ_ERR_INVALID_INPUT, "%s: workspace of %llu bytes, needs %llu", what, (unsigned long long)have,
+                    (unsigned long long)need);
+    if (need && !aligned16(ws)) return fail(RFXQ_ERR_OTHER, "%s: workspace is not 16-byte aligned", what);
+    *out = ws;
+    return RFXQ_OK;
+}
+
+// Row tiles that `rows` rows in `groups` groups can need: every group may end
+// inside one.
+uint32_t max_tiles(uint32_t rows, uint32_t groups, uint32_t bm) { return rows / bm + std::min(rows, groups); }
+
+// ------------------------------------------------------------------ grouped GEMM
+
+// f32 activations in pieces of the weights' type: rows of whole 64-element steps
+struct Pieces {
+    uint32_t count, ld;
+    uint64_t plane, exp_at, total;
+};
+Pieces pieces_of(uint32_t ty, uint32_t rows, uint32_t k) {
+    Pieces p;
+    p.count = ty == RFXQ_TYPE_F16 ? 2u : 3u;
+    p.ld = (uint32_t)(((uint64_t)k + 63u) / 64u * 64u);
+    p.plane = (uint64_t)rows * p.ld;
+    p.exp_at = align256(p.plane * p.count * 2u);
+    p.total = p.exp_at + align256(4ull * rows);
+    return p;
+}
+
+// ------------------------------------------------------------------ adapters
+
+// The launch of rfxq_lora_down: ranges of K until the workgroups fill the CUs
+// twice, of at least 256 values each.
+struct LoraPlan {
+    uint32_t ldv, tiles, splits, k_split;
+    uint64_t total;
+};
+LoraPlan lora_plan(uint32_t k, uint32_t rank, uint32_t groups, uint32_t rows, uint32_t cus) {
+    LoraPlan p;
+    p.ldv = (rank + 15u) & ~15u;
+    p.tiles = max_tiles(rows, groups, 16u);
+    const uint32_t want = (2u * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
+    p.splits = std::max(1u, std::min({want, most, 32u}));
+    p.k_split = ((k + p.splits - 1u) / p.splits + 63u) & ~63u;
+    p.splits = (k + p.k_split - 1u) / p.k_split;
+    p.total = align256(4ull * p.splits * rows * p.ldv);
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order,
+                    hipStream_t stream) {
+    if (groups == 0 || groups > kMaxGroups)
+        return fail(RFXQ_ERR_OTHER, "group_rows: groups=%u (1..=%u)", groups, kMaxGroups);
+    if (n > kMaxGroupRows) return fail(RFXQ_ERR_OTHER, "group_rows: n=%u (at most %u)", n, kMaxGroupRows);
+    if (!offsets || (n && (!ids || !order))) return fail(RFXQ_ERR_INVALID_INPUT, "group_rows: NULL pointer");
+    if ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(order)) % 4u)
+        return fail(RFXQ_ERR_OTHER, "group_rows: a pointer is not 4-byte aligned");
+    if (overlap(ids, 4ull * n, order, 4ull * n) || overlap(ids, 4ull * n, offsets, 4ull * (groups + 1u)) ||
+        overlap(order, 4ull * n, offsets, 4ull * (groups + 1u)))
+        return fail(RFXQ_ERR_INVALID_INPUT, "group_rows: ids, offsets and order overlap");
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    const uint32_t rounds = n > 64u * kGroupThreads ? 4u : 1u;
+    GroupRowsArgs a = {ids, offsets, order, n, groups, rounds, 0};
+    const uint32_t keys = groups + 1u, lds = 8u * keys + 4u * ((16u * keys + 1u) / 2u);
+    const uint32_t grid = std::max(1u, (n + kGroupThreads * rounds - 1u) / (kGroupThreads * rounds));
+    if (int rc = launch(c->half.group_rows, grid, lds, stream, &a, sizeof a, "rfxq_group_rows launch", kGroupThreads))
+        return rc;
+    return ok();
+}
+
+uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows, uint32_t x_type) {
+    if (!w || x_type != RFXQ_TYPE_F32 || !half_type(w->ggml_type) || x_rows == 0) return 0;
+    return pieces_of(w->ggml_type, x_rows, w->in_features).total;
+}
+
+int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
+                      const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
+                      void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+    if (int rc = check_stack(w, false, "grouped_gemm")) return rc;
+    if (int rc = check_rows(x, w->in_features, "grouped_gemm", "x")) return rc;
+    if (int rc = check_rows(y, w->out_features, "grouped_gemm", "y")) return rc;
+    const uint32_t ty = w->ggml_type, k = w->in_features, n = w->out_features;
+    if (x->type != RFXQ_TYPE_F32 && x->type != ty)
+        return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: x of type %u with weights of type %u (F32 or the weights')",
+                    x->type, ty);
+    if (y->type != RFXQ_TYPE_F32 && y->type != ty)
+        return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: y of type %u with weights of type %u (F32 or the weights')",
+                    y->type, ty);
+    if (rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "grouped_gemm: rows=%u", rows);
+    if (x_div == 0) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: x_div=0");
+    if (!x_index && x_div != 1) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: x_div=%u without x_index", x_div);
+    if (rows == 0 || x->rows == 0 || y->rows == 0) return ok();
+    if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: offsets is NULL");
+    if (overlap(x->data, rows_span(x, k), y->data, rows_span(y, n)))
+        return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: x and y overlap");
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    const uint32_t t = ty == RFXQ_TYPE_F16 ? 0u : 1u, groups = std::max(w->expert_count, 1u);
+    GroupedArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.x = x->data;
+    a.w = w->data;
+    a.y = y->data;
+    a.offsets = offsets;
+    a.x_index = x_index;
+    a.y_index = y_index;
+    a.ldx = x->stride;
+    a.ldy = y->stride;
+    a.w_stride = (uint64_t)k * n;
+    a.rows = rows;
+    a.x_rows = x->rows;
+    a.y_rows = y->rows;
+    a.x_div = x_div;
+    a.k = k;
+    a.n = n;
+    a.groups = groups;
+    a.pieces = 1;
+    a.y_f32 = y->type == RFXQ_TYPE_F32 ? 1u : 0u;
+    constexpr uint32_t bm = 64, bn = 128;
+    a.tiles_m = max_tiles(rows, groups, bm);
+    a.tiles_n = (n + bn - 1u) / bn;
+    a.sm = 4;
+    a.sn = 8;
+    const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
+    const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
+    if (grid > 0x7FFFFFFFull)
+        return fail(RFXQ_ERR_OTHER, "grouped_gemm: %u rows x %u columns need %llu workgroups", rows, n,
+                    (unsigned long long)grid);
+    if (x->type == RFXQ_TYPE_F32) {
+        const Pieces p = pieces_of(ty, x->rows, k);
+        void* ws = nullptr;
+        if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "grouped_gemm", &ws)) return rc;
+        uint8_t* base = static_cast<uint8_t*>(ws);
+        int32_t* exp = reinterpret_cast<int32_t*>(base + p.exp_at);
+        SplitArgs s = {static_cast<const float*>(x->data), ws, exp, x->stride, p.plane, x->rows, k, p.ld, 0};
+        if (int rc = launch(c->half.split[t], std::min((x->rows + 3u) / 4u, 16384u), 0, stream, &s, sizeof s,
+                            "rfxq_split launch"))
+            return rc;
+        a.x = ws;
+        a.ldx = p.ld;
+        a.plane = p.plane;
+        a.pieces = p.count;
+        a.x_exp = exp;
+    }
+    if (int rc = launch(c->half.any[t], (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch")) return rc;
+    return ok();
+}
+
+uint64_t rfxq_lora_add_workspace_size(const rfxq_weight* a, uint32_t rows) {
+    if (!a || rows == 0 || a->in_features == 0 || a->out_features == 0) return 0;
+    const Ctx* c = loaded_ctx();
+    // What any number of rows up to `rows` needs: there are at least rows / 16
+    // tiles, so the ranges are fewer than 32 CUs / rows + 1 (fewer rows can take
+    // more ranges, and more memory, than the most rows do).
+    const uint64_t ldv = (a->out_features + 15ull) & ~15ull, cus = c ? (uint64_t)c->cus : 256u;
+    return align256(4u * ldv * std::min<uint64_t>(32ull * rows, 32u * cus + rows));
+}
+
+int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b, const int32_t* ranks,
+                  const float* scales, const int32_t* offsets, const int32_t* order, const rfxq_rows* y,
+                  const rfxq_rows* out, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+    if (int rc = check_stack(a, true, "lora_add a")) return rc;
+    if (int rc = check_stack(b, true, "lora_add b")) return rc;
+    const uint32_t k = a->in_features, rank = a->out_features, n = b->out_features;
+    if (b->in_features != rank || b->expert_count != a->expert_count || b->ggml_type != a->ggml_type)
+        return fail(RFXQ_ERR_OTHER, "lora_add: a [%u, %u, %u] of type %u and b [%u, %u, %u] of type %u", k, rank,
+                    a->expert_count, a->ggml_type, b->in_features, n, b->expert_count, b->ggml_type);
+    if (int rc = check_rows(x, k, "lora_add", "x")) return rc;
+    if (int rc = check_rows(y, n, "lora_add", "y")) return rc;
+    if (int rc = check_rows(out, n, "lora_add", "out")) return rc;
+    if (x->rows != y->rows || x->rows != out->rows)
+        return fail(RFXQ_ERR_OTHER, "lora_add: %u rows of x, %u of y, %u of out", x->rows, y->rows, out->rows);
+    if (x->type != y->type || x->type != out->type || (x->type != RFXQ_TYPE_F32 && x->type != a->ggml_type))
+        return fail(RFXQ_ERR_INVALID_INPUT,
+                    "lora_add: x of type %u, y %u, out %u with adapters of type %u (one type, F32 or the adapters')",
+                    x->type, y->type, out->type, a->ggml_type);
+    const uint32_t rows = x->rows, groups = std::max(a->expert_count, 1u);
+    if (rows == 0) return ok();
+    if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "lora_add: offsets is NULL");
+    const uint64_t sx = rows_span(x, k), sy = rows_span(y, n), so = rows_span(out, n);
+    if (overlap(x->data, sx, out->data, so)) return fail(RFXQ_ERR_INVALID_INPUT, "lora_add: x and out overlap");
+    if (!(y->data == out->data && y->stride == out->stride) && overlap(y->data, sy, out->data, so))
+        return fail(RFXQ_ERR_INVALID_INPUT, "lora_add: y and out overlap without being the same rows");
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    const LoraPlan p = lora_plan(k, rank, groups, rows, (uint32_t)c->cus);
+    const uint32_t tiles_n = (n + 255u) / 256u;
+    const uint64_t up = (uint64_t)(p.tiles + 1u) * tiles_n;
+    if (up > 0x7FFFFFFFull || (uint64_t)p.tiles * p.splits > 0x7FFFFFFFull)
+        return fail(RFXQ_ERR_OTHER, "lora_add: %u rows x %u columns need %llu workgroups", rows, n,
+                    (unsigned long long)up);
+    void* ws = nullptr;
+    if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "lora_add", &ws)) return rc;
+    const uint32_t xe = 16u / elem_bytes(x->type), we = 16u / elem_bytes(a->ggml_type);
+    LoraArgs l;
+    std::memset(&l, 0, sizeof l);
+    l.x = x->data;
+    l.a = a->data;
+    l.b = b->data;
+    l.ranks = ranks;
+    l.scales = scales;
+    l.offsets = offsets;
+    l.order = order;
+    l.y = y->data;
+    l.out = out->data;
+    l.v = static_cast<float*>(ws);
+    l.ldx = x->stride;
+    l.ldy = y->stride;
+    l.ldo = out->stride;
+    l.rows = l.x_rows = rows;
+    l.k = k;
+    l.n = n;
+    l.rank = rank;
+    l.ldv = p.ldv;
+    l.groups = groups;
+    l.splits = p.splits;
+    l.k_split = p.k_split;
+    l.tiles = p.tiles;
+    l.tiles_n = tiles_n;
+    l.vec = (aligned16(x->data) && x->stride % xe == 0 ? 1u : 0u) | (aligned16(a->data) && k % we == 0 ? 2u : 0u) |
+            (aligned16(b->data) && rank % we == 0 ? 4u : 0u);
+    const uint32_t t = x->type == RFXQ_TYPE_F32 ? (a->ggml_type == RFXQ_TYPE_F32 ? 0u : a->ggml_type == RFXQ_TYPE_F16 ? 1u : 2u)
+                       : x->type == RFXQ_TYPE_F16 ? 3u : 4u;
+    if (int rc = launch(c->half.lora_down[t], p.tiles * p.splits, 0, stream, &l, sizeof l, "rfxq_lora_down launch"))
+        return rc;
+    if (int rc = launch(c->half.lora_up[t], (uint32_t)up, 0, stream, &l, sizeof l, "rfxq_lora_up launch")) return rc;
+    return ok();
+}
+
+}  // extern "C"

@@ -36,6 +36,7 @@
 
 extern "C" const unsigned char rfxq_code_object[];
 extern "C" const unsigned char rfxq_code_object_end[];
+extern "C" const unsigned char rfxq_half_code_object[];
 
 namespace {
 
@@ -144,6 +145,15 @@ constexpr uint32_t kNormRowsPerWg = 4;  // rows per rfxq_rmsnorm_q8_1 workgroup 
 
 // ------------------------------------------------------------------ per-device module
 
+// kernels of the second code object (half_host.hpp)
+struct HalfKernels {
+    hipFunction_t group_rows = nullptr;
+    // [F16, BF16]
+    hipFunction_t any[2] = {}, split[2] = {};
+    // [f32 x F32, f32 x F16, f32 x BF16, F16, BF16]
+    hipFunction_t lora_down[5] = {}, lora_up[5] = {};
+};
+
 struct Ctx {
     int device = -1;
     int cus = 256;
@@ -162,6 +172,8 @@ struct Ctx {
     hipFunction_t moe_route = nullptr, moe_route_w = nullptr, moe_plan = nullptr;
     // MoE decode kernels: [Q4_K, Q6_K, Q8_0][4, 8, 16, 32 lanes per row]
     hipFunction_t moe_dec_gu[3][4] = {}, moe_dec_dn[3][4] = {};
+    hipModule_t half_mod = nullptr;  // half.hip: grouped rows, half-typed stacks, adapters
+    HalfKernels half;
     void* ws = nullptr;
     uint64_t ws_bytes = 0;
     void* scratch = nullptr;  // this device's fixed scratch array (rfxq_gemm_no_alloc)
@@ -189,6 +201,34 @@ std::map<int, std::unique_ptr<Ctx>> g_ctx;
 uint64_t align256(uint64_t v) { return (v + 255u) & ~(uint64_t)255u; }
 
 int type_index(uint32_t ty) { return ty == RFXQ_TYPE_Q4_K ? 0 : ty == RFXQ_TYPE_Q6_K ? 1 : 2; }
+
+int load_half(hipModule_t mod, HalfKernels* h) {
+    struct {
+        hipFunction_t* f;
+        const char* name;
+    } fns[] = {
+        {&h->group_rows, "rfxq_group_rows"},
+        {&h->any[0], "rfxq_grouped_any_f16"},
+        {&h->any[1], "rfxq_grouped_any_bf16"},
+        {&h->split[0], "rfxq_split_f16"},
+        {&h->split[1], "rfxq_split_bf16"},
+    };
+    for (auto& f : fns) {
+        hipError_t e = hipModuleGetFunction(f.f, mod, f.name);
+        if (e != hipSuccess)
+            return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", f.name, hipGetErrorString(e));
+    }
+    static const char* const kLora[5] = {"f32_f32", "f32_f16", "f32_bf16", "f16_f16", "bf16_bf16"};
+    for (int t = 0; t < 5; t++)
+        for (int up = 0; up < 2; up++) {
+            char name[64];
+            std::snprintf(name, sizeof name, "rfxq_lora_%s_%s", up ? "up" : "down", kLora[t]);
+            hipError_t e = hipModuleGetFunction(up ? &h->lora_up[t] : &h->lora_down[t], mod, name);
+            if (e != hipSuccess)
+                return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name, hipGetErrorString(e));
+        }
+    return RFXQ_OK;
+}
 
 int load_ctx(int device, Ctx** out) {
     std::lock_guard<std::mutex> lk(g_mu);
@@ -275,6 +315,8 @@ int load_ctx(int device, Ctx** out) {
                 if (e != hipSuccess)
                     return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name, hipGetErrorString(e));
             }
+    HIPCHK(hipModuleLoadData(&c->half_mod, rfxq_half_code_object), "hipModuleLoadData(embedded gfx950 code object)");
+    if (int rc = load_half(c->half_mod, &c->half)) return rc;
     // the fixed scratch of rfxq_gemm_no_alloc, resolved now (the device is
     // current); a failure disables only that entry point, which reports it
     c->scratch_err = rfxq_scratch::setup(device, &c->scratch);
@@ -3716,3 +3758,5 @@ int rfxq_gguf_upload(const rfxq_gguf* g, const uint64_t* indices, uint32_t count
 }
 
 }  // extern "C"
+
+#include "half_host.hpp"

@@ -1,0 +1,174 @@
+// Rows grouped by an id (rfxq_group_rows), and the search of the products that
+// work on such groups for the tile a workgroup computes.
+//
+// key_i = id_i, or `groups` for an id outside [0, groups);
+//   offsets[g] = #{ i : key_i < g }, g = 0..groups
+//   order      = the rows i sorted by (key_i, i)
+// a stable counting sort: the place of row i is
+//   offsets[key_i] + #{ j < i : key_j = key_i }.
+#pragma once
+#include "common.hpp"
+
+constexpr uint32_t kMaxGroups = 1024;
+
+// Inclusive sum over the wave's lanes: within 16-lane rows by row shifts, then
+// the rows' last lanes carried over (row_bcast 15 and 31).
+RFXQ_DEV uint32_t wave_scan(uint32_t v) {
+#define RFXQ_SCAN(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, (ctrl), (rows), 0xF, false)
+    RFXQ_SCAN(0x111, 0xF);
+    RFXQ_SCAN(0x112, 0xF);
+    RFXQ_SCAN(0x114, 0xF);
+    RFXQ_SCAN(0x118, 0xF);
+    RFXQ_SCAN(0x142, 0xA);
+    RFXQ_SCAN(0x143, 0xC);
+#undef RFXQ_SCAN
+    return v;
+}
+
+// The rows [beg, end) of one tile of at most `bm` rows, all of one group; where
+// there is none (any = false), `beg` is the tile's number behind the last one.
+struct RowTile {
+    uint32_t group, beg, end;
+    bool any;
+};
+
+// Tile t of the grouped rows: the groups' tiles counted in order, each group
+// starting a tile of its own. Every wave searches by itself (no LDS, no
+// barrier): lane l holds `per` neighbouring groups. Offsets are taken as they
+// are found: clamped to [0, rows] and to what came before, so that no value
+// there leads outside the arrays.
+RFXQ_DEV RowTile find_tile(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t bm, uint32_t t) {
+    const uint32_t lane = threadIdx.x & 63u, per = (groups + 63u) / 64u;
+    const uint32_t g0 = lane * per < groups ? lane * per : groups;
+    const uint32_t g1 = g0 + per < groups ? g0 + per : groups;
+    const auto at = [&](uint32_t g) {
+        const int32_t o = offsets[g];
+        return o < 0 ? 0u : (uint32_t)o < rows ? (uint32_t)o : rows;
+    };
+    uint32_t mine = 0;
+    for (uint32_t g = g0; g < g1; g++) {
+        const uint32_t b = at(g), e = at(g + 1u);
+        mine += e > b ? (e - b + bm - 1u) / bm : 0u;
+    }
+    const uint32_t upto = wave_scan(mine);
+    const uint64_t has = __builtin_amdgcn_ballot_w64(upto > t);
+    RowTile r = {0, t - (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), 0, false};
+    if (!has) return r;
+    const uint32_t l = (uint32_t)__builtin_ctzll(has);
+    uint32_t left = t - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), (int)l);  // among lane l's tiles
+    const uint32_t e0 = l * per, e1 = e0 + per < groups ? e0 + per : groups;
+    for (uint32_t g = e0; g < e1; g++) {
+        const uint32_t b = at(g), e = at(g + 1u);
+        const uint32_t n = e > b ? (e - b + bm - 1u) / bm : 0u;
+        if (left < n) {
+            r.group = g;
+            r.beg = b + left * bm;
+            r.end = r.beg + bm < e ? r.beg + bm : e;
+            r.any = true;
+            break;
+        }
+        left -= n;
+    }
+    r.group = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.group);
+    r.beg = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.beg);
+    r.end = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.end);
+    return r;
+}
+
+struct GroupRowsArgs {
+    const int32_t* ids;
+    int32_t* offsets;
+    int32_t* order;
+    uint32_t n, groups, rounds, pad;
+};
+
+constexpr uint32_t kGroupThreads = 1024, kGroupWaves = kGroupThreads / 64u, kGroupRounds = 4;
+
+// Workgroup b places rows [b c, (b + 1) c), c = 1024 rounds, and counts the
+// ids of all n rows by itself, those before its own apart: one launch, no
+// scratch memory and no waiting between workgroups. The ids are read once by
+// every workgroup (from L2).
+//
+// Dynamic LDS: cnt[2][groups + 1] (rows before the workgroup's own; the
+// others), then wcnt[16][groups + 1] (16 bits: a wave's own rows).
+extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs a) {
+    extern __shared__ uint32_t lds[];
+    const uint32_t keys = a.groups + 1u, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    uint32_t* before = lds;
+    uint32_t* rest = lds + keys;
+    uint16_t* wcnt = reinterpret_cast<uint16_t*>(lds + 2u * keys);
+    __shared__ uint32_t part[kGroupWaves];
+    const uint32_t words = 2u * keys + (kGroupWaves * keys + 1u) / 2u;
+    for (uint32_t i = tid; i < words; i += kGroupThreads) lds[i] = 0;
+    __syncthreads();
+
+    const uint32_t chunk = kGroupThreads * a.rounds, begin = blockIdx.x * chunk;
+    const auto key_of = [&](uint32_t i) {
+        const uint32_t id = (uint32_t)a.ids[i];
+        return id < a.groups ? id : a.groups;
+    };
+    for (uint32_t i = tid; i < a.n; i += kGroupThreads) atomicAdd(&(i < begin ? before : rest)[key_of(i)], 1u);
+    __syncthreads();
+
+    // exclusive sums over the groups' counts, a thread per group
+    const uint32_t all = tid < a.groups ? before[tid] + rest[tid] : 0u;
+    const uint32_t incl = wave_scan(all);
+    if (lane == 63u) part[wave] = incl;
+    __syncthreads();
+    uint32_t base = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kGroupWaves; w++) {
+        base += w < wave ? part[w] : 0u;
+        total += part[w];
+    }
+    base += incl - all;
+    if (blockIdx.x == 0) {
+        if (tid < a.groups) a.offsets[tid] = (int32_t)base;
+        if (tid == 0) a.offsets[a.groups] = (int32_t)total;
+    }
+    if (tid < a.groups) before[tid] += base;
+    if (tid == 0) before[a.groups] += total;
+
+    // the own rows: a wave takes 64 neighbouring rows a round; lanes of one
+    // key find each other by ballots over the key's bits
+    const uint32_t bits = 32u - (uint32_t)__builtin_clz(a.groups);
+    const uint64_t below = ((uint64_t)1 << lane) - 1u;
+    uint32_t key[kGroupRounds], rank[kGroupRounds];
+#pragma unroll
+    for (uint32_t r = 0; r < kGroupRounds; r++) {
+        if (r >= a.rounds) break;
+        const uint32_t i = begin + (wave * a.rounds + r) * 64u + lane;
+        const bool own = i < a.n;
+        key[r] = own ? key_of(i) : 0u;
+        uint64_t same = __builtin_amdgcn_ballot_w64(own);
+        for (uint32_t b = 0; b < bits; b++) {
+            const uint64_t set = __builtin_amdgcn_ballot_w64((key[r] >> b) & 1u);
+            same &= (key[r] >> b) & 1u ? set : ~set;
+        }
+        if (own) {
+            volatile uint16_t* c = &wcnt[wave * keys + key[r]];
+            const uint32_t had = *c, ahead = (uint32_t)__builtin_popcountll(same & below);
+            rank[r] = had + ahead;
+            __builtin_amdgcn_wave_barrier();
+            if (ahead == 0u) *c = (uint16_t)(had + (uint32_t)__builtin_popcountll(same));
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (uint32_t k = tid; k < keys; k += kGroupThreads) {  // each wave's first place of a key
+        uint32_t run = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kGroupWaves; w++) {
+            const uint32_t v = wcnt[w * keys + k];
+            wcnt[w * keys + k] = (uint16_t)run;
+            run += v;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t r = 0; r < kGroupRounds; r++) {
+        if (r >= a.rounds) break;
+        const uint32_t i = begin + (wave * a.rounds + r) * 64u + lane;
+        if (i < a.n) a.order[before[key[r]] + wcnt[wave * keys + key[r]] + rank[r]] = (int32_t)i;
+    }
+}

@@ -16,7 +16,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from . import RfxqGemmPolicy, RfxqGemvItem, RfxqOptions, RfxqWeight, lib
+from . import RfxqGemmPolicy, RfxqGemvItem, RfxqOptions, RfxqRows, RfxqWeight, lib
 
 __all__ = [
     "ReflexError", "GgmlError", "GpuError", "OutOfMemoryError", "InvalidInputError", "IoError", "GgufFile",
@@ -29,6 +29,7 @@ __all__ = [
     "moe_route_device", "moe_ffn_grouped_device",
     "act_q8_1_size", "quantize_act_q8_1", "rmsnorm_q8_1", "silu_and_mul_q8_1", "gemm_q8_1", "gemm_q8_1_batch",
     "gemm_gate_up_silu_q8_1",
+    "RowGroups", "group_rows", "grouped_gemm", "grouped_gemm_workspace_size", "lora_add", "lora_add_workspace_size",
     "get_options", "set_options", "options", "gemm_policy", "PATH_GEMV_ROWS", "PATH_MMQ_INT8", "PATH_MMQ_F16",
 ]
 
@@ -110,6 +111,7 @@ class GgmlType(enum.IntEnum):
     Q8_1 = 9
     Q4K = 12
     Q6K = 14
+    BF16 = 30
 
 
 def ggml_type_block_dims(ty: int) -> tuple[int, int]:
@@ -118,6 +120,9 @@ def ggml_type_block_dims(ty: int) -> tuple[int, int]:
     _check(lib().rfxq_block_dims(int(ty), ctypes.byref(qk), ctypes.byref(bb)))
     return qk.value, bb.value
 
+
+_FLOAT_TYPES = {torch.float32: GgmlType.F32, torch.float16: GgmlType.F16, torch.bfloat16: GgmlType.BF16}
+_FLOAT_DTYPES = {int(v): k for k, v in _FLOAT_TYPES.items()}
 
 # ------------------------------------------------------------------ weights (src/model/loading.rs)
 
@@ -169,6 +174,17 @@ class Weight:
         t = torch.from_numpy(np.ascontiguousarray(blocks).view(np.uint8)).to(device)
         shape = [in_features, out_features] + ([expert_count] if expert_count else [])
         return cls(GgmlType(ty), t, shape)
+
+    @classmethod
+    def from_tensor(cls, t: torch.Tensor) -> "Weight":
+        """A contiguous f32, f16 or bf16 device tensor [out, in] or [count, out, in] as a weight
+        (no copy: the weight reads the tensor's memory)."""
+        if t.dtype not in _FLOAT_TYPES or t.dim() not in (2, 3):
+            raise InvalidInputError(11, f"Weight.from_tensor: {t.dtype} of {t.dim()} dimensions "
+                                        "(f32, f16 or bf16 of 2 or 3)")
+        if not t.is_contiguous():
+            raise InvalidInputError(11, "Weight.from_tensor: the tensor is not contiguous")
+        return cls(_FLOAT_TYPES[t.dtype], t, list(reversed(t.shape)), len=t.numel() * t.element_size())
 
     def quant_ptr(self) -> int:
         return self.arena.data_ptr() + self.offset
@@ -588,6 +604,133 @@ def moe_ffn_grouped_device(x: torch.Tensor, rows: int, hidden: int, router_logit
         _check(lib().rfxq_moe_ffn_grouped_device(x.data_ptr(), rows, hidden, router_logits.data_ptr(), expert_count,
                                                  top_k, int(normalize), float(weight_scale), gate.cref(), up.cref(),
                                                  down.cref(), out.data_ptr(), _stream()))
+
+
+# ------------------------------------------------------------------ grouped rows, half-typed stacks, adapters
+
+@dataclass
+class RowGroups:
+    """Rows grouped by an id (``rfxq_group_rows``): group g's rows are
+    ``order[offsets[g]:offsets[g + 1]]``, rows in no group come last."""
+
+    offsets: torch.Tensor  # int32 [groups + 1]
+    order: torch.Tensor    # int32 [rows]
+
+
+def _ints(t: torch.Tensor | None, least: int, like: torch.Tensor, what: str) -> int | None:
+    """The address of an int32 device tensor of at least ``least`` values."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least or t.device != like.device:
+        raise InvalidInputError(11, f"{what}: needs {least} contiguous int32 values on {like.device}, got "
+                                    f"{t.numel()} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, columns: int, like: torch.Tensor, what: str) -> RfxqRows:
+    """``rfxq_rows`` of a 2-D tensor whose rows are contiguous."""
+    ty = _FLOAT_TYPES.get(t.dtype)
+    if ty is None or t.dim() != 2 or t.shape[1] != columns or t.device != like.device:
+        raise InvalidInputError(11, f"{what}: {t.dtype} {list(t.shape)} on {t.device} (f32, f16 or bf16 "
+                                    f"[rows, {columns}] on {like.device})")
+    rows = t.shape[0]
+    if (columns > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < columns):
+        raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
+    return RfxqRows(t.data_ptr(), ty, rows, t.stride(0) if rows > 1 else columns)
+
+
+def _space(t: torch.Tensor | None, like: torch.Tensor, what: str) -> tuple[int | None, int]:
+    if t is None:
+        return None, 0
+    if not t.is_contiguous() or t.device != like.device:
+        raise InvalidInputError(11, f"{what}: the workspace must be contiguous and on {like.device}")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _check_stack(w: Weight, like: torch.Tensor, what: str) -> None:
+    if w.arena.device != like.device:
+        raise InvalidInputError(11, f"{what}: weight on {w.arena.device}, rows on {like.device}")
+
+
+def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None) -> RowGroups:
+    """Rows grouped by an int32 device id (a routed expert, a request's adapter); an id
+    outside [0, groups) is a row in no group. Stable: a group's rows keep their order."""
+    n = ids.numel()
+    if not ids.is_cuda:
+        raise InvalidInputError(11, f"group_rows: ids on {ids.device}")
+    src = _ints(ids, n, ids, "group_rows ids")
+    if out is None:
+        if groups < 0:
+            raise InvalidInputError(11, f"group_rows: groups={groups}")
+        out = RowGroups(torch.empty(groups + 1, dtype=torch.int32, device=ids.device),
+                        torch.empty(n, dtype=torch.int32, device=ids.device))
+    with _dev(ids):
+        _check(lib().rfxq_group_rows(src, n, groups, _ints(out.offsets, groups + 1, ids, "group_rows offsets"),
+                                     _ints(out.order, n, ids, "group_rows order"), _stream()))
+    return out
+
+
+def grouped_gemm_workspace_size(w: Weight, x_rows: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace ``grouped_gemm`` needs for x of this many rows and type."""
+    return int(lib().rfxq_grouped_gemm_workspace_size(w.cref(), x_rows, int(_FLOAT_TYPES[dtype])))
+
+
+def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
+                 x_div: int = 1, y_index: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Products of grouped rows with a stack of F16 / BF16 matrices: for the places p of group g,
+    ``out[y_index[p]] = x[x_index[p] // x_div] @ W[g].T`` (either index may be left out: place p itself).
+    The counterpart of ``expert_gemm`` for all experts at once. Without ``out``, a new tensor of x's type with
+    ``rows`` rows, zero where no place of a group writes."""
+    count = int(w.shape[2]) if len(w.shape) > 2 else 1
+    if not x.is_cuda:
+        raise InvalidInputError(11, f"grouped_gemm: x on {x.device}")
+    _check_stack(w, x, "grouped_gemm")
+    if rows < 0 or x_div < 1:
+        raise InvalidInputError(11, f"grouped_gemm: rows={rows} x_div={x_div}")
+    xr = _rows(x, w.in_features, x, "grouped_gemm x")
+    y = out if out is not None else torch.zeros(rows, w.out_features, dtype=x.dtype, device=x.device)
+    yr = _rows(y, w.out_features, x, "grouped_gemm out")
+    space, size = _space(workspace, x, "grouped_gemm")
+    with _dev(x):
+        _check(lib().rfxq_grouped_gemm(ctypes.byref(xr), w.cref(), _ints(offsets, count + 1, x, "grouped_gemm offsets"),
+                                       rows, _ints(x_index, rows, x, "grouped_gemm x_index"), x_div,
+                                       _ints(y_index, rows, x, "grouped_gemm y_index"), ctypes.byref(yr), space, size,
+                                       _stream()))
+    return y
+
+
+def lora_add_workspace_size(a: Weight, rows: int) -> int:
+    """Bytes of workspace ``lora_add`` needs for up to this many rows."""
+    return int(lib().rfxq_lora_add_workspace_size(a.cref(), rows))
+
+
+def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.Tensor,
+             ranks: torch.Tensor | None = None, scales: torch.Tensor | None = None, out: torch.Tensor | None = None,
+             workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection: ``out[r] = y[r] + scales[g] * B[g] (A[g] x[r])``
+    for the rows r of group g, ``out[r] = y[r]`` for rows in no group. a [count, rank, in] and b [count, out, rank]
+    are stacks; adapter g is their first ``ranks[g]`` rows and columns. ``groups``: the rows grouped by their adapter
+    ids (``group_rows``). Without ``out``, y itself is updated."""
+    count = int(a.shape[2]) if len(a.shape) > 2 else 1
+    if not x.is_cuda:
+        raise InvalidInputError(11, f"lora_add: x on {x.device}")
+    _check_stack(a, x, "lora_add a")
+    _check_stack(b, x, "lora_add b")
+    out = y if out is None else out
+    xr = _rows(x, a.in_features, x, "lora_add x")
+    yr, outr = (_rows(t, b.out_features, x, f"lora_add {m}") for t, m in ((y, "y"), (out, "out")))
+    if scales is not None and (scales.dtype != torch.float32 or scales.numel() < count or not scales.is_contiguous()
+                               or scales.device != x.device):
+        raise InvalidInputError(11, f"lora_add: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
+                                    f"(f32, {count} values)")
+    space, size = _space(workspace, x, "lora_add")
+    with _dev(x):
+        _check(lib().rfxq_lora_add(ctypes.byref(xr), a.cref(), b.cref(), _ints(ranks, count, x, "lora_add ranks"),
+                                   _ptr(scales), _ints(groups.offsets, count + 1, x, "lora_add offsets"),
+                                   _ints(groups.order, x.shape[0], x, "lora_add order"), ctypes.byref(yr),
+                                   ctypes.byref(outr), space, size, _stream()))
+    return out
 
 
 # ------------------------------------------------------------------ GGUF files

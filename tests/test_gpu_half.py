@@ -1,0 +1,497 @@
+"""Grouped rows, products with F16 / BF16 stacks and low-rank adapters (rfxq_group_rows,
+rfxq_grouped_gemm, rfxq_lora_add) against their definitions in 64 bits on the CPU.
+
+Bounds, per result: a half-typed output is off by half a step, eps / 2 of its value; a sum of K products
+held in f32 by at most 2^-23 of the sum of the products' sizes per addition, with K / 32 + 32 additions in
+a row (the matrix instructions add 32 products, or 4 of f32 operands, to the sum at once; parts of a sum that are
+added later are counted in). f32 activations beside f16 weights are split into two f16 pieces, which leave
+2^-22 of a value (half a step of the second piece, 2^-11 of 2^-11) and 2^-39 of its row's largest (half a
+step of f16's smallest number, 2^-25, at a largest of 2^14 or more); beside bf16 weights three pieces are
+exact but for what is below f32's range. A value below f32's or f16's normal range keeps an absolute step."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TINY = {F32: 2.0 ** -149, F16: 2.0 ** -24, BF16: 2.0 ** -133}
+
+
+def _say(*what):
+    print(*what, flush=True)
+
+
+# ------------------------------------------------------------------ group_rows
+
+def _grouped(ids, groups):
+    key = np.where((ids >= 0) & (ids < groups), ids, groups)
+    order = np.argsort(key, kind="stable").astype(np.int32)
+    offsets = np.searchsorted(key[order], np.arange(groups + 1)).astype(np.int32)
+    return offsets, order
+
+
+def _ids(n, groups, how, seed=0):
+    r = np.random.default_rng(seed + n + groups)
+    if how == "any":  # some in no group, on either side
+        return r.integers(-1, groups + 1, n).astype(np.int32)
+    if how == "one":
+        return np.full(n, groups - 1, np.int32)
+    if how == "none":
+        return np.where(r.random(n) < 0.5, -(1 << 31), (1 << 31) - 1).astype(np.int32)
+    if how == "rising":
+        return np.sort(r.integers(0, groups, n)).astype(np.int32)
+    return r.integers(0, groups, n).astype(np.int32)
+
+
+@pytest.mark.parametrize("how", ["any", "one", "none", "rising", "all"])
+@pytest.mark.parametrize("n,groups", [(0, 5), (1, 1), (2, 3), (63, 2), (64, 128), (65, 1024), (300, 37), (1000, 128),
+                                      (1024, 7), (1025, 1023), (4096, 128), (65536, 64), (65537, 1024),
+                                      (131077, 129)])
+def test_group_rows(rq, n, groups, how):
+    _say("group_rows", n, groups, how)
+    ids = _ids(n, groups, how)
+    guard = 77
+    offsets = torch.full((groups + 1 + 8,), guard, dtype=torch.int32, device=DEV)
+    order = torch.full((n + 8,), guard, dtype=torch.int32, device=DEV)
+    g = rq.group_rows(torch.from_numpy(ids).to(DEV), groups, out=rq.RowGroups(offsets, order))
+    want_offsets, want_order = _grouped(ids, groups)
+    assert np.array_equal(g.offsets.cpu().numpy()[:groups + 1], want_offsets)
+    assert np.array_equal(g.order.cpu().numpy()[:n], want_order)
+    assert (offsets[groups + 1:] == guard).all() and (order[n:] == guard).all()
+
+
+def test_group_rows_unaligned_ids_and_new_outputs(rq):
+    ids = _ids(5001, 37, "any")
+    t = torch.from_numpy(np.concatenate([ids[:1], ids])).to(DEV)[1:]  # starts 4 bytes into its memory
+    g = rq.group_rows(t, 37)
+    want_offsets, want_order = _grouped(ids, 37)
+    assert np.array_equal(g.offsets.cpu().numpy(), want_offsets) and np.array_equal(g.order.cpu().numpy(), want_order)
+
+
+# ------------------------------------------------------------------ grouped_gemm
+
+def _strided(values, stride, shift, pad):
+    """`values` [rows, cols] on the GPU as a view of rows `stride` apart, `shift` elements into memory that
+    holds `pad` elsewhere."""
+    rows, cols = values.shape
+    memory = torch.full((shift + max(rows, 1) * stride + 8,), pad, dtype=values.dtype, device=DEV)
+    view = memory[shift:shift + rows * stride].view(rows, stride)[:, :cols]
+    view.copy_(values)
+    return view, memory
+
+
+def _product_bound(x, w, y64, x_type, w_type, y_type, pieces=None):
+    """Largest allowed |error| per result of x @ w.T (64-bit arrays)."""
+    k = x.shape[1]
+    size = np.abs(x) @ np.abs(w).T
+    count = {F32: 2 if w_type == F16 else 3}.get(x_type, 1)
+    b = (count * (k / 32) + 32) * 2.0 ** -23 * size
+    if x_type == F32:
+        b = b + 2.0 ** -22 * size + 2.0 ** -39 * np.abs(x).max(1, keepdims=True, initial=0) * np.abs(w).sum(1)
+    return b + torch.finfo(y_type).eps / 2 * (np.abs(y64) + b) + TINY[y_type]
+
+
+def _case(rows, groups, k, n, x_type, w_type, seed, x_rows=None):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(x_rows or rows, k, generator=gen)
+    if k > 1:
+        x[:, k // 2] *= 8
+    w = (torch.randn(groups, n, k, generator=gen) * 0.05).to(w_type)
+    return x.to(x_type), w
+
+
+def _run_grouped(rq, x, w, offsets, rows, x_index, x_div, y_index, y_type, y_rows, xs=(0, 0), ys=(0, 0), ws=0,
+                 workspace=None):
+    """grouped_gemm on strided and shifted copies: (y, what lies around y unchanged)."""
+    k, n = x.shape[1], w.shape[1]
+    xv, _ = _strided(x.to(DEV), k + xs[0], xs[1], float("nan"))
+    yv, ymem = _strided(torch.full((y_rows, n), 123.0, dtype=y_type, device=DEV), n + ys[0], ys[1], 99.0)
+    wmem = torch.full((w.numel() + ws + 8,), float("nan"), dtype=w.dtype, device=DEV)
+    wmem[ws:ws + w.numel()] = w.reshape(-1).to(DEV)
+    weight = rq.Weight.from_tensor(wmem[ws:ws + w.numel()].view(w.shape))
+    dev = lambda v: None if v is None else torch.from_numpy(np.asarray(v, np.int32)).to(DEV)  # noqa: E731
+    rq.grouped_gemm(xv, weight, dev(offsets), rows, x_index=dev(x_index), x_div=x_div, y_index=dev(y_index), out=yv,
+                    workspace=workspace)
+    torch.cuda.synchronize()
+    around = ymem.clone()
+    around[ys[1]:ys[1] + y_rows * (n + ys[0])].view(y_rows, -1)[:, :n] = 99.0
+    return yv.cpu(), bool((around == 99.0).all())
+
+
+def _check_grouped(x, w, offsets, x_index, x_div, y_index, y):
+    """Every row of y: its product's within the bound, or what it was."""
+    want = np.full(y.shape, 123.0)
+    bound = np.zeros(y.shape)
+    x64, w64 = x.double().numpy(), w.double().numpy()
+    for g in range(w.shape[0]):
+        p = np.arange(offsets[g], offsets[g + 1])
+        src = p if x_index is None else np.where(np.asarray(x_index)[p] < 0, -1, np.asarray(x_index)[p] // x_div)
+        dst = p if y_index is None else np.asarray(y_index)[p]
+        fine = (src >= 0) & (src < x.shape[0]) & (dst >= 0) & (dst < y.shape[0])
+        src, dst = src[fine], dst[fine]
+        want[dst] = x64[src] @ w64[g].T
+        bound[dst] = _product_bound(x64[src], w64[g], want[dst], x.dtype, w.dtype, y.dtype)
+    off = np.abs(y.double().numpy() - want)
+    assert np.isfinite(off).all()
+    worst = np.unravel_index(np.argmax(off - bound), off.shape)
+    assert (off <= bound).all(), (worst, off[worst], bound[worst])
+    rel = np.linalg.norm(off) / np.linalg.norm(want)
+    # rounding errors of either sign: well under a half step of y, and for f32 under 2^-19 (a lost piece
+    # of the activations would leave 2^-13)
+    assert rel <= (torch.finfo(y.dtype).eps / 2 if y.dtype != F32 else 2.0 ** -19), rel
+
+
+TYPES = [(F16, F16, F16), (BF16, BF16, BF16), (F32, F16, F32), (F32, BF16, F32), (F16, F16, F32), (F32, BF16, BF16)]
+
+
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES)
+@pytest.mark.parametrize("rows,groups,k,n", [
+    (1, 1, 1, 1), (1, 8, 64, 128), (2, 3, 7, 15), (8, 128, 256, 96), (17, 4, 72, 64), (33, 2, 128, 129), (64, 5, 8, 16),
+    (65, 3, 200, 300), (130, 7, 1235, 153), (300, 1, 576, 257), (513, 40, 320, 128), (700, 6, 2056, 384)])
+def test_grouped_gemm(rq, rows, groups, k, n, x_type, w_type, y_type):
+    _say("grouped_gemm", rows, groups, k, n, x_type, w_type, y_type)
+    x, w = _case(rows, groups, k, n, x_type, w_type, rows + k)
+    ids = _ids(rows, groups, "all")
+    offsets, _ = _grouped(ids, groups)
+    y, kept = _run_grouped(rq, x, w, offsets, rows, None, 1, None, y_type, rows)
+    _check_grouped(x, w, offsets, None, 1, None, y)
+    assert kept
+
+
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES[:4])
+@pytest.mark.parametrize("xs,ys,ws", [((8, 0), (8, 0), 0), ((3, 1), (5, 3), 1), ((0, 2), (0, 0), 0), ((0, 0), (1, 0), 2),
+                                      ((16, 8), (16, 8), 8)])
+def test_grouped_gemm_strides(rq, xs, ys, ws, x_type, w_type, y_type):
+    """Rows with space behind them (NaN in it), and memory that starts anywhere."""
+    _say("grouped_gemm strides", xs, ys, ws, x_type, w_type, y_type)
+    rows, groups, k, n = 90, 4, 136, 144
+    x, w = _case(rows, groups, k, n, x_type, w_type, 5)
+    offsets, _ = _grouped(_ids(rows, groups, "all"), groups)
+    y, kept = _run_grouped(rq, x, w, offsets, rows, None, 1, None, y_type, rows, xs, ys, ws)
+    _check_grouped(x, w, offsets, None, 1, None, y)
+    assert kept
+
+
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES[:4])
+@pytest.mark.parametrize("tokens,top_k", [(1, 1), (1, 8), (5, 3), (40, 4), (200, 6)])
+def test_grouped_gemm_indexes(rq, tokens, top_k, x_type, w_type, y_type):
+    """A router's pairs: gathered into groups, and scattered back; pairs that ask for no expert."""
+    _say("grouped_gemm indexes", tokens, top_k, x_type, w_type, y_type)
+    groups, k, n, pairs = 12, 96, 80, tokens * top_k
+    ids = _ids(pairs, groups, "any")
+    offsets, order = _grouped(ids, groups)
+    x, w = _case(pairs, groups, k, n, x_type, w_type, tokens, x_rows=tokens)
+    y, kept = _run_grouped(rq, x, w, offsets, pairs, order, top_k, None, y_type, pairs)
+    _check_grouped(x, w, offsets, order, top_k, None, y)
+    assert kept
+    x, w = _case(pairs, groups, k, n, x_type, w_type, tokens)
+    y, kept = _run_grouped(rq, x, w, offsets, pairs, None, 1, order, y_type, pairs)
+    _check_grouped(x, w, offsets, None, 1, order, y)
+    assert kept
+
+
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES[:4])
+def test_grouped_gemm_indexes_out_of_range(rq, x_type, w_type, y_type):
+    rows, groups, k, n = 70, 3, 64, 72
+    x, w = _case(rows, groups, k, n, x_type, w_type, 3)
+    offsets = np.array([0, 30, 30, 66], np.int32)
+    r = np.random.default_rng(4)
+    xi, yi = np.arange(rows) * 2, r.permutation(rows)
+    xi[[0, 5, 31, 65]] = [-1, 2 * rows, -(1 << 31), (1 << 31) - 1]
+    yi[[1, 7, 40]] = [rows, -5, (1 << 31) - 1]
+    y, kept = _run_grouped(rq, x, w, offsets, rows, xi, 2, yi, y_type, rows)
+    _check_grouped(x, w, offsets, xi, 2, yi, y)
+    assert kept
+
+
+@pytest.mark.parametrize("offsets", [[5, 9, 9, 20], [0, 40, 10, 50], [-7, 3, 1 << 30, 50], [0, 0, 0, 0], [50, 50, 0, 0]])
+def test_grouped_gemm_odd_offsets(rq, offsets):
+    """Offsets that do not rise from 0 to the rows stay inside the arrays: rows of no group are left alone."""
+    x, w = _case(50, 3, 64, 64, F16, F16, 9)
+    y, kept = _run_grouped(rq, x, w, offsets, 50, None, 1, None, F16, 50)
+    assert kept and bool(torch.isfinite(y).all())
+    inside = np.zeros(50, bool)
+    for b, e in zip(offsets, offsets[1:]):
+        inside[max(b, 0):max(min(e, 50), 0)] = True
+    assert bool((y[~inside] == 123.0).all())
+
+
+@pytest.mark.parametrize("w_type", [F16, BF16])
+@pytest.mark.parametrize("k", [64, 203])
+def test_grouped_gemm_not_finite_rows(rq, w_type, k):
+    """Infinities and NaN stay in their own rows; f32 values at the ends of their range."""
+    rows, n = 40, 64
+    x, w = _case(rows, 2, k, n, F32, w_type, 11)
+    x[3, 5], x[8, 0], x[20] = float("inf"), float("nan"), 0.0
+    x[21] *= 1e37
+    x[22] *= 1e-37
+    x[23], x[23, 1] = 0.0, 3e38
+    offsets = np.array([0, 17, rows], np.int32)
+    y, _ = _run_grouped(rq, x, w, offsets, rows, None, 1, None, F32, rows)
+    x64, w64 = x.double().numpy(), w.double().numpy()
+    with np.errstate(invalid="ignore"):
+        want = np.concatenate([x64[:17] @ w64[0].T, x64[17:] @ w64[1].T])
+    assert torch.isinf(y[3]).all() and np.array_equal(np.sign(y[3].numpy()), np.sign(want[3]))
+    assert torch.isnan(y[8]).all() and (y[20] == 0).all()
+    fine = [r for r in range(rows) if r not in (3, 8)]
+    g = np.array([0] * 17 + [1] * (rows - 17))
+    for r in fine:
+        b = _product_bound(x64[r:r + 1], w64[g[r]], want[r:r + 1], F32, w_type, F32)[0]
+        # pieces below f32's range are lost: k products of 2^-149 and a weight
+        b = b + k * 2.0 ** -149 * (1 + np.abs(w64[g[r]]).max())
+        assert (np.abs(y[r].double().numpy() - want[r]) <= b).all(), r
+
+
+def test_grouped_gemm_own_workspace_and_2d_weight(rq):
+    x, w = _case(50, 1, 100, 40, F32, F16, 2)
+    weight = rq.Weight.from_tensor(w[0].contiguous().to(DEV))
+    size = rq.grouped_gemm_workspace_size(weight, 50, F32)
+    ws = torch.full((size + 64,), 7, dtype=torch.uint8, device=DEV)
+    offsets = torch.tensor([0, 50], dtype=torch.int32, device=DEV)
+    y = rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[:size])
+    _check_grouped(x, w, [0, 50], None, 1, None, y.cpu())
+    assert (ws[size:] == 7).all()
+    with pytest.raises(rq.InvalidInputError, match="needs"):
+        rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[:size - 1])
+    with pytest.raises(rq.ReflexError, match="16-byte aligned"):
+        rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[8:])
+
+
+# ------------------------------------------------------------------ lora_add
+
+def _run_lora(rq, x, a, b, ids, ranks, scales, y, in_place, xs=(0, 0), ys=(0, 0), shift=0):
+    count = a.shape[0]
+    k, n = x.shape[1], y.shape[1]
+    xv, _ = _strided(x.to(DEV), k + xs[0], xs[1], float("nan"))
+    yv, ymem = _strided(y.to(DEV), n + ys[0], ys[1], 99.0)
+    wa, wb = (torch.full((w.numel() + shift + 8,), float("nan"), dtype=w.dtype, device=DEV) for w in (a, b))
+    for m, w in ((wa, a), (wb, b)):
+        m[shift:shift + w.numel()] = w.reshape(-1).to(DEV)
+    wa, wb = (rq.Weight.from_tensor(m[shift:shift + w.numel()].view(w.shape)) for m, w in ((wa, a), (wb, b)))
+    groups = rq.group_rows(torch.from_numpy(ids).to(DEV), count)
+    out = None
+    if not in_place:
+        out = torch.full(y.shape, 123.0, dtype=y.dtype, device=DEV)
+    dev = lambda v, t: None if v is None else torch.tensor(v, dtype=t, device=DEV)  # noqa: E731
+    got = rq.lora_add(xv, wa, wb, groups, yv, ranks=dev(ranks, torch.int32), scales=dev(scales, F32), out=out)
+    torch.cuda.synchronize()
+    if not in_place:
+        assert torch.equal(yv.cpu(), y)
+    around = ymem.clone()
+    around[ys[1]:ys[1] + y.shape[0] * (n + ys[0])].view(y.shape[0], -1)[:, :n] = 99.0
+    assert bool((around == 99.0).all())
+    return got.cpu()
+
+
+def _check_lora(x, a, b, ids, ranks, scales, y, got):
+    count, rank, k = a.shape
+    x64, y64 = x.double().numpy(), y.double().numpy()
+    want, bound = y64.copy(), np.zeros(y64.shape)
+    for g in range(count):
+        r = rank if ranks is None else min(max(ranks[g], 0), rank)
+        s = 1.0 if scales is None else np.float64(np.float32(scales[g]))
+        rows = np.flatnonzero(ids == g)
+        if not len(rows) or not r:
+            continue
+        a64, b64 = a[g, :r].double().numpy(), b[g, :, :r].double().numpy()
+        low, low_size = x64[rows] @ a64.T, np.abs(x64[rows]) @ np.abs(a64).T
+        # v is off by its own sum's error (x's pieces as in the grouped products, where it is split), which B carries on
+        low_bound = ((k / 4 + 64) * 2.0 ** -23 + 2.0 ** -22) * low_size
+        low_bound += 2.0 ** -39 * np.abs(x64[rows]).max(1, keepdims=True) * np.abs(a64).sum(1)
+        delta = s * (low @ b64.T)
+        size = np.abs(s) * (np.abs(low) @ np.abs(b64).T)
+        e = np.abs(s) * (low_bound @ np.abs(b64).T) + (r / 4 + 40) * 2.0 ** -23 * size
+        e += 2.0 ** -15 * size if x.dtype == BF16 else 2.0 ** -21 * size if x.dtype == F16 else 2.0 ** -22 * size
+        want[rows] = y64[rows] + delta
+        e += 2.0 ** -23 * (np.abs(y64[rows]) + np.abs(delta))
+        bound[rows] = e + torch.finfo(y.dtype).eps / 2 * (np.abs(want[rows]) + e) + TINY[y.dtype]
+    off = np.abs(got.double().numpy() - want)
+    assert np.isfinite(off).all()
+    worst = np.unravel_index(np.argmax(off - bound), off.shape)
+    assert (off <= bound).all(), (worst, off[worst], bound[worst])
+
+
+def _lora_case(rows, count, rank, k, n, x_type, w_type, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, k, generator=gen).to(x_type)
+    a = (torch.randn(count, rank, k, generator=gen) * 0.05).to(w_type)
+    b = (torch.randn(count, n, rank, generator=gen) * 0.05).to(w_type)
+    y = torch.randn(rows, n, generator=gen).to(x_type)
+    r = np.random.default_rng(seed)
+    ids = r.integers(-1, count + 1, rows).astype(np.int32)
+    ranks = r.integers(0, rank + 1, count).tolist()
+    scales = r.uniform(-2, 4, count).tolist()
+    for g in range(count):  # what lies past an adapter's rank is not used
+        a[g, ranks[g]:] = float("nan")
+        b[g, :, ranks[g]:] = float("inf")
+    return x, a, b, ids, ranks, scales, y
+
+
+LORA_TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,k,n", [
+    (1, 1, 1, 1, 1), (1, 3, 16, 64, 256), (2, 2, 8, 40, 17), (16, 16, 16, 512, 300), (17, 1, 13, 1235, 153),
+    (40, 5, 64, 128, 257), (129, 4, 130, 264, 512), (300, 9, 32, 2048, 80), (700, 3, 24, 136, 264), (65, 70, 33, 72, 40)])
+def test_lora_add(rq, rows, count, rank, k, n, x_type, w_type):
+    _say("lora_add", rows, count, rank, k, n, x_type, w_type)
+    c = _lora_case(rows, count, rank, k, n, x_type, w_type, rows + k)
+    for in_place in (False, True):
+        _check_lora(*c, _run_lora(rq, *c, in_place))
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("xs,ys,shift", [((8, 0), (8, 0), 0), ((3, 1), (5, 3), 1), ((0, 2), (0, 0), 0), ((16, 8), (16, 8), 8)])
+def test_lora_add_strides(rq, xs, ys, shift, x_type, w_type):
+    _say("lora_add strides", xs, ys, shift, x_type, w_type)
+    c = _lora_case(50, 4, 24, 136, 144, x_type, w_type, 3)
+    for in_place in (False, True):
+        _check_lora(*c, _run_lora(rq, *c, in_place, xs, ys, shift))
+
+
+def test_lora_add_whole_ranks_and_one_scale(rq):
+    x, a, b, ids, _, _, y = _lora_case(40, 3, 16, 96, 64, F32, F16, 8)
+    a, b = (torch.where(torch.isfinite(t), t, 0.25) for t in (a, b))
+    _check_lora(x, a, b, ids, None, None, y, _run_lora(rq, x, a, b, ids, None, None, y, True))
+    # ranks out of range are taken as the nearest that is not
+    ranks = [-3, 99, 16]
+    _check_lora(x, a, b, ids, ranks, None, y, _run_lora(rq, x, a, b, ids, ranks, None, y, False))
+
+
+def test_lora_add_no_row_in_a_group(rq):
+    c = list(_lora_case(20, 3, 16, 96, 64, F16, F16, 8))
+    c[3] = np.full(20, -1, np.int32)
+    for in_place in (False, True):
+        assert torch.equal(_run_lora(rq, *c, in_place), c[6])
+
+
+# ------------------------------------------------------------------ together, captured, on other streams
+
+def _expert_layer(rq, x, logits, weights, top_k):
+    """Routed experts of half-typed stacks in the library's own f32 activations."""
+    tokens, groups = logits.shape
+    ids, share = rq.moe_route_device(logits.reshape(-1), tokens, groups, top_k, True)
+    g = rq.group_rows(ids.reshape(-1), groups)
+    pairs = tokens * top_k
+    gate, up = (rq.grouped_gemm(x, w, g.offsets, pairs, x_index=g.order, x_div=top_k) for w in weights[:2])
+    inner = rq.silu_and_mul(gate, up)
+    down = rq.grouped_gemm(inner, weights[2], g.offsets, pairs, y_index=g.order)
+    return (down.view(tokens, top_k, -1) * share.unsqueeze(2)).sum(1), ids, share
+
+
+def _layer_inputs(tokens, groups, hidden, ffn, w_type, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, hidden, generator=gen)
+    logits = torch.randn(tokens, groups, generator=gen)
+    w = [(torch.randn(groups, *s, generator=gen) * 0.05).to(w_type) for s in ((ffn, hidden), (ffn, hidden), (hidden, ffn))]
+    return x, logits, w
+
+
+def _layer_64(x, ids, share, w):
+    x, w = x.double(), [t.double() for t in w]
+    out = torch.zeros_like(x)
+    for t in range(x.shape[0]):
+        for e, s in zip(ids[t].tolist(), share[t].tolist()):
+            gate, up = w[0][e] @ x[t], w[1][e] @ x[t]
+            out[t] += s * (w[2][e] @ (gate / (1 + torch.exp(-gate)) * up))
+    return out
+
+
+@pytest.mark.parametrize("w_type", [F16, BF16])
+@pytest.mark.parametrize("tokens", [1, 7, 90])
+def test_expert_layer_and_adapters(rq, tokens, w_type):
+    """Route, group, three grouped products; then adapters beside a quantized projection of the result.
+    Each product is f32 through and through, so the layer is within 2^-17 of 64 bits in norm (three products
+    of 2^-19 each and SiLU's few steps)."""
+    from reflex_amd import synth
+
+    hidden, ffn, groups, top_k = 256, 192, 16, 4
+    x, logits, w = _layer_inputs(tokens, groups, hidden, ffn, w_type, tokens)
+    weights = [rq.Weight.from_tensor(t.to(DEV)) for t in w]
+    out, ids, share = _expert_layer(rq, x.to(DEV), logits.to(DEV), weights, top_k)
+    want = _layer_64(x, ids.cpu(), share.cpu(), w)
+    assert (out.cpu().double() - want).norm() <= 2.0 ** -17 * want.norm()
+
+    n, rank, count = 320, 8, 3
+    q = rq.Weight.from_blocks(12, synth.weights(12, n, hidden, 5), hidden, n, device=DEV)
+    y = rq.gemm(out.reshape(-1), q, tokens).view(tokens, n)
+    base = y.cpu()
+    _, a, b, _, _, scales, _ = _lora_case(1, count, rank, hidden, n, F32, w_type, 4)
+    a, b = (torch.where(torch.isfinite(t), t, 0.25) for t in (a, b))
+    adapter = (np.arange(tokens) % (count + 1)).astype(np.int32)
+    g = rq.group_rows(torch.from_numpy(adapter).to(DEV), count)
+    wa, wb = rq.Weight.from_tensor(a.to(DEV)), rq.Weight.from_tensor(b.to(DEV))
+    rq.lora_add(out, wa, wb, g, y, scales=torch.tensor(scales, device=DEV))
+    _check_lora(out.cpu(), a, b, adapter, None, scales, base, y.cpu())
+
+
+def test_captured_and_replayed(rq):
+    """The whole run in one graph, replayed on new inputs, with eager work between."""
+    tokens, hidden, ffn, groups, top_k = 33, 128, 96, 8, 2
+    x, logits, w = _layer_inputs(tokens, groups, hidden, ffn, F16, 1)
+    weights = [rq.Weight.from_tensor(t.to(DEV)) for t in w]
+    pairs = tokens * top_k
+    xd, ld, ids = x.to(DEV), logits.to(DEV), torch.empty(pairs, dtype=torch.int32, device=DEV)
+    g = rq.RowGroups(torch.empty(groups + 1, dtype=torch.int32, device=DEV), torch.empty_like(ids))
+    gate, y = (torch.empty(pairs, m, device=DEV) for m in (ffn, hidden))
+    ws = torch.empty(max(rq.grouped_gemm_workspace_size(weights[0], tokens, F32),
+                         rq.grouped_gemm_workspace_size(weights[2], pairs, F32)), dtype=torch.uint8, device=DEV)
+    a = rq.Weight.from_tensor((torch.randn(groups, 5, ffn) * 0.1).half().to(DEV))
+    b = rq.Weight.from_tensor((torch.randn(groups, hidden, 5) * 0.1).half().to(DEV))
+    lws = torch.empty(rq.lora_add_workspace_size(a, pairs), dtype=torch.uint8, device=DEV)
+
+    def step():
+        ids.copy_(ld.topk(top_k, dim=1).indices.reshape(-1))
+        rq.group_rows(ids, groups, out=g)
+        rq.grouped_gemm(xd, weights[0], g.offsets, pairs, x_index=g.order, x_div=top_k, out=gate, workspace=ws)
+        rq.grouped_gemm(gate, weights[2], g.offsets, pairs, y_index=g.order, out=y, workspace=ws)
+        rq.lora_add(gate, a, b, g, y, workspace=lws)
+        return y
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for r in range(4):
+        xd.copy_(torch.randn(tokens, hidden))
+        ld.copy_(torch.randn(tokens, groups))
+        y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = y.clone()
+        want = step().clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), f"replay {r}"
+
+
+def test_other_stream(rq):
+    """Calls go to the current stream, behind the work that makes their inputs there."""
+    x, w = _case(200, 5, 256, 128, F16, F16, 6)
+    offsets, _ = _grouped(_ids(200, 5, "all"), 5)
+    weight, od = rq.Weight.from_tensor(w.to(DEV)), torch.from_numpy(offsets).to(DEV)
+    s = torch.cuda.Stream()
+    xd = torch.zeros(200, 256, dtype=F16, device=DEV)
+    src = x.to(DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        big = torch.randn(2048, 2048, device=DEV)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        xd.copy_(src)
+        y = rq.grouped_gemm(xd, weight, od, 200)
+    s.synchronize()
+    _check_grouped(x, w, offsets, None, 1, None, y.cpu())
+
+
+def test_same_results_every_time(rq):
+    x, a, b, ids, ranks, scales, y = _lora_case(37, 4, 16, 4096, 512, F32, F16, 2)
+    first = _run_lora(rq, x, a, b, ids, ranks, scales, y, False)
+    for _ in range(3):
+        assert torch.equal(_run_lora(rq, x, a, b, ids, ranks, scales, y, False), first)

@@ -1,0 +1,165 @@
+"""Refusals and workspace sizes of the entry points on grouped rows (rfxq_group_rows,
+rfxq_grouped_gemm, rfxq_lora_add): all of them are decided on the host, before any launch, so
+they run without a GPU (addresses that are never read)."""
+import ctypes
+
+import pytest
+import torch
+
+P = 1 << 20  # a plausible device address
+F32, F16, BF16, Q4K = 0, 1, 30, 12
+
+
+@pytest.fixture(scope="module")
+def L():
+    import reflex_amd
+
+    return reflex_amd.lib()
+
+
+def _weight(ty=F16, k=64, n=32, e=4, data=P, length=None):
+    import reflex_amd as rq
+
+    size = {F32: 4, F16: 2, BF16: 2}.get(ty, 2)
+    return rq.RfxqWeight(ty, k, n, e, data, k * n * max(e, 1) * size if length is None else length)
+
+
+def _rows(ty=F16, rows=8, stride=64, data=2 * P):
+    import reflex_amd as rq
+
+    return rq.RfxqRows(data, ty, rows, stride)
+
+
+def _expect(L, rc, code, text):
+    assert rc == code and text in L.rfxq_last_error().decode(), (rc, L.rfxq_last_error())
+
+
+@pytest.mark.parametrize("change,code,text", [
+    ({"groups": 0}, 12, "groups=0"),
+    ({"groups": 1025}, 12, "groups=1025"),
+    ({"n": (1 << 24) + 1}, 12, "at most"),
+    ({"ids": None}, 11, "NULL"),
+    ({"offsets": None}, 11, "NULL"),
+    ({"order": None}, 11, "NULL"),
+    ({"ids": P + 2}, 12, "4-byte aligned"),
+    ({"order": P}, 11, "overlap"),
+    ({"order": P + 4}, 11, "overlap"),
+    ({"offsets": 3 * P + 8}, 11, "overlap"),
+])
+def test_group_rows_refusals(L, change, code, text):
+    a = {"ids": P, "n": 100, "groups": 8, "offsets": 2 * P, "order": 3 * P, **change}
+    _expect(L, L.rfxq_group_rows(a["ids"], a["n"], a["groups"], a["offsets"], a["order"], None), code, text)
+
+
+def _grouped(L, x=None, w=None, offsets=5 * P, rows=8, x_index=None, x_div=1, y_index=None, y=None, ws=None, ws_bytes=0):
+    ref = lambda v: None if v is None else ctypes.byref(v)  # noqa: E731
+    return L.rfxq_grouped_gemm(ref(x), ref(w), offsets, rows, x_index, x_div, y_index, ref(y), ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    ({"w": None}, 11, "weight is NULL"),
+    ({"w": {"ty": Q4K}}, 1, "F16 or BF16"),
+    ({"w": {"ty": F32}}, 1, "F16 or BF16"),
+    ({"w": {"k": 0}}, 12, "shape"),
+    ({"w": {"n": 0}}, 12, "shape"),
+    ({"w": {"e": 1025}}, 12, "expert_count=1025"),
+    ({"w": {"length": 64 * 32 * 4 * 2 - 1}}, 12, "needs"),
+    ({"w": {"k": 0xFFFFFFFF, "n": 0xFFFFFFFF, "length": 1 << 40}}, 12, "needs"),
+    ({"w": {"data": None}}, 11, "data is NULL"),
+    ({"w": {"data": P + 1}}, 12, "aligned"),
+    ({"x": None}, 11, "x is NULL"),
+    ({"x": {"ty": Q4K}}, 1, "of type 12"),
+    ({"x": {"ty": BF16}}, 11, "x of type 30"),
+    ({"x": {"stride": 63}}, 12, "stride=63"),
+    ({"x": {"data": None}}, 11, "x data is NULL"),
+    ({"x": {"data": P + 1}}, 12, "aligned"),
+    ({"y": None}, 11, "y is NULL"),
+    ({"y": {"ty": BF16}}, 11, "y of type 30"),
+    ({"y": {"stride": 31}}, 12, "stride=31"),
+    ({"y": {"data": 2 * P + 64}}, 11, "overlap"),
+    ({"rows": 1 << 31}, 12, "rows="),
+    ({"x_div": 0}, 11, "x_div=0"),
+    ({"x_div": 2}, 11, "without x_index"),
+    ({"offsets": None}, 11, "offsets is NULL"),
+])
+def test_grouped_gemm_refusals(L, change, code, text):
+    a = {"x": {}, "w": {}, "y": {}, **change}
+    for m, make in (("x", _rows), ("w", _weight), ("y", lambda **c: _rows(**{"stride": 32, "data": 4 * P, **c}))):
+        if a[m] is not None:
+            a[m] = make(**a[m])
+    _expect(L, _grouped(L, **a), code, text)
+
+
+@pytest.mark.parametrize("empty", ["rows", "x", "y"])
+def test_grouped_gemm_of_nothing(L, empty):
+    a = {"x": _rows(), "w": _weight(), "y": _rows(stride=32, data=4 * P)}
+    if empty == "rows":
+        a["rows"] = 0
+    else:
+        a[empty].rows = 0
+    assert _grouped(L, **a) == 0
+
+
+def _lora(L, x=None, a=None, b=None, y=None, out=None, offsets=9 * P, ws=None, ws_bytes=0):
+    ref = lambda v: None if v is None else ctypes.byref(v)  # noqa: E731
+    return L.rfxq_lora_add(ref(x), ref(a), ref(b), None, None, offsets, None, ref(y), ref(out), ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("change,code,text", [
+    ({"a": None}, 11, "a: weight is NULL"),
+    ({"b": None}, 11, "b: weight is NULL"),
+    ({"a": {"ty": Q4K}}, 1, "F32, F16 or BF16"),
+    ({"b": {"ty": BF16}}, 12, "of type 30"),
+    ({"b": {"k": 7}}, 12, "lora_add: a"),
+    ({"b": {"e": 3}}, 12, "lora_add: a"),
+    ({"x": {"rows": 9}}, 12, "9 rows of x"),
+    ({"out": {"rows": 9}}, 12, "9 of out"),
+    ({"x": {"ty": F32}}, 11, "x of type 0"),
+    ({"x": {"ty": BF16}, "y": {"ty": BF16}, "out": {"ty": BF16}}, 11, "x of type 30"),
+    ({"y": {"stride": 47}}, 12, "stride=47"),
+    ({"offsets": None}, 11, "offsets is NULL"),
+    ({"out": {"data": 2 * P}}, 11, "x and out overlap"),
+    ({"out": {"data": 6 * P + 96}}, 11, "y and out overlap"),
+    ({"out": {"data": 6 * P, "stride": 50}}, 11, "y and out overlap"),
+])
+def test_lora_add_refusals(L, change, code, text):
+    base = {"x": dict(data=2 * P), "a": dict(n=6), "b": dict(k=6, n=48, data=4 * P), "y": dict(stride=48, data=6 * P),
+            "out": dict(stride=48, data=8 * P)}
+    a = {}
+    for m, c in base.items():
+        if m in change and change[m] is None:
+            a[m] = None
+        else:
+            a[m] = (_weight if m in "ab" else _rows)(**{**c, **change.get(m, {})})
+    if "offsets" in change:
+        a["offsets"] = change["offsets"]
+    _expect(L, _lora(L, **a), code, text)
+
+
+def test_workspace_sizes(L):
+    w16, wb = _weight(k=100), _weight(ty=BF16, k=100)
+    size = lambda w, rows, ty: L.rfxq_grouped_gemm_workspace_size(ctypes.byref(w), rows, ty)  # noqa: E731
+    assert size(w16, 7, F16) == 0 and size(_weight(ty=Q4K), 7, F32) == 0 and size(w16, 0, F32) == 0
+    assert size(w16, 7, F32) >= 2 * 7 * 128 * 2 + 4 * 7  # two pieces in rows of 128, exponents
+    assert size(wb, 7, F32) >= 3 * 7 * 128 * 2
+    # a buffer for the most rows holds any fewer rows' needs
+    a = _weight(k=4096, n=64, e=64)
+    sizes = [L.rfxq_lora_add_workspace_size(ctypes.byref(a), r) for r in range(1, 9000, 7)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+
+
+def test_python_checks():
+    import reflex_amd as rq
+
+    w = rq.Weight.from_tensor(torch.zeros(3, 16, 8, dtype=torch.float16))
+    assert (w.ty, w.shape, w._c.len) == (rq.GgmlType.F16, [8, 16, 3], 3 * 16 * 8 * 2)
+    for bad in (torch.zeros(4, 4, dtype=torch.int32), torch.zeros(4), torch.zeros(4, 6).t()):
+        with pytest.raises(rq.InvalidInputError):
+            rq.Weight.from_tensor(bad)
+    x, ids = torch.zeros(4, 8, dtype=torch.float16), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(rq.InvalidInputError, match="ids on cpu"):
+        rq.group_rows(ids, 3)
+    with pytest.raises(rq.InvalidInputError, match="x on cpu"):
+        rq.grouped_gemm(x, w, ids, 4)
+    with pytest.raises(rq.InvalidInputError, match="x on cpu"):
+        rq.lora_add(x, w, w, rq.RowGroups(ids, ids), x)
