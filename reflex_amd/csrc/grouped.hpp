@@ -118,6 +118,36 @@ RFXQ_DEV void st_row(const GroupedArgs& a, int64_t row, uint32_t n, const f4v_t 
     }
 }
 
+// 4 neighbouring results of one row.
+template <typename T>
+RFXQ_DEV void st_four(const GroupedArgs& a, int64_t row, uint32_t n, f4v_t v) {
+    const uint32_t have = a.n > n ? a.n - n : 0u;
+    const uint64_t at = (uint64_t)row * a.ldy + n;
+    if (a.y_f32) {
+        float* y = static_cast<float*>(a.y) + at;
+        if (have >= 4u && (reinterpret_cast<uintptr_t>(y) & 15u) == 0u) {
+            *(RFXQ_GLOBAL f4v_t*)y = v;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++)
+                if (i < have) stf(y + i, v[i]);
+        }
+        return;
+    }
+    typedef T t4_t __attribute__((ext_vector_type(4)));
+    T* y = static_cast<T*>(a.y) + at;
+    t4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = (T)v[i];
+    if (have >= 4u && (reinterpret_cast<uintptr_t>(y) & 7u) == 0u) {
+        *(RFXQ_GLOBAL t4_t*)y = r;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            if (i < have) ((RFXQ_GLOBAL T*)y)[i] = r[i];
+    }
+}
+
 // Place of 16-byte piece c (of 8) of LDS row r: rows of 128 bytes, pieces
 // xor'ed with the row so that 8 rows' pieces of one column lie in 8 banks' groups.
 RFXQ_DEV uint32_t lds_piece(uint32_t r, uint32_t c) { return r * 8u + (c ^ (r & 7u)); }
@@ -127,30 +157,36 @@ RFXQ_DEV uint32_t lds_piece(uint32_t r, uint32_t c) { return r * 8u + (c ^ (r & 
 // four operands of a wave's 64 columns give it 16 neighbouring ones.
 RFXQ_DEV uint32_t col_of(uint32_t j) { return (j & ~63u) + ((j >> 2) & 3u) * 16u + ((j >> 4) & 3u) * 4u + (j & 3u); }
 
-// The wave's 16 MF x 64 tile of one 64-wide step of K, both operands in LDS.
-template <typename T, int MF>
+// The wave's 16 MF x 64 tile of one 64-wide step of K, both operands in LDS
+// (the activations' pieces XS apart).
+template <typename T, int MF, uint32_t PIECES, uint32_t XS>
 RFXQ_DEV void tile_step(const u4_t* xs, const u4_t* ws, uint32_t xr, uint32_t wr, f4v_t (&acc)[MF][4]) {
     const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4;
 #pragma unroll
     for (uint32_t h = 0; h < 2u; h++) {
-        u4_t wf[4], xf[MF];
+        u4_t wf[4];
 #pragma unroll
         for (uint32_t f = 0; f < 4u; f++) wf[f] = ws[lds_piece(wr + 16u * f + l, 4u * h + q)];
 #pragma unroll
-        for (uint32_t m = 0; m < (uint32_t)MF; m++) xf[m] = xs[lds_piece(xr + 16u * m + l, 4u * h + q)];
+        for (uint32_t j = 0; j < PIECES; j++) {
+            u4_t xf[MF];
 #pragma unroll
-        for (uint32_t m = 0; m < (uint32_t)MF; m++)
+            for (uint32_t m = 0; m < (uint32_t)MF; m++) xf[m] = xs[j * XS + lds_piece(xr + 16u * m + l, 4u * h + q)];
 #pragma unroll
-            for (uint32_t f = 0; f < 4u; f++) acc[m][f] = mfma32<T>(wf[f], xf[m], acc[m][f]);
+            for (uint32_t m = 0; m < (uint32_t)MF; m++)
+#pragma unroll
+                for (uint32_t f = 0; f < 4u; f++) acc[m][f] = mfma32<T>(wf[f], xf[m], acc[m][f]);
+        }
     }
 }
 
-template <typename T, int MF>
+// 16-row operand m holds the tile's rows m0 + STEP m and on.
+template <typename T, int MF, uint32_t STEP = 16>
 RFXQ_DEV void tile_out(const GroupedArgs& a, const RowTile& t, uint32_t m0, uint32_t n0, const f4v_t (&acc)[MF][4]) {
     const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4;
 #pragma unroll
     for (uint32_t m = 0; m < (uint32_t)MF; m++) {
-        const uint32_t p = t.beg + m0 + 16u * m + l;
+        const uint32_t p = t.beg + m0 + STEP * m + l;
         if (p >= t.end) continue;
         const int64_t src = src_row(a, p), dst = dst_row(a, p);
         if (src < 0 || dst < 0) continue;
@@ -165,11 +201,12 @@ RFXQ_DEV void tile_out(const GroupedArgs& a, const RowTile& t, uint32_t m0, uint
 }
 
 // Any alignment and any K: operands through registers, element by element at
-// a row's end. 64 x 128 tiles, 4 waves of 32 x 64.
-template <typename T>
+// a row's end, the next step's loads in flight during the products. 64 x 128
+// tiles, 4 waves of 32 x 64; PIECES row tiles beside one tile of weights.
+template <typename T, uint32_t PIECES>
 RFXQ_DEV void grouped_any(const GroupedArgs& a) {
     constexpr uint32_t BM = 64, BN = 128, NX = BM * 8u / 256u, NW = BN * 8u / 256u;
-    __shared__ u4_t xs[BM * 8u], ws[BN * 8u];
+    __shared__ u4_t xs[PIECES][BM * 8u], ws[BN * 8u];
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
     const RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, tm);
@@ -190,32 +227,328 @@ RFXQ_DEV void grouped_any(const GroupedArgs& a) {
         wp[i] = n < a.n ? w + (uint64_t)n * a.k : nullptr;
     }
     f4v_t acc[2][4] = {};
-    const uint32_t steps = (a.k + 63u) / 64u * a.pieces, c = tid & 7u;
-    u4_t xv[NX], wv[NW];
+    const uint32_t steps = (a.k + 63u) / 64u, c = tid & 7u;
+    u4_t xv[PIECES][NX], wv[NW];
     const auto load = [&](uint32_t s) {
-        const uint32_t k = s / a.pieces * 64u + 8u * c, have = k < a.k ? a.k - k : 0u;
-        const uint64_t at = (uint64_t)(s % a.pieces) * a.plane + k;
-#pragma unroll
-        for (uint32_t i = 0; i < NX; i++) xv[i] = xp[i] && have ? ld_halves(xp[i] + at, have) : u4_t{0, 0, 0, 0};
+        const uint32_t k = s * 64u + 8u * c, have = k < a.k ? a.k - k : 0u;
 #pragma unroll
         for (uint32_t i = 0; i < NW; i++) wv[i] = wp[i] && have ? ld_halves(wp[i] + k, have) : u4_t{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t j = 0; j < PIECES; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < NX; i++)
+                xv[j][i] = xp[i] && have ? PIECES > 1 ? ld16(xp[i] + j * a.plane + k) : ld_halves(xp[i] + k, have) : u4_t{0, 0, 0, 0};
     };
     load(0);
     for (uint32_t s = 0; s < steps; s++) {
         __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < NX; i++) xs[lds_piece((tid >> 3) + 32u * i, c)] = xv[i];
+        for (uint32_t j = 0; j < PIECES; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < NX; i++) xs[j][lds_piece((tid >> 3) + 32u * i, c)] = xv[j][i];
 #pragma unroll
         for (uint32_t i = 0; i < NW; i++) ws[lds_piece((tid >> 3) + 32u * i, c)] = wv[i];
         __syncthreads();
         if (s + 1u < steps) load(s + 1u);
-        tile_step<T, 2>(xs, ws, (wave >> 1) * 32u, (wave & 1u) * 64u, acc);
+        tile_step<T, 2, PIECES, BM * 8u>(xs[0], ws, (wave >> 1) * 32u, (wave & 1u) * 64u, acc);
     }
     tile_out<T, 2>(a, t, (wave >> 1) * 32u, n0 + (wave & 1u) * 64u, acc);
 }
 
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f16(GroupedArgs a) { grouped_any<half_t>(a); }
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_bf16(GroupedArgs a) { grouped_any<__bf16>(a); }
+extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f16(GroupedArgs a) { grouped_any<half_t, 1>(a); }
+extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_bf16(GroupedArgs a) { grouped_any<__bf16, 1>(a); }
+extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f32_f16(GroupedArgs a) { grouped_any<half_t, 2>(a); }
+extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f32_bf16(GroupedArgs a) { grouped_any<__bf16, 3>(a); }
+
+// ---------------------------------------------------------------- tiles filled by asynchronous copies
+
+// BM x BN tiles of WM x WN waves (each BM / WM rows x 64 columns), 64-wide
+// steps of K in STAGES buffers: copies global -> LDS run STAGES - 1 steps
+// ahead of the products, without registers between. P pieces of the activations
+// beside one tile of weights; where P is less than there are, the steps go
+// through the pieces. Rows of x and W start at whole 16 bytes; what lies past a
+// row's end or the tile's last row is copied from past the buffer's end, which
+// fills it with zeros. Offsets within x and within one matrix stay below 4 GiB
+// (the host's rule).
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, uint32_t P>
+struct GroupedTile {
+    static constexpr uint32_t THREADS = 64u * WM * WN, MF = BM / WM / 16;
+    static constexpr uint32_t NX = BM * 8u / THREADS, NW = BN * 8u / THREADS, LOADS = P * NX + NW;
+    static constexpr uint32_t PAST = 0xFFFFFFF0u;
+    static_assert(BN == 64 * WN && NX >= 1 && NW >= 1 && STAGES >= 2 && STAGES <= 4 && (STAGES - 2) * LOADS < 64);
+
+    RowTile t;
+    rsrc_t xr, wr;
+    uint32_t xo[NX], wo[NW];  // lanes' byte offsets at k = 0
+    uint32_t lane, wave, piece, n0, k, pieces, plane, steps;
+    uint32_t at_k = 0, at_p = 0;  // of the next step to copy
+
+    __device__ __forceinline__ void issue(u4_t* xs, u4_t* ws) {
+        // past the end: as many copies, so that waits count the same
+        const bool more = at_k < k, there = more && (at_k + 64u <= k || at_k + 8u * piece < k);
+        const uint32_t xb = more ? 2u * at_k + at_p * plane : 0u, wb = more ? 2u * at_k : 0u;
+#pragma unroll
+        for (uint32_t j = 0; j < P; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < NX; i++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, RFXQ_LDSP(xs + j * BM * 8 + (wave * NX + i) * 64u), 16,
+                                                         there ? xo[i] : PAST, more ? xb + j * plane : 0u, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < NW; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, RFXQ_LDSP(ws + (wave * NW + i) * 64u), 16, there ? wo[i] : PAST, wb,
+                                                     0, 0);
+        at_p += P;
+        if (at_p >= pieces) {
+            at_p = 0;
+            at_k += 64u;
+        }
+    }
+
+    // the tile, and where its rows are; false: there is none
+    __device__ __forceinline__ bool begin(const GroupedArgs& a) {
+        uint32_t tm, tn;
+        if (!tile_place(a, blockIdx.x, tm, tn)) return false;
+        t = find_tile(a.offsets, a.groups, a.rows, BM, tm);
+        if (!t.any) return false;
+        lane = threadIdx.x & 63u;
+        n0 = tn * BN;
+        wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        piece = (lane & 7u) ^ (lane >> 3);
+        k = a.k;
+        pieces = a.pieces;
+        plane = (uint32_t)(2u * a.plane);
+        const uint64_t xbytes = ((uint64_t)a.plane * (a.pieces - 1u) + (uint64_t)(a.x_rows - 1u) * a.ldx + a.k) * 2u;
+        xr = make_rsrc(a.x, (uint32_t)xbytes);
+        wr = make_rsrc(a.w + (uint64_t)t.group * a.w_stride, (uint32_t)(2u * a.w_stride));
+#pragma unroll
+        for (uint32_t i = 0; i < NX; i++) {
+            const uint32_t p = t.beg + (wave * NX + i) * 8u + (lane >> 3);
+            const int64_t s = p < t.end ? src_row(a, p) : -1;
+            xo[i] = s < 0 ? PAST : (uint32_t)((uint64_t)s * a.ldx * 2u) + 16u * piece;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NW; i++) {
+            const uint32_t n = n0 + col_of((wave * NW + i) * 8u + (lane >> 3));
+            wo[i] = n < a.n ? n * a.k * 2u + 16u * piece : PAST;
+        }
+        steps = (a.k + 63u) / 64u * (a.pieces / P);
+        return true;
+    }
+
+    __device__ __forceinline__ void run(const GroupedArgs& a) {
+        constexpr uint32_t XS = P * BM * 8u;
+        __shared__ u4_t xs0[XS], xs1[XS], xs2[STAGES > 2 ? XS : 1u], xs3[STAGES > 3 ? XS : 1u];
+        __shared__ u4_t ws0[BN * 8], ws1[BN * 8], ws2[STAGES > 2 ? BN * 8 : 1], ws3[STAGES > 3 ? BN * 8 : 1];
+        if (!begin(a)) return;
+        f4v_t acc[MF][4] = {};
+        const uint32_t row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * 64u;
+        issue(xs0, ws0);
+        if constexpr (STAGES > 2) issue(xs1, ws1);
+        if constexpr (STAGES > 3) issue(xs2, ws2);
+        const auto step = [&](const u4_t* xs, const u4_t* ws, u4_t* nx, u4_t* nw) {
+            constexpr uint32_t left = (STAGES - 2) * LOADS;  // copies of later steps
+            __builtin_amdgcn_s_waitcnt(0x0F70 | (left & 15u) | (left >> 4) << 14);
+            lds_barrier();
+            issue(nx, nw);
+            tile_step<T, MF, P, BM * 8u>(xs, ws, row0, col0, acc);
+        };
+        for (uint32_t s = 0; s < steps; s += STAGES) {
+            if constexpr (STAGES == 2) {
+                step(xs0, ws0, xs1, ws1);
+                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
+            } else if constexpr (STAGES == 3) {
+                step(xs0, ws0, xs2, ws2);
+                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
+                if (s + 2u < steps) step(xs2, ws2, xs1, ws1);
+            } else {
+                step(xs0, ws0, xs3, ws3);
+                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
+                if (s + 2u < steps) step(xs2, ws2, xs1, ws1);
+                if (s + 3u < steps) step(xs3, ws3, xs2, ws2);
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the workgroup
+        tile_out<T, MF>(a, t, row0, n0 + col0, acc);
+    }
+
+    // 256 x 256 tiles, 8 waves. The waves of a SIMD (w and w + 4) take turns: while
+    // one multiplies 32 of K from its registers, the other reads its next operands
+    // from LDS. A turn ends with a barrier, the upper waves are a turn behind.
+    // Reads of a step end with the upper waves' fourth turn, so the copies into its
+    // buffer begin in the first turn of the next step; they are waited for at the
+    // end of that step's last turn (the upper waves' last reading turn).
+    // The lower and the upper waves take every other 16 rows of the tile, and leave
+    // out those behind the group's last row: FULL has none.
+    template <bool FULL>
+    __device__ __forceinline__ void turns(u4_t* xs0, u4_t* xs1, u4_t* ws0, u4_t* ws1, f4v_t (&acc)[MF][4]) {
+        const uint32_t upper = wave >> 2, l = lane & 15u, q = lane >> 4, row0 = upper * 16u, col0 = (wave & 3u) * 64u;
+        const uint32_t rows = t.end - t.beg, some = rows > row0 ? (rows - row0 + 31u) / 32u : 0u;
+        u4_t wf[4], xf[MF];
+        const auto turn_over = [] {
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const auto read = [&](const u4_t* xs, const u4_t* ws, uint32_t h) {
+#pragma unroll
+            for (uint32_t f = 0; f < 4u; f++) wf[f] = ws[lds_piece(col0 + 16u * f + l, 4u * h + q)];
+#pragma unroll
+            for (uint32_t m = 0; m < MF; m++)
+                if (FULL || m < some) xf[m] = xs[lds_piece(row0 + 32u * m + l, 4u * h + q)];
+        };
+        const auto multiply = [&] {
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (uint32_t m = 0; m < MF; m++)
+                if (FULL || m < some) {
+#pragma unroll
+                    for (uint32_t f = 0; f < 4u; f++) acc[m][f] = mfma32<T>(wf[f], xf[m], acc[m][f]);
+                }
+            __builtin_amdgcn_s_setprio(0);
+        };
+        const auto step = [&](const u4_t* xs, const u4_t* ws, u4_t* nx, u4_t* nw) {
+            read(xs, ws, 0);
+            issue(nx, nw);
+            turn_over();
+            multiply();
+            turn_over();
+            read(xs, ws, 1);
+            if (upper) __builtin_amdgcn_s_waitcnt(0x0F70);
+            turn_over();
+            multiply();
+            if (!upper) __builtin_amdgcn_s_waitcnt(0x0F70);
+            turn_over();
+        };
+        issue(xs0, ws0);
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        turn_over();
+        if (upper) turn_over();
+        for (uint32_t s = 0; s < steps; s += 2u) {
+            step(xs0, ws0, xs1, ws1);
+            if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
+        }
+        if (!upper) turn_over();
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the workgroup
+    }
+    __device__ __forceinline__ void run_turns(const GroupedArgs& a) {
+        static_assert(WM * WN == 8 && WN == 4 && STAGES == 2 && P == 1);
+        __shared__ u4_t xs0[BM * 8], xs1[BM * 8], ws0[BN * 8], ws1[BN * 8];
+        if (!begin(a)) return;
+        f4v_t acc[MF][4] = {};
+        if (t.end - t.beg == BM)
+            turns<true>(xs0, xs1, ws0, ws1, acc);
+        else
+            turns<false>(xs0, xs1, ws0, ws1, acc);
+        tile_out<T, MF, 32>(a, t, (wave >> 2) * 16u, n0 + (wave & 3u) * 64u, acc);
+    }
+};
+
+#define RFXQ_GROUPED_TILE(name, T, BM, BN, WM, WN, STAGES, P, RUN)                                   \
+    extern "C" __global__ __launch_bounds__(64 * WM * WN) void rfxq_grouped_##name(GroupedArgs a) { \
+        GroupedTile<T, BM, BN, WM, WN, STAGES, P> t;                                                 \
+        t.RUN(a);                                                                                    \
+    }
+RFXQ_GROUPED_TILE(64_f16, half_t, 64, 128, 2, 2, 3, 1, run)
+RFXQ_GROUPED_TILE(64_bf16, __bf16, 64, 128, 2, 2, 3, 1, run)
+RFXQ_GROUPED_TILE(64_f32_f16, half_t, 64, 128, 2, 2, 2, 2, run)
+RFXQ_GROUPED_TILE(64_f32_bf16, __bf16, 64, 128, 2, 2, 2, 3, run)
+RFXQ_GROUPED_TILE(256_f16, half_t, 256, 256, 2, 4, 2, 1, run_turns)
+RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, 1, run_turns)
+
+// ---------------------------------------------------------------- few rows a group
+
+// Decode: what a group's matrix weighs is all that counts, so its rows go from
+// memory straight into the matrix instructions' registers, each once, as their
+// 16-row operand; up to 16 activation rows are the other one. A wave takes 16 NT
+// columns and all of K (WK = 1) or, where that makes too few waves, a quarter of K
+// (WK = 4, the workgroup's waves add their parts in LDS). Loads run a block of 128 of K
+// ahead of the products.
+// f32 activations are multiplied as they are (f32 matrix instructions, the weights
+// widened): 32 cycles for 4 of K, which stays below the time of the
+// weights' memory reads at 16 rows, and spares the pieces' launch.
+template <typename TX, typename TW, uint32_t NT, uint32_t WK>
+RFXQ_DEV void grouped_few(const GroupedArgs& a) {
+    constexpr bool F32 = __is_same(TX, float);
+    constexpr uint32_t XV = F32 ? 2u : 1u;  // 16-byte loads of 8 activations
+    __shared__ f4v_t part[WK > 1 ? (WK - 1) * NT * 64u : 1u];
+    constexpr uint32_t COLS = 16u * NT * 4u / WK;  // a workgroup's
+    const uint32_t tn = blockIdx.x % a.tiles_n;
+    const RowTile t = find_tile(a.offsets, a.groups, a.rows, 16, blockIdx.x / a.tiles_n);
+    if (!t.any) return;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4;
+    const uint32_t n0 = tn * COLS + (WK == 1 ? wave * 16u * NT : 0u);
+    const uint32_t blocks = (a.k + 127u) / 128u, each = (blocks + WK - 1u) / WK;
+    const uint32_t b0 = WK == 1 ? 0u : min(wave * each, blocks), b1 = WK == 1 ? blocks : min(b0 + each, blocks);
+    const uint32_t p = t.beg + l;
+    const int64_t src = p < t.end ? src_row(a, p) : -1;
+    const TX* x = reinterpret_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
+    const TW* w[NT];
+#pragma unroll
+    for (uint32_t f = 0; f < NT; f++)
+        w[f] = reinterpret_cast<const TW*>(a.w) + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.k;
+    f4v_t acc[NT] = {};
+    u4_t wv[2][4][NT], xv[2][4][XV];
+    const auto load = [&](uint32_t s, uint32_t b) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const uint32_t k = 128u * b + 32u * i + 8u * q;
+            const bool have = k < a.k;
+#pragma unroll
+            for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = have ? ld16(w[f] + k) : u4_t{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = have && src >= 0 ? ld16(x + k + 4u * v) : u4_t{0, 0, 0, 0};
+        }
+    };
+    const auto multiply = [&](uint32_t s) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+#pragma unroll
+            for (uint32_t f = 0; f < NT; f++) {
+                if constexpr (F32) {
+                    typedef TW t8_t __attribute__((ext_vector_type(8)));
+                    const t8_t w8 = __builtin_bit_cast(t8_t, wv[s][i][f]);
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++)
+                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)w8[j], as_f32(xv[s][i][j >> 2][j & 3u]), acc[f], 0, 0, 0);
+                } else {
+                    acc[f] = mfma32<TW>(wv[s][i][f], xv[s][i][0], acc[f]);
+                }
+            }
+    };
+    if (b0 < b1) load(0, b0);
+    for (uint32_t b = b0; b < b1; b += 2u) {
+        if (b + 1u < b1) load(1, b + 1u);
+        multiply(0);
+        if (b + 2u < b1) load(0, b + 2u);
+        if (b + 1u < b1) multiply(1);
+    }
+    if constexpr (WK > 1) {
+        if (wave) {
+#pragma unroll
+            for (uint32_t f = 0; f < NT; f++) part[((wave - 1u) * NT + f) * 64u + lane] = acc[f];
+        }
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (uint32_t v = 0; v + 1u < WK; v++)
+#pragma unroll
+            for (uint32_t f = 0; f < NT; f++) acc[f] += part[(v * NT + f) * 64u + lane];
+    }
+    if (src < 0) return;
+    const int64_t dst = dst_row(a, p);
+    if (dst < 0) return;
+#pragma unroll
+    for (uint32_t f = 0; f < NT; f++) st_four<TW>(a, dst, n0 + 16u * f + 4u * q, acc[f]);
+}
+
+#define RFXQ_GROUPED_FEW(name, TX, TW)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_few_##name(GroupedArgs a) { grouped_few<TX, TW, 2, 1>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_few4_##name(GroupedArgs a) { grouped_few<TX, TW, 1, 4>(a); }
+RFXQ_GROUPED_FEW(f16, half_t, half_t)
+RFXQ_GROUPED_FEW(bf16, __bf16, __bf16)
+RFXQ_GROUPED_FEW(f32_f16, float, half_t)
+RFXQ_GROUPED_FEW(f32_bf16, float, __bf16)
 
 // ---------------------------------------------------------------- f32 activations as pieces
 

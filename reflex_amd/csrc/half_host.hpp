@@ -125,6 +125,8 @@ uint32_t max_tiles(uint32_t rows, uint32_t groups, uint32_t bm) { return rows / 
 
 // ------------------------------------------------------------------ grouped GEMM
 
+constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offsets reach
+
 // f32 activations in pieces of the weights' type: rows of whole 64-element steps
 struct Pieces {
     uint32_t count, ld;
@@ -138,6 +140,42 @@ Pieces pieces_of(uint32_t ty, uint32_t rows, uint32_t k) {
     p.exp_at = align256(p.plane * p.count * 2u);
     p.total = p.exp_at + align256(4ull * rows);
     return p;
+}
+
+// The kernel of a grouped product, by the mean rows of the groups that can have
+// any, measured with stacks of 128 matrices of 768 x 2048 and 2048 x 768 and of 8 of
+// 14336 x 4096 and 4096 x 14336 (N x K; us, bf16):
+//   few rows  16 rows, weights straight from memory: up to 4 rows (64 against 72 on
+//             128 x 768 x 2048 at 4 rows, 88 against 88 at 8); f32 activations, whose
+//             pieces the tiles have to multiply one by one, up to 8 (121 against 128);
+//             short K up to 2, where the tiles keep more loads in flight (54 against
+//             51 at 2 rows, 61 against 66 at 4)
+//   tiles     64 x 128 through registers: the rest
+//   pipelined 64 x 128 copied ahead into three buffers: where the tiles do not fill the
+//             CUs twice, each workgroup has to hide its own latency (8 x 4096 x 14336 at
+//             32 rows: 186 against 247); 896 tiles are faster without (176 against 163)
+//   large     256 x 256: from where its larger steps pay (8 x 14336 x 4096: 327 against
+//             324 at 128 rows, 358 against 395 at 200); for f32 activations it goes
+//             through the pieces, reading the weights again (1372 against 1289 at 400)
+struct GroupedVariant {
+    hipFunction_t f;
+    uint32_t bm, bn, threads;
+    bool few;
+};
+GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool split_x, uint32_t rows, uint32_t groups, uint32_t k,
+                               uint32_t n, bool direct, bool copies) {
+    const uint32_t used = std::min(rows, groups), mean = rows / used, xt = split_x ? 0u : 1u;
+    const uint64_t fill = 2ull * c->cus;
+    if (direct && mean <= (k < 1024u ? 2u : split_x ? 8u : 4u)) {
+        // a wave's columns over all of K, unless that leaves CUs without work or long K
+        // to one wave (128 x 768 x 2048, 8 rows in 8 groups: 20 against 8 us)
+        if (k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
+        return {c->half.few4[xt][t], 16, 16, 256, true};
+    }
+    if (copies && mean > (split_x ? 512u : 160u)) return {c->half.t256[t], 256, 256, 512, false};
+    if (copies && mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill)
+        return {c->half.t64[xt][t], 64, 128, 256, false};
+    return {c->half.any[xt][t], 64, 128, 256, false};
 }
 
 // ------------------------------------------------------------------ adapters
@@ -234,18 +272,24 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.groups = groups;
     a.pieces = 1;
     a.y_f32 = y->type == RFXQ_TYPE_F32 ? 1u : 0u;
-    constexpr uint32_t bm = 64, bn = 128;
-    a.tiles_m = max_tiles(rows, groups, bm);
-    a.tiles_n = (n + bn - 1u) / bn;
+    // asynchronous copies: rows at whole 16 bytes, 32-bit offsets
+    const bool split_x = x->type == RFXQ_TYPE_F32;
+    const Pieces p = split_x ? pieces_of(ty, x->rows, k) : Pieces{};
+    const uint64_t xb = split_x ? 2u * p.plane * p.count : rows_span(x, k);
+    const bool copies = (split_x || (aligned16(x->data) && x->stride % 8u == 0)) && aligned16(w->data) && k % 8u == 0 &&
+                        xb < kMaxOffset && 2ull * k * n < kMaxOffset;
+    const bool direct = aligned16(x->data) && x->stride % (split_x ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
+    const GroupedVariant v = grouped_variant(c, t, split_x, rows, groups, k, n, direct, copies);
+    a.tiles_m = max_tiles(rows, groups, v.bm);
+    a.tiles_n = (n + v.bn - 1u) / v.bn;
     a.sm = 4;
     a.sn = 8;
     const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
-    const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
+    const uint64_t grid = v.few ? (uint64_t)a.tiles_m * a.tiles_n : (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid > 0x7FFFFFFFull)
         return fail(RFXQ_ERR_OTHER, "grouped_gemm: %u rows x %u columns need %llu workgroups", rows, n,
                     (unsigned long long)grid);
-    if (x->type == RFXQ_TYPE_F32) {
-        const Pieces p = pieces_of(ty, x->rows, k);
+    if (split_x && !v.few) {
         void* ws = nullptr;
         if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "grouped_gemm", &ws)) return rc;
         uint8_t* base = static_cast<uint8_t*>(ws);
@@ -260,7 +304,7 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
         a.pieces = p.count;
         a.x_exp = exp;
     }
-    if (int rc = launch(c->half.any[t], (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch")) return rc;
+    if (int rc = launch(v.f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch", v.threads)) return rc;
     return ok();
 }
 

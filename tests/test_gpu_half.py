@@ -160,6 +160,40 @@ def test_grouped_gemm(rq, rows, groups, k, n, x_type, w_type, y_type):
     assert kept
 
 
+# sizes at which each kernel is chosen, whole and ragged: few rows over short K with many columns,
+# few rows, tiles copied ahead, tiles through registers, large tiles (f32: above 512 rows a group)
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES)
+@pytest.mark.parametrize("rows,groups,k,n", [
+    (150, 128, 128, 520), (70, 64, 1160, 200), (40, 9, 1152, 48), (64, 3, 640, 1032), (20, 1, 264, 24),
+    (400, 4, 200, 136), (1000, 3, 328, 520), (1030, 4, 64, 272), (1500, 2, 136, 264), (1200, 1, 8, 256)])
+def test_grouped_gemm_each_kernel(rq, rows, groups, k, n, x_type, w_type, y_type):
+    _say("grouped_gemm kernels", rows, groups, k, n, x_type, w_type, y_type)
+    x, w = _case(rows, groups, k, n, x_type, w_type, rows + k)
+    offsets, order = _grouped(_ids(rows, groups, "all"), groups)
+    y, kept = _run_grouped(rq, x, w, offsets, rows, order, 1, order, y_type, rows, (8, 8), (8, 0), 8)
+    _check_grouped(x, w, offsets, order, 1, order, y)
+    assert kept
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_grouped_gemm_rows_past_4_gib(rq, rows):
+    """Rows of x, y and matrices of a stack whose bytes lie past 32-bit offsets."""
+    _say("grouped_gemm past 4 GiB", rows)
+    k, n, far, count = 1024, 2200, 2_200_000, 1000
+    x, w = _case(rows, 2, k, n, F16, F16, 1)
+    xd = torch.empty(far, k, dtype=F16, device=DEV)
+    at = torch.arange(far - rows, far, device=DEV)
+    xd[at] = x.to(DEV)
+    yd = torch.empty(far, n, dtype=F16, device=DEV)
+    stack = torch.empty(count, n, k, dtype=F16, device=DEV)
+    stack[-2:] = w.to(DEV)
+    idx = at.to(torch.int32)
+    offsets = torch.zeros(count + 1, dtype=torch.int32, device=DEV)
+    offsets[-2], offsets[-1] = rows // 2, rows
+    rq.grouped_gemm(xd, rq.Weight.from_tensor(stack), offsets, rows, x_index=idx, y_index=idx, out=yd)
+    _check_grouped(x, w, [0, rows // 2, rows], None, 1, None, yd[at].cpu())
+
+
 @pytest.mark.parametrize("x_type,w_type,y_type", TYPES[:4])
 @pytest.mark.parametrize("xs,ys,ws", [((8, 0), (8, 0), 0), ((3, 1), (5, 3), 1), ((0, 2), (0, 0), 0), ((0, 0), (1, 0), 2),
                                       ((16, 8), (16, 8), 8)])
