@@ -429,7 +429,7 @@ uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows,
 /* Low-rank adapters of many requests beside a projection that all rows share:
  * for the rows r = order[p] (NULL: p) of group g, offsets[g] <= p < offsets[g + 1],
  *   out[r] = y[r] + scales[g] * B_g (A_g x[r])
- * over the first ranks[g] rows of A_g and columns of B_g; rows in no group:
+ * over the first ranks[g] rows of A_g and columns of B_g (rank <= 512); rows in no group:
  * out[r] = y[r]. y is what the shared projection gave (rfxq_gemm, rfxq_gemv_rows);
  * out may be y. a: a stack [in, rank, adapters], b: a stack [rank, out, adapters],
  * of one type (F32, F16 or BF16), such as a pool whose places hold adapters of up

@@ -30,6 +30,16 @@ RFXQ_DEV f4v_t mfma32(u4_t a, u4_t b, f4v_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
 }
 
+// Between a run of matrix instructions that ends at a branch and the first reads
+// of their results. The compiler's own wait states have come out short there: a
+// result read as the first instruction behind a branch was read too early.
+// 32 wait states, more than the longest of the instructions used here needs.
+RFXQ_DEV void mfma_settle() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 struct GroupedArgs {
     const uint16_t* x;  // rows of halves (pieces: plane p of `plane` elements)
     const uint16_t* w;
@@ -184,6 +194,7 @@ RFXQ_DEV void tile_step(const u4_t* xs, const u4_t* ws, uint32_t xr, uint32_t wr
 template <typename T, int MF, uint32_t STEP = 16>
 RFXQ_DEV void tile_out(const GroupedArgs& a, const RowTile& t, uint32_t m0, uint32_t n0, const f4v_t (&acc)[MF][4]) {
     const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4;
+    mfma_settle();
 #pragma unroll
     for (uint32_t m = 0; m < (uint32_t)MF; m++) {
         const uint32_t p = t.beg + m0 + STEP * m + l;
@@ -523,6 +534,7 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
         if (b + 2u < b1) load(0, b + 2u);
         if (b + 1u < b1) multiply(1);
     }
+    mfma_settle();
     if constexpr (WK > 1) {
         if (wave) {
 #pragma unroll

@@ -8,6 +8,7 @@ namespace {
 
 constexpr uint32_t kMaxGroups = 1024;         // rows.hpp
 constexpr uint32_t kMaxGroupRows = 1u << 24;  // rows of rfxq_group_rows
+constexpr uint32_t kMaxRank = 512;            // v of a 16-row tile in LDS
 constexpr uint32_t kGroupThreads = 1024;      // of its workgroups, 1 to 4 rows each
 
 // Mirrors of the device structs.
@@ -57,7 +58,7 @@ struct LoraArgs {
     uint64_t ldx, ldy, ldo;
     uint32_t rows, x_rows, k, n;
     uint32_t rank, ldv, groups, splits;
-    uint32_t k_split, tiles, tiles_n, vec;
+    uint32_t k_split, tiles, across, pad;
 };
 static_assert(sizeof(LoraArgs) == 152, "LoraArgs layout");
 
@@ -180,19 +181,21 @@ GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool split_x, uint32_t 
 
 // ------------------------------------------------------------------ adapters
 
-// The launch of rfxq_lora_down: ranges of K until the workgroups fill the CUs
-// twice, of at least 256 values each.
+// 32-row tiles from 17 rows a group on. The ranges of K of rfxq_lora_down: until
+// the workgroups fill the CUs, of at least 256 values each.
 struct LoraPlan {
-    uint32_t ldv, tiles, splits, k_split;
+    uint32_t ldv, bm, tiles, splits, k_split;
     uint64_t total;
 };
 LoraPlan lora_plan(uint32_t k, uint32_t rank, uint32_t groups, uint32_t rows, uint32_t cus) {
     LoraPlan p;
     p.ldv = (rank + 15u) & ~15u;
-    p.tiles = max_tiles(rows, groups, 16u);
-    const uint32_t want = (2u * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
+    p.bm = rows / std::min(rows, groups) > 16u && rank <= 256u ? 32u : 16u;
+    p.tiles = max_tiles(rows, groups, p.bm);
+    const uint32_t fill = getenv("RFXQ_FILL") ? atoi(getenv("RFXQ_FILL")) : 2;
+    const uint32_t want = (fill * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
     p.splits = std::max(1u, std::min({want, most, 32u}));
-    p.k_split = ((k + p.splits - 1u) / p.splits + 63u) & ~63u;
+    p.k_split = ((k + p.splits - 1u) / p.splits + 127u) & ~127u;
     p.splits = (k + p.k_split - 1u) / p.k_split;
     p.total = align256(4ull * p.splits * rows * p.ldv);
     return p;
@@ -311,11 +314,11 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
 uint64_t rfxq_lora_add_workspace_size(const rfxq_weight* a, uint32_t rows) {
     if (!a || rows == 0 || a->in_features == 0 || a->out_features == 0) return 0;
     const Ctx* c = loaded_ctx();
-    // What any number of rows up to `rows` needs: there are at least rows / 16
-    // tiles, so the ranges are fewer than 32 CUs / rows + 1 (fewer rows can take
-    // more ranges, and more memory, than the most rows do).
+    // What any number of rows up to `rows` needs: there are at least rows / 32 tiles,
+    // so the ranges are fewer than 64 CUs / rows + 1 (fewer rows can take more
+    // ranges, and more memory, than the most rows do).
     const uint64_t ldv = (a->out_features + 15ull) & ~15ull, cus = c ? (uint64_t)c->cus : 256u;
-    return align256(4u * ldv * std::min<uint64_t>(32ull * rows, 32u * cus + rows));
+    return align256(4u * ldv * std::min<uint64_t>(32ull * rows, 64u * cus + rows));
 }
 
 int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b, const int32_t* ranks,
@@ -327,6 +330,7 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     if (b->in_features != rank || b->expert_count != a->expert_count || b->ggml_type != a->ggml_type)
         return fail(RFXQ_ERR_OTHER, "lora_add: a [%u, %u, %u] of type %u and b [%u, %u, %u] of type %u", k, rank,
                     a->expert_count, a->ggml_type, b->in_features, n, b->expert_count, b->ggml_type);
+    if (rank > kMaxRank) return fail(RFXQ_ERR_OTHER, "lora_add: rank=%u (at most %u)", rank, kMaxRank);
     if (int rc = check_rows(x, k, "lora_add", "x")) return rc;
     if (int rc = check_rows(y, n, "lora_add", "y")) return rc;
     if (int rc = check_rows(out, n, "lora_add", "out")) return rc;
@@ -346,14 +350,14 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
     const LoraPlan p = lora_plan(k, rank, groups, rows, (uint32_t)c->cus);
-    const uint32_t tiles_n = (n + 255u) / 256u;
-    const uint64_t up = (uint64_t)(p.tiles + 1u) * tiles_n;
+    // strips of 32 columns shared by as many workgroups as fill the CUs (4 of a CU's waves each)
+    const uint32_t fillu = getenv("RFXQ_FILLU") ? atoi(getenv("RFXQ_FILLU")) : 4;
+    const uint32_t across = std::max(1u, std::min((fillu * (uint32_t)c->cus + p.tiles - 1u) / p.tiles, (n + 127u) / 128u));
+    const uint64_t up = (uint64_t)(p.tiles + 1u) * across;
     if (up > 0x7FFFFFFFull || (uint64_t)p.tiles * p.splits > 0x7FFFFFFFull)
-        return fail(RFXQ_ERR_OTHER, "lora_add: %u rows x %u columns need %llu workgroups", rows, n,
-                    (unsigned long long)up);
+        return fail(RFXQ_ERR_OTHER, "lora_add: %u rows need %llu workgroups", rows, (unsigned long long)up);
     void* ws = nullptr;
     if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "lora_add", &ws)) return rc;
-    const uint32_t xe = 16u / elem_bytes(x->type), we = 16u / elem_bytes(a->ggml_type);
     LoraArgs l;
     std::memset(&l, 0, sizeof l);
     l.x = x->data;
@@ -378,14 +382,16 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     l.splits = p.splits;
     l.k_split = p.k_split;
     l.tiles = p.tiles;
-    l.tiles_n = tiles_n;
-    l.vec = (aligned16(x->data) && x->stride % xe == 0 ? 1u : 0u) | (aligned16(a->data) && k % we == 0 ? 2u : 0u) |
-            (aligned16(b->data) && rank % we == 0 ? 4u : 0u);
+    l.across = across;
     const uint32_t t = x->type == RFXQ_TYPE_F32 ? (a->ggml_type == RFXQ_TYPE_F32 ? 0u : a->ggml_type == RFXQ_TYPE_F16 ? 1u : 2u)
                        : x->type == RFXQ_TYPE_F16 ? 3u : 4u;
-    if (int rc = launch(c->half.lora_down[t], p.tiles * p.splits, 0, stream, &l, sizeof l, "rfxq_lora_down launch"))
+    const uint32_t wide = p.bm == 32u ? 1u : 0u, ldl = (rank + 31u) & ~31u;
+    const uint32_t pieces = x->type == RFXQ_TYPE_F32 && a->ggml_type == RFXQ_TYPE_BF16 ? 3u : 2u;
+    const uint32_t lds = a->ggml_type == RFXQ_TYPE_F32 ? 4u * p.bm * (ldl + 4u)
+                                                       : 2u * pieces * p.bm * (ldl + 8u) + 4u * p.bm * (ldl / 32u);
+    if (int rc = launch(c->half.lora_down[t][wide], p.tiles * p.splits, 0, stream, &l, sizeof l, "rfxq_lora_down launch"))
         return rc;
-    if (int rc = launch(c->half.lora_up[t], (uint32_t)up, 0, stream, &l, sizeof l, "rfxq_lora_up launch")) return rc;
+    if (int rc = launch(c->half.lora_up[t][wide], (uint32_t)up, lds, stream, &l, sizeof l, "rfxq_lora_up launch")) return rc;
     return ok();
 }
 

@@ -5,6 +5,17 @@
 // leaves v (f32) in the workspace, in ranges of K where rows are few, and
 // rfxq_lora_up_* adds the ranges in order, so results do not change from call
 // to call.
+//
+// Both read their operands straight into the matrix instructions' registers:
+// lane (l, q) of a wave holds 8 neighbouring values of row l, from 8 q on, of a
+// 32-wide step (the order within a step is free, as long as both operands keep
+// it). Activations and adapters of one half type multiply exactly. f32 values (x,
+// and v always) beside half-typed adapters are split for each step into pieces of
+// the adapters' type, scaled by a power of two per row and step so that the row's
+// largest lies in [2^14, 2^15): 2 pieces of f16 (2^-22 of a value), 3 of bf16
+// (exact; 2 for bf16 results, 2^-15 of v). f32 matrix instructions take 256 cycles for
+// what 2 or 3 half-typed ones and four multiply-adds take about 50 for; they are left
+// for f32 adapters.
 #pragma once
 #include "common.hpp"
 #include "grouped.hpp"
@@ -24,27 +35,139 @@ struct LoraArgs {
     uint64_t ldx, ldy, ldo;
     uint32_t rows, x_rows, k, n;
     uint32_t rank, ldv, groups, splits;
-    uint32_t k_split, tiles, tiles_n, vec;  // vec: 1 rows of x, 2 of A, 4 of B start at whole 16 bytes
+    uint32_t k_split, tiles, across, pad;
 };
 
-template <typename T>
-RFXQ_DEV float to_f32(T v) { return (float)v; }
+// Vectors that may start at any element.
+typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h8a2_t __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 b8a2_t __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 h4a2_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 b4a2_t __attribute__((ext_vector_type(4), aligned(2)));
 
-// 4 values at p, of which the first `have` are there: the others are 0.
+// 8 neighbouring values of a row as they lie in memory.
 template <typename T>
-RFXQ_DEV f4v_t ld_four(const T* p, uint32_t have, bool vec) {
-    typedef T t4_t __attribute__((ext_vector_type(4)));
-    f4v_t r = {0, 0, 0, 0};
-    if (vec && have >= 4u) {
-        const t4_t t = *(const RFXQ_GLOBAL t4_t*)p;
+struct Eight {
+    u4_t v;
+    __device__ __forceinline__ float at(uint32_t j) const {
+        if constexpr (__is_same(T, half_t))
+            return (float)__builtin_bit_cast(h8_t, v)[j];
+        else
+            return (float)__builtin_bit_cast(b8_t, v)[j];
+    }
+};
+template <>
+struct Eight<float> {
+    f4v_t v[2];
+    __device__ __forceinline__ float at(uint32_t j) const { return v[j >> 2][j & 3u]; }
+};
+
+// The 8 values at p.
+template <typename T>
+RFXQ_DEV Eight<T> ld_eight(const T* p) {
+    Eight<T> r;
+    if constexpr (__is_same(T, float)) {
+        r.v[0] = *(const RFXQ_GLOBAL f4a4_t*)p;
+        r.v[1] = *(const RFXQ_GLOBAL f4a4_t*)(p + 4);
+    } else {
+        r.v = *(const RFXQ_GLOBAL u4a2_t*)p;
+    }
+    return r;
+}
+// The first `have` of the 8 values at p, then zeros; `room`: elements from p to the
+// end of its array. What follows the row is read too, where it is there.
+template <typename T>
+RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have, uint64_t room) {
+    Eight<T> r = {};
+    if (have == 0) return r;
+    if (room >= 8u) {
+        r = ld_eight(p);
+        if constexpr (__is_same(T, float)) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = (float)t[i];
+            for (uint32_t i = 0; i < 8u; i++) r.v[i >> 2][i & 3u] = i < have ? r.v[i >> 2][i & 3u] : 0.0f;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++)
+                r.v[i] &= have > 2u * i + 1u ? 0xFFFFFFFFu : have > 2u * i ? 0xFFFFu : 0u;
+        }
+        return r;
+    }
+    T t[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) t[i] = i < have ? ((const RFXQ_GLOBAL T*)p)[i] : (T)0.0f;
+    __builtin_memcpy(&r, t, sizeof t);
+    return r;
+}
+
+// 4 neighbouring values of a row; the first `have` of them.
+template <typename T>
+RFXQ_DEV f4v_t ld_four(const T* p, uint32_t have) {
+    f4v_t r = {0, 0, 0, 0};
+    if (have >= 4u) {
+        if constexpr (__is_same(T, float)) {
+            r = *(const RFXQ_GLOBAL f4a4_t*)p;
+        } else if constexpr (__is_same(T, half_t)) {
+            r = __builtin_convertvector(*(const RFXQ_GLOBAL h4a2_t*)p, f4v_t);
+        } else {
+            r = __builtin_convertvector(*(const RFXQ_GLOBAL b4a2_t*)p, f4v_t);
+        }
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++)
             if (i < have) r[i] = (float)((const RFXQ_GLOBAL T*)p)[i];
     }
     return r;
+}
+template <typename T>
+RFXQ_DEV void st_four_any(T* p, uint32_t have, f4v_t v) {
+    if (have >= 4u) {
+        if constexpr (__is_same(T, float))
+            *(RFXQ_GLOBAL f4a4_t*)p = v;
+        else if constexpr (__is_same(T, half_t))
+            *(RFXQ_GLOBAL h4a2_t*)p = __builtin_convertvector(v, h4a2_t);
+        else
+            *(RFXQ_GLOBAL b4a2_t*)p = __builtin_convertvector(v, b4a2_t);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            if (i < have) ((RFXQ_GLOBAL T*)p)[i] = (T)v[i];
+    }
+}
+
+// f32 values of a step as pieces of T, times 2^e (the scale's exponent)
+template <typename T, uint32_t NP>
+RFXQ_DEV void split_eight(const Eight<float>& x, float scale, u4_t (&out)[NP]) {
+    float left[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) left[i] = x.at(i) * scale;
+#pragma unroll
+    for (uint32_t n = 0; n < NP; n++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const T a = (T)left[2 * i], b = (T)left[2 * i + 1];
+            out[n][i] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+            left[2 * i] -= (float)a;
+            left[2 * i + 1] -= (float)b;
+        }
+}
+// The exponent e at which `top` is 2^e times a value in [2^14, 2^15), kept so that 2^e and 2^-e are f32 values
+RFXQ_DEV int step_exp(float top) { return max(__builtin_amdgcn_frexp_expf(top) - 15, -126); }
+RFXQ_DEV float pow2(int e) { return as_f32((uint32_t)(e + 127) << 23); }
+
+// the largest of the four lanes (l, 0..3)
+RFXQ_DEV float max_over_q(float v) {
+    uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    v = fmaxf(as_f32(r[0]), as_f32(r[1]));
+    b = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(as_f32(s[0]), as_f32(s[1]));
+}
+RFXQ_DEV float max_of_eight(const Eight<float>& x) {
+    float t = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) t = fmaxf(t, __builtin_fabsf(x.at(i)));
+    return t;
 }
 
 RFXQ_DEV uint32_t lora_rank(const LoraArgs& a, uint32_t g) {
@@ -59,114 +182,315 @@ RFXQ_DEV int64_t lora_row(const LoraArgs& a, uint32_t p) {
     return r >= 0 && (uint32_t)r < a.x_rows ? (int64_t)r : -1;
 }
 
-constexpr uint32_t kLoraRows = 16, kLoraCols = 256;
+// The state of a workgroup of rfxq_lora_down_*, and its passes over up to 64 rows of A.
+template <typename TX, typename TW, uint32_t MT>
+struct LoraDown {
+    const TX* x[MT];
+    bool there[MT];
+    const TX* x_end;
+    const TW* a_end;
+    RowTile t;
+    uint32_t rank, split, wave, lane, k0, k1;
 
-// v: 16 rows of one group, one range of K; the workgroup's 4 waves take
-// quarters of it and add them in LDS.
-template <typename TX, typename TW>
-RFXQ_DEV void lora_down(const LoraArgs& a) {
-    __shared__ f4v_t part[3][4][64];
-    const uint32_t split = blockIdx.x / a.tiles;
-    const RowTile t = find_tile(a.offsets, a.groups, a.rows, kLoraRows, blockIdx.x % a.tiles);
-    if (!t.any) return;
-    const uint32_t rank = lora_rank(a, t.group), wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t l = lane & 15u, q = lane >> 4;
-    const uint32_t p = t.beg + l;
-    const int64_t row = p < t.end ? lora_row(a, p) : -1;
-    const TX* x = static_cast<const TX*>(a.x) + (row < 0 ? 0 : (uint64_t)row * a.ldx);
-    const uint32_t quarter = (a.k_split / 4u + 15u) & ~15u;
-    const uint32_t k_end = min(a.k, (split + 1u) * a.k_split);
-    const uint32_t k0 = split * a.k_split + wave * quarter, k1 = min(k_end, k0 + quarter);
-    for (uint32_t r0 = 0; r0 < rank; r0 += 64u) {
-        f4v_t acc[4] = {};
-        const TW* w[4];
+    // RT 16-row operands from row r0 of A. The number is known at compile time: the
+    // products of a step and what reads them stay free of branches (mfma_settle).
+    template <uint32_t RT>
+    __device__ __forceinline__ void pass(const LoraArgs& a, uint32_t r0, f4v_t (*part)[MT][4][64]) const {
+        const uint32_t l = lane & 15u, q = lane >> 4;
+        const uint32_t full = (k1 - k0) / 32u, tail = (k1 - k0) % 32u;
+        f4v_t acc[MT][RT] = {};
+        const TW* w[RT];
 #pragma unroll
-        for (uint32_t f = 0; f < 4u; f++)
-            w[f] = static_cast<const TW*>(a.a) + ((uint64_t)t.group * a.rank + min(r0 + 16u * f + l, a.rank - 1u)) * a.k;
-        for (uint32_t k = k0 + 4u * q; k < k0 + quarter; k += 16u) {
-            const uint32_t have = k < k1 ? k1 - k : 0u;
-            const f4v_t xv = ld_four(x + k, row < 0 ? 0u : have, a.vec & 1u);
-#pragma unroll
-            for (uint32_t f = 0; f < 4u; f++) {
-                if (r0 + 16u * f >= rank) break;
-                const f4v_t wv = ld_four(w[f] + k, r0 + 16u * f + l < rank ? have : 0u, a.vec & 2u);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[j], xv[j], acc[f], 0, 0, 0);
-            }
+        for (uint32_t f = 0; f < RT; f++) {
+            // rows past the rank read the last one; their results are dropped below
+            w[f] = static_cast<const TW*>(a.a) + ((uint64_t)t.group * a.rank + min(r0 + 16u * f + l, rank - 1u)) * a.k + 8u * q;
         }
+        Eight<TX> xv[2][MT];
+        Eight<TW> wv[2][RT];
+        const auto load = [&](uint32_t s, uint32_t k) {
+#pragma unroll
+            for (uint32_t f = 0; f < RT; f++) wv[s][f] = ld_eight(w[f] + k);
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) xv[s][m] = there[m] ? ld_eight(x[m] + k) : Eight<TX>{};
+        };
+        const auto multiply = [&](uint32_t s) {
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) {
+                if constexpr (__is_same(TW, float)) {
+#pragma unroll
+                    for (uint32_t f = 0; f < RT; f++)
+#pragma unroll
+                        for (uint32_t j = 0; j < 8u; j++)
+                            acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[s][f].at(j), xv[s][m].at(j), acc[m][f], 0, 0, 0);
+                } else if constexpr (__is_same(TX, TW)) {
+#pragma unroll
+                    for (uint32_t f = 0; f < RT; f++) acc[m][f] = mfma32<TW>(wv[s][f].v, xv[s][m].v, acc[m][f]);
+                } else {
+                    constexpr uint32_t NP = __is_same(TW, half_t) ? 2u : 3u;
+                    const int e = step_exp(max_over_q(max_of_eight(xv[s][m])));
+                    const float back = pow2(e);
+                    u4_t xp[NP];
+                    split_eight<TW, NP>(xv[s][m], pow2(-e), xp);
+#pragma unroll
+                    for (uint32_t f = 0; f < RT; f++) {
+                        f4v_t d = {0, 0, 0, 0};
+#pragma unroll
+                        for (uint32_t n = 0; n < NP; n++) d = mfma32<TW>(wv[s][f].v, xp[NP - 1u - n], d);
+                        acc[m][f] += d * back;
+                    }
+                }
+            }
+        };
+        if (full) load(0, k0);
+        for (uint32_t i = 0; i < full; i += 2u) {
+            if (i + 1u < full) load(1, k0 + 32u * (i + 1u));
+            multiply(0);
+            if (i + 2u < full) load(0, k0 + 32u * (i + 2u));
+            if (i + 1u < full) multiply(1);
+        }
+        if (tail) {
+            const uint32_t k = k0 + 32u * full, have = tail > 8u * q ? tail - 8u * q : 0u;
+#pragma unroll
+            for (uint32_t f = 0; f < RT; f++)
+                wv[0][f] = ld_eight(w[f] + k, have, (uint64_t)(a_end - (w[f] + k)));
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) xv[0][m] = ld_eight(x[m] + k, there[m] ? have : 0u, (uint64_t)(x_end - (x[m] + k)));
+            multiply(0);
+        }
+        mfma_settle();
         __syncthreads();
         if (wave) {
 #pragma unroll
-            for (int f = 0; f < 4; f++) part[wave - 1u][f][lane] = acc[f];
+            for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+                for (uint32_t f = 0; f < RT; f++) part[wave - 1u][m][f][lane] = acc[m][f];
         }
         __syncthreads();
-        if (wave == 0 && p < t.end) {
-            float* v = a.v + ((uint64_t)split * a.rows + p) * a.ldv + r0 + 4u * q;
+        if (wave == 0) {
 #pragma unroll
-            for (uint32_t f = 0; f < 4u; f++) {
-                if (r0 + 16u * f >= rank) break;
-                const f4v_t s = ((acc[f] + part[0][f][lane]) + part[1][f][lane]) + part[2][f][lane];
-                *(RFXQ_GLOBAL f4v_t*)(v + 16u * f) = s;  // rows rank.. of the last 16 are 0
+            for (uint32_t m = 0; m < MT; m++) {
+                const uint32_t p = t.beg + 16u * m + l;
+                if (p >= t.end) break;
+                float* v = a.v + ((uint64_t)split * a.rows + p) * a.ldv + r0 + 4u * q;
+#pragma unroll
+                for (uint32_t f = 0; f < RT; f++) {
+                    if (r0 + 16u * f >= rank) break;
+                    f4v_t s = ((acc[m][f] + part[0][m][f][lane]) + part[1][m][f][lane]) + part[2][m][f][lane];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4u; i++)
+                        if (r0 + 16u * f + 4u * q + i >= rank) s[i] = 0.0f;
+                    *(RFXQ_GLOBAL f4v_t*)(v + 16u * f) = s;
+                }
             }
         }
     }
+};
+
+// v: 16 MT rows of one group, one range of K; the workgroup's 4 waves take
+// quarters of it (whole steps of 32) and add them in LDS.
+template <typename TX, typename TW, uint32_t MT>
+RFXQ_DEV void lora_down(const LoraArgs& a) {
+    __shared__ f4v_t part[3][MT][4][64];
+    LoraDown<TX, TW, MT> d;
+    d.split = blockIdx.x / a.tiles;
+    d.t = find_tile(a.offsets, a.groups, a.rows, 16u * MT, blockIdx.x % a.tiles);
+    if (!d.t.any) return;
+    d.rank = lora_rank(a, d.t.group);
+    d.lane = threadIdx.x & 63u;
+    d.wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++) {
+        const uint32_t p = d.t.beg + 16u * m + (d.lane & 15u);
+        const int64_t row = p < d.t.end ? lora_row(a, p) : -1;
+        d.there[m] = row >= 0;
+        d.x[m] = static_cast<const TX*>(a.x) + (row < 0 ? 0 : (uint64_t)row * a.ldx) + 8u * (d.lane >> 4);
+    }
+    d.x_end = static_cast<const TX*>(a.x) + (uint64_t)(a.x_rows - 1u) * a.ldx + a.k;
+    d.a_end = static_cast<const TW*>(a.a) + (uint64_t)a.groups * a.rank * a.k;
+    const uint32_t quarter = (a.k_split / 4u + 31u) & ~31u;
+    const uint32_t end = min(a.k, (d.split + 1u) * a.k_split);
+    d.k0 = min(d.split * a.k_split + d.wave * quarter, end);
+    d.k1 = min(d.k0 + quarter, end);
+    for (uint32_t r0 = 0; r0 < d.rank; r0 += 64u) {
+        const uint32_t left = d.rank - r0;
+        if (left <= 16u)
+            d.template pass<1>(a, r0, part);
+        else if (left <= 32u)
+            d.template pass<2>(a, r0, part);
+        else
+            d.template pass<4>(a, r0, part);
+    }
 }
 
-// out: 16 rows x 256 columns, a wave 64 columns.
-template <typename TX, typename TW>
+// out: 16 MT rows, strips of 16 NF columns: a.across workgroups share a tile's strips,
+// a wave takes every (4 across)th. v, added up and in pieces, lies in LDS for
+// all of them; B's values and y of the next strip are loaded during a strip.
+//
+// LDS: f32 adapters: v [16 MT][ldv + 4]. Others: the pieces [NP][16 MT][ldl + 8]
+// (halves, ldl = rank in whole steps of 32), then 2^e [16 MT][ldl / 32].
+template <typename TX, typename TW, uint32_t MT, uint32_t NF>
 RFXQ_DEV void lora_up(const LoraArgs& a) {
-    const uint32_t tn = blockIdx.x % a.tiles_n;
-    RowTile t = find_tile(a.offsets, a.groups, a.rows, kLoraRows, blockIdx.x / a.tiles_n);
+    constexpr bool F32 = __is_same(TW, float);
+    constexpr uint32_t BM = 16u * MT, NP = __is_same(TW, __bf16) && __is_same(TX, float) ? 3u : 2u;
+    extern __shared__ uint32_t lds[];
+    RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, blockIdx.x / a.across);
     if (!t.any) {  // rows in no group
         if (a.y == a.out) return;
         const int32_t o = a.offsets[a.groups];
-        t.beg = (o < 0 ? 0u : (uint32_t)o) + t.beg * kLoraRows;
+        t.beg = (o < 0 ? 0u : (uint32_t)o) + t.beg * BM;
         if (t.beg >= a.rows) return;
-        t.end = min(t.beg + kLoraRows, a.rows);
+        t.end = min(t.beg + BM, a.rows);
         t.group = a.groups;
     }
-    const uint32_t rank = lora_rank(a, t.group), wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const uint32_t rank = lora_rank(a, t.group), lane = threadIdx.x & 63u;
     if (rank == 0 && a.y == a.out) return;
-    const uint32_t l = lane & 15u, q = lane >> 4, p = t.beg + l, n0 = tn * kLoraCols + wave * 64u;
-    const int64_t row = p < t.end ? lora_row(a, p) : -1;
-    f4v_t acc[4] = {};
-    const float* v = a.v + (uint64_t)min(p, t.end - 1u) * a.ldv;
-    const TW* w[4];
-    uint32_t cols = 0;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t l = lane & 15u, q = lane >> 4, strips = (a.n + 16u * NF - 1u) / (16u * NF);
+    const uint32_t group = min(t.group, a.groups - 1u);
+    const uint32_t steps = (rank + 31u) / 32u, ldl = (a.rank + 31u) & ~31u;
+    const TX* y[MT];
+    TX* o[MT];
+    bool there[MT];
 #pragma unroll
-    for (uint32_t f = 0; f < 4u; f++) {
-        const uint32_t n = n0 + (l >> 2) * 16u + 4u * f + (l & 3u);
-        cols |= n < a.n ? 1u << f : 0u;
-        w[f] = static_cast<const TW*>(a.b) + ((uint64_t)min(t.group, a.groups - 1u) * a.n + min(n, a.n - 1u)) * a.rank;
+    for (uint32_t m = 0; m < MT; m++) {
+        const uint32_t p = t.beg + 16u * m + l;
+        const int64_t row = p < t.end ? lora_row(a, p) : -1;
+        there[m] = row >= 0;
+        y[m] = static_cast<const TX*>(a.y) + (row < 0 ? 0 : (uint64_t)row * a.ldy);
+        o[m] = static_cast<TX*>(a.out) + (row < 0 ? 0 : (uint64_t)row * a.ldo);
     }
-    for (uint32_t r = 4u * q; r < ((rank + 15u) & ~15u); r += 16u) {
-        f4v_t vv = {0, 0, 0, 0};
-        for (uint32_t s = 0; s < a.splits; s++) vv += *(const RFXQ_GLOBAL f4v_t*)(v + (uint64_t)s * a.rows * a.ldv + r);
-        const uint32_t have = r < rank ? rank - r : 0u;
+    const TW* b_end = static_cast<const TW*>(a.b) + (uint64_t)a.groups * a.n * a.rank;
+
+    struct Strip {
+        Eight<TW> w[2][NF];  // the first 64 of the rank
+        f4v_t y[MT][NF];
+    };
+    const auto row_of = [&](uint32_t n0, uint32_t f) {
+        return static_cast<const TW*>(a.b) + ((uint64_t)group * a.n + min(n0 + 16u * f + l, a.n - 1u)) * a.rank + 8u * q;
+    };
+    const auto load_w = [&](Eight<TW>(&w)[NF], uint32_t n0, uint32_t r) {
+        if (r + 32u <= rank) {
 #pragma unroll
-        for (uint32_t f = 0; f < 4u; f++) {
-            const f4v_t wv = ld_four(w[f] + r, cols >> f & 1u ? have : 0u, a.vec & 4u);
+            for (uint32_t f = 0; f < NF; f++) w[f] = ld_eight(row_of(n0, f) + r);
+        } else {
+            const uint32_t at = r + 8u * q, have = rank > at ? rank - at : 0u;
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[j], vv[j], acc[f], 0, 0, 0);
+            for (uint32_t f = 0; f < NF; f++) {
+                const TW* p = row_of(n0, f) + r;
+                w[f] = ld_eight(p, have, (uint64_t)(b_end - p));
+            }
+        }
+    };
+    const auto load = [&](Strip& s, uint32_t n0) {
+        if (rank) load_w(s.w[0], n0, 0);
+        if (rank > 32u) load_w(s.w[1], n0, 32u);
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+            for (uint32_t f = 0; f < NF; f++) {
+                const uint32_t n = n0 + 16u * f + 4u * q;
+                s.y[m][f] = ld_four(y[m] + n, !there[m] || n >= a.n ? 0u : a.n - n);
+            }
+    };
+    const uint32_t first = (blockIdx.x % a.across) * 4u + wave, by = 4u * a.across;
+    Strip s[2];
+    if (first < strips) load(s[0], 16u * NF * first);
+
+    // v into LDS: a lane's 8 values of a row and step, the ranges of K added in
+    // order; v is written, with zeros, up to the next whole 16
+    for (uint32_t j = wave; j < MT * steps; j += 4u) {
+        const uint32_t m = j % MT, r = 32u * (j / MT) + 8u * q, p = t.beg + 16u * m + l;
+        Eight<float> sum = {};
+        if (p < t.end && r < rank) {
+            const float* v = a.v + (uint64_t)p * a.ldv + r;
+#pragma unroll 4
+            for (uint32_t i = 0; i < a.splits; i++) {
+                const float* vs = v + (uint64_t)i * a.rows * a.ldv;
+                sum.v[0] += *(const RFXQ_GLOBAL f4v_t*)vs;
+                sum.v[1] += *(const RFXQ_GLOBAL f4v_t*)(vs + 4);
+            }
+        }
+        if constexpr (F32) {
+            f4v_t* to = reinterpret_cast<f4v_t*>(lds + (16u * m + l) * (ldl + 4u) + r);
+            to[0] = sum.v[0];
+            to[1] = sum.v[1];
+        } else {
+            const int e = step_exp(max_over_q(max_of_eight(sum)));
+            u4_t out[NP];
+            split_eight<TW, NP>(sum, pow2(-e), out);
+#pragma unroll
+            for (uint32_t n = 0; n < NP; n++)
+                *reinterpret_cast<u4_t*>(reinterpret_cast<uint16_t*>(lds) + (n * BM + 16u * m + l) * (ldl + 8u) + r) = out[n];
+            if (q == 0)
+                reinterpret_cast<float*>(lds + NP * BM * (ldl + 8u) / 2u)[(16u * m + l) * (ldl / 32u) + j / MT] = pow2(e);
         }
     }
-    if (row < 0) return;
+    __syncthreads();
     const float scale = t.group < a.groups && a.scales ? a.scales[t.group] : 1.0f;
-    const TX* y = static_cast<const TX*>(a.y) + (uint64_t)row * a.ldy;
-    TX* o = static_cast<TX*>(a.out) + (uint64_t)row * a.ldo;
+
+    const auto multiply = [&](const Eight<TW>(&w)[NF], uint32_t step, f4v_t(&acc)[MT][NF]) {
 #pragma unroll
-    for (uint32_t f = 0; f < 4u; f++)
+        for (uint32_t m = 0; m < MT; m++) {
+            if constexpr (F32) {
+                Eight<float> v;
+                const f4v_t* at = reinterpret_cast<const f4v_t*>(lds + (16u * m + l) * (ldl + 4u) + 32u * step + 8u * q);
+                v.v[0] = at[0];
+                v.v[1] = at[1];
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) {
-            const uint32_t n = n0 + 16u * q + 4u * f + i;
-            if (n < a.n) o[n] = rank ? (TX)((float)y[n] + scale * acc[f][i]) : y[n];
+                for (uint32_t f = 0; f < NF; f++)
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++)
+                        acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[f].at(j), v.at(j), acc[m][f], 0, 0, 0);
+            } else {
+                u4_t v[NP];
+#pragma unroll
+                for (uint32_t n = 0; n < NP; n++)
+                    v[n] = *reinterpret_cast<const u4_t*>(reinterpret_cast<const uint16_t*>(lds) +
+                                                          (n * BM + 16u * m + l) * (ldl + 8u) + 32u * step + 8u * q);
+                const float back = reinterpret_cast<const float*>(lds + NP * BM * (ldl + 8u) / 2u)[(16u * m + l) * (ldl / 32u) + step];
+#pragma unroll
+                for (uint32_t f = 0; f < NF; f++) {
+                    f4v_t d = {0, 0, 0, 0};
+#pragma unroll
+                    for (uint32_t n = 0; n < NP; n++) d = mfma32<TW>(w[f].v, v[NP - 1u - n], d);
+                    acc[m][f] += d * back;
+                }
+            }
         }
+    };
+    const auto finish = [&](const Strip& s, uint32_t n0) {
+        f4v_t acc[MT][NF] = {};
+        if (rank) multiply(s.w[0], 0, acc);
+        if (rank > 32u) multiply(s.w[1], 1, acc);
+        for (uint32_t step = 2; step < steps; step++) {
+            Eight<TW> w[NF];
+            load_w(w, n0, 32u * step);
+            multiply(w, step, acc);
+        }
+        if constexpr (F32) mfma_settle();
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+            for (uint32_t f = 0; f < NF; f++) {
+                const uint32_t n = n0 + 16u * f + 4u * q;
+                const f4v_t r = rank ? s.y[m][f] + scale * acc[m][f] : s.y[m][f];
+                st_four_any(o[m] + n, !there[m] || n >= a.n ? 0u : a.n - n, r);
+            }
+    };
+    for (uint32_t i = first; i < strips; i += 2u * by) {
+        if (i + by < strips) load(s[1], 16u * NF * (i + by));
+        finish(s[0], 16u * NF * i);
+        if (i + by >= strips) break;
+        if (i + 2u * by < strips) load(s[0], 16u * NF * (i + 2u * by));
+        finish(s[1], 16u * NF * (i + by));
+    }
 }
 
-#define RFXQ_LORA(name, TX, TW)                                                                                    \
-    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name(LoraArgs a) { lora_down<TX, TW>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name(LoraArgs a) { lora_up<TX, TW>(a); }
+#define RFXQ_LORA(name, TX, TW)                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name(LoraArgs a) { lora_down<TX, TW, 1>(a); }    \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name(LoraArgs a) { lora_up<TX, TW, 1, 2>(a); }        \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name##_32(LoraArgs a) { lora_down<TX, TW, 2>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name##_32(LoraArgs a) { lora_up<TX, TW, 2, 2>(a); }
 RFXQ_LORA(f32_f32, float, float)
 RFXQ_LORA(f32_f16, float, half_t)
 RFXQ_LORA(f32_bf16, float, __bf16)
