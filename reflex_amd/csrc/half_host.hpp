@@ -181,16 +181,19 @@ GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool split_x, uint32_t 
 
 // ------------------------------------------------------------------ adapters
 
+// whole vectors in every row of b and out (lora.hpp)
+bool lora_vec(uint32_t rank, uint32_t n) { return rank % 8u == 0 && n % 4u == 0; }
+
 // 32-row tiles from 17 rows a group on. The ranges of K of rfxq_lora_down: until
 // the workgroups fill the CUs, of at least 256 values each.
 struct LoraPlan {
     uint32_t ldv, bm, tiles, splits, k_split;
     uint64_t total;
 };
-LoraPlan lora_plan(uint32_t k, uint32_t rank, uint32_t groups, uint32_t rows, uint32_t cus) {
+LoraPlan lora_plan(uint32_t k, uint32_t n, uint32_t rank, uint32_t groups, uint32_t rows, uint32_t cus) {
     LoraPlan p;
     p.ldv = (rank + 15u) & ~15u;
-    p.bm = rows / std::min(rows, groups) > 16u && rank <= 256u ? 32u : 16u;
+    p.bm = rows / std::min(rows, groups) > 16u && rank <= 256u && lora_vec(rank, n) ? 32u : 16u;
     p.tiles = max_tiles(rows, groups, p.bm);
     const uint32_t fill = getenv("RFXQ_FILL") ? atoi(getenv("RFXQ_FILL")) : 2;
     const uint32_t want = (fill * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
@@ -349,7 +352,7 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
         return fail(RFXQ_ERR_INVALID_INPUT, "lora_add: y and out overlap without being the same rows");
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
-    const LoraPlan p = lora_plan(k, rank, groups, rows, (uint32_t)c->cus);
+    const LoraPlan p = lora_plan(k, n, rank, groups, rows, (uint32_t)c->cus);
     // strips of 32 columns shared by as many workgroups as fill the CUs (4 of a CU's waves each)
     const uint32_t fillu = getenv("RFXQ_FILLU") ? atoi(getenv("RFXQ_FILLU")) : 4;
     const uint32_t across = std::max(1u, std::min((fillu * (uint32_t)c->cus + p.tiles - 1u) / p.tiles, (n + 127u) / 128u));
@@ -385,13 +388,13 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     l.across = across;
     const uint32_t t = x->type == RFXQ_TYPE_F32 ? (a->ggml_type == RFXQ_TYPE_F32 ? 0u : a->ggml_type == RFXQ_TYPE_F16 ? 1u : 2u)
                        : x->type == RFXQ_TYPE_F16 ? 3u : 4u;
-    const uint32_t wide = p.bm == 32u ? 1u : 0u, ldl = (rank + 31u) & ~31u;
+    const uint32_t wide = p.bm == 32u ? 1u : 0u, form = lora_vec(rank, n) ? wide : 2u, ldl = (rank + 31u) & ~31u;
     const uint32_t pieces = x->type == RFXQ_TYPE_F32 && a->ggml_type == RFXQ_TYPE_BF16 ? 3u : 2u;
     const uint32_t lds = a->ggml_type == RFXQ_TYPE_F32 ? 4u * p.bm * (ldl + 4u)
                                                        : 2u * pieces * p.bm * (ldl + 8u) + 4u * p.bm * (ldl / 32u);
     if (int rc = launch(c->half.lora_down[t][wide], p.tiles * p.splits, 0, stream, &l, sizeof l, "rfxq_lora_down launch"))
         return rc;
-    if (int rc = launch(c->half.lora_up[t][wide], (uint32_t)up, lds, stream, &l, sizeof l, "rfxq_lora_up launch")) return rc;
+    if (int rc = launch(c->half.lora_up[t][form], (uint32_t)up, lds, stream, &l, sizeof l, "rfxq_lora_up launch")) return rc;
     return ok();
 }
 

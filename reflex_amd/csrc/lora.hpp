@@ -40,10 +40,6 @@ struct LoraArgs {
 
 // Vectors that may start at any element.
 typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
-typedef _Float16 h8a2_t __attribute__((ext_vector_type(8), aligned(2)));
-typedef __bf16 b8a2_t __attribute__((ext_vector_type(8), aligned(2)));
-typedef _Float16 h4a2_t __attribute__((ext_vector_type(4), aligned(2)));
-typedef __bf16 b4a2_t __attribute__((ext_vector_type(4), aligned(2)));
 
 // 8 neighbouring values of a row as they lie in memory.
 template <typename T>
@@ -74,64 +70,63 @@ RFXQ_DEV Eight<T> ld_eight(const T* p) {
     }
     return r;
 }
-// The first `have` of the 8 values at p, then zeros; `room`: elements from p to the
-// end of its array. What follows the row is read too, where it is there.
+// The first `have` of the 8 values at p, one by one, then zeros.
 template <typename T>
-RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have, uint64_t room) {
-    Eight<T> r = {};
-    if (have == 0) return r;
-    if (room >= 8u) {
-        r = ld_eight(p);
-        if constexpr (__is_same(T, float)) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) r.v[i >> 2][i & 3u] = i < have ? r.v[i >> 2][i & 3u] : 0.0f;
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; i++)
-                r.v[i] &= have > 2u * i + 1u ? 0xFFFFFFFFu : have > 2u * i ? 0xFFFFu : 0u;
-        }
-        return r;
-    }
+RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have) {
+    if (have >= 8u) return ld_eight(p);
     T t[8];
 #pragma unroll
     for (uint32_t i = 0; i < 8u; i++) t[i] = i < have ? ((const RFXQ_GLOBAL T*)p)[i] : (T)0.0f;
+    Eight<T> r;
     __builtin_memcpy(&r, t, sizeof t);
     return r;
 }
 
-// 4 neighbouring values of a row; the first `have` of them.
+// 4 neighbouring values of a row as they lie in memory, at any element.
 template <typename T>
-RFXQ_DEV f4v_t ld_four(const T* p, uint32_t have) {
-    f4v_t r = {0, 0, 0, 0};
-    if (have >= 4u) {
-        if constexpr (__is_same(T, float)) {
-            r = *(const RFXQ_GLOBAL f4a4_t*)p;
-        } else if constexpr (__is_same(T, half_t)) {
-            r = __builtin_convertvector(*(const RFXQ_GLOBAL h4a2_t*)p, f4v_t);
-        } else {
-            r = __builtin_convertvector(*(const RFXQ_GLOBAL b4a2_t*)p, f4v_t);
-        }
-    } else {
+struct FourOf {
+    typedef T type __attribute__((ext_vector_type(4)));
+    typedef T any __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+template <typename T>
+using Four = typename FourOf<T>::type;
+
+template <typename T>
+RFXQ_DEV Four<T> ld_four(const T* p) {
+    return *(const RFXQ_GLOBAL typename FourOf<T>::any*)p;
+}
+template <typename T>
+RFXQ_DEV Four<T> ld_four(const T* p, uint32_t have) {
+    if (have >= 4u) return ld_four(p);
+    Four<T> r = {};
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; i++)
-            if (i < have) r[i] = (float)((const RFXQ_GLOBAL T*)p)[i];
-    }
+    for (uint32_t i = 0; i < 4u; i++)
+        if (i < have) r[i] = ((const RFXQ_GLOBAL T*)p)[i];
     return r;
 }
 template <typename T>
-RFXQ_DEV void st_four_any(T* p, uint32_t have, f4v_t v) {
+RFXQ_DEV void st_four(T* p, uint32_t have, f4v_t v) {
+    const Four<T> r = __builtin_convertvector(v, Four<T>);
     if (have >= 4u) {
-        if constexpr (__is_same(T, float))
-            *(RFXQ_GLOBAL f4a4_t*)p = v;
-        else if constexpr (__is_same(T, half_t))
-            *(RFXQ_GLOBAL h4a2_t*)p = __builtin_convertvector(v, h4a2_t);
-        else
-            *(RFXQ_GLOBAL b4a2_t*)p = __builtin_convertvector(v, b4a2_t);
+        *(RFXQ_GLOBAL typename FourOf<T>::any*)p = r;
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++)
-            if (i < have) ((RFXQ_GLOBAL T*)p)[i] = (T)v[i];
+            if (i < have) ((RFXQ_GLOBAL T*)p)[i] = r[i];
     }
+}
+
+// The first `have` of 8 values, then zeros.
+template <typename T>
+RFXQ_DEV Eight<T> first_of(Eight<T> r, uint32_t have) {
+    if constexpr (__is_same(T, float)) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) r.v[i >> 2][i & 3u] = i < have ? r.v[i >> 2][i & 3u] : 0.0f;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) r.v[i] &= have > 2u * i + 1u ? 0xFFFFFFFFu : have > 2u * i ? 0xFFFFu : 0u;
+    }
+    return r;
 }
 
 // f32 values of a step as pieces of T, times 2^e (the scale's exponent)
@@ -186,9 +181,6 @@ RFXQ_DEV int64_t lora_row(const LoraArgs& a, uint32_t p) {
 template <typename TX, typename TW, uint32_t MT>
 struct LoraDown {
     const TX* x[MT];
-    bool there[MT];
-    const TX* x_end;
-    const TW* a_end;
     RowTile t;
     uint32_t rank, split, wave, lane, k0, k1;
 
@@ -211,7 +203,7 @@ struct LoraDown {
 #pragma unroll
             for (uint32_t f = 0; f < RT; f++) wv[s][f] = ld_eight(w[f] + k);
 #pragma unroll
-            for (uint32_t m = 0; m < MT; m++) xv[s][m] = there[m] ? ld_eight(x[m] + k) : Eight<TX>{};
+            for (uint32_t m = 0; m < MT; m++) xv[s][m] = ld_eight(x[m] + k);
         };
         const auto multiply = [&](uint32_t s) {
 #pragma unroll
@@ -251,10 +243,9 @@ struct LoraDown {
         if (tail) {
             const uint32_t k = k0 + 32u * full, have = tail > 8u * q ? tail - 8u * q : 0u;
 #pragma unroll
-            for (uint32_t f = 0; f < RT; f++)
-                wv[0][f] = ld_eight(w[f] + k, have, (uint64_t)(a_end - (w[f] + k)));
+            for (uint32_t f = 0; f < RT; f++) wv[0][f] = ld_eight(w[f] + k, have);
 #pragma unroll
-            for (uint32_t m = 0; m < MT; m++) xv[0][m] = ld_eight(x[m] + k, there[m] ? have : 0u, (uint64_t)(x_end - (x[m] + k)));
+            for (uint32_t m = 0; m < MT; m++) xv[0][m] = ld_eight(x[m] + k, have);
             multiply(0);
         }
         mfma_settle();
@@ -302,11 +293,9 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
     for (uint32_t m = 0; m < MT; m++) {
         const uint32_t p = d.t.beg + 16u * m + (d.lane & 15u);
         const int64_t row = p < d.t.end ? lora_row(a, p) : -1;
-        d.there[m] = row >= 0;
+        // places without a row read the first one: what comes of it is not used
         d.x[m] = static_cast<const TX*>(a.x) + (row < 0 ? 0 : (uint64_t)row * a.ldx) + 8u * (d.lane >> 4);
     }
-    d.x_end = static_cast<const TX*>(a.x) + (uint64_t)(a.x_rows - 1u) * a.ldx + a.k;
-    d.a_end = static_cast<const TW*>(a.a) + (uint64_t)a.groups * a.rank * a.k;
     const uint32_t quarter = (a.k_split / 4u + 31u) & ~31u;
     const uint32_t end = min(a.k, (d.split + 1u) * a.k_split);
     d.k0 = min(d.split * a.k_split + d.wave * quarter, end);
@@ -326,9 +315,13 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
 // a wave takes every (4 across)th. v, added up and in pieces, lies in LDS for
 // all of them; B's values and y of the next strip are loaded during a strip.
 //
+// VEC: rank is a multiple of 8 and n of 4. Then no load has a condition: what does not
+// exist reads the row's first values and is left out where it is used, so loads
+// stay in flight until then. (Loads under a condition are waited for at its end.)
+//
 // LDS: f32 adapters: v [16 MT][ldv + 4]. Others: the pieces [NP][16 MT][ldl + 8]
 // (halves, ldl = rank in whole steps of 32), then 2^e [16 MT][ldl / 32].
-template <typename TX, typename TW, uint32_t MT, uint32_t NF>
+template <typename TX, typename TW, uint32_t MT, uint32_t NF, bool VEC>
 RFXQ_DEV void lora_up(const LoraArgs& a) {
     constexpr bool F32 = __is_same(TW, float);
     constexpr uint32_t BM = 16u * MT, NP = __is_same(TW, __bf16) && __is_same(TX, float) ? 3u : 2u;
@@ -359,26 +352,20 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
         y[m] = static_cast<const TX*>(a.y) + (row < 0 ? 0 : (uint64_t)row * a.ldy);
         o[m] = static_cast<TX*>(a.out) + (row < 0 ? 0 : (uint64_t)row * a.ldo);
     }
-    const TW* b_end = static_cast<const TW*>(a.b) + (uint64_t)a.groups * a.n * a.rank;
-
     struct Strip {
         Eight<TW> w[2][NF];  // the first 64 of the rank
-        f4v_t y[MT][NF];
+        Four<TX> y[MT][NF];
     };
-    const auto row_of = [&](uint32_t n0, uint32_t f) {
-        return static_cast<const TW*>(a.b) + ((uint64_t)group * a.n + min(n0 + 16u * f + l, a.n - 1u)) * a.rank + 8u * q;
-    };
+    const TW* matrix = static_cast<const TW*>(a.b) + (uint64_t)group * a.n * a.rank;
     const auto load_w = [&](Eight<TW>(&w)[NF], uint32_t n0, uint32_t r) {
-        if (r + 32u <= rank) {
+        const uint32_t at = r + 8u * q;
 #pragma unroll
-            for (uint32_t f = 0; f < NF; f++) w[f] = ld_eight(row_of(n0, f) + r);
-        } else {
-            const uint32_t at = r + 8u * q, have = rank > at ? rank - at : 0u;
-#pragma unroll
-            for (uint32_t f = 0; f < NF; f++) {
-                const TW* p = row_of(n0, f) + r;
-                w[f] = ld_eight(p, have, (uint64_t)(b_end - p));
-            }
+        for (uint32_t f = 0; f < NF; f++) {
+            const TW* row = matrix + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.rank;
+            if constexpr (VEC)
+                w[f] = ld_eight(row + (at < rank ? at : 0u));
+            else
+                w[f] = ld_eight(row + at, rank > at ? rank - at : 0u);
         }
     };
     const auto load = [&](Strip& s, uint32_t n0) {
@@ -389,7 +376,10 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
 #pragma unroll
             for (uint32_t f = 0; f < NF; f++) {
                 const uint32_t n = n0 + 16u * f + 4u * q;
-                s.y[m][f] = ld_four(y[m] + n, !there[m] || n >= a.n ? 0u : a.n - n);
+                if constexpr (VEC)
+                    s.y[m][f] = ld_four(y[m] + (n < a.n ? n : 0u));
+                else
+                    s.y[m][f] = ld_four(y[m] + n, n >= a.n ? 0u : a.n - n);
             }
     };
     const uint32_t first = (blockIdx.x % a.across) * 4u + wave, by = 4u * a.across;
@@ -428,7 +418,15 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
     __syncthreads();
     const float scale = t.group < a.groups && a.scales ? a.scales[t.group] : 1.0f;
 
-    const auto multiply = [&](const Eight<TW>(&w)[NF], uint32_t step, f4v_t(&acc)[MT][NF]) {
+    const auto multiply = [&](const Eight<TW>(&loaded)[NF], uint32_t step, f4v_t(&acc)[MT][NF]) {
+        Eight<TW> w[NF];
+#pragma unroll
+        for (uint32_t f = 0; f < NF; f++) w[f] = loaded[f];
+        if (VEC && 32u * (step + 1u) > rank) {
+            const uint32_t at = 32u * step + 8u * q;
+#pragma unroll
+            for (uint32_t f = 0; f < NF; f++) w[f] = first_of(loaded[f], rank > at ? rank - at : 0u);
+        }
 #pragma unroll
         for (uint32_t m = 0; m < MT; m++) {
             if constexpr (F32) {
@@ -473,8 +471,13 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
 #pragma unroll
             for (uint32_t f = 0; f < NF; f++) {
                 const uint32_t n = n0 + 16u * f + 4u * q;
-                const f4v_t r = rank ? s.y[m][f] + scale * acc[m][f] : s.y[m][f];
-                st_four_any(o[m] + n, !there[m] || n >= a.n ? 0u : a.n - n, r);
+                f4v_t r = __builtin_convertvector(s.y[m][f], f4v_t);
+                if (rank) r += scale * acc[m][f];
+                if constexpr (VEC) {
+                    if (there[m] && n < a.n) st_four(o[m] + n, 4u, r);
+                } else {
+                    st_four(o[m] + n, !there[m] || n >= a.n ? 0u : a.n - n, r);
+                }
             }
     };
     for (uint32_t i = first; i < strips; i += 2u * by) {
@@ -486,11 +489,14 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
     }
 }
 
-#define RFXQ_LORA(name, TX, TW)                                                                                          \
-    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name(LoraArgs a) { lora_down<TX, TW, 1>(a); }    \
-    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name(LoraArgs a) { lora_up<TX, TW, 1, 2>(a); }        \
+#define RFXQ_LORA(name, TX, TW)                                                                                            \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name(LoraArgs a) { lora_down<TX, TW, 1>(a); }      \
     extern "C" __global__ __launch_bounds__(256) void rfxq_lora_down_##name##_32(LoraArgs a) { lora_down<TX, TW, 2>(a); } \
-    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name##_32(LoraArgs a) { lora_up<TX, TW, 2, 2>(a); }
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name(LoraArgs a) { lora_up<TX, TW, 1, 2, true>(a); } \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name##_32(LoraArgs a) {                             \
+        lora_up<TX, TW, 2, 2, true>(a);                                                                                    \
+    }                                                                                                                      \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_lora_up_##name##_any(LoraArgs a) { lora_up<TX, TW, 1, 2, false>(a); }
 RFXQ_LORA(f32_f32, float, float)
 RFXQ_LORA(f32_f16, float, half_t)
 RFXQ_LORA(f32_bf16, float, __bf16)

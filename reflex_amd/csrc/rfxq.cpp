@@ -152,7 +152,7 @@ struct HalfKernels {
     hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {}, t64[2][2] = {};
     hipFunction_t t256[2] = {}, split[2] = {};  // halves, one piece of K after another
     // [f32 x F32, f32 x F16, f32 x BF16, F16, BF16]
-    hipFunction_t lora_down[5][2] = {}, lora_up[5][2] = {};  // [16, 32 rows]
+    hipFunction_t lora_down[5][2] = {}, lora_up[5][3] = {};  // [16, 32 rows, 16 rows of any rank and columns]
 };
 
 struct Ctx {
@@ -237,14 +237,14 @@ int load_half(hipModule_t mod, HalfKernels* h) {
     }
     static const char* const kLora[5] = {"f32_f32", "f32_f16", "f32_bf16", "f16_f16", "bf16_bf16"};
     for (int t = 0; t < 5; t++)
-        for (int wide = 0; wide < 2; wide++)
-            for (int up = 0; up < 2; up++) {
-                char name[64];
-                std::snprintf(name, sizeof name, "rfxq_lora_%s_%s%s", up ? "up" : "down", kLora[t], wide ? "_32" : "");
-                hipError_t e = hipModuleGetFunction(up ? &h->lora_up[t][wide] : &h->lora_down[t][wide], mod, name);
-                if (e != hipSuccess)
-                    return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name, hipGetErrorString(e));
-            }
+        for (int v = 0; v < 5; v++) {
+            static const char* const kForm[5][2] = {{"down", ""}, {"down", "_32"}, {"up", ""}, {"up", "_32"}, {"up", "_any"}};
+            char name[64];
+            std::snprintf(name, sizeof name, "rfxq_lora_%s_%s%s", kForm[v][0], kLora[t], kForm[v][1]);
+            hipError_t e = hipModuleGetFunction(v < 2 ? &h->lora_down[t][v] : &h->lora_up[t][v - 2], mod, name);
+            if (e != hipSuccess)
+                return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name, hipGetErrorString(e));
+        }
     return RFXQ_OK;
 }
 
