@@ -393,11 +393,12 @@ typedef struct rfxq_rows {
  *                order[offsets[g]] .. order[offsets[g + 1] - 1]; rows in no group last.
  * ids and order: n values, offsets: groups + 1, all in device memory; order must
  * not overlap ids. 1 <= groups <= 1024; n up to 2^24; n = 0 clears the offsets
- * (ids and order may then be NULL). One launch, no workspace, no host
- * synchronisation: it can be captured. The reference groups on the host
- * (src/model/dense.rs:1523-1546). */
-int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order,
-                    hipStream_t stream);
+ * (ids and order may then be NULL). `workspace`: rfxq_group_rows_workspace_size
+ * bytes, 16-byte aligned, or NULL for the library's own (see rfxq_gemm); small n need
+ * none. The reference groups on the host (src/model/dense.rs:1523-1546). */
+int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order, void* workspace,
+                    uint64_t workspace_bytes, hipStream_t stream);
+uint64_t rfxq_group_rows_workspace_size(uint32_t n, uint32_t groups);
 
 /* Products of grouped rows with a stack of matrices that a GGUF file keeps in F16
  * or BF16 ([in, out, expert_count]; a 2-D weight is a stack of one): for every

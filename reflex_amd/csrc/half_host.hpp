@@ -16,9 +16,10 @@ struct GroupRowsArgs {
     const int32_t* ids;
     int32_t* offsets;
     int32_t* order;
+    uint32_t* counts;
     uint32_t n, groups, rounds, pad;
 };
-static_assert(sizeof(GroupRowsArgs) == 40, "GroupRowsArgs layout");
+static_assert(sizeof(GroupRowsArgs) == 48, "GroupRowsArgs layout");
 
 struct GroupedArgs {
     const void* x;
@@ -124,6 +125,26 @@ int take_workspace(Ctx* c, void* ws, uint64_t have, uint64_t need, hipStream_t s
 // inside one.
 uint32_t max_tiles(uint32_t rows, uint32_t groups, uint32_t bm) { return rows / bm + std::min(rows, groups); }
 
+// ------------------------------------------------------------------ grouping
+
+struct GroupPlan {
+    uint32_t rounds, grid;
+    uint64_t counts;  // bytes of the workgroups' counts, 0: each counts all rows
+};
+GroupPlan group_plan(uint32_t n, uint32_t groups) {
+    GroupPlan p;
+    // One launch, in which every workgroup counts all ids, or a launch of counts before
+    // it (us, 128 groups: 7.4 against 8.0 at 32768 rows, 9.9 against 9.2 at 65536, 15.4
+    // against 10.5 at 131072; 1024 groups, whose counts are longer to add up: 14.8 against
+    // 24 at 131072). 2 rows a thread there (12.0 with 1, 11.4 with 4), 4 from a million on
+    // (33 against 23).
+    const bool many = n > (groups > 256u ? 262144u : 65536u);
+    p.rounds = !many ? 1u : n <= 262144u ? 2u : 4u;
+    p.grid = std::max(1u, (n + kGroupThreads * p.rounds - 1u) / (kGroupThreads * p.rounds));
+    p.counts = many ? align256(4ull * p.grid * (groups + 1u)) : 0u;
+    return p;
+}
+
 // ------------------------------------------------------------------ grouped GEMM
 
 constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offsets reach
@@ -208,8 +229,13 @@ LoraPlan lora_plan(uint32_t k, uint32_t n, uint32_t rank, uint32_t groups, uint3
 
 extern "C" {
 
-int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order,
-                    hipStream_t stream) {
+uint64_t rfxq_group_rows_workspace_size(uint32_t n, uint32_t groups) {
+    if (n > kMaxGroupRows || groups == 0 || groups > kMaxGroups) return 0;
+    return group_plan(n, groups).counts;
+}
+
+int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* offsets, int32_t* order, void* workspace,
+                    uint64_t workspace_bytes, hipStream_t stream) {
     if (groups == 0 || groups > kMaxGroups)
         return fail(RFXQ_ERR_OTHER, "group_rows: groups=%u (1..=%u)", groups, kMaxGroups);
     if (n > kMaxGroupRows) return fail(RFXQ_ERR_OTHER, "group_rows: n=%u (at most %u)", n, kMaxGroupRows);
@@ -221,11 +247,17 @@ int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* of
         return fail(RFXQ_ERR_INVALID_INPUT, "group_rows: ids, offsets and order overlap");
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
-    const uint32_t rounds = n > 64u * kGroupThreads ? 4u : 1u;
-    GroupRowsArgs a = {ids, offsets, order, n, groups, rounds, 0};
+    const GroupPlan p = group_plan(n, groups);
+    void* ws = nullptr;
+    if (p.counts)
+        if (int rc = take_workspace(c, workspace, workspace_bytes, p.counts, stream, "group_rows", &ws)) return rc;
+    GroupRowsArgs a = {ids, offsets, order, static_cast<uint32_t*>(ws), n, groups, p.rounds, 0};
     const uint32_t keys = groups + 1u, lds = 8u * keys + 4u * ((16u * keys + 1u) / 2u);
-    const uint32_t grid = std::max(1u, (n + kGroupThreads * rounds - 1u) / (kGroupThreads * rounds));
-    if (int rc = launch(c->half.group_rows, grid, lds, stream, &a, sizeof a, "rfxq_group_rows launch", kGroupThreads))
+    if (p.counts)
+        if (int rc = launch(c->half.group_count, p.grid, 4u * keys, stream, &a, sizeof a, "rfxq_group_count launch",
+                            kGroupThreads))
+            return rc;
+    if (int rc = launch(c->half.group_rows, p.grid, lds, stream, &a, sizeof a, "rfxq_group_rows launch", kGroupThreads))
         return rc;
     return ok();
 }

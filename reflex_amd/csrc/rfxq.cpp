@@ -147,7 +147,7 @@ constexpr uint32_t kNormRowsPerWg = 4;  // rows per rfxq_rmsnorm_q8_1 workgroup 
 
 // kernels of the second code object (half_host.hpp)
 struct HalfKernels {
-    hipFunction_t group_rows = nullptr;
+    hipFunction_t group_rows = nullptr, group_count = nullptr;
     // [f32 activations, the weights' type][F16, BF16]
     hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {}, t64[2][2] = {};
     hipFunction_t t256[2] = {}, split[2] = {};  // halves, one piece of K after another
@@ -209,6 +209,7 @@ int load_half(hipModule_t mod, HalfKernels* h) {
         const char* name;
     } fns[] = {
         {&h->group_rows, "rfxq_group_rows"},
+        {&h->group_count, "rfxq_group_count"},
         {&h->any[0][0], "rfxq_grouped_any_f32_f16"},
         {&h->any[0][1], "rfxq_grouped_any_f32_bf16"},
         {&h->any[1][0], "rfxq_grouped_any_f16"},

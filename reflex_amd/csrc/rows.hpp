@@ -79,18 +79,51 @@ struct GroupRowsArgs {
     const int32_t* ids;
     int32_t* offsets;
     int32_t* order;
+    uint32_t* counts;  // rfxq_group_count's: [workgroups][groups + 1], or NULL
     uint32_t n, groups, rounds, pad;
 };
 
 constexpr uint32_t kGroupThreads = 1024, kGroupWaves = kGroupThreads / 64u, kGroupRounds = 4;
 
-// Workgroup b places rows [b c, (b + 1) c), c = 1024 rounds, and counts the
-// ids of all n rows by itself, those before its own apart: one launch, no
-// scratch memory and no waiting between workgroups. The ids are read once by
-// every workgroup (from L2).
+RFXQ_DEV uint32_t group_key(const GroupRowsArgs& a, uint32_t i) {
+    const uint32_t id = (uint32_t)((const RFXQ_GLOBAL int32_t*)a.ids)[i];
+    return id < a.groups ? id : a.groups;
+}
+
+// The rows of each key in [begin, end) added to LDS counters, 8 ids a thread in
+// flight.
+RFXQ_DEV void count_keys(const GroupRowsArgs& a, uint32_t begin, uint32_t end, uint32_t* cnt) {
+    uint32_t i = begin + threadIdx.x;
+    for (; i + 7u * kGroupThreads < end; i += 8u * kGroupThreads) {
+        uint32_t key[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j++) key[j] = group_key(a, i + j * kGroupThreads);
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j++) atomicAdd(cnt + key[j], 1u);
+    }
+    for (; i < end; i += kGroupThreads) atomicAdd(cnt + group_key(a, i), 1u);
+}
+
+// Many rows: each workgroup's rows by key, for rfxq_group_rows. Dynamic LDS:
+// groups + 1 counters.
+extern "C" __global__ __launch_bounds__(1024) void rfxq_group_count(GroupRowsArgs a) {
+    extern __shared__ uint32_t lds[];
+    const uint32_t keys = a.groups + 1u, chunk = kGroupThreads * a.rounds, begin = blockIdx.x * chunk;
+    for (uint32_t k = threadIdx.x; k < keys; k += kGroupThreads) lds[k] = 0;
+    __syncthreads();
+    count_keys(a, begin, min(begin + chunk, a.n), lds);
+    __syncthreads();
+    for (uint32_t k = threadIdx.x; k < keys; k += kGroupThreads) a.counts[(uint64_t)blockIdx.x * keys + k] = lds[k];
+}
+
+// Workgroup b places rows [b c, (b + 1) c), c = 1024 rounds. It needs each key's
+// rows before its own and in all: up to some ten thousand rows it counts
+// them itself (one launch, no scratch memory; the ids come from L2, the LDS
+// atomics bound it: 15.4 us for 131072 rows, 128 groups), for more it adds up what
+// rfxq_group_count left (10.5 us).
 //
-// Dynamic LDS: cnt[2][groups + 1] (rows before the workgroup's own; the
-// others), then wcnt[16][groups + 1] (16 bits: a wave's own rows).
+// Dynamic LDS: before[groups + 1], rest[groups + 1] (rows before the
+// workgroup's own; the others), then wcnt[16][groups + 1] (16 bits: a wave's own rows).
 extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs a) {
     extern __shared__ uint32_t lds[];
     const uint32_t keys = a.groups + 1u, tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -103,11 +136,25 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
     __syncthreads();
 
     const uint32_t chunk = kGroupThreads * a.rounds, begin = blockIdx.x * chunk;
-    const auto key_of = [&](uint32_t i) {
-        const uint32_t id = (uint32_t)a.ids[i];
-        return id < a.groups ? id : a.groups;
-    };
-    for (uint32_t i = tid; i < a.n; i += kGroupThreads) atomicAdd(&(i < begin ? before : rest)[key_of(i)], 1u);
+    if (a.counts) {
+        // the threads of one key take every `parts`th workgroup's counts
+        const uint32_t parts = max(kGroupThreads / keys, 1u);
+        for (uint32_t j = tid; j < parts * keys; j += kGroupThreads) {
+            const uint32_t k = j % keys;
+            uint32_t ahead = 0, behind = 0;
+#pragma unroll 8
+            for (uint32_t w = j / keys; w < gridDim.x; w += parts) {
+                const uint32_t c = a.counts[(uint64_t)w * keys + k];
+                ahead += w < blockIdx.x ? c : 0u;
+                behind += w < blockIdx.x ? 0u : c;
+            }
+            atomicAdd(before + k, ahead);
+            atomicAdd(rest + k, behind);
+        }
+    } else {
+        count_keys(a, 0, begin, before);
+        count_keys(a, begin, a.n, rest);
+    }
     __syncthreads();
 
     // exclusive sums over the groups' counts, a thread per group
@@ -139,7 +186,7 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
         if (r >= a.rounds) break;
         const uint32_t i = begin + (wave * a.rounds + r) * 64u + lane;
         const bool own = i < a.n;
-        key[r] = own ? key_of(i) : 0u;
+        key[r] = own ? group_key(a, i) : 0u;
         uint64_t same = __builtin_amdgcn_ballot_w64(own);
         for (uint32_t b = 0; b < bits; b++) {
             const uint64_t set = __builtin_amdgcn_ballot_w64((key[r] >> b) & 1u);

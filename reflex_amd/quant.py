@@ -29,7 +29,7 @@ __all__ = [
     "moe_route_device", "moe_ffn_grouped_device",
     "act_q8_1_size", "quantize_act_q8_1", "rmsnorm_q8_1", "silu_and_mul_q8_1", "gemm_q8_1", "gemm_q8_1_batch",
     "gemm_gate_up_silu_q8_1",
-    "RowGroups", "group_rows", "grouped_gemm", "grouped_gemm_workspace_size", "lora_add", "lora_add_workspace_size",
+    "RowGroups", "group_rows", "group_rows_workspace_size", "grouped_gemm", "grouped_gemm_workspace_size", "lora_add", "lora_add_workspace_size",
     "get_options", "set_options", "options", "gemm_policy", "PATH_GEMV_ROWS", "PATH_MMQ_INT8", "PATH_MMQ_F16",
 ]
 
@@ -617,62 +617,86 @@ class RowGroups:
     order: torch.Tensor    # int32 [rows]
 
 
-def _ints(t: torch.Tensor | None, least: int, like: torch.Tensor, what: str) -> int | None:
+# The checks below run on every call beside launches of a few microseconds: they compare
+# device numbers and plain integers, not torch.device and enum objects.
+
+_ROW_TYPES = {d: int(t) for d, t in _FLOAT_TYPES.items()}
+
+
+def _on(t: torch.Tensor, what: str) -> int:
+    """The number of the GPU that t is on."""
+    dev = t.get_device()
+    if dev < 0:
+        raise InvalidInputError(11, f"{what} on {t.device}")
+    return dev
+
+
+def _ints(t: torch.Tensor | None, least: int, dev: int, what: str) -> int | None:
     """The address of an int32 device tensor of at least ``least`` values."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < least or t.device != like.device:
-        raise InvalidInputError(11, f"{what}: needs {least} contiguous int32 values on {like.device}, got "
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.numel() < least or not t.is_contiguous():
+        raise InvalidInputError(11, f"{what}: needs {least} contiguous int32 values on cuda:{dev}, got "
                                     f"{t.numel()} of {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, columns: int, like: torch.Tensor, what: str) -> RfxqRows:
+def _rows(t: torch.Tensor, columns: int, dev: int, what: str) -> RfxqRows:
     """``rfxq_rows`` of a 2-D tensor whose rows are contiguous."""
-    ty = _FLOAT_TYPES.get(t.dtype)
-    if ty is None or t.dim() != 2 or t.shape[1] != columns or t.device != like.device:
-        raise InvalidInputError(11, f"{what}: {t.dtype} {list(t.shape)} on {t.device} (f32, f16 or bf16 "
-                                    f"[rows, {columns}] on {like.device})")
-    rows = t.shape[0]
-    if (columns > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < columns):
+    ty = _ROW_TYPES.get(t.dtype)
+    shape = t.shape
+    if ty is None or len(shape) != 2 or shape[1] != columns or t.get_device() != dev:
+        raise InvalidInputError(11, f"{what}: {t.dtype} {list(shape)} on {t.device} (f32, f16 or bf16 "
+                                    f"[rows, {columns}] on cuda:{dev})")
+    rows, (step, one) = shape[0], t.stride()
+    if rows <= 1:
+        step = columns
+    if step < columns or (one != 1 and columns > 1):
         raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
-    return RfxqRows(t.data_ptr(), ty, rows, t.stride(0) if rows > 1 else columns)
+    return RfxqRows(t.data_ptr(), ty, rows, step)
 
 
-def _space(t: torch.Tensor | None, like: torch.Tensor, what: str) -> tuple[int | None, int]:
+def _space(t: torch.Tensor | None, dev: int, what: str) -> tuple[int | None, int]:
     if t is None:
         return None, 0
-    if not t.is_contiguous() or t.device != like.device:
-        raise InvalidInputError(11, f"{what}: the workspace must be contiguous and on {like.device}")
+    if t.get_device() != dev or not t.is_contiguous():
+        raise InvalidInputError(11, f"{what}: the workspace must be contiguous and on cuda:{dev}")
     return t.data_ptr(), t.numel() * t.element_size()
 
 
-def _check_stack(w: Weight, like: torch.Tensor, what: str) -> None:
-    if w.arena.device != like.device:
-        raise InvalidInputError(11, f"{what}: weight on {w.arena.device}, rows on {like.device}")
+def _stack(w: Weight, dev: int, what: str) -> int:
+    """The number of matrices of a weight on this GPU."""
+    if w.arena.get_device() != dev:
+        raise InvalidInputError(11, f"{what}: weight on {w.arena.device}, rows on cuda:{dev}")
+    return w._c.expert_count or 1
 
 
-def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None) -> RowGroups:
+def group_rows_workspace_size(n: int, groups: int) -> int:
+    """Bytes of workspace ``group_rows`` needs for n ids (0 for few)."""
+    return int(lib().rfxq_group_rows_workspace_size(n, groups))
+
+
+def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None,
+               workspace: torch.Tensor | None = None) -> RowGroups:
     """Rows grouped by an int32 device id (a routed expert, a request's adapter); an id
     outside [0, groups) is a row in no group. Stable: a group's rows keep their order."""
+    dev = _on(ids, "group_rows: ids")
     n = ids.numel()
-    if not ids.is_cuda:
-        raise InvalidInputError(11, f"group_rows: ids on {ids.device}")
-    src = _ints(ids, n, ids, "group_rows ids")
+    src = _ints(ids, n, dev, "group_rows ids")
     if out is None:
         if groups < 0:
             raise InvalidInputError(11, f"group_rows: groups={groups}")
-        out = RowGroups(torch.empty(groups + 1, dtype=torch.int32, device=ids.device),
-                        torch.empty(n, dtype=torch.int32, device=ids.device))
+        out = RowGroups(ids.new_empty(groups + 1), ids.new_empty(n))
+    space, size = _space(workspace, dev, "group_rows")
     with _dev(ids):
-        _check(lib().rfxq_group_rows(src, n, groups, _ints(out.offsets, groups + 1, ids, "group_rows offsets"),
-                                     _ints(out.order, n, ids, "group_rows order"), _stream()))
+        _check(lib().rfxq_group_rows(src, n, groups, _ints(out.offsets, groups + 1, dev, "group_rows offsets"),
+                                     _ints(out.order, n, dev, "group_rows order"), space, size, _stream()))
     return out
 
 
 def grouped_gemm_workspace_size(w: Weight, x_rows: int, dtype: torch.dtype) -> int:
     """Bytes of workspace ``grouped_gemm`` needs for x of this many rows and type."""
-    return int(lib().rfxq_grouped_gemm_workspace_size(w.cref(), x_rows, int(_FLOAT_TYPES[dtype])))
+    return int(lib().rfxq_grouped_gemm_workspace_size(w.cref(), x_rows, _ROW_TYPES[dtype]))
 
 
 def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
@@ -682,21 +706,19 @@ def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x
     ``out[y_index[p]] = x[x_index[p] // x_div] @ W[g].T`` (either index may be left out: place p itself).
     The counterpart of ``expert_gemm`` for all experts at once. Without ``out``, a new tensor of x's type with
     ``rows`` rows, zero where no place of a group writes."""
-    count = int(w.shape[2]) if len(w.shape) > 2 else 1
-    if not x.is_cuda:
-        raise InvalidInputError(11, f"grouped_gemm: x on {x.device}")
-    _check_stack(w, x, "grouped_gemm")
+    dev = _on(x, "grouped_gemm: x")
+    count = _stack(w, dev, "grouped_gemm")
     if rows < 0 or x_div < 1:
         raise InvalidInputError(11, f"grouped_gemm: rows={rows} x_div={x_div}")
-    xr = _rows(x, w.in_features, x, "grouped_gemm x")
-    y = out if out is not None else torch.zeros(rows, w.out_features, dtype=x.dtype, device=x.device)
-    yr = _rows(y, w.out_features, x, "grouped_gemm out")
-    space, size = _space(workspace, x, "grouped_gemm")
+    c = w._c
+    xr = _rows(x, c.in_features, dev, "grouped_gemm x")
+    y = out if out is not None else torch.zeros(rows, c.out_features, dtype=x.dtype, device=x.device)
+    yr = _rows(y, c.out_features, dev, "grouped_gemm out")
+    space, size = _space(workspace, dev, "grouped_gemm")
     with _dev(x):
-        _check(lib().rfxq_grouped_gemm(ctypes.byref(xr), w.cref(), _ints(offsets, count + 1, x, "grouped_gemm offsets"),
-                                       rows, _ints(x_index, rows, x, "grouped_gemm x_index"), x_div,
-                                       _ints(y_index, rows, x, "grouped_gemm y_index"), ctypes.byref(yr), space, size,
-                                       _stream()))
+        _check(lib().rfxq_grouped_gemm(xr, c, _ints(offsets, count + 1, dev, "grouped_gemm offsets"), rows,
+                                       _ints(x_index, rows, dev, "grouped_gemm x_index"), x_div,
+                                       _ints(y_index, rows, dev, "grouped_gemm y_index"), yr, space, size, _stream()))
     return y
 
 
@@ -712,24 +734,30 @@ def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.
     for the rows r of group g, ``out[r] = y[r]`` for rows in no group. a [count, rank, in] and b [count, out, rank]
     are stacks; adapter g is their first ``ranks[g]`` rows and columns. ``groups``: the rows grouped by their adapter
     ids (``group_rows``). Without ``out``, y itself is updated."""
-    count = int(a.shape[2]) if len(a.shape) > 2 else 1
-    if not x.is_cuda:
-        raise InvalidInputError(11, f"lora_add: x on {x.device}")
-    _check_stack(a, x, "lora_add a")
-    _check_stack(b, x, "lora_add b")
-    out = y if out is None else out
-    xr = _rows(x, a.in_features, x, "lora_add x")
-    yr, outr = (_rows(t, b.out_features, x, f"lora_add {m}") for t, m in ((y, "y"), (out, "out")))
-    if scales is not None and (scales.dtype != torch.float32 or scales.numel() < count or not scales.is_contiguous()
-                               or scales.device != x.device):
+    dev = _on(x, "lora_add: x")
+    count = _stack(a, dev, "lora_add a")
+    _stack(b, dev, "lora_add b")
+    ca, cb = a._c, b._c
+    xr = _rows(x, ca.in_features, dev, "lora_add x")
+    yr = _rows(y, cb.out_features, dev, "lora_add y")
+    if out is None:
+        out, outr = y, yr
+    else:
+        outr = _rows(out, cb.out_features, dev, "lora_add out")
+    if scales is None:
+        sp = None
+    elif (scales.dtype is not torch.float32 or scales.get_device() != dev or scales.numel() < count
+          or not scales.is_contiguous()):
         raise InvalidInputError(11, f"lora_add: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
-                                    f"(f32, {count} values)")
-    space, size = _space(workspace, x, "lora_add")
+                                    f"(f32, {count} values on cuda:{dev})")
+    else:
+        sp = scales.data_ptr()
+    space, size = _space(workspace, dev, "lora_add")
     with _dev(x):
-        _check(lib().rfxq_lora_add(ctypes.byref(xr), a.cref(), b.cref(), _ints(ranks, count, x, "lora_add ranks"),
-                                   _ptr(scales), _ints(groups.offsets, count + 1, x, "lora_add offsets"),
-                                   _ints(groups.order, x.shape[0], x, "lora_add order"), ctypes.byref(yr),
-                                   ctypes.byref(outr), space, size, _stream()))
+        _check(lib().rfxq_lora_add(xr, ca, cb, _ints(ranks, count, dev, "lora_add ranks"), sp,
+                                   _ints(groups.offsets, count + 1, dev, "lora_add offsets"),
+                                   _ints(groups.order, xr.rows, dev, "lora_add order"), yr, outr, space, size,
+                                   _stream()))
     return out
 
 

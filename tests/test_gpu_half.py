@@ -48,7 +48,7 @@ def _ids(n, groups, how, seed=0):
 @pytest.mark.parametrize("how", ["any", "one", "none", "rising", "all"])
 @pytest.mark.parametrize("n,groups", [(0, 5), (1, 1), (2, 3), (63, 2), (64, 128), (65, 1024), (300, 37), (1000, 128),
                                       (1024, 7), (1025, 1023), (4096, 128), (65536, 64), (65537, 1024),
-                                      (131077, 129)])
+                                      (131077, 129), (270001, 256), (300007, 1000)])
 def test_group_rows(rq, n, groups, how):
     _say("group_rows", n, groups, how)
     ids = _ids(n, groups, how)
@@ -68,6 +68,23 @@ def test_group_rows_unaligned_ids_and_new_outputs(rq):
     g = rq.group_rows(t, 37)
     want_offsets, want_order = _grouped(ids, 37)
     assert np.array_equal(g.offsets.cpu().numpy(), want_offsets) and np.array_equal(g.order.cpu().numpy(), want_order)
+
+
+def test_group_rows_own_workspace(rq):
+    n, groups = 100_001, 200
+    ids = _ids(n, groups, "any")
+    t = torch.from_numpy(ids).to(DEV)
+    size = rq.group_rows_workspace_size(n, groups)
+    ws = torch.full((size + 64,), 7, dtype=torch.uint8, device=DEV)
+    g = rq.group_rows(t, groups, workspace=ws[:size])
+    want_offsets, want_order = _grouped(ids, groups)
+    assert np.array_equal(g.offsets.cpu().numpy(), want_offsets) and np.array_equal(g.order.cpu().numpy(), want_order)
+    assert (ws[size:] == 7).all()
+    with pytest.raises(rq.InvalidInputError, match="needs"):
+        rq.group_rows(t, groups, workspace=ws[:size - 1])
+    with pytest.raises(rq.ReflexError, match="16-byte aligned"):
+        rq.group_rows(t, groups, workspace=ws[8:])
+    assert rq.group_rows_workspace_size(1000, groups) == 0
 
 
 # ------------------------------------------------------------------ grouped_gemm

@@ -48,7 +48,7 @@ def _expect(L, rc, code, text):
 ])
 def test_group_rows_refusals(L, change, code, text):
     a = {"ids": P, "n": 100, "groups": 8, "offsets": 2 * P, "order": 3 * P, **change}
-    _expect(L, L.rfxq_group_rows(a["ids"], a["n"], a["groups"], a["offsets"], a["order"], None), code, text)
+    _expect(L, L.rfxq_group_rows(a["ids"], a["n"], a["groups"], a["offsets"], a["order"], None, 0, None), code, text)
 
 
 def _grouped(L, x=None, w=None, offsets=5 * P, rows=8, x_index=None, x_div=1, y_index=None, y=None, ws=None, ws_bytes=0):
