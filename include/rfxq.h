@@ -414,18 +414,15 @@ uint64_t rfxq_group_rows_workspace_size(uint32_t n, uint32_t groups);
  * x: f32, or the weights' type; y: f32, or the weights' type (its rows must not
  * overlap x). Accumulation is f32, each result is rounded once; f32 activations
  * keep f32 accuracy (they are split into 2 (F16) or 3 (BF16) pieces of the
- * weights' type in the workspace; a weight that is infinite gives a result that is
- * not finite, of either kind). Any in_features, stride and alignment of whole
- * elements; rows of x and W that start at multiples of 16 bytes (in_features and
- * strides multiples of 8) are faster. `workspace`: rfxq_grouped_gemm_workspace_size
- * bytes, 16-byte aligned, or NULL for the library's own (see rfxq_gemm). The
- * counterpart of rfxq_expert_gemm for all experts at once
+ * weights' type; a weight that is infinite gives a result that is not finite, of
+ * either kind). Any in_features, stride and alignment of whole elements; rows of x
+ * and W that start at multiples of 16 bytes (in_features and strides multiples of
+ * 8) are faster. One launch, no workspace, no host synchronisation: it can be
+ * captured. The counterpart of rfxq_expert_gemm for all experts at once
  * (src/model/dense.rs:1086-1115, 1531-1548). */
 int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
                       const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
-                      void* workspace, uint64_t workspace_bytes, hipStream_t stream);
-/* 0 unless x_type is RFXQ_TYPE_F32 (or the weight or type has no product). */
-uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows, uint32_t x_type);
+                      hipStream_t stream);
 
 /* Low-rank adapters of many requests beside a projection that all rows share:
  * for the rows r = order[p] (NULL: p) of group g, offsets[g] <= p < offsets[g + 1],
@@ -441,7 +438,9 @@ uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows,
  * of x once (a row that it does not list keeps what out held). x, y and out have
  * one type: f32 (any adapters), or the adapters' F16 / BF16; as many rows each.
  * A x is kept in f32, accumulation is f32, each result is rounded once.
- * `workspace` as for rfxq_grouped_gemm. No counterpart in the reference. */
+ * `workspace`: rfxq_lora_add_workspace_size bytes for up to `rows` rows, 16-byte
+ * aligned, or NULL for the library's own (see rfxq_gemm). No counterpart in the
+ * reference. */
 int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b, const int32_t* ranks,
                   const float* scales, const int32_t* offsets, const int32_t* order, const rfxq_rows* y,
                   const rfxq_rows* out, void* workspace, uint64_t workspace_bytes, hipStream_t stream);

@@ -126,8 +126,7 @@ SIGNATURES = {
     "rfxq_gemm_q8_1_plan_create": (_I, [_P, _U32, _U32, _I, ctypes.POINTER(_P)]),
     "rfxq_group_rows": (_I, [_P, _U32, _U32, _P, _P, _P, _U64, _P]),
     "rfxq_group_rows_workspace_size": (_U64, [_U32, _U32]),
-    "rfxq_grouped_gemm": (_I, [_RP, _WP, _P, _U32, _P, _U32, _P, _RP, _P, _U64, _P]),
-    "rfxq_grouped_gemm_workspace_size": (_U64, [_WP, _U32, _U32]),
+    "rfxq_grouped_gemm": (_I, [_RP, _WP, _P, _U32, _P, _U32, _P, _RP, _P]),
     "rfxq_lora_add": (_I, [_RP, _WP, _WP, _P, _P, _P, _P, _RP, _RP, _P, _U64, _P]),
     "rfxq_lora_add_workspace_size": (_U64, [_WP, _U32]),
 }

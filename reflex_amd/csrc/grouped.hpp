@@ -2,15 +2,15 @@
 // (rfxq_grouped_gemm): y[dst_p][n] = sum_k x[src_p][k] W_g[n][k] for the rows p
 // of group g, f32 accumulation, one rounding to the type of y.
 //
-// f32 activations keep their accuracy: a first launch splits each value into
-// pieces of the weights' type that add up to it, and the products run over the
-// pieces (the same weights, f32 accumulation).
-// Rows are scaled by a power of two first, so that a row's largest value lies
-// in [2^14, 2^15) (the matrix instructions take subnormal bf16 operands as 0):
-//   f16:  hi = RN16(x), lo = RN16(x - hi): 22 bits or more of every value above
-//         2^-17 of the row's largest, 2^-39 of the largest of every other
-//   bf16: three truncations of 8 bits each: exact for every value above 2^-100
-//         of the row's largest
+// f32 activations keep their accuracy: few rows go through f32 matrix
+// instructions, more are split, as a tile is staged, into pieces of the weights'
+// type that add up to them and multiply the same weights. A row's 64 values of a
+// step are scaled by a power of two first, so that the largest lies in [2^14,
+// 2^15) (the matrix instructions take subnormal bf16 operands as 0), and the
+// step's sum is scaled back as it is added:
+//   f16:  x = RN16(x) + RN16(the rest): 22 bits or more of every value above
+//         2^-17 of the step's largest, 2^-39 of the largest of every other
+//   bf16: three roundings of 8 bits each: exact
 // Products of the pieces cost 2 (f16) or 3 (bf16) times the matrix
 // instructions; one rounding of x to the weights' type would cost 2^-12 or 2^-9
 // of every value, which f32 outputs show.
@@ -41,21 +41,17 @@ RFXQ_DEV void mfma_settle() {
 }
 
 struct GroupedArgs {
-    const uint16_t* x;  // rows of halves (pieces: plane p of `plane` elements)
+    const void* x;
     const uint16_t* w;
     void* y;
     const int32_t* offsets;
     const int32_t* x_index;
     const int32_t* y_index;
-    const int32_t* x_exp;  // pieces: the results are taken times 2^x_exp[src], or NULL
-    uint64_t ldx, ldy, plane, w_stride;
+    uint64_t ldx, ldy, w_stride;
     uint32_t rows, x_rows, y_rows, x_div;
-    uint32_t k, n, groups, pieces;
-    uint32_t y_f32, tiles_m, tiles_n, sm, sn, pad;
+    uint32_t k, n, groups, y_f32;
+    uint32_t tiles_m, tiles_n, sm, sn;
 };
-
-// 16 zero bytes that lanes past a row's end copy from
-__device__ const u4_t rfxq_zero16 = {0, 0, 0, 0};
 
 // Row p's source and destination; -1 where an index is out of range (such a row
 // is not computed).
@@ -71,6 +67,99 @@ RFXQ_DEV int64_t dst_row(const GroupedArgs& a, uint32_t p) {
     return i >= 0 && (uint32_t)i < a.y_rows ? (int64_t)i : -1;
 }
 
+// Vectors that may start at any element.
+typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// 8 neighbouring values of a row as they lie in memory.
+template <typename T>
+struct Eight {
+    u4_t v;
+    __device__ __forceinline__ float at(uint32_t j) const {
+        if constexpr (__is_same(T, half_t))
+            return (float)__builtin_bit_cast(h8_t, v)[j];
+        else
+            return (float)__builtin_bit_cast(b8_t, v)[j];
+    }
+};
+template <>
+struct Eight<float> {
+    f4v_t v[2];
+    __device__ __forceinline__ float at(uint32_t j) const { return v[j >> 2][j & 3u]; }
+};
+
+// The 8 values at p.
+template <typename T>
+RFXQ_DEV Eight<T> ld_eight(const T* p) {
+    Eight<T> r;
+    if constexpr (__is_same(T, float)) {
+        r.v[0] = *(const RFXQ_GLOBAL f4a4_t*)p;
+        r.v[1] = *(const RFXQ_GLOBAL f4a4_t*)(p + 4);
+    } else {
+        r.v = *(const RFXQ_GLOBAL u4a2_t*)p;
+    }
+    return r;
+}
+// The first `have` of the 8 values at p, one by one, then zeros.
+template <typename T>
+RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have) {
+    if (have >= 8u) return ld_eight(p);
+    T t[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) t[i] = i < have ? ((const RFXQ_GLOBAL T*)p)[i] : (T)0.0f;
+    Eight<T> r;
+    __builtin_memcpy(&r, t, sizeof t);
+    return r;
+}
+
+RFXQ_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
+
+// 8 f32 values of a step as pieces of T that add up to them times `scale`.
+// Infinities and NaN are whole in the first.
+template <typename T, uint32_t NP>
+RFXQ_DEV void split_eight(const Eight<float>& x, float scale, u4_t (&out)[NP]) {
+    float left[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) left[i] = x.at(i) * scale;
+#pragma unroll
+    for (uint32_t n = 0; n < NP; n++)
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const T a = (T)left[2 * i], b = (T)left[2 * i + 1];
+            out[n][i] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+            left[2 * i] = finite(left[2 * i]) ? left[2 * i] - (float)a : 0.0f;
+            left[2 * i + 1] = finite(left[2 * i + 1]) ? left[2 * i + 1] - (float)b : 0.0f;
+        }
+}
+// The exponent e at which `top` is 2^e times a value in [2^14, 2^15), kept so that 2^e and 2^-e are f32 values
+RFXQ_DEV int step_exp(float top) { return max(__builtin_amdgcn_frexp_expf(top) - 15, -126); }
+RFXQ_DEV float pow2(int e) { return as_f32((uint32_t)(e + 127) << 23); }
+
+// the largest of the four lanes (l, 0..3)
+RFXQ_DEV float max_over_q(float v) {
+    uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    v = fmaxf(as_f32(r[0]), as_f32(r[1]));
+    b = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(as_f32(s[0]), as_f32(s[1]));
+}
+// the largest of the finite ones' sizes
+RFXQ_DEV float max_of_eight(const Eight<float>& x) {
+    float t = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        const float v = __builtin_fabsf(x.at(i));
+        t = v < __builtin_inff() ? fmaxf(t, v) : t;
+    }
+    return t;
+}
+// the largest of 8 neighbouring lanes
+RFXQ_DEV float max_over_8(float v) {
+    v = fmaxf(v, RFXQ_DPP(v, 0xB1));
+    v = fmaxf(v, RFXQ_DPP(v, 0x4E));
+    return fmaxf(v, RFXQ_DPP(v, 0x141));
+}
+
 // Workgroup b's place in the grid of tiles: workgroups go round-robin to the 8
 // XCDs, and each XCD takes blocks of sm x sn neighbouring tiles, whose rows
 // and columns meet in its L2.
@@ -80,18 +169,6 @@ RFXQ_DEV bool tile_place(const GroupedArgs& a, uint32_t b, uint32_t& tm, uint32_
     tm = (block / across) * a.sm + r % a.sm;
     tn = (block % across) * a.sn + r / a.sm;
     return tm < a.tiles_m && tn < a.tiles_n;
-}
-
-// 8 halves at p, of which the first `have` are there: the others are 0.
-RFXQ_DEV u4_t ld_halves(const uint16_t* p, uint32_t have) {
-    if (have >= 8u) return *(const RFXQ_GLOBAL u4a2_t*)p;
-    uint16_t v[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) v[i] = i < have ? ((const RFXQ_GLOBAL uint16_t*)p)[i] : (uint16_t)0;
-    u4_t r;
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; i++) r[i] = (uint32_t)v[2 * i] | (uint32_t)v[2 * i + 1] << 16;
-    return r;
 }
 
 // 16 neighbouring results of one row, of which the first `have` are there.
@@ -168,7 +245,7 @@ RFXQ_DEV uint32_t lds_piece(uint32_t r, uint32_t c) { return r * 8u + (c ^ (r & 
 RFXQ_DEV uint32_t col_of(uint32_t j) { return (j & ~63u) + ((j >> 2) & 3u) * 16u + ((j >> 4) & 3u) * 4u + (j & 3u); }
 
 // The wave's 16 MF x 64 tile of one 64-wide step of K, both operands in LDS
-// (the activations' pieces XS apart).
+// (the activations' pieces XS apart, the last ones first).
 template <typename T, int MF, uint32_t PIECES, uint32_t XS>
 RFXQ_DEV void tile_step(const u4_t* xs, const u4_t* ws, uint32_t xr, uint32_t wr, f4v_t (&acc)[MF][4]) {
     const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4;
@@ -181,7 +258,8 @@ RFXQ_DEV void tile_step(const u4_t* xs, const u4_t* ws, uint32_t xr, uint32_t wr
         for (uint32_t j = 0; j < PIECES; j++) {
             u4_t xf[MF];
 #pragma unroll
-            for (uint32_t m = 0; m < (uint32_t)MF; m++) xf[m] = xs[j * XS + lds_piece(xr + 16u * m + l, 4u * h + q)];
+            for (uint32_t m = 0; m < (uint32_t)MF; m++)
+                xf[m] = xs[(PIECES - 1u - j) * XS + lds_piece(xr + 16u * m + l, 4u * h + q)];
 #pragma unroll
             for (uint32_t m = 0; m < (uint32_t)MF; m++)
 #pragma unroll
@@ -201,118 +279,135 @@ RFXQ_DEV void tile_out(const GroupedArgs& a, const RowTile& t, uint32_t m0, uint
         if (p >= t.end) continue;
         const int64_t src = src_row(a, p), dst = dst_row(a, p);
         if (src < 0 || dst < 0) continue;
-        f4v_t v[4];
-        const int e = a.x_exp ? a.x_exp[src] : 0;
-#pragma unroll
-        for (int f = 0; f < 4; f++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[f][i] = a.x_exp ? __builtin_ldexpf(acc[m][f][i], e) : acc[m][f][i];
-        st_row<T>(a, dst, n0 + 16u * q, v);
+        st_row<T>(a, dst, n0 + 16u * q, acc[m]);
     }
 }
 
-// Any alignment and any K: operands through registers, element by element at
-// a row's end, the next step's loads in flight during the products. 64 x 128
-// tiles, 4 waves of 32 x 64; PIECES row tiles beside one tile of weights.
-template <typename T, uint32_t PIECES>
+// Any alignment and any K: operands through registers, the next step's loads in
+// flight during the products. 64 x 128 tiles, 4 waves of 32 x 64. Loads of
+// whole steps have no condition: rows and columns past the tile read others,
+// whose results are not stored. The last, partial step is loaded element by
+// element, with zeros behind the end of both operands.
+// TX float: split into pieces on the way to LDS, all against one tile of weights.
+template <typename TX, typename T>
 RFXQ_DEV void grouped_any(const GroupedArgs& a) {
+    constexpr bool F32 = __is_same(TX, float);
+    constexpr uint32_t P = !F32 ? 1u : __is_same(T, half_t) ? 2u : 3u;
     constexpr uint32_t BM = 64, BN = 128, NX = BM * 8u / 256u, NW = BN * 8u / 256u;
-    __shared__ u4_t xs[PIECES][BM * 8u], ws[BN * 8u];
+    __shared__ u4_t xs[P][BM * 8u], ws[BN * 8u];
+    __shared__ float back[F32 ? BM : 1u];  // of the step's rows
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
     const RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, tm);
     if (!t.any) return;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, n0 = tn * BN;
-    const uint16_t* w = a.w + (uint64_t)t.group * a.w_stride;
-    const uint16_t* xp[NX];
-    const uint16_t* wp[NW];
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, n0 = tn * BN, c = tid & 7u, l = tid & 15u;
+    const T* w = reinterpret_cast<const T*>(a.w) + (uint64_t)t.group * a.w_stride;
+    const TX* xp[NX];
+    const T* wp[NW];
 #pragma unroll
     for (uint32_t i = 0; i < NX; i++) {
-        const uint32_t p = t.beg + (tid >> 3) + 32u * i;
-        const int64_t s = p < t.end ? src_row(a, p) : -1;
-        xp[i] = s < 0 ? nullptr : a.x + (uint64_t)s * a.ldx;
+        const int64_t s = src_row(a, min(t.beg + (tid >> 3) + 32u * i, t.end - 1u));
+        xp[i] = static_cast<const TX*>(a.x) + (s < 0 ? 0 : (uint64_t)s * a.ldx) + 8u * c;
     }
 #pragma unroll
-    for (uint32_t i = 0; i < NW; i++) {
-        const uint32_t n = n0 + col_of((tid >> 3) + 32u * i);
-        wp[i] = n < a.n ? w + (uint64_t)n * a.k : nullptr;
-    }
+    for (uint32_t i = 0; i < NW; i++)
+        wp[i] = w + (uint64_t)min(n0 + col_of((tid >> 3) + 32u * i), a.n - 1u) * a.k + 8u * c;
     f4v_t acc[2][4] = {};
-    const uint32_t steps = (a.k + 63u) / 64u, c = tid & 7u;
-    u4_t xv[PIECES][NX], wv[NW];
+    const uint32_t full = a.k / 64u, tail = a.k % 64u, steps = full + (tail ? 1u : 0u);
+    const uint32_t row0 = (wave >> 1) * 32u, col0 = (wave & 1u) * 64u;
+    Eight<TX> xv[NX];
+    Eight<T> wv[NW];
     const auto load = [&](uint32_t s) {
-        const uint32_t k = s * 64u + 8u * c, have = k < a.k ? a.k - k : 0u;
+        const uint32_t k = s * 64u;
+        if (s < full) {
 #pragma unroll
-        for (uint32_t i = 0; i < NW; i++) wv[i] = wp[i] && have ? ld_halves(wp[i] + k, have) : u4_t{0, 0, 0, 0};
+            for (uint32_t i = 0; i < NW; i++) wv[i] = ld_eight(wp[i] + k);
 #pragma unroll
-        for (uint32_t j = 0; j < PIECES; j++)
+            for (uint32_t i = 0; i < NX; i++) xv[i] = ld_eight(xp[i] + k);
+        } else if (s < steps) {
+            const uint32_t have = tail > 8u * c ? tail - 8u * c : 0u;
 #pragma unroll
-            for (uint32_t i = 0; i < NX; i++)
-                xv[j][i] = xp[i] && have ? PIECES > 1 ? ld16(xp[i] + j * a.plane + k) : ld_halves(xp[i] + k, have) : u4_t{0, 0, 0, 0};
+            for (uint32_t i = 0; i < NW; i++) wv[i] = ld_eight(wp[i] + k, have);
+#pragma unroll
+            for (uint32_t i = 0; i < NX; i++) xv[i] = ld_eight(xp[i] + k, have);
+        }
     };
     load(0);
     for (uint32_t s = 0; s < steps; s++) {
         __syncthreads();
 #pragma unroll
-        for (uint32_t j = 0; j < PIECES; j++)
+        for (uint32_t i = 0; i < NX; i++) {
+            const uint32_t r = (tid >> 3) + 32u * i;
+            if constexpr (F32) {
+                const int e = step_exp(max_over_8(max_of_eight(xv[i])));
+                u4_t p[P];
+                split_eight<T, P>(xv[i], pow2(-e), p);
 #pragma unroll
-            for (uint32_t i = 0; i < NX; i++) xs[j][lds_piece((tid >> 3) + 32u * i, c)] = xv[j][i];
+                for (uint32_t j = 0; j < P; j++) xs[j][lds_piece(r, c)] = p[j];
+                if (c == 0) back[r] = pow2(e);
+            } else {
+                xs[0][lds_piece(r, c)] = xv[i].v;
+            }
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < NW; i++) ws[lds_piece((tid >> 3) + 32u * i, c)] = wv[i];
+        for (uint32_t i = 0; i < NW; i++) ws[lds_piece((tid >> 3) + 32u * i, c)] = wv[i].v;
         __syncthreads();
-        if (s + 1u < steps) load(s + 1u);
-        tile_step<T, 2, PIECES, BM * 8u>(xs[0], ws, (wave >> 1) * 32u, (wave & 1u) * 64u, acc);
+        load(s + 1u);
+        if constexpr (F32) {
+            f4v_t d[2][4] = {};
+            tile_step<T, 2, P, BM * 8u>(xs[0], ws, row0, col0, d);
+#pragma unroll
+            for (uint32_t m = 0; m < 2u; m++) {
+                const float scale = back[row0 + 16u * m + l];
+#pragma unroll
+                for (uint32_t f = 0; f < 4u; f++) acc[m][f] += d[m][f] * scale;
+            }
+        } else {
+            tile_step<T, 2, 1, 0>(xs[0], ws, row0, col0, acc);
+        }
     }
-    tile_out<T, 2>(a, t, (wave >> 1) * 32u, n0 + (wave & 1u) * 64u, acc);
+    tile_out<T, 2>(a, t, row0, n0 + col0, acc);
 }
 
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f16(GroupedArgs a) { grouped_any<half_t, 1>(a); }
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_bf16(GroupedArgs a) { grouped_any<__bf16, 1>(a); }
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f32_f16(GroupedArgs a) { grouped_any<half_t, 2>(a); }
-extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_any_f32_bf16(GroupedArgs a) { grouped_any<__bf16, 3>(a); }
+extern "C" __global__ __launch_bounds__(256, 4) void rfxq_grouped_any_f16(GroupedArgs a) { grouped_any<half_t, half_t>(a); }
+extern "C" __global__ __launch_bounds__(256, 4) void rfxq_grouped_any_bf16(GroupedArgs a) { grouped_any<__bf16, __bf16>(a); }
+extern "C" __global__ __launch_bounds__(256, 3) void rfxq_grouped_any_f32_f16(GroupedArgs a) { grouped_any<float, half_t>(a); }
+extern "C" __global__ __launch_bounds__(256, 3) void rfxq_grouped_any_f32_bf16(GroupedArgs a) { grouped_any<float, __bf16>(a); }
 
 // ---------------------------------------------------------------- tiles filled by asynchronous copies
 
 // BM x BN tiles of WM x WN waves (each BM / WM rows x 64 columns), 64-wide
 // steps of K in STAGES buffers: copies global -> LDS run STAGES - 1 steps
-// ahead of the products, without registers between. P pieces of the activations
-// beside one tile of weights; where P is less than there are, the steps go
-// through the pieces. Rows of x and W start at whole 16 bytes; what lies past a
-// row's end or the tile's last row is copied from past the buffer's end, which
-// fills it with zeros. Offsets within x and within one matrix stay below 4 GiB
-// (the host's rule).
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, uint32_t P>
+// ahead of the products, without registers between. Rows of x and W start at
+// whole 16 bytes; what lies past a row's end or the tile's last row is copied
+// from past the buffer's end, which fills it with zeros. Offsets within x and
+// within one matrix stay below 4 GiB (the host's rule).
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 struct GroupedTile {
     static constexpr uint32_t THREADS = 64u * WM * WN, MF = BM / WM / 16;
-    static constexpr uint32_t NX = BM * 8u / THREADS, NW = BN * 8u / THREADS, LOADS = P * NX + NW;
+    static constexpr uint32_t NX = BM * 8u / THREADS, NW = BN * 8u / THREADS, LOADS = NX + NW;
     static constexpr uint32_t PAST = 0xFFFFFFF0u;
     static_assert(BN == 64 * WN && NX >= 1 && NW >= 1 && STAGES >= 2 && STAGES <= 4 && (STAGES - 2) * LOADS < 64);
 
     RowTile t;
     rsrc_t xr, wr;
     uint32_t xo[NX], wo[NW];  // lanes' byte offsets at k = 0
-    uint32_t lane, wave, piece, n0, k, pieces, plane, steps;
-    uint32_t at_k = 0, at_p = 0;  // of the next step to copy
+    uint32_t lane, wave, piece, n0, k, steps;
+    uint32_t at = 0;  // of the next step to copy
 
     __device__ __forceinline__ void issue(u4_t* xs, u4_t* ws) {
         // past the end: as many copies, so that waits count the same
-        const bool more = at_k < k, there = more && (at_k + 64u <= k || at_k + 8u * piece < k);
-        const uint32_t xb = more ? 2u * at_k + at_p * plane : 0u, wb = more ? 2u * at_k : 0u;
+        const bool there = at + 64u <= k || at + 8u * piece < k;
+        const uint32_t by = at < k ? 2u * at : 0u;
 #pragma unroll
-        for (uint32_t j = 0; j < P; j++)
-#pragma unroll
-            for (uint32_t i = 0; i < NX; i++)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, RFXQ_LDSP(xs + j * BM * 8 + (wave * NX + i) * 64u), 16,
-                                                         there ? xo[i] : PAST, more ? xb + j * plane : 0u, 0, 0);
+        for (uint32_t i = 0; i < NX; i++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, RFXQ_LDSP(xs + (wave * NX + i) * 64u), 16, there ? xo[i] : PAST, by,
+                                                     0, 0);
 #pragma unroll
         for (uint32_t i = 0; i < NW; i++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, RFXQ_LDSP(ws + (wave * NW + i) * 64u), 16, there ? wo[i] : PAST, wb,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, RFXQ_LDSP(ws + (wave * NW + i) * 64u), 16, there ? wo[i] : PAST, by,
                                                      0, 0);
-        at_p += P;
-        if (at_p >= pieces) {
-            at_p = 0;
-            at_k += 64u;
-        }
+        at += 64u;
     }
 
     // the tile, and where its rows are; false: there is none
@@ -326,9 +421,7 @@ struct GroupedTile {
         wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         piece = (lane & 7u) ^ (lane >> 3);
         k = a.k;
-        pieces = a.pieces;
-        plane = (uint32_t)(2u * a.plane);
-        const uint64_t xbytes = ((uint64_t)a.plane * (a.pieces - 1u) + (uint64_t)(a.x_rows - 1u) * a.ldx + a.k) * 2u;
+        const uint64_t xbytes = ((uint64_t)(a.x_rows - 1u) * a.ldx + a.k) * 2u;
         xr = make_rsrc(a.x, (uint32_t)xbytes);
         wr = make_rsrc(a.w + (uint64_t)t.group * a.w_stride, (uint32_t)(2u * a.w_stride));
 #pragma unroll
@@ -342,13 +435,12 @@ struct GroupedTile {
             const uint32_t n = n0 + col_of((wave * NW + i) * 8u + (lane >> 3));
             wo[i] = n < a.n ? n * a.k * 2u + 16u * piece : PAST;
         }
-        steps = (a.k + 63u) / 64u * (a.pieces / P);
+        steps = (a.k + 63u) / 64u;
         return true;
     }
 
     __device__ __forceinline__ void run(const GroupedArgs& a) {
-        constexpr uint32_t XS = P * BM * 8u;
-        __shared__ u4_t xs0[XS], xs1[XS], xs2[STAGES > 2 ? XS : 1u], xs3[STAGES > 3 ? XS : 1u];
+        __shared__ u4_t xs0[BM * 8], xs1[BM * 8], xs2[STAGES > 2 ? BM * 8 : 1], xs3[STAGES > 3 ? BM * 8 : 1];
         __shared__ u4_t ws0[BN * 8], ws1[BN * 8], ws2[STAGES > 2 ? BN * 8 : 1], ws3[STAGES > 3 ? BN * 8 : 1];
         if (!begin(a)) return;
         f4v_t acc[MF][4] = {};
@@ -361,7 +453,7 @@ struct GroupedTile {
             __builtin_amdgcn_s_waitcnt(0x0F70 | (left & 15u) | (left >> 4) << 14);
             lds_barrier();
             issue(nx, nw);
-            tile_step<T, MF, P, BM * 8u>(xs, ws, row0, col0, acc);
+            tile_step<T, MF, 1, 0>(xs, ws, row0, col0, acc);
         };
         for (uint32_t s = 0; s < steps; s += STAGES) {
             if constexpr (STAGES == 2) {
@@ -442,7 +534,7 @@ struct GroupedTile {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the workgroup
     }
     __device__ __forceinline__ void run_turns(const GroupedArgs& a) {
-        static_assert(WM * WN == 8 && WN == 4 && STAGES == 2 && P == 1);
+        static_assert(WM * WN == 8 && WN == 4 && STAGES == 2);
         __shared__ u4_t xs0[BM * 8], xs1[BM * 8], ws0[BN * 8], ws1[BN * 8];
         if (!begin(a)) return;
         f4v_t acc[MF][4] = {};
@@ -454,17 +546,15 @@ struct GroupedTile {
     }
 };
 
-#define RFXQ_GROUPED_TILE(name, T, BM, BN, WM, WN, STAGES, P, RUN)                                   \
+#define RFXQ_GROUPED_TILE(name, T, BM, BN, WM, WN, STAGES, RUN)                                      \
     extern "C" __global__ __launch_bounds__(64 * WM * WN) void rfxq_grouped_##name(GroupedArgs a) { \
-        GroupedTile<T, BM, BN, WM, WN, STAGES, P> t;                                                 \
+        GroupedTile<T, BM, BN, WM, WN, STAGES> t;                                                    \
         t.RUN(a);                                                                                    \
     }
-RFXQ_GROUPED_TILE(64_f16, half_t, 64, 128, 2, 2, 3, 1, run)
-RFXQ_GROUPED_TILE(64_bf16, __bf16, 64, 128, 2, 2, 3, 1, run)
-RFXQ_GROUPED_TILE(64_f32_f16, half_t, 64, 128, 2, 2, 2, 2, run)
-RFXQ_GROUPED_TILE(64_f32_bf16, __bf16, 64, 128, 2, 2, 2, 3, run)
-RFXQ_GROUPED_TILE(256_f16, half_t, 256, 256, 2, 4, 2, 1, run_turns)
-RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, 1, run_turns)
+RFXQ_GROUPED_TILE(64_f16, half_t, 64, 128, 2, 2, 3, run)
+RFXQ_GROUPED_TILE(64_bf16, __bf16, 64, 128, 2, 2, 3, run)
+RFXQ_GROUPED_TILE(256_f16, half_t, 256, 256, 2, 4, 2, run_turns)
+RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, run_turns)
 
 // ---------------------------------------------------------------- few rows a group
 
@@ -475,8 +565,8 @@ RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, 1, run_turns)
 // (WK = 4, the workgroup's waves add their parts in LDS). Loads run a block of 128 of K
 // ahead of the products.
 // f32 activations are multiplied as they are (f32 matrix instructions, the weights
-// widened): 32 cycles for 4 of K, which stays below the time of the
-// weights' memory reads at 16 rows, and spares the pieces' launch.
+// widened): 32 cycles for 4 of K, which stays below the time of the weights'
+// memory reads.
 template <typename TX, typename TW, uint32_t NT, uint32_t WK>
 RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     constexpr bool F32 = __is_same(TX, float);
@@ -493,22 +583,33 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     const uint32_t b0 = WK == 1 ? 0u : min(wave * each, blocks), b1 = WK == 1 ? blocks : min(b0 + each, blocks);
     const uint32_t p = t.beg + l;
     const int64_t src = p < t.end ? src_row(a, p) : -1;
-    const TX* x = reinterpret_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
+    const TX* x = static_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
     const TW* w[NT];
 #pragma unroll
     for (uint32_t f = 0; f < NT; f++)
         w[f] = reinterpret_cast<const TW*>(a.w) + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.k;
     f4v_t acc[NT] = {};
     u4_t wv[2][4][NT], xv[2][4][XV];
+    // blocks of 128 that are whole, without conditions; then the last values of K
     const auto load = [&](uint32_t s, uint32_t b) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            const uint32_t k = 128u * b + 32u * i + 8u * q;
+#pragma unroll
+            for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = ld16(w[f] + k);
+#pragma unroll
+            for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = ld16(x + k + 4u * v);
+        }
+    };
+    const auto load_tail = [&](uint32_t b) {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
             const uint32_t k = 128u * b + 32u * i + 8u * q;
             const bool have = k < a.k;
 #pragma unroll
-            for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = have ? ld16(w[f] + k) : u4_t{0, 0, 0, 0};
+            for (uint32_t f = 0; f < NT; f++) wv[0][i][f] = have ? ld16(w[f] + k) : u4_t{0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = have && src >= 0 ? ld16(x + k + 4u * v) : u4_t{0, 0, 0, 0};
+            for (uint32_t v = 0; v < XV; v++) xv[0][i][v] = have ? ld16(x + k + 4u * v) : u4_t{0, 0, 0, 0};
         }
     };
     const auto multiply = [&](uint32_t s) {
@@ -527,12 +628,17 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
                 }
             }
     };
-    if (b0 < b1) load(0, b0);
-    for (uint32_t b = b0; b < b1; b += 2u) {
-        if (b + 1u < b1) load(1, b + 1u);
+    const uint32_t whole = min(b1, a.k / 128u);
+    if (b0 < whole) load(0, b0);
+    for (uint32_t b = b0; b < whole; b += 2u) {
+        if (b + 1u < whole) load(1, b + 1u);
         multiply(0);
-        if (b + 2u < b1) load(0, b + 2u);
-        if (b + 1u < b1) multiply(1);
+        if (b + 2u < whole) load(0, b + 2u);
+        if (b + 1u < whole) multiply(1);
+    }
+    if (whole < b1 && b0 < b1) {
+        load_tail(b1 - 1u);
+        multiply(0);
     }
     mfma_settle();
     if constexpr (WK > 1) {
@@ -561,53 +667,3 @@ RFXQ_GROUPED_FEW(f16, half_t, half_t)
 RFXQ_GROUPED_FEW(bf16, __bf16, __bf16)
 RFXQ_GROUPED_FEW(f32_f16, float, half_t)
 RFXQ_GROUPED_FEW(f32_bf16, float, __bf16)
-
-// ---------------------------------------------------------------- f32 activations as pieces
-
-struct SplitArgs {
-    const float* x;
-    uint16_t* out;    // [pieces][rows][ldo]
-    int32_t* exp;     // the rows' exponents
-    uint64_t ldx, plane;
-    uint32_t rows, k, ldo, pad;
-};
-
-// A wave per row; columns k..ldo-1 are 0.
-template <bool F16>
-RFXQ_DEV void split_rows(const SplitArgs& a) {
-    const uint32_t lane = threadIdx.x & 63u;
-    for (uint32_t r = blockIdx.x * 4u + (threadIdx.x >> 6); r < a.rows; r += gridDim.x * 4u) {
-        const float* x = a.x + (uint64_t)r * a.ldx;
-        uint16_t* o = a.out + (uint64_t)r * a.ldo;
-        float top = 0.0f;  // of the finite values: infinities and NaN stay what they are
-        for (uint32_t i = lane; i < a.k; i += 64u) {
-            const float v = __builtin_fabsf(x[i]);
-            top = v < __builtin_inff() ? fmaxf(top, v) : top;
-        }
-        top = wave_max(top);
-        const int e = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;  // top / 2^e in [2^14, 2^15)
-        if (lane == 0) a.exp[r] = e;
-        for (uint32_t i = lane; i < a.ldo; i += 64u) {
-            const float s = i < a.k ? __builtin_ldexpf(x[i], -e) : 0.0f;
-            const bool fine = __builtin_fabsf(s) < __builtin_inff();
-            if (F16) {
-                const half_t hi = (half_t)s;
-                const half_t lo = fine ? (half_t)(s - (float)hi) : (half_t)0.0f;
-                o[i] = __builtin_bit_cast(uint16_t, hi);
-                o[a.plane + i] = __builtin_bit_cast(uint16_t, lo);
-            } else {
-                const uint32_t h = __builtin_bit_cast(uint32_t, s) & 0xFFFF0000u;
-                const float left = fine ? s - as_f32(h) : 0.0f;
-                const uint32_t m = __builtin_bit_cast(uint32_t, left) & 0xFFFF0000u;
-                const float last = left - as_f32(m);
-                // a NaN keeps a set fraction bit
-                o[i] = (uint16_t)(h >> 16 | (s != s ? 0x40u : 0u));
-                o[a.plane + i] = (uint16_t)(m >> 16);
-                o[2u * a.plane + i] = (uint16_t)(__builtin_bit_cast(uint32_t, last) >> 16);
-            }
-        }
-    }
-}
-
-extern "C" __global__ __launch_bounds__(256) void rfxq_split_f16(SplitArgs a) { split_rows<true>(a); }
-extern "C" __global__ __launch_bounds__(256) void rfxq_split_bf16(SplitArgs a) { split_rows<false>(a); }

@@ -28,22 +28,12 @@ struct GroupedArgs {
     const int32_t* offsets;
     const int32_t* x_index;
     const int32_t* y_index;
-    const int32_t* x_exp;
-    uint64_t ldx, ldy, plane, w_stride;
+    uint64_t ldx, ldy, w_stride;
     uint32_t rows, x_rows, y_rows, x_div;
-    uint32_t k, n, groups, pieces;
-    uint32_t y_f32, tiles_m, tiles_n, sm, sn, pad;
+    uint32_t k, n, groups, y_f32;
+    uint32_t tiles_m, tiles_n, sm, sn;
 };
-static_assert(sizeof(GroupedArgs) == 144, "GroupedArgs layout");
-
-struct SplitArgs {
-    const float* x;
-    void* out;
-    int32_t* exp;
-    uint64_t ldx, plane;
-    uint32_t rows, k, ldo, pad;
-};
-static_assert(sizeof(SplitArgs) == 56, "SplitArgs layout");
+static_assert(sizeof(GroupedArgs) == 120, "GroupedArgs layout");
 
 struct LoraArgs {
     const void* x;
@@ -149,21 +139,6 @@ GroupPlan group_plan(uint32_t n, uint32_t groups) {
 
 constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offsets reach
 
-// f32 activations in pieces of the weights' type: rows of whole 64-element steps
-struct Pieces {
-    uint32_t count, ld;
-    uint64_t plane, exp_at, total;
-};
-Pieces pieces_of(uint32_t ty, uint32_t rows, uint32_t k) {
-    Pieces p;
-    p.count = ty == RFXQ_TYPE_F16 ? 2u : 3u;
-    p.ld = (uint32_t)(((uint64_t)k + 63u) / 64u * 64u);
-    p.plane = (uint64_t)rows * p.ld;
-    p.exp_at = align256(p.plane * p.count * 2u);
-    p.total = p.exp_at + align256(4ull * rows);
-    return p;
-}
-
 // The kernel of a grouped product, by the mean rows of the groups that can have
 // any, measured with stacks of 128 matrices of 768 x 2048 and 2048 x 768 and of 8 of
 // 14336 x 4096 and 4096 x 14336 (N x K; us, bf16):
@@ -184,19 +159,21 @@ struct GroupedVariant {
     uint32_t bm, bn, threads;
     bool few;
 };
-GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool split_x, uint32_t rows, uint32_t groups, uint32_t k,
-                               uint32_t n, bool direct, bool copies) {
-    const uint32_t used = std::min(rows, groups), mean = rows / used, xt = split_x ? 0u : 1u;
+GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n,
+                               bool direct, bool copies) {
+    const uint32_t used = std::min(rows, groups), mean = rows / used, xt = f32 ? 0u : 1u;
     const uint64_t fill = 2ull * c->cus;
-    if (direct && mean <= (k < 1024u ? 2u : split_x ? 8u : 4u)) {
+    const char* env = getenv("RFXQ_TILE");
+    const int sel = env ? atoi(env) : -1;
+    if (direct && (sel >= 0 ? sel == 1 || sel == 4 : mean <= (k < 1024u ? 2u : f32 ? 8u : 4u))) {
         // a wave's columns over all of K, unless that leaves CUs without work or long K
         // to one wave (128 x 768 x 2048, 8 rows in 8 groups: 20 against 8 us)
-        if (k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
+        if (sel >= 0 ? sel == 1 : k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
         return {c->half.few4[xt][t], 16, 16, 256, true};
     }
-    if (copies && mean > (split_x ? 512u : 160u)) return {c->half.t256[t], 256, 256, 512, false};
-    if (copies && mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill)
-        return {c->half.t64[xt][t], 64, 128, 256, false};
+    if (copies && (sel >= 0 ? sel == 256 : mean > 160u)) return {c->half.t256[t], 256, 256, 512, false};
+    if (copies && (sel >= 0 ? sel == 64 : mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill))
+        return {c->half.t64[t], 64, 128, 256, false};
     return {c->half.any[xt][t], 64, 128, 256, false};
 }
 
@@ -262,14 +239,9 @@ int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* of
     return ok();
 }
 
-uint64_t rfxq_grouped_gemm_workspace_size(const rfxq_weight* w, uint32_t x_rows, uint32_t x_type) {
-    if (!w || x_type != RFXQ_TYPE_F32 || !half_type(w->ggml_type) || x_rows == 0) return 0;
-    return pieces_of(w->ggml_type, x_rows, w->in_features).total;
-}
-
 int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
                       const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
-                      void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+                      hipStream_t stream) {
     if (int rc = check_stack(w, false, "grouped_gemm")) return rc;
     if (int rc = check_rows(x, w->in_features, "grouped_gemm", "x")) return rc;
     if (int rc = check_rows(y, w->out_features, "grouped_gemm", "y")) return rc;
@@ -308,40 +280,24 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.k = k;
     a.n = n;
     a.groups = groups;
-    a.pieces = 1;
     a.y_f32 = y->type == RFXQ_TYPE_F32 ? 1u : 0u;
     // asynchronous copies: rows at whole 16 bytes, 32-bit offsets
-    const bool split_x = x->type == RFXQ_TYPE_F32;
-    const Pieces p = split_x ? pieces_of(ty, x->rows, k) : Pieces{};
-    const uint64_t xb = split_x ? 2u * p.plane * p.count : rows_span(x, k);
-    const bool copies = (split_x || (aligned16(x->data) && x->stride % 8u == 0)) && aligned16(w->data) && k % 8u == 0 &&
-                        xb < kMaxOffset && 2ull * k * n < kMaxOffset;
-    const bool direct = aligned16(x->data) && x->stride % (split_x ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
-    const GroupedVariant v = grouped_variant(c, t, split_x, rows, groups, k, n, direct, copies);
+    const bool f32 = x->type == RFXQ_TYPE_F32;
+    const bool direct = aligned16(x->data) && x->stride % (f32 ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
+    // asynchronous copies: 32-bit offsets
+    const bool copies = direct && !f32 && rows_span(x, k) < kMaxOffset && 2ull * k * n < kMaxOffset;
+    const GroupedVariant v = grouped_variant(c, t, f32, rows, groups, k, n, direct, copies);
     a.tiles_m = max_tiles(rows, groups, v.bm);
     a.tiles_n = (n + v.bn - 1u) / v.bn;
+    // XCD blocks of 4 row tiles and up to 4 column tiles, evenly cut
+    const uint32_t across = (a.tiles_n + 3u) / 4u;
     a.sm = 4;
-    a.sn = 8;
+    a.sn = (a.tiles_n + across - 1u) / across;
     const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
     const uint64_t grid = v.few ? (uint64_t)a.tiles_m * a.tiles_n : (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid > 0x7FFFFFFFull)
         return fail(RFXQ_ERR_OTHER, "grouped_gemm: %u rows x %u columns need %llu workgroups", rows, n,
                     (unsigned long long)grid);
-    if (split_x && !v.few) {
-        void* ws = nullptr;
-        if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "grouped_gemm", &ws)) return rc;
-        uint8_t* base = static_cast<uint8_t*>(ws);
-        int32_t* exp = reinterpret_cast<int32_t*>(base + p.exp_at);
-        SplitArgs s = {static_cast<const float*>(x->data), ws, exp, x->stride, p.plane, x->rows, k, p.ld, 0};
-        if (int rc = launch(c->half.split[t], std::min((x->rows + 3u) / 4u, 16384u), 0, stream, &s, sizeof s,
-                            "rfxq_split launch"))
-            return rc;
-        a.x = ws;
-        a.ldx = p.ld;
-        a.plane = p.plane;
-        a.pieces = p.count;
-        a.x_exp = exp;
-    }
     if (int rc = launch(v.f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch", v.threads)) return rc;
     return ok();
 }

@@ -38,50 +38,6 @@ struct LoraArgs {
     uint32_t k_split, tiles, across, pad;
 };
 
-// Vectors that may start at any element.
-typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
-
-// 8 neighbouring values of a row as they lie in memory.
-template <typename T>
-struct Eight {
-    u4_t v;
-    __device__ __forceinline__ float at(uint32_t j) const {
-        if constexpr (__is_same(T, half_t))
-            return (float)__builtin_bit_cast(h8_t, v)[j];
-        else
-            return (float)__builtin_bit_cast(b8_t, v)[j];
-    }
-};
-template <>
-struct Eight<float> {
-    f4v_t v[2];
-    __device__ __forceinline__ float at(uint32_t j) const { return v[j >> 2][j & 3u]; }
-};
-
-// The 8 values at p.
-template <typename T>
-RFXQ_DEV Eight<T> ld_eight(const T* p) {
-    Eight<T> r;
-    if constexpr (__is_same(T, float)) {
-        r.v[0] = *(const RFXQ_GLOBAL f4a4_t*)p;
-        r.v[1] = *(const RFXQ_GLOBAL f4a4_t*)(p + 4);
-    } else {
-        r.v = *(const RFXQ_GLOBAL u4a2_t*)p;
-    }
-    return r;
-}
-// The first `have` of the 8 values at p, one by one, then zeros.
-template <typename T>
-RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have) {
-    if (have >= 8u) return ld_eight(p);
-    T t[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) t[i] = i < have ? ((const RFXQ_GLOBAL T*)p)[i] : (T)0.0f;
-    Eight<T> r;
-    __builtin_memcpy(&r, t, sizeof t);
-    return r;
-}
-
 // 4 neighbouring values of a row as they lie in memory, at any element.
 template <typename T>
 struct FourOf {
@@ -127,42 +83,6 @@ RFXQ_DEV Eight<T> first_of(Eight<T> r, uint32_t have) {
         for (uint32_t i = 0; i < 4u; i++) r.v[i] &= have > 2u * i + 1u ? 0xFFFFFFFFu : have > 2u * i ? 0xFFFFu : 0u;
     }
     return r;
-}
-
-// f32 values of a step as pieces of T, times 2^e (the scale's exponent)
-template <typename T, uint32_t NP>
-RFXQ_DEV void split_eight(const Eight<float>& x, float scale, u4_t (&out)[NP]) {
-    float left[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) left[i] = x.at(i) * scale;
-#pragma unroll
-    for (uint32_t n = 0; n < NP; n++)
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) {
-            const T a = (T)left[2 * i], b = (T)left[2 * i + 1];
-            out[n][i] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
-            left[2 * i] -= (float)a;
-            left[2 * i + 1] -= (float)b;
-        }
-}
-// The exponent e at which `top` is 2^e times a value in [2^14, 2^15), kept so that 2^e and 2^-e are f32 values
-RFXQ_DEV int step_exp(float top) { return max(__builtin_amdgcn_frexp_expf(top) - 15, -126); }
-RFXQ_DEV float pow2(int e) { return as_f32((uint32_t)(e + 127) << 23); }
-
-// the largest of the four lanes (l, 0..3)
-RFXQ_DEV float max_over_q(float v) {
-    uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-    v = fmaxf(as_f32(r[0]), as_f32(r[1]));
-    b = __builtin_bit_cast(uint32_t, v);
-    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(as_f32(s[0]), as_f32(s[1]));
-}
-RFXQ_DEV float max_of_eight(const Eight<float>& x) {
-    float t = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) t = fmaxf(t, __builtin_fabsf(x.at(i)));
-    return t;
 }
 
 RFXQ_DEV uint32_t lora_rank(const LoraArgs& a, uint32_t g) {

@@ -148,9 +148,8 @@ constexpr uint32_t kNormRowsPerWg = 4;  // rows per rfxq_rmsnorm_q8_1 workgroup 
 // kernels of the second code object (half_host.hpp)
 struct HalfKernels {
     hipFunction_t group_rows = nullptr, group_count = nullptr;
-    // [f32 activations, the weights' type][F16, BF16]
-    hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {}, t64[2][2] = {};
-    hipFunction_t t256[2] = {}, split[2] = {};  // halves, one piece of K after another
+    hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {};  // [f32 activations, the weights' type][F16, BF16]
+    hipFunction_t t64[2] = {}, t256[2] = {};                       // activations of the weights' type
     // [f32 x F32, f32 x F16, f32 x BF16, F16, BF16]
     hipFunction_t lora_down[5][2] = {}, lora_up[5][3] = {};  // [16, 32 rows, 16 rows of any rank and columns]
 };
@@ -222,14 +221,10 @@ int load_half(hipModule_t mod, HalfKernels* h) {
         {&h->few4[0][1], "rfxq_grouped_few4_f32_bf16"},
         {&h->few4[1][0], "rfxq_grouped_few4_f16"},
         {&h->few4[1][1], "rfxq_grouped_few4_bf16"},
-        {&h->t64[0][0], "rfxq_grouped_64_f32_f16"},
-        {&h->t64[0][1], "rfxq_grouped_64_f32_bf16"},
-        {&h->t64[1][0], "rfxq_grouped_64_f16"},
-        {&h->t64[1][1], "rfxq_grouped_64_bf16"},
+        {&h->t64[0], "rfxq_grouped_64_f16"},
+        {&h->t64[1], "rfxq_grouped_64_bf16"},
         {&h->t256[0], "rfxq_grouped_256_f16"},
         {&h->t256[1], "rfxq_grouped_256_bf16"},
-        {&h->split[0], "rfxq_split_f16"},
-        {&h->split[1], "rfxq_split_bf16"},
     };
     for (auto& f : fns) {
         hipError_t e = hipModuleGetFunction(f.f, mod, f.name);

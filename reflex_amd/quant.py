@@ -29,7 +29,7 @@ __all__ = [
     "moe_route_device", "moe_ffn_grouped_device",
     "act_q8_1_size", "quantize_act_q8_1", "rmsnorm_q8_1", "silu_and_mul_q8_1", "gemm_q8_1", "gemm_q8_1_batch",
     "gemm_gate_up_silu_q8_1",
-    "RowGroups", "group_rows", "group_rows_workspace_size", "grouped_gemm", "grouped_gemm_workspace_size", "lora_add", "lora_add_workspace_size",
+    "RowGroups", "group_rows", "group_rows_workspace_size", "grouped_gemm", "lora_add", "lora_add_workspace_size",
     "get_options", "set_options", "options", "gemm_policy", "PATH_GEMV_ROWS", "PATH_MMQ_INT8", "PATH_MMQ_F16",
 ]
 
@@ -694,14 +694,8 @@ def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None,
     return out
 
 
-def grouped_gemm_workspace_size(w: Weight, x_rows: int, dtype: torch.dtype) -> int:
-    """Bytes of workspace ``grouped_gemm`` needs for x of this many rows and type."""
-    return int(lib().rfxq_grouped_gemm_workspace_size(w.cref(), x_rows, _ROW_TYPES[dtype]))
-
-
 def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
-                 x_div: int = 1, y_index: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                 workspace: torch.Tensor | None = None) -> torch.Tensor:
+                 x_div: int = 1, y_index: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Products of grouped rows with a stack of F16 / BF16 matrices: for the places p of group g,
     ``out[y_index[p]] = x[x_index[p] // x_div] @ W[g].T`` (either index may be left out: place p itself).
     The counterpart of ``expert_gemm`` for all experts at once. Without ``out``, a new tensor of x's type with
@@ -714,11 +708,10 @@ def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x
     xr = _rows(x, c.in_features, dev, "grouped_gemm x")
     y = out if out is not None else torch.zeros(rows, c.out_features, dtype=x.dtype, device=x.device)
     yr = _rows(y, c.out_features, dev, "grouped_gemm out")
-    space, size = _space(workspace, dev, "grouped_gemm")
     with _dev(x):
         _check(lib().rfxq_grouped_gemm(xr, c, _ints(offsets, count + 1, dev, "grouped_gemm offsets"), rows,
                                        _ints(x_index, rows, dev, "grouped_gemm x_index"), x_div,
-                                       _ints(y_index, rows, dev, "grouped_gemm y_index"), yr, space, size, _stream()))
+                                       _ints(y_index, rows, dev, "grouped_gemm y_index"), yr, _stream()))
     return y
 
 

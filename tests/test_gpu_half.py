@@ -5,9 +5,9 @@ Bounds, per result: a half-typed output is off by half a step, eps / 2 of its va
 held in f32 by at most 2^-23 of the sum of the products' sizes per addition, with K / 32 + 32 additions in
 a row (the matrix instructions add 32 products, or 4 of f32 operands, to the sum at once; parts of a sum that are
 added later are counted in). f32 activations beside f16 weights are split into two f16 pieces, which leave
-2^-22 of a value (half a step of the second piece, 2^-11 of 2^-11) and 2^-39 of its row's largest (half a
-step of f16's smallest number, 2^-25, at a largest of 2^14 or more); beside bf16 weights three pieces are
-exact but for what is below f32's range. A value below f32's or f16's normal range keeps an absolute step."""
+2^-22 of a value (half a step of the second piece, 2^-11 of 2^-11) and 2^-39 of the largest of its row or of
+its step of the row (half a step of f16's smallest number, 2^-25, at a largest of 2^14 or more); beside bf16
+weights three pieces are exact but for what is below f32's range. A value below f32's or f16's normal range keeps an absolute step."""
 import numpy as np
 import pytest
 import torch
@@ -119,8 +119,7 @@ def _case(rows, groups, k, n, x_type, w_type, seed, x_rows=None):
     return x.to(x_type), w
 
 
-def _run_grouped(rq, x, w, offsets, rows, x_index, x_div, y_index, y_type, y_rows, xs=(0, 0), ys=(0, 0), ws=0,
-                 workspace=None):
+def _run_grouped(rq, x, w, offsets, rows, x_index, x_div, y_index, y_type, y_rows, xs=(0, 0), ys=(0, 0), ws=0):
     """grouped_gemm on strided and shifted copies: (y, what lies around y unchanged)."""
     k, n = x.shape[1], w.shape[1]
     xv, _ = _strided(x.to(DEV), k + xs[0], xs[1], float("nan"))
@@ -129,8 +128,7 @@ def _run_grouped(rq, x, w, offsets, rows, x_index, x_div, y_index, y_type, y_row
     wmem[ws:ws + w.numel()] = w.reshape(-1).to(DEV)
     weight = rq.Weight.from_tensor(wmem[ws:ws + w.numel()].view(w.shape))
     dev = lambda v: None if v is None else torch.from_numpy(np.asarray(v, np.int32)).to(DEV)  # noqa: E731
-    rq.grouped_gemm(xv, weight, dev(offsets), rows, x_index=dev(x_index), x_div=x_div, y_index=dev(y_index), out=yv,
-                    workspace=workspace)
+    rq.grouped_gemm(xv, weight, dev(offsets), rows, x_index=dev(x_index), x_div=x_div, y_index=dev(y_index), out=yv)
     torch.cuda.synchronize()
     around = ymem.clone()
     around[ys[1]:ys[1] + y_rows * (n + ys[0])].view(y_rows, -1)[:, :n] = 99.0
@@ -295,19 +293,14 @@ def test_grouped_gemm_not_finite_rows(rq, w_type, k):
         assert (np.abs(y[r].double().numpy() - want[r]) <= b).all(), r
 
 
-def test_grouped_gemm_own_workspace_and_2d_weight(rq):
+def test_grouped_gemm_2d_weight_and_new_output(rq):
     x, w = _case(50, 1, 100, 40, F32, F16, 2)
     weight = rq.Weight.from_tensor(w[0].contiguous().to(DEV))
-    size = rq.grouped_gemm_workspace_size(weight, 50, F32)
-    ws = torch.full((size + 64,), 7, dtype=torch.uint8, device=DEV)
-    offsets = torch.tensor([0, 50], dtype=torch.int32, device=DEV)
-    y = rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[:size])
-    _check_grouped(x, w, [0, 50], None, 1, None, y.cpu())
-    assert (ws[size:] == 7).all()
-    with pytest.raises(rq.InvalidInputError, match="needs"):
-        rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[:size - 1])
-    with pytest.raises(rq.ReflexError, match="16-byte aligned"):
-        rq.grouped_gemm(x.to(DEV), weight, offsets, 50, workspace=ws[8:])
+    offsets = torch.tensor([0, 47], dtype=torch.int32, device=DEV)
+    y = rq.grouped_gemm(x.to(DEV), weight, offsets, 50).cpu()
+    assert (y[47:] == 0).all()
+    y[47:] = 123.0
+    _check_grouped(x, w, [0, 47], None, 1, None, y)
 
 
 # ------------------------------------------------------------------ lora_add
@@ -488,8 +481,6 @@ def test_captured_and_replayed(rq):
     xd, ld, ids = x.to(DEV), logits.to(DEV), torch.empty(pairs, dtype=torch.int32, device=DEV)
     g = rq.RowGroups(torch.empty(groups + 1, dtype=torch.int32, device=DEV), torch.empty_like(ids))
     gate, y = (torch.empty(pairs, m, device=DEV) for m in (ffn, hidden))
-    ws = torch.empty(max(rq.grouped_gemm_workspace_size(weights[0], tokens, F32),
-                         rq.grouped_gemm_workspace_size(weights[2], pairs, F32)), dtype=torch.uint8, device=DEV)
     a = rq.Weight.from_tensor((torch.randn(groups, 5, ffn) * 0.1).half().to(DEV))
     b = rq.Weight.from_tensor((torch.randn(groups, hidden, 5) * 0.1).half().to(DEV))
     lws = torch.empty(rq.lora_add_workspace_size(a, pairs), dtype=torch.uint8, device=DEV)
@@ -497,8 +488,8 @@ def test_captured_and_replayed(rq):
     def step():
         ids.copy_(ld.topk(top_k, dim=1).indices.reshape(-1))
         rq.group_rows(ids, groups, out=g)
-        rq.grouped_gemm(xd, weights[0], g.offsets, pairs, x_index=g.order, x_div=top_k, out=gate, workspace=ws)
-        rq.grouped_gemm(gate, weights[2], g.offsets, pairs, y_index=g.order, out=y, workspace=ws)
+        rq.grouped_gemm(xd, weights[0], g.offsets, pairs, x_index=g.order, x_div=top_k, out=gate)
+        rq.grouped_gemm(gate, weights[2], g.offsets, pairs, y_index=g.order, out=y)
         rq.lora_add(gate, a, b, g, y, workspace=lws)
         return y
 
