@@ -163,16 +163,14 @@ GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows
                                bool direct, bool copies) {
     const uint32_t used = std::min(rows, groups), mean = rows / used, xt = f32 ? 0u : 1u;
     const uint64_t fill = 2ull * c->cus;
-    const char* env = getenv("RFXQ_TILE");
-    const int sel = env ? atoi(env) : -1;
-    if (direct && (sel >= 0 ? sel == 1 || sel == 4 : mean <= (k < 1024u ? 2u : f32 ? 8u : 4u))) {
+    if (direct && mean <= (k < 1024u ? 2u : f32 ? 8u : 4u)) {
         // a wave's columns over all of K, unless that leaves CUs without work or long K
         // to one wave (128 x 768 x 2048, 8 rows in 8 groups: 20 against 8 us)
-        if (sel >= 0 ? sel == 1 : k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
+        if (k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
         return {c->half.few4[xt][t], 16, 16, 256, true};
     }
-    if (copies && (sel >= 0 ? sel == 256 : mean > 160u)) return {c->half.t256[t], 256, 256, 512, false};
-    if (copies && (sel >= 0 ? sel == 64 : mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill))
+    if (copies && mean > 160u) return {c->half.t256[t], 256, 256, 512, false};
+    if (copies && mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill)
         return {c->half.t64[t], 64, 128, 256, false};
     return {c->half.any[xt][t], 64, 128, 256, false};
 }
@@ -193,8 +191,7 @@ LoraPlan lora_plan(uint32_t k, uint32_t n, uint32_t rank, uint32_t groups, uint3
     p.ldv = (rank + 15u) & ~15u;
     p.bm = rows / std::min(rows, groups) > 16u && rank <= 256u && lora_vec(rank, n) ? 32u : 16u;
     p.tiles = max_tiles(rows, groups, p.bm);
-    const uint32_t fill = getenv("RFXQ_FILL") ? atoi(getenv("RFXQ_FILL")) : 2;
-    const uint32_t want = (fill * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
+    const uint32_t want = (2u * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
     p.splits = std::max(1u, std::min({want, most, 32u}));
     p.k_split = ((k + p.splits - 1u) / p.splits + 127u) & ~127u;
     p.splits = (k + p.k_split - 1u) / p.k_split;
@@ -341,9 +338,9 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
     const LoraPlan p = lora_plan(k, n, rank, groups, rows, (uint32_t)c->cus);
-    // strips of 32 columns shared by as many workgroups as fill the CUs (4 of a CU's waves each)
-    const uint32_t fillu = getenv("RFXQ_FILLU") ? atoi(getenv("RFXQ_FILLU")) : 4;
-    const uint32_t across = std::max(1u, std::min((fillu * (uint32_t)c->cus + p.tiles - 1u) / p.tiles, (n + 127u) / 128u));
+    // a tile's strips of 32 columns are shared by as many workgroups as give 8 a CU (4096 rows of 4096
+    // columns, rank 64: 61.7 us; 4 a CU: 66, 2: 68)
+    const uint32_t across = std::max(1u, std::min((8u * (uint32_t)c->cus + p.tiles - 1u) / p.tiles, (n + 127u) / 128u));
     const uint64_t up = (uint64_t)(p.tiles + 1u) * across;
     if (up > 0x7FFFFFFFull || (uint64_t)p.tiles * p.splits > 0x7FFFFFFFull)
         return fail(RFXQ_ERR_OTHER, "lora_add: %u rows need %llu workgroups", rows, (unsigned long long)up);
@@ -387,3 +384,91 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
 }
 
 }  // extern "C"
+
+namespace {
+
+bool half_layer(const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down) {
+    return gate && up && down && half_type(gate->ggml_type) && half_type(up->ggml_type) && half_type(down->ggml_type);
+}
+
+// rfxq_moe_ffn_grouped(_device) over F16 or BF16 stacks: the routing (from the
+// device's logits, or the host's, copied up), rfxq_group_rows, three grouped
+// products of f32 activations and the combine in increasing expert order.
+int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits, const uint32_t* host_idx,
+             const float* host_w, uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
+             const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out, hipStream_t stream) {
+    if (!x || !out) return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped: NULL argument");
+    if (rows == 0) return ok();
+    if (gate->expert_count != expert_count || up->expert_count != expert_count || down->expert_count != expert_count)
+        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: expert tensors must have expert_count=%u", expert_count);
+    if (gate->in_features != hidden || up->in_features != hidden || down->out_features != hidden ||
+        gate->out_features != up->out_features || down->in_features != gate->out_features)
+        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: shapes gate [%u,%u] up [%u,%u] down [%u,%u] hidden %u",
+                    gate->in_features, gate->out_features, up->in_features, up->out_features, down->in_features,
+                    down->out_features, hidden);
+    if (expert_count == 0 || expert_count > kRouteMaxE)
+        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: expert_count=%u (1..=%u)", expert_count, kRouteMaxE);
+    if (top_k == 0 || top_k > expert_count || top_k > 64u)
+        return fail(RFXQ_ERR_OTHER, "route_top_k: k (%u) must be in 1..=%u (logits.len())", top_k,
+                    std::min(expert_count, 64u));
+    if (int rc = check_stack(gate, false, "moe_ffn_grouped gate")) return rc;
+    if (int rc = check_stack(up, false, "moe_ffn_grouped up")) return rc;
+    if (int rc = check_stack(down, false, "moe_ffn_grouped down")) return rc;
+    const uint64_t P64 = (uint64_t)rows * top_k;
+    if (P64 > kMaxGroupRows)
+        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: %llu routed pairs (at most %u)", (unsigned long long)P64,
+                    kMaxGroupRows);
+    const uint32_t P = (uint32_t)P64, ffn = gate->out_features;
+    if (overlap(x, 4ull * rows * hidden, out, 4ull * rows * hidden))
+        return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped: x and out overlap");
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    const uint64_t pairs = align256(4ull * P), wide = align256(4ull * P * ffn);
+    const uint64_t o_w = pairs, o_order = o_w + pairs, o_pair = o_order + pairs, o_pair_w = o_pair + pairs;
+    const uint64_t o_off = o_pair_w + pairs, o_cnt = o_off + align256(4ull * (expert_count + 1u));
+    const uint64_t cnt = rfxq_group_rows_workspace_size(P, expert_count);
+    const uint64_t o_gate = o_cnt + cnt, o_up = o_gate + wide, o_s = o_up + wide, o_down = o_s + wide;
+    void* ws;
+    if (int rc = ctx_workspace(c, o_down + align256(4ull * P * hidden), &ws, stream)) return rc;
+    uint8_t* base = static_cast<uint8_t*>(ws);
+    int32_t* idx = reinterpret_cast<int32_t*>(base);
+    float* w = reinterpret_cast<float*>(base + o_w);
+    int32_t* order = reinterpret_cast<int32_t*>(base + o_order);
+    int32_t* pair = reinterpret_cast<int32_t*>(base + o_pair);
+    float* pair_w = reinterpret_cast<float*>(base + o_pair_w);
+    int32_t* offsets = reinterpret_cast<int32_t*>(base + o_off);
+    float* g = reinterpret_cast<float*>(base + o_gate);
+    float* u = reinterpret_cast<float*>(base + o_up);
+    float* inner = reinterpret_cast<float*>(base + o_s);
+    float* d = reinterpret_cast<float*>(base + o_down);
+    if (router_logits) {
+        if (int rc = moe_route_launch(c, router_logits, rows, expert_count, top_k, normalize, weight_scale, idx, w, nullptr,
+                                      0, nullptr, nullptr, nullptr, stream))
+            return rc;
+    } else {
+        if (int rc = stage_upload(c, idx, host_idx, 4ull * P, stream)) return rc;
+        if (int rc = stage_upload(c, w, host_w, 4ull * P, stream)) return rc;
+    }
+    if (int rc = rfxq_group_rows(idx, P, expert_count, offsets, order, cnt ? base + o_cnt : nullptr, cnt, stream)) return rc;
+    const rfxq_rows xr = {const_cast<float*>(x), RFXQ_TYPE_F32, rows, hidden};
+    const rfxq_rows gr = {g, RFXQ_TYPE_F32, P, ffn}, ur = {u, RFXQ_TYPE_F32, P, ffn}, sr = {inner, RFXQ_TYPE_F32, P, ffn};
+    const rfxq_rows dr = {d, RFXQ_TYPE_F32, P, hidden};
+    if (int rc = rfxq_grouped_gemm(&xr, gate, offsets, P, order, top_k, nullptr, &gr, stream)) return rc;
+    if (int rc = rfxq_grouped_gemm(&xr, up, offsets, P, order, top_k, nullptr, &ur, stream)) return rc;
+    if (int rc = rfxq_silu_and_mul(g, u, inner, (uint64_t)P * ffn, stream)) return rc;
+    if (int rc = rfxq_grouped_gemm(&sr, down, offsets, P, nullptr, 1, order, &dr, stream)) return rc;
+    struct {
+        const int32_t* ids;
+        const float* w;
+        int32_t* pair;
+        float* pair_w;
+        uint32_t pairs, k;
+    } a = {idx, w, pair, pair_w, P, top_k};
+    if (int rc = launch(c->half.moe_order, std::min((P + 255u) / 256u, 16384u), 0, stream, &a, sizeof a,
+                        "rfxq_moe_order launch"))
+        return rc;
+    if (int rc = launch_combine(c, d, pair, pair_w, out, rows, top_k, hidden, stream)) return rc;
+    return ok();
+}
+
+}  // namespace

@@ -147,7 +147,7 @@ constexpr uint32_t kNormRowsPerWg = 4;  // rows per rfxq_rmsnorm_q8_1 workgroup 
 
 // kernels of the second code object (half_host.hpp)
 struct HalfKernels {
-    hipFunction_t group_rows = nullptr, group_count = nullptr;
+    hipFunction_t group_rows = nullptr, group_count = nullptr, moe_order = nullptr;
     hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {};  // [f32 activations, the weights' type][F16, BF16]
     hipFunction_t t64[2] = {}, t256[2] = {};                       // activations of the weights' type
     // [f32 x F32, f32 x F16, f32 x BF16, F16, BF16]
@@ -209,6 +209,7 @@ int load_half(hipModule_t mod, HalfKernels* h) {
     } fns[] = {
         {&h->group_rows, "rfxq_group_rows"},
         {&h->group_count, "rfxq_group_count"},
+        {&h->moe_order, "rfxq_moe_order"},
         {&h->any[0][0], "rfxq_grouped_any_f32_f16"},
         {&h->any[0][1], "rfxq_grouped_any_f32_bf16"},
         {&h->any[1][0], "rfxq_grouped_any_f16"},
@@ -2973,6 +2974,11 @@ int moe_grouped_device(const float* x, uint32_t rows, uint32_t hidden, const flo
                        const uint32_t* host_idx, const float* host_w, uint32_t expert_count, uint32_t top_k,
                        int normalize, float weight_scale, const rfxq_weight* gate, const rfxq_weight* up,
                        const rfxq_weight* down, float* out, hipStream_t stream);
+// the same layer with F16 or BF16 stacks (half_host.hpp)
+bool half_layer(const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down);
+int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits, const uint32_t* host_idx,
+             const float* host_w, uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
+             const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out, hipStream_t stream);
 }  // namespace
 
 extern "C" {
@@ -2992,13 +2998,16 @@ int rfxq_moe_ffn_grouped(const float* x, uint32_t rows, uint32_t hidden, const f
                     gate->in_features, gate->out_features, up->in_features, up->out_features, down->in_features,
                     down->out_features, hidden);
     const uint32_t ffn = gate->out_features;
+    const bool half = half_layer(gate, up, down);
     rfxq_weight g0, u0, d0;
     if (int rc = expert_slice(gate, 0, &g0, "moe_ffn_grouped gate")) return rc;
     if (int rc = expert_slice(up, 0, &u0, "moe_ffn_grouped up")) return rc;
     if (int rc = expert_slice(down, 0, &d0, "moe_ffn_grouped down")) return rc;
-    if (int rc = check_mmq_weight(&g0, "moe_ffn_grouped gate")) return rc;
-    if (int rc = check_mmq_weight(&u0, "moe_ffn_grouped up")) return rc;
-    if (int rc = check_mmq_weight(&d0, "moe_ffn_grouped down")) return rc;
+    if (!half) {
+        if (int rc = check_mmq_weight(&g0, "moe_ffn_grouped gate")) return rc;
+        if (int rc = check_mmq_weight(&u0, "moe_ffn_grouped up")) return rc;
+        if (int rc = check_mmq_weight(&d0, "moe_ffn_grouped down")) return rc;
+    }
     if (gate->ggml_type != up->ggml_type)
         return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: gate and up must share a type");
     if (reinterpret_cast<uintptr_t>(x) % 16u) return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: x not 16-byte aligned");
@@ -3021,6 +3030,11 @@ int rfxq_moe_ffn_grouped(const float* x, uint32_t rows, uint32_t hidden, const f
     if (bad >= 0)
         return route_top_k(router_logits_host + (uint64_t)bad * expert_count, expert_count, top_k, normalize != 0,
                            ridx.data() + (uint64_t)bad * top_k, rwts.data() + (uint64_t)bad * top_k);
+    if (half) {
+        for (float& w : rwts) w *= weight_scale;
+        return moe_half(x, rows, hidden, nullptr, ridx.data(), rwts.data(), expert_count, top_k, normalize, weight_scale,
+                        gate, up, down, out, stream);
+    }
     // grouping by expert, tokens in order (a counting sort)
     const uint32_t P = rows * top_k;
     std::vector<uint32_t> off(expert_count + 1, 0), fill(rows, 0);
@@ -3276,6 +3290,9 @@ int rfxq_moe_ffn_grouped_device(const float* x, uint32_t rows, uint32_t hidden, 
                                 const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out,
                                 hipStream_t stream) {
     if (!router_logits) return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped_device: NULL argument");
+    if (half_layer(gate, up, down))
+        return moe_half(x, rows, hidden, router_logits, nullptr, nullptr, expert_count, top_k, normalize, weight_scale,
+                        gate, up, down, out, stream);
     return moe_grouped_device(x, rows, hidden, router_logits, nullptr, nullptr, expert_count, top_k, normalize,
                               weight_scale, gate, up, down, out, stream);
 }

@@ -219,3 +219,20 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
         if (i < a.n) a.order[before[key[r]] + wcnt[wave * keys + key[r]] + rank[r]] = (int32_t)i;
     }
 }
+
+// A token's pairs in increasing expert order, as rfxq_moe_combine adds them
+// up: ids and weights [tokens][k] in selection order -> pair numbers and
+// weights. A pair's place is the number of those before it (equal ids by their
+// place, so that the places are a permutation for any ids).
+extern "C" __global__ __launch_bounds__(256) void rfxq_moe_order(const int32_t* __restrict__ ids,
+                                                                const float* __restrict__ w, int32_t* __restrict__ pair,
+                                                                float* __restrict__ pair_w, uint32_t pairs, uint32_t k) {
+    for (uint32_t p = blockIdx.x * 256u + threadIdx.x; p < pairs; p += gridDim.x * 256u) {
+        const uint32_t first = p - p % k;
+        const int32_t mine = ids[p];
+        uint32_t at = first;
+        for (uint32_t j = first; j < first + k; j++) at += ids[j] < mine || (ids[j] == mine && j < p) ? 1u : 0u;
+        pair[at] = (int32_t)p;
+        pair_w[at] = w[p];
+    }
+}

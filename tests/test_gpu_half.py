@@ -472,6 +472,71 @@ def test_expert_layer_and_adapters(rq, tokens, w_type):
     _check_lora(out.cpu(), a, b, adapter, None, scales, base, y.cpu())
 
 
+@pytest.mark.parametrize("gate_type,down_type", [(F16, F16), (BF16, BF16), (F16, BF16)])
+@pytest.mark.parametrize("tokens,groups,hidden,ffn,top_k", [(1, 8, 128, 96, 2), (5, 3, 100, 77, 3), (64, 16, 256, 192, 4),
+                                                            (300, 12, 264, 160, 5)])
+def test_moe_ffn_grouped_half_stacks(rq, tokens, groups, hidden, ffn, top_k, gate_type, down_type):
+    """The library's own expert layer over F16 / BF16 stacks, routed on the device and on the host.
+    Within 2^-17 of 64 bits in norm (see test_expert_layer_and_adapters)."""
+    _say("moe_ffn_grouped half", tokens, groups, hidden, ffn, top_k, gate_type, down_type)
+    x, logits, w = _layer_inputs(tokens, groups, hidden, ffn, gate_type, tokens)
+    w[2] = w[2].to(down_type)
+    weights = [rq.Weight.from_tensor(t.to(DEV)) for t in w]
+    xd, ld = x.to(DEV).reshape(-1), logits.to(DEV).reshape(-1)
+    ids, share = rq.moe_route_device(ld, tokens, groups, top_k, True, 1.5)
+    want = _layer_64(x, ids.cpu(), share.cpu(), w)
+    out = torch.full((tokens * hidden,), float("nan"), device=DEV)
+    rq.moe_ffn_grouped_device(xd, tokens, hidden, ld, groups, top_k, True, 1.5, *weights, out)
+    first = out.cpu()
+    assert (first.view(tokens, hidden).double() - want).norm() <= 2.0 ** -17 * want.norm()
+    out.fill_(float("nan"))
+    rq.moe_ffn_grouped_device(xd, tokens, hidden, ld, groups, top_k, True, 1.5, *weights, out)
+    assert torch.equal(out.cpu(), first)
+    out.fill_(float("nan"))
+    rq.moe_ffn_grouped(xd, tokens, hidden, logits.numpy(), groups, top_k, True, 1.5, *weights, out)
+    assert (out.cpu().view(tokens, hidden).double() - want).norm() <= 2.0 ** -17 * want.norm()
+
+
+def test_moe_ffn_grouped_half_refusals(rq):
+    x, logits, w = _layer_inputs(4, 4, 64, 48, F16, 1)
+    g, u, d = (rq.Weight.from_tensor(t.to(DEV)) for t in w)
+    q = rq.Weight.from_blocks(12, np.zeros(4 * 256 * 144, np.uint8), 256, 256, expert_count=4, device=DEV)
+    xd, ld, out = x.to(DEV), logits.to(DEV), torch.empty(4 * 64, device=DEV)
+    run = lambda *a, k=2, o=out: rq.moe_ffn_grouped_device(xd, 4, 64, ld, 4, k, True, 1.0, *a, o)  # noqa: E731
+    with pytest.raises(rq.ReflexError, match="shapes"):
+        run(g, u, u)
+    with pytest.raises(rq.ReflexError, match="k \\(5\\)"):
+        run(g, u, d, k=5)
+    with pytest.raises(rq.InvalidInputError, match="overlap"):
+        run(g, u, d, o=xd)
+    with pytest.raises(rq.ReflexError):  # half-typed and quantized stacks in one layer
+        run(g, u, q)
+
+
+def test_moe_ffn_grouped_half_captured(rq):
+    tokens, hidden, ffn, groups, top_k = 40, 128, 96, 8, 2
+    x, logits, w = _layer_inputs(tokens, groups, hidden, ffn, BF16, 3)
+    weights = [rq.Weight.from_tensor(t.to(DEV)) for t in w]
+    xd, ld = x.to(DEV), logits.to(DEV)
+    out = torch.empty(tokens * hidden, device=DEV)
+    step = lambda: rq.moe_ffn_grouped_device(xd, tokens, hidden, ld, groups, top_k, True, 1.0, *weights, out)  # noqa: E731
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for r in range(3):
+        xd.copy_(torch.randn(tokens, hidden))
+        ld.copy_(torch.randn(tokens, groups))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, out), f"replay {r}"
+
+
 def test_captured_and_replayed(rq):
     """The whole run in one graph, replayed on new inputs, with eager work between."""
     tokens, hidden, ffn, groups, top_k = 33, 128, 96, 8, 2
