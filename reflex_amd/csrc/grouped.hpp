@@ -10,7 +10,7 @@
 // step's sum is scaled back as it is added:
 //   f16:  x = RN16(x) + RN16(the rest): 22 bits or more of every value above
 //         2^-17 of the step's largest, 2^-39 of the largest of every other
-//   bf16: three roundings of 8 bits each: exact
+//   bf16: three truncations of 8 bits each: exact
 // Products of the pieces cost 2 (f16) or 3 (bf16) times the matrix
 // instructions; one rounding of x to the weights' type would cost 2^-12 or 2^-9
 // of every value, which f32 outputs show.
@@ -111,53 +111,82 @@ RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have) {
     return r;
 }
 
-RFXQ_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
-
-// 8 f32 values of a step as pieces of T that add up to them times `scale`.
-// Infinities and NaN are whole in the first.
-template <typename T, uint32_t NP>
-RFXQ_DEV void split_eight(const Eight<float>& x, float scale, u4_t (&out)[NP]) {
-    float left[8];
+// The largest of 8 values' sizes, as bits: sizes order like their bits, and
+// infinities and NaN lie above every finite one.
+constexpr uint32_t kInfBits = 0x7F800000u;
+RFXQ_DEV uint32_t top_of_eight(const Eight<float>& x) {
+    uint32_t t = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) left[i] = x.at(i) * scale;
-#pragma unroll
-    for (uint32_t n = 0; n < NP; n++)
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) {
-            const T a = (T)left[2 * i], b = (T)left[2 * i + 1];
-            out[n][i] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
-            left[2 * i] = finite(left[2 * i]) ? left[2 * i] - (float)a : 0.0f;
-            left[2 * i + 1] = finite(left[2 * i + 1]) ? left[2 * i + 1] - (float)b : 0.0f;
-        }
-}
-// The exponent e at which `top` is 2^e times a value in [2^14, 2^15), kept so that 2^e and 2^-e are f32 values
-RFXQ_DEV int step_exp(float top) { return max(__builtin_amdgcn_frexp_expf(top) - 15, -126); }
-RFXQ_DEV float pow2(int e) { return as_f32((uint32_t)(e + 127) << 23); }
-
-// the largest of the four lanes (l, 0..3)
-RFXQ_DEV float max_over_q(float v) {
-    uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-    v = fmaxf(as_f32(r[0]), as_f32(r[1]));
-    b = __builtin_bit_cast(uint32_t, v);
-    const auto s = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(as_f32(s[0]), as_f32(s[1]));
-}
-// the largest of the finite ones' sizes
-RFXQ_DEV float max_of_eight(const Eight<float>& x) {
-    float t = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) {
-        const float v = __builtin_fabsf(x.at(i));
-        t = v < __builtin_inff() ? fmaxf(t, v) : t;
-    }
+    for (uint32_t i = 0; i < 8u; i++) t = max(t, __builtin_bit_cast(uint32_t, x.at(i)) & 0x7FFFFFFFu);
     return t;
 }
+#define RFXQ_DPP_U32(v, ctrl) (uint32_t) __builtin_amdgcn_update_dpp(0, (int)(v), (ctrl), 0xF, 0xF, false)
 // the largest of 8 neighbouring lanes
-RFXQ_DEV float max_over_8(float v) {
-    v = fmaxf(v, RFXQ_DPP(v, 0xB1));
-    v = fmaxf(v, RFXQ_DPP(v, 0x4E));
-    return fmaxf(v, RFXQ_DPP(v, 0x141));
+RFXQ_DEV uint32_t top_over_8(uint32_t v) {
+    v = max(v, RFXQ_DPP_U32(v, 0xB1));
+    v = max(v, RFXQ_DPP_U32(v, 0x4E));
+    return max(v, RFXQ_DPP_U32(v, 0x141));
+}
+// the largest of the four lanes (l, 0..3)
+RFXQ_DEV uint32_t top_over_q(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+    const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)s[0], (uint32_t)s[1]);
+}
+
+// The scale of a row's values of a step, from the largest of their sizes: 2^e
+// and 2^-e with that one times 2^-e in [2^14, 2^15), kept so that both are f32
+// values. Steps with infinities or NaN are not scaled up: what is finite there
+// does not show.
+struct StepScale {
+    float up, back;
+};
+RFXQ_DEV StepScale step_scale(uint32_t top) {
+    const int e = max((int)(top >> 23) - 127 - 14, -126);
+    return {as_f32((uint32_t)(127 - e) << 23), as_f32((uint32_t)(127 + e) << 23)};
+}
+
+// 8 f32 values of a step as pieces of T that add up to them times `scale`.
+// Infinities and NaN (anywhere in the wave: `top`) are whole in the first piece.
+template <typename T, uint32_t NP>
+RFXQ_DEV void split_eight(const Eight<float>& x, float scale, uint32_t top, u4_t (&out)[NP]) {
+    float v[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) v[i] = x.at(i) * scale;
+    const auto pieces = [&](bool all_finite) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) {
+            float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+            for (uint32_t n = 0; n < NP; n++) {
+                float pa, pb;
+                if constexpr (__is_same(T, half_t)) {
+                    const h2_t h = {(half_t)a, (half_t)b};
+                    out[n][i] = h2_bits(h);
+                    pa = (float)h[0];
+                    pb = (float)h[1];
+                } else {  // truncated: the upper halves of the bits (a NaN keeps a set fraction bit there)
+                    uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
+                    if (!all_finite) {
+                        ua |= a != a ? 0x400000u : 0u;
+                        ub |= b != b ? 0x400000u : 0u;
+                    }
+                    out[n][i] = ua >> 16 | (ub & 0xFFFF0000u);
+                    pa = as_f32(ua & 0xFFFF0000u);
+                    pb = as_f32(ub & 0xFFFF0000u);
+                }
+                if (n + 1u < NP) {
+                    a = all_finite || __builtin_fabsf(a) < __builtin_inff() ? a - pa : 0.0f;
+                    b = all_finite || __builtin_fabsf(b) < __builtin_inff() ? b - pb : 0.0f;
+                }
+            }
+        }
+    };
+    if (__builtin_amdgcn_ballot_w64(top >= kInfBits))
+        pieces(false);
+    else
+        pieces(true);
 }
 
 // Workgroup b's place in the grid of tiles: workgroups go round-robin to the 8
@@ -339,12 +368,13 @@ RFXQ_DEV void grouped_any(const GroupedArgs& a) {
         for (uint32_t i = 0; i < NX; i++) {
             const uint32_t r = (tid >> 3) + 32u * i;
             if constexpr (F32) {
-                const int e = step_exp(max_over_8(max_of_eight(xv[i])));
+                const uint32_t top = top_over_8(top_of_eight(xv[i]));
+                const StepScale scale = step_scale(top);
                 u4_t p[P];
-                split_eight<T, P>(xv[i], pow2(-e), p);
+                split_eight<T, P>(xv[i], scale.up, top, p);
 #pragma unroll
                 for (uint32_t j = 0; j < P; j++) xs[j][lds_piece(r, c)] = p[j];
-                if (c == 0) back[r] = pow2(e);
+                if (c == 0) back[r] = scale.back;
             } else {
                 xs[0][lds_piece(r, c)] = xv[i].v;
             }

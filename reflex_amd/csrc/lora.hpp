@@ -139,10 +139,11 @@ struct LoraDown {
                     for (uint32_t f = 0; f < RT; f++) acc[m][f] = mfma32<TW>(wv[s][f].v, xv[s][m].v, acc[m][f]);
                 } else {
                     constexpr uint32_t NP = __is_same(TW, half_t) ? 2u : 3u;
-                    const int e = step_exp(max_over_q(max_of_eight(xv[s][m])));
-                    const float back = pow2(e);
+                    const uint32_t top = top_over_q(top_of_eight(xv[s][m]));
+                    const StepScale scale = step_scale(top);
+                    const float back = scale.back;
                     u4_t xp[NP];
-                    split_eight<TW, NP>(xv[s][m], pow2(-e), xp);
+                    split_eight<TW, NP>(xv[s][m], scale.up, top, xp);
 #pragma unroll
                     for (uint32_t f = 0; f < RT; f++) {
                         f4v_t d = {0, 0, 0, 0};
@@ -325,14 +326,15 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
             to[0] = sum.v[0];
             to[1] = sum.v[1];
         } else {
-            const int e = step_exp(max_over_q(max_of_eight(sum)));
+            const uint32_t top = top_over_q(top_of_eight(sum));
+            const StepScale step = step_scale(top);
             u4_t out[NP];
-            split_eight<TW, NP>(sum, pow2(-e), out);
+            split_eight<TW, NP>(sum, step.up, top, out);
 #pragma unroll
             for (uint32_t n = 0; n < NP; n++)
                 *reinterpret_cast<u4_t*>(reinterpret_cast<uint16_t*>(lds) + (n * BM + 16u * m + l) * (ldl + 8u) + r) = out[n];
             if (q == 0)
-                reinterpret_cast<float*>(lds + NP * BM * (ldl + 8u) / 2u)[(16u * m + l) * (ldl / 32u) + j / MT] = pow2(e);
+                reinterpret_cast<float*>(lds + NP * BM * (ldl + 8u) / 2u)[(16u * m + l) * (ldl / 32u) + j / MT] = step.back;
         }
     }
     __syncthreads();
