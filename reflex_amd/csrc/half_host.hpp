@@ -181,7 +181,8 @@ GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows
 bool lora_vec(uint32_t rank, uint32_t n) { return rank % 8u == 0 && n % 4u == 0; }
 
 // 32-row tiles from 17 rows a group on. The ranges of K of rfxq_lora_down: until
-// the workgroups fill the CUs, of at least 256 values each.
+// the workgroups fill the CUs twice (16-row tiles) or once (32: 4096 rows of 4096 60.6 us, twice
+// 65.2), of at least 256 values each.
 struct LoraPlan {
     uint32_t ldv, bm, tiles, splits, k_split;
     uint64_t total;
@@ -191,7 +192,7 @@ LoraPlan lora_plan(uint32_t k, uint32_t n, uint32_t rank, uint32_t groups, uint3
     p.ldv = (rank + 15u) & ~15u;
     p.bm = rows / std::min(rows, groups) > 16u && rank <= 256u && lora_vec(rank, n) ? 32u : 16u;
     p.tiles = max_tiles(rows, groups, p.bm);
-    const uint32_t want = (2u * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
+    const uint32_t want = ((p.bm == 32u ? 1u : 2u) * cus + p.tiles - 1u) / p.tiles, most = (k + 255u) / 256u;
     p.splits = std::max(1u, std::min({want, most, 32u}));
     p.k_split = ((k + p.splits - 1u) / p.splits + 127u) & ~127u;
     p.splits = (k + p.k_split - 1u) / p.k_split;
