@@ -295,7 +295,7 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.sn = (a.tiles_n + across - 1u) / across;
     const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
     const uint64_t grid = v.few ? (uint64_t)a.tiles_m * a.tiles_n : (blocks + 7u) / 8u * 8u * a.sm * a.sn;
-    if (grid > 0x7FFFFFFFull)
+    if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
         return fail(RFXQ_ERR_OTHER, "grouped_gemm: %u rows x %u columns need %llu workgroups", rows, n,
                     (unsigned long long)grid);
     if (int rc = launch(v.f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch", v.threads)) return rc;
@@ -345,7 +345,7 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     // columns, rank 64: 61.7 us; 4 a CU: 66, 2: 68)
     const uint32_t across = std::max(1u, std::min((8u * (uint32_t)c->cus + p.tiles - 1u) / p.tiles, (n + 127u) / 128u));
     const uint64_t up = (uint64_t)(p.tiles + 1u) * across;
-    if (up > 0x7FFFFFFFull || (uint64_t)p.tiles * p.splits > 0x7FFFFFFFull)
+    if (up * 256u > 0xFFFFFFFFull || (uint64_t)p.tiles * p.splits * 256u > 0xFFFFFFFFull)
         return fail(RFXQ_ERR_OTHER, "lora_add: %u rows need %llu workgroups", rows, (unsigned long long)up);
     void* ws = nullptr;
     if (int rc = take_workspace(c, workspace, workspace_bytes, p.total, stream, "lora_add", &ws)) return rc;

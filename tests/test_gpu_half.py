@@ -412,6 +412,72 @@ def test_lora_add_no_row_in_a_group(rq):
         assert torch.equal(_run_lora(rq, *c, in_place), c[6])
 
 
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,k,n", [(20, 2, 512, 64, 40), (33, 1, 256, 96, 64), (90, 2, 264, 40, 136),
+                                                  (50, 3, 300, 33, 12), (200, 1, 8, 8200, 4)])
+def test_lora_add_long_ranks_and_rows(rq, rows, count, rank, k, n, x_type, w_type):
+    _say("lora_add long", rows, count, rank, k, n, x_type, w_type)
+    c = _lora_case(rows, count, rank, k, n, x_type, w_type, rows)
+    _check_lora(*c, _run_lora(rq, *c, False))
+
+
+@pytest.mark.parametrize("w_type", [F16, BF16])
+def test_lora_add_values_at_the_ends_of_f32(rq, w_type):
+    """Steps of large and of small values, of both in one row, and of infinities: finite rows keep the bound
+    (of v's own steps: values below 2^-39 of a step's largest may be lost), the others do not come out finite."""
+    rows, k, n, rank = 12, 96, 32, 16
+    x, a, b, _, _, _, y = _lora_case(rows, 1, rank, k, n, F32, w_type, 6)
+    a, b = (torch.where(torch.isfinite(t), t, 0.25) for t in (a, b))
+    x[1] *= 1e30
+    x[2] *= 1e-30
+    x[3, :32] *= 1e25
+    x[4, 40] = 1e-38
+    x[5] = 0.0
+    x[6, 3], x[7, 90] = float("inf"), float("nan")
+    y[1:4] = 0.0
+    ids = np.zeros(rows, np.int32)
+    got = _run_lora(rq, x, a, b, ids, None, None, y, False)
+    assert not torch.isfinite(got[6]).any() and torch.isnan(got[7]).all() and torch.equal(got[5], y[5])
+    fine = [r for r in range(rows) if r not in (6, 7)]
+    _check_lora(x[fine], a, b, ids[fine], None, None, y[fine], got[fine])
+
+
+def test_lora_add_own_workspace(rq):
+    x, a, b, ids, ranks, scales, y = _lora_case(30, 3, 16, 4096, 64, F32, F16, 4)
+    wa, wb = rq.Weight.from_tensor(a.to(DEV)), rq.Weight.from_tensor(b.to(DEV))
+    g = rq.group_rows(torch.from_numpy(ids).to(DEV), 3)
+    size = rq.lora_add_workspace_size(wa, 30)
+    ws = torch.full((size + 64,), 7, dtype=torch.uint8, device=DEV)
+    yd, rd, sd = y.to(DEV), torch.tensor(ranks, dtype=torch.int32, device=DEV), torch.tensor(scales, device=DEV)
+    rq.lora_add(x.to(DEV), wa, wb, g, yd, ranks=rd, scales=sd, workspace=ws[:size])
+    _check_lora(x, a, b, ids, ranks, scales, y, yd.cpu())
+    assert (ws[size:] == 7).all()
+    with pytest.raises(rq.InvalidInputError, match="needs"):
+        rq.lora_add(x.to(DEV), wa, wb, g, yd, workspace=ws[:16])
+    with pytest.raises(rq.ReflexError, match="16-byte aligned"):
+        rq.lora_add(x.to(DEV), wa, wb, g, yd, workspace=ws[8:])
+
+
+def test_stacks_from_a_file(rq, tmp_path):
+    """F16 and BF16 expert tensors of a GGUF file, uploaded and multiplied."""
+    from test_gguf import write_gguf
+
+    k, n, groups, rows = 72, 40, 3, 30
+    stacks = {}
+    tensors = []
+    for name, t, ty in (("a", F16, 1), ("b", BF16, 30)):
+        x, w = _case(rows, groups, k, n, t, t, ty)
+        stacks[name] = (x, w)
+        tensors.append((name, [k, n, groups], ty, w.view(torch.int16).numpy().tobytes()))
+    write_gguf(tmp_path / "f.gguf", [], tensors)
+    weights = rq.GgufFile(tmp_path / "f.gguf").upload(["a", "b"], device=DEV)
+    offsets, _ = _grouped(_ids(rows, groups, "all"), groups)
+    for name, (x, w) in stacks.items():
+        assert weights[name].shape == [k, n, groups]
+        y = rq.grouped_gemm(x.to(DEV), weights[name], torch.from_numpy(offsets).to(DEV), rows)
+        _check_grouped(x, w, offsets, None, 1, None, y.cpu())
+
+
 # ------------------------------------------------------------------ together, captured, on other streams
 
 def _expert_layer(rq, x, logits, weights, top_k):

@@ -158,3 +158,70 @@ def test_python_checks():
         rq.grouped_gemm(x, w, ids, 4)
     with pytest.raises(rq.InvalidInputError, match="x on cpu"):
         rq.lora_add(x, w, w, rq.RowGroups(ids, ids), x)
+
+
+def test_matrix_results_are_not_read_too_early(tmp_path):
+    """The kernels' listing: on no path is a matrix instruction's result read before the wait states that the
+    compiler itself keeps in straight code (10 behind v_mfma_f32_16x16x4_f32, 8 behind the 16x16x32 ones). It
+    has left them out where the reading instruction is the first behind a branch."""
+    import os
+    import re
+    import subprocess
+
+    from reflex_amd import build
+
+    listing = tmp_path / "half.s"
+    flags = [f for f in build.DEVICE_FLAGS if f != "--no-gpu-bundle-output"]
+    subprocess.run([os.path.join(build.ROCM, "bin", "hipcc"), *flags, "-S", os.path.join(build.CSRC, "half.hip"), "-o",
+                    str(listing)], check=True, capture_output=True)
+    code, labels, kernel = [], {}, None
+    for line in listing.read_text().split("\n"):
+        m = re.match(r"^([\w.$]+):", line)
+        if m:
+            labels[m.group(1)] = len(code)
+            kernel = m.group(1) if m.group(1).startswith("rfxq") else kernel
+            continue
+        text = line.split(";")[0].strip()
+        if text and not text.startswith("."):
+            code.append((text, kernel))
+
+    def registers(operand):
+        found = set()
+        for m in re.finditer(r"\b([av])(?:\[(\d+):(\d+)\]|(\d+)\b)", operand):
+            lo, hi = (m.group(2), m.group(3)) if m.group(2) else (m.group(4), m.group(4))
+            found |= {(m.group(1), i) for i in range(int(lo), int(hi) + 1)}
+        return found
+
+    early, products = [], 0
+    for i, (text, kernel) in enumerate(code):
+        if not text.startswith("v_mfma"):
+            continue
+        products += 1
+        need = 10 if "x4_f32" in text else 8
+        paths, seen = [(i + 1, 0, frozenset(registers(text.split(None, 1)[1].split(", ")[0])))], set()
+        while paths:
+            at, waited, live = state = paths.pop()
+            if waited >= need or not live or at >= len(code) or state in seen:
+                continue
+            seen.add(state)
+            name, _, rest = code[at][0].partition(" ")
+            operands = rest.split(", ")
+            if name == "s_endpgm":
+                continue
+            if name == "s_nop":
+                paths.append((at + 1, waited + int(rest, 0) + 1, live))
+                continue
+            if name.startswith(("s_branch", "s_cbranch")):
+                paths.append((labels[rest.strip()], waited + 1, live))
+                if name == "s_branch":
+                    continue
+            elif name.startswith(("v_", "ds_", "global_", "buffer_", "flat_")):
+                writes = set() if "store" in name or "ds_write" in name else registers(operands[0])
+                reads = set().union(*map(registers, operands[1:] if writes else operands))
+                if name.startswith("v_mfma"):  # the next product may add to the same result
+                    reads = registers(operands[1]) | registers(operands[2])
+                if reads & live:
+                    early.append((kernel, text, code[at][0], waited))
+                live = frozenset(live - writes)
+            paths.append((at + 1, waited + 1, live))
+    assert products > 500 and not early, early[:5]
