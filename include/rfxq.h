@@ -414,11 +414,11 @@ uint64_t rfxq_group_rows_workspace_size(uint32_t n, uint32_t groups);
  * order[p] / top_k), its down product y_index = order. Rows that no place
  * names, and places in no group, with an index out of range or behind
  * x->rows, leave y as it was; a destination named twice holds one of its results.
- * x: f32, or the weights' type; y: f32, or the weights' type (its rows must not
- * overlap x). Accumulation is f32, each result is rounded once; f32 activations
+ * x: f32, or the weights' type; y: f32, or the weights' type (the memory from its
+ * first element to its last must not overlap x's). Accumulation is f32, each result is rounded once; f32 activations
  * keep f32 accuracy (they are split into 2 (F16) or 3 (BF16) pieces of the
- * weights' type; a weight that is infinite gives a result that is not finite, of
- * either kind). Any in_features, stride and alignment of whole elements; rows of x
+ * weights' type; a weight that is infinite, or of 2^100 and more, can give a
+ * result that is not finite, of either kind). Any in_features, stride and alignment of whole elements; rows of x
  * and W that start at multiples of 16 bytes (in_features and strides multiples of
  * 8) are faster. One launch, no workspace, no host synchronisation: it can be
  * captured. The counterpart of rfxq_expert_gemm for all experts at once
@@ -432,13 +432,15 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
  *   out[r] = y[r] + scales[g] * B_g (A_g x[r])
  * over the first ranks[g] rows of A_g and columns of B_g (rank <= 512); rows in no group:
  * out[r] = y[r]. y is what the shared projection gave (rfxq_gemm, rfxq_gemv_rows);
- * out may be y. a: a stack [in, rank, adapters], b: a stack [rank, out, adapters],
+ * out may be y; otherwise neither y nor x may overlap it, from its first element
+ * to its last. a: a stack [in, rank, adapters], b: a stack [rank, out, adapters],
  * of one type (F32, F16 or BF16), such as a pool whose places hold adapters of up
  * to `rank`; what lies past an adapter's own rank is not used. ranks (values
  * clamped to [0, rank]; NULL: all of it) and scales (NULL: 1): device memory,
  * a value per adapter. offsets and order as rfxq_group_rows writes them from the
  * rows' adapter ids, once for all projections of a step; order lists every row
- * of x once (a row that it does not list keeps what out held). x, y and out have
+ * of x once (a row that it does not list keeps what out held), and offsets rise
+ * from 0. x, y and out have
  * one type: f32 (any adapters), or the adapters' F16 / BF16; as many rows each.
  * A x is kept in f32, accumulation is f32, each result is rounded once.
  * `workspace`: rfxq_lora_add_workspace_size bytes for up to `rows` rows, 16-byte

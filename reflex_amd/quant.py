@@ -641,6 +641,13 @@ def _ints(t: torch.Tensor | None, least: int, dev: int, what: str) -> int | None
     return t.data_ptr()
 
 
+def _count(n: int, least: int, what: str) -> int:
+    """A count as the library takes it: below 2^31."""
+    if not least <= n <= 0x7FFFFFFF:
+        raise InvalidInputError(11, f"{what}={n}")
+    return n
+
+
 def _rows(t: torch.Tensor, columns: int, dev: int, what: str) -> RfxqRows:
     """``rfxq_rows`` of a 2-D tensor whose rows are contiguous."""
     ty = _ROW_TYPES.get(t.dtype)
@@ -653,7 +660,7 @@ def _rows(t: torch.Tensor, columns: int, dev: int, what: str) -> RfxqRows:
         step = columns
     if step < columns or (one != 1 and columns > 1):
         raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
-    return RfxqRows(t.data_ptr(), ty, rows, step)
+    return RfxqRows(t.data_ptr(), ty, _count(rows, 0, f"{what}: rows"), step)
 
 
 def _space(t: torch.Tensor | None, dev: int, what: str) -> tuple[int | None, int]:
@@ -673,7 +680,7 @@ def _stack(w: Weight, dev: int, what: str) -> int:
 
 def group_rows_workspace_size(n: int, groups: int) -> int:
     """Bytes of workspace ``group_rows`` needs for n ids (0 for few)."""
-    return int(lib().rfxq_group_rows_workspace_size(n, groups))
+    return int(lib().rfxq_group_rows_workspace_size(_count(n, 0, "group_rows: n"), _count(groups, 0, "group_rows: groups")))
 
 
 def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None,
@@ -681,11 +688,10 @@ def group_rows(ids: torch.Tensor, groups: int, out: RowGroups | None = None,
     """Rows grouped by an int32 device id (a routed expert, a request's adapter); an id
     outside [0, groups) is a row in no group. Stable: a group's rows keep their order."""
     dev = _on(ids, "group_rows: ids")
-    n = ids.numel()
+    n = _count(ids.numel(), 0, "group_rows: n")
+    _count(groups, 0, "group_rows: groups")
     src = _ints(ids, n, dev, "group_rows ids")
     if out is None:
-        if groups < 0:
-            raise InvalidInputError(11, f"group_rows: groups={groups}")
         out = RowGroups(ids.new_empty(groups + 1), ids.new_empty(n))
     space, size = _space(workspace, dev, "group_rows")
     with _dev(ids):
@@ -702,8 +708,8 @@ def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x
     ``rows`` rows, zero where no place of a group writes."""
     dev = _on(x, "grouped_gemm: x")
     count = _stack(w, dev, "grouped_gemm")
-    if rows < 0 or x_div < 1:
-        raise InvalidInputError(11, f"grouped_gemm: rows={rows} x_div={x_div}")
+    _count(rows, 0, "grouped_gemm: rows")
+    _count(x_div, 1, "grouped_gemm: x_div")
     c = w._c
     xr = _rows(x, c.in_features, dev, "grouped_gemm x")
     y = out if out is not None else torch.zeros(rows, c.out_features, dtype=x.dtype, device=x.device)
@@ -717,7 +723,7 @@ def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x
 
 def lora_add_workspace_size(a: Weight, rows: int) -> int:
     """Bytes of workspace ``lora_add`` needs for up to this many rows."""
-    return int(lib().rfxq_lora_add_workspace_size(a.cref(), rows))
+    return int(lib().rfxq_lora_add_workspace_size(a.cref(), _count(rows, 0, "lora_add: rows")))
 
 
 def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.Tensor,

@@ -458,6 +458,20 @@ def test_lora_add_own_workspace(rq):
         rq.lora_add(x.to(DEV), wa, wb, g, yd, workspace=ws[8:])
 
 
+def test_python_counts_do_not_wrap(rq):
+    x = torch.zeros(4, 8, dtype=F16, device=DEV)
+    w = rq.Weight.from_tensor(torch.zeros(2, 8, 8, dtype=F16, device=DEV))
+    offsets = torch.zeros(3, dtype=torch.int32, device=DEV)
+    out = torch.zeros(4, 8, dtype=F16, device=DEV)
+    for n in (-1, 1 << 31, (1 << 32) + 4):
+        with pytest.raises(rq.InvalidInputError, match="rows="):
+            rq.grouped_gemm(x, w, offsets, n, out=out)
+        with pytest.raises(rq.InvalidInputError, match="x_div="):
+            rq.grouped_gemm(x, w, offsets, 2, x_index=offsets, x_div=n, out=out)
+        with pytest.raises(rq.InvalidInputError, match="groups="):
+            rq.group_rows(offsets, n)
+
+
 def test_stacks_from_a_file(rq, tmp_path):
     """F16 and BF16 expert tensors of a GGUF file, uploaded and multiplied."""
     from test_gguf import write_gguf

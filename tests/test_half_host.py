@@ -160,6 +160,18 @@ def test_python_checks():
         rq.lora_add(x, w, w, rq.RowGroups(ids, ids), x)
 
 
+def test_python_counts_do_not_wrap():
+    import reflex_amd as rq
+
+    for n in (-1, 1 << 31, 1 << 32):
+        with pytest.raises(rq.InvalidInputError, match="group_rows: n="):
+            rq.group_rows_workspace_size(n, 4)
+        with pytest.raises(rq.InvalidInputError, match="groups="):
+            rq.group_rows_workspace_size(4, n)
+        with pytest.raises(rq.InvalidInputError, match="rows="):
+            rq.lora_add_workspace_size(rq.Weight.from_tensor(torch.zeros(4, 8)), n)
+
+
 def test_matrix_results_are_not_read_too_early(tmp_path):
     """The kernels' listing: on no path is a matrix instruction's result read before the wait states that the
     compiler itself keeps in straight code (10 behind v_mfma_f32_16x16x4_f32, 8 behind the 16x16x32 ones). It
