@@ -54,13 +54,12 @@ struct GroupedArgs {
 };
 
 // Row p's source and destination; -1 where an index is out of range (such a row
-// is not computed).
+// is not computed). The load has no condition (without an index it reads the first
+// offset), so that nothing waits for it where it is issued.
 RFXQ_DEV int64_t src_row(const GroupedArgs& a, uint32_t p) {
-    if (!a.x_index) return p < a.x_rows ? (int64_t)p : -1;
-    const int32_t i = a.x_index[p];
-    if (i < 0) return -1;
-    const uint32_t s = (uint32_t)i / a.x_div;
-    return s < a.x_rows ? (int64_t)s : -1;
+    const int32_t i = ((const RFXQ_GLOBAL int32_t*)(a.x_index ? a.x_index : a.offsets))[a.x_index ? p : 0u];
+    const uint32_t s = a.x_index ? (uint32_t)i / a.x_div : p;
+    return (i >= 0 || !a.x_index) && s < a.x_rows ? (int64_t)s : -1;
 }
 RFXQ_DEV int64_t dst_row(const GroupedArgs& a, uint32_t p) {
     const int32_t i = a.y_index ? a.y_index[p] : (int32_t)p;
@@ -612,8 +611,6 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     const uint32_t blocks = (a.k + 127u) / 128u, each = (blocks + WK - 1u) / WK;
     const uint32_t b0 = WK == 1 ? 0u : min(wave * each, blocks), b1 = WK == 1 ? blocks : min(b0 + each, blocks);
     const uint32_t p = t.beg + l;
-    const int64_t src = p < t.end ? src_row(a, p) : -1;
-    const TX* x = static_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
     const TW* w[NT];
 #pragma unroll
     for (uint32_t f = 0; f < NT; f++)
@@ -621,14 +618,26 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     f4v_t acc[NT] = {};
     u4_t wv[2][4][NT], xv[2][4][XV];
     // blocks of 128 that are whole, without conditions; then the last values of K
+    const auto load_w = [&](uint32_t s, uint32_t b, uint32_t i) {
+#pragma unroll
+        for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = ld16(w[f] + 128u * b + 32u * i + 8u * q);
+    };
+    const uint32_t whole = min(b1, a.k / 128u);
+    if (b0 < whole) {  // on their way while the rows are looked up
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) load_w(0, b0, i);
+    }
+    const int64_t found = src_row(a, min(p, t.end - 1u)), src = p < t.end ? found : -1;
+    const TX* x = static_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
+    const auto load_x = [&](uint32_t s, uint32_t b, uint32_t i) {
+#pragma unroll
+        for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = ld16(x + 128u * b + 32u * i + 8u * q + 4u * v);
+    };
     const auto load = [&](uint32_t s, uint32_t b) {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
-            const uint32_t k = 128u * b + 32u * i + 8u * q;
-#pragma unroll
-            for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = ld16(w[f] + k);
-#pragma unroll
-            for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = ld16(x + k + 4u * v);
+            load_w(s, b, i);
+            load_x(s, b, i);
         }
     };
     const auto load_tail = [&](uint32_t b) {
@@ -658,8 +667,10 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
                 }
             }
     };
-    const uint32_t whole = min(b1, a.k / 128u);
-    if (b0 < whole) load(0, b0);
+    if (b0 < whole) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++) load_x(0, b0, i);
+    }
     for (uint32_t b = b0; b < whole; b += 2u) {
         if (b + 1u < whole) load(1, b + 1u);
         multiply(0);

@@ -85,22 +85,23 @@ RFXQ_DEV Eight<T> first_of(Eight<T> r, uint32_t have) {
     return r;
 }
 
-RFXQ_DEV uint32_t lora_rank(const LoraArgs& a, uint32_t g) {
-    if (g >= a.groups) return 0;
-    if (!a.ranks) return a.rank;
-    const int32_t r = a.ranks[g];
-    return r < 0 ? 0u : (uint32_t)r < a.rank ? (uint32_t)r : a.rank;
+// the rank of a tile's group (`extra` of find_tile: its value of ranks)
+RFXQ_DEV uint32_t lora_rank(const LoraArgs& a, const RowTile& t) {
+    if (!t.any) return 0;
+    return a.ranks ? min((uint32_t)max(t.extra, 0), a.rank) : a.rank;
 }
 
+// Place p's row; a load without a condition (without an order it reads the first offset).
 RFXQ_DEV int64_t lora_row(const LoraArgs& a, uint32_t p) {
-    const int32_t r = a.order ? a.order[p] : (int32_t)p;
+    const int32_t i = ((const RFXQ_GLOBAL int32_t*)(a.order ? a.order : a.offsets))[a.order ? p : 0u];
+    const int32_t r = a.order ? i : (int32_t)p;
     return r >= 0 && (uint32_t)r < a.x_rows ? (int64_t)r : -1;
 }
 
 // The state of a workgroup of rfxq_lora_down_*, and its passes over up to 64 rows of A.
 template <typename TX, typename TW, uint32_t MT>
 struct LoraDown {
-    const TX* x[MT];
+    int64_t row[MT];  // -1: a place without a row
     RowTile t;
     uint32_t rank, split, wave, lane, k0, k1;
 
@@ -119,11 +120,22 @@ struct LoraDown {
         }
         Eight<TX> xv[2][MT];
         Eight<TW> wv[2][RT];
-        const auto load = [&](uint32_t s, uint32_t k) {
+        const auto load_w = [&](uint32_t s, uint32_t k) {
 #pragma unroll
             for (uint32_t f = 0; f < RT; f++) wv[s][f] = ld_eight(w[f] + k);
+        };
+        if (full) load_w(0, k0);  // on their way while the rows are looked up
+        const TX* x[MT];
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++)  // places without a row read the first one: what comes of it is not used
+            x[m] = static_cast<const TX*>(a.x) + (row[m] < 0 ? 0 : (uint64_t)row[m] * a.ldx) + 8u * q;
+        const auto load_x = [&](uint32_t s, uint32_t k) {
 #pragma unroll
             for (uint32_t m = 0; m < MT; m++) xv[s][m] = ld_eight(x[m] + k);
+        };
+        const auto load = [&](uint32_t s, uint32_t k) {
+            load_w(s, k);
+            load_x(s, k);
         };
         const auto multiply = [&](uint32_t s) {
 #pragma unroll
@@ -154,7 +166,7 @@ struct LoraDown {
                 }
             }
         };
-        if (full) load(0, k0);
+        if (full) load_x(0, k0);
         for (uint32_t i = 0; i < full; i += 2u) {
             if (i + 1u < full) load(1, k0 + 32u * (i + 1u));
             multiply(0);
@@ -205,17 +217,16 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
     __shared__ f4v_t part[3][MT][4][64];
     LoraDown<TX, TW, MT> d;
     d.split = blockIdx.x / a.tiles;
-    d.t = find_tile(a.offsets, a.groups, a.rows, 16u * MT, blockIdx.x % a.tiles);
+    d.t = find_tile(a.offsets, a.groups, a.rows, 16u * MT, blockIdx.x % a.tiles, a.ranks);
     if (!d.t.any) return;
-    d.rank = lora_rank(a, d.t.group);
+    d.rank = lora_rank(a, d.t);
     d.lane = threadIdx.x & 63u;
     d.wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 #pragma unroll
     for (uint32_t m = 0; m < MT; m++) {
         const uint32_t p = d.t.beg + 16u * m + (d.lane & 15u);
-        const int64_t row = p < d.t.end ? lora_row(a, p) : -1;
-        // places without a row read the first one: what comes of it is not used
-        d.x[m] = static_cast<const TX*>(a.x) + (row < 0 ? 0 : (uint64_t)row * a.ldx) + 8u * (d.lane >> 4);
+        const int64_t found = lora_row(a, min(p, d.t.end - 1u));
+        d.row[m] = p < d.t.end ? found : -1;
     }
     const uint32_t quarter = (a.k_split / 4u + 31u) & ~31u;
     const uint32_t end = min(a.k, (d.split + 1u) * a.k_split);
@@ -247,7 +258,7 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
     constexpr bool F32 = __is_same(TW, float);
     constexpr uint32_t BM = 16u * MT, NP = __is_same(TW, __bf16) && __is_same(TX, float) ? 3u : 2u;
     extern __shared__ uint32_t lds[];
-    RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, blockIdx.x / a.across);
+    RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, blockIdx.x / a.across, a.ranks);
     if (!t.any) {  // rows in no group
         if (a.y == a.out) return;
         const int32_t o = a.offsets[a.groups];
@@ -256,23 +267,12 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
         t.end = min(t.beg + BM, a.rows);
         t.group = a.groups;
     }
-    const uint32_t rank = lora_rank(a, t.group), lane = threadIdx.x & 63u;
+    const uint32_t rank = lora_rank(a, t), lane = threadIdx.x & 63u;
     if (rank == 0 && a.y == a.out) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t l = lane & 15u, q = lane >> 4, strips = (a.n + 16u * NF - 1u) / (16u * NF);
     const uint32_t group = min(t.group, a.groups - 1u);
     const uint32_t steps = (rank + 31u) / 32u, ldl = (a.rank + 31u) & ~31u;
-    const TX* y[MT];
-    TX* o[MT];
-    bool there[MT];
-#pragma unroll
-    for (uint32_t m = 0; m < MT; m++) {
-        const uint32_t p = t.beg + 16u * m + l;
-        const int64_t row = p < t.end ? lora_row(a, p) : -1;
-        there[m] = row >= 0;
-        y[m] = static_cast<const TX*>(a.y) + (row < 0 ? 0 : (uint64_t)row * a.ldy);
-        o[m] = static_cast<TX*>(a.out) + (row < 0 ? 0 : (uint64_t)row * a.ldo);
-    }
     struct Strip {
         Eight<TW> w[2][NF];  // the first 64 of the rank
         Four<TX> y[MT][NF];
@@ -289,9 +289,25 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
                 w[f] = ld_eight(row + at, rank > at ? rank - at : 0u);
         }
     };
-    const auto load = [&](Strip& s, uint32_t n0) {
+    const auto load_ws = [&](Strip& s, uint32_t n0) {
         if (rank) load_w(s.w[0], n0, 0);
         if (rank > 32u) load_w(s.w[1], n0, 32u);
+    };
+    const uint32_t first = (blockIdx.x % a.across) * 4u + wave, by = 4u * a.across;
+    Strip s[2];
+    if (first < strips) load_ws(s[0], 16u * NF * first);  // on their way while the rows are looked up
+    const TX* y[MT];
+    TX* o[MT];
+    bool there[MT];
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++) {
+        const uint32_t p = t.beg + 16u * m + l;
+        const int64_t found = lora_row(a, min(p, t.end - 1u)), row = p < t.end ? found : -1;
+        there[m] = row >= 0;
+        y[m] = static_cast<const TX*>(a.y) + (row < 0 ? 0 : (uint64_t)row * a.ldy);
+        o[m] = static_cast<TX*>(a.out) + (row < 0 ? 0 : (uint64_t)row * a.ldo);
+    }
+    const auto load_ys = [&](Strip& s, uint32_t n0) {
 #pragma unroll
         for (uint32_t m = 0; m < MT; m++)
 #pragma unroll
@@ -303,9 +319,11 @@ RFXQ_DEV void lora_up(const LoraArgs& a) {
                     s.y[m][f] = ld_four(y[m] + n, n >= a.n ? 0u : a.n - n);
             }
     };
-    const uint32_t first = (blockIdx.x % a.across) * 4u + wave, by = 4u * a.across;
-    Strip s[2];
-    if (first < strips) load(s[0], 16u * NF * first);
+    const auto load = [&](Strip& s, uint32_t n0) {
+        load_ws(s, n0);
+        load_ys(s, n0);
+    };
+    if (first < strips) load_ys(s[0], 16u * NF * first);
 
     // v into LDS: a lane's 8 values of a row and step, the ranges of K added in
     // order; v is written, with zeros, up to the next whole 16

@@ -29,49 +29,64 @@ RFXQ_DEV uint32_t wave_scan(uint32_t v) {
 // there is none (any = false), `beg` is the tile's number behind the last one.
 struct RowTile {
     uint32_t group, beg, end;
+    int32_t extra;
     bool any;
+};
+
+template <uint32_t N>
+struct Count {
+    static constexpr uint32_t value = N;
 };
 
 // Tile t of the grouped rows: the groups' tiles counted in order, each group
 // starting a tile of its own. Every wave searches by itself (no LDS, no
-// barrier): lane l holds `per` neighbouring groups. Offsets are taken as they
-// are found: clamped to [0, rows] and to what came before, so that no value
-// there leads outside the arrays.
-RFXQ_DEV RowTile find_tile(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t bm, uint32_t t) {
-    const uint32_t lane = threadIdx.x & 63u, per = (groups + 63u) / 64u;
-    const uint32_t g0 = lane * per < groups ? lane * per : groups;
-    const uint32_t g1 = g0 + per < groups ? g0 + per : groups;
-    const auto at = [&](uint32_t g) {
-        const int32_t o = offsets[g];
-        return o < 0 ? 0u : (uint32_t)o < rows ? (uint32_t)o : rows;
-    };
-    uint32_t mine = 0;
-    for (uint32_t g = g0; g < g1; g++) {
-        const uint32_t b = at(g), e = at(g + 1u);
-        mine += e > b ? (e - b + bm - 1u) / bm : 0u;
-    }
-    const uint32_t upto = wave_scan(mine);
-    const uint64_t has = __builtin_amdgcn_ballot_w64(upto > t);
-    RowTile r = {0, t - (uint32_t)__builtin_amdgcn_readlane((int)upto, 63), 0, false};
-    if (!has) return r;
-    const uint32_t l = (uint32_t)__builtin_ctzll(has);
-    uint32_t left = t - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), (int)l);  // among lane l's tiles
-    const uint32_t e0 = l * per, e1 = e0 + per < groups ? e0 + per : groups;
-    for (uint32_t g = e0; g < e1; g++) {
-        const uint32_t b = at(g), e = at(g + 1u);
-        const uint32_t n = e > b ? (e - b + bm - 1u) / bm : 0u;
-        if (left < n) {
-            r.group = g;
-            r.beg = b + left * bm;
-            r.end = r.beg + bm < e ? r.beg + bm : e;
-            r.any = true;
-            break;
+// barrier), a group a lane: the offsets of up to 256 groups are one trip to memory,
+// which every kernel here waits for before it knows what to read (two and more trips,
+// with neighbouring groups in a lane: FIND_FIGURES).
+// Offsets are taken as they are found: clamped to [0, rows], and a group
+// whose end lies before its start has no tiles, so that no value there leads
+// outside the arrays. `extra`: a value per group, returned for the tile's.
+RFXQ_DEV RowTile find_tile(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t bm, uint32_t t,
+                           const int32_t* extra = nullptr) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t before = 0;  // tiles of the groups looked at
+    RowTile r = {0, 0, 0, 0, false};
+    const auto look = [&](auto n, uint32_t g0) {
+        constexpr uint32_t N = decltype(n)::value;
+        int32_t b[N], e[N], x[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            const uint32_t g = g0 + 64u * i + lane;
+            b[i] = ((const RFXQ_GLOBAL int32_t*)offsets)[min(g, groups)];
+            e[i] = ((const RFXQ_GLOBAL int32_t*)offsets)[min(g + 1u, groups)];
+            x[i] = extra ? ((const RFXQ_GLOBAL int32_t*)extra)[min(g, groups - 1u)] : 0;
         }
-        left -= n;
-    }
-    r.group = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.group);
-    r.beg = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.beg);
-    r.end = (uint32_t)__builtin_amdgcn_readfirstlane((int)r.end);
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            const uint32_t bi = min((uint32_t)max(b[i], 0), rows), ei = min((uint32_t)max(e[i], 0), rows);
+            const uint32_t mine = ei > bi ? (ei - bi + bm - 1u) / bm : 0u;
+            const uint32_t upto = before + wave_scan(mine);
+            const uint64_t has = __builtin_amdgcn_ballot_w64(upto > t);
+            if (has) {
+                const int l = __builtin_ctzll(has);
+                const uint32_t left = t - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), l);
+                if (left >= (uint32_t)__builtin_amdgcn_readlane((int)mine, l)) return;  // a sum that wrapped
+                const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)ei, l);
+                r.group = g0 + 64u * i + (uint32_t)l;
+                r.beg = (uint32_t)__builtin_amdgcn_readlane((int)bi, l) + left * bm;
+                r.end = min(r.beg + bm, end);
+                r.extra = __builtin_amdgcn_readlane(x[i], l);
+                r.any = true;
+                return;
+            }
+            before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        }
+    };
+    if (groups <= 64u)
+        look(Count<1>{}, 0);
+    else
+        for (uint32_t g0 = 0; g0 < groups && !r.any; g0 += 256u) look(Count<4>{}, g0);
+    if (!r.any) r.beg = t - before;
     return r;
 }
 
