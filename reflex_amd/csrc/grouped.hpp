@@ -585,6 +585,141 @@ RFXQ_GROUPED_TILE(64_bf16, __bf16, 64, 128, 2, 2, 3, run)
 RFXQ_GROUPED_TILE(256_f16, half_t, 256, 256, 2, 4, 2, run_turns)
 RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, run_turns)
 
+// ---------------------------------------------------------------- ranges of K, a wave each
+
+// 16 MT rows times 16 RT columns over [k0, k1) of K, a wave by itself: both operands
+// from memory straight into registers, 64 of K (whole 128-byte lines of half-typed
+// rows) a step. w, and x as rows() gives it, point to the lane's first values, 8
+// (lane / 16) on from k = 0. The numbers of operands are known at compile time: the
+// products of a step and what reads them stay free of branches (mfma_settle). Other
+// waves hide the loads: with steps in flight ahead a wave needs the registers of two
+// (rfxq_lora_down, 4096 rows of 4096 values, rank 64: 58.0 us with rfxq_lora_up, 56.4 without).
+template <typename TX, typename TW, uint32_t MT, uint32_t RT, typename Rows>
+RFXQ_DEV void k_range(const TW* const (&w)[RT], const Rows& rows, uint32_t k0, uint32_t k1, f4v_t (&acc)[MT][RT]) {
+    const uint32_t full = (k1 - k0) / 64u, tail = (k1 - k0) % 64u;
+    Eight<TX> xv[MT][2];
+    Eight<TW> wv[RT][2];
+    const TX* x[MT];
+    const auto load_w = [&](uint32_t k) {
+#pragma unroll
+        for (uint32_t f = 0; f < RT; f++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) wv[f][h] = ld_eight(w[f] + k + 32u * h);
+    };
+    const auto load_x = [&](uint32_t k) {
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) xv[m][h] = ld_eight(x[m] + k + 32u * h);
+    };
+    const auto multiply = [&](uint32_t h) {
+#pragma unroll
+        for (uint32_t m = 0; m < MT; m++) {
+            if constexpr (__is_same(TW, float)) {
+#pragma unroll
+                for (uint32_t f = 0; f < RT; f++)
+#pragma unroll
+                    for (uint32_t j = 0; j < 8u; j++)
+                        acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[f][h].at(j), xv[m][h].at(j), acc[m][f], 0, 0, 0);
+            } else if constexpr (__is_same(TX, TW)) {
+#pragma unroll
+                for (uint32_t f = 0; f < RT; f++) acc[m][f] = mfma32<TW>(wv[f][h].v, xv[m][h].v, acc[m][f]);
+            } else {
+                constexpr uint32_t NP = __is_same(TW, half_t) ? 2u : 3u;
+                const uint32_t top = top_over_q(top_of_eight(xv[m][h]));
+                const StepScale scale = step_scale(top);
+                const float back = scale.back;
+                u4_t xp[NP];
+                split_eight<TW, NP>(xv[m][h], scale.up, top, xp);
+#pragma unroll
+                for (uint32_t f = 0; f < RT; f++) {
+                    f4v_t d = {0, 0, 0, 0};
+#pragma unroll
+                    for (uint32_t n = 0; n < NP; n++) d = mfma32<TW>(wv[f][h].v, xp[NP - 1u - n], d);
+                    acc[m][f] += d * back;
+                }
+            }
+        }
+    };
+    if (full) load_w(k0);  // on their way while the rows are looked up
+    rows(x);
+    for (uint32_t i = 0; i < full; i++) {
+        if (i) load_w(k0 + 64u * i);
+        load_x(k0 + 64u * i);
+        multiply(0);
+        multiply(1);
+    }
+    mfma_settle();
+    if (tail) {
+        const uint32_t q = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++) {
+            const uint32_t k = k0 + 64u * full + 32u * h, have = tail > 32u * h + 8u * q ? tail - 32u * h - 8u * q : 0u;
+#pragma unroll
+            for (uint32_t f = 0; f < RT; f++) wv[f][h] = ld_eight(w[f] + k, have);
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) xv[m][h] = ld_eight(x[m] + k, have);
+        }
+        multiply(0);
+        multiply(1);
+        mfma_settle();
+    }
+}
+
+// f32 activations where 64 x 128 tiles leave CUs without work or are mostly empty: 32 x 64,
+// the workgroup's waves take quarters of K and add them in LDS, any alignment. A
+// tile's time there is that of its steps, a quarter as many here (8 groups of 64
+// rows, N x K 1024 x 4096: 38 us against 95; a CU's loads bound it: the same with
+// steps copied ahead).
+template <typename TX, typename TW>
+RFXQ_DEV void grouped_quarters(const GroupedArgs& a) {
+    constexpr uint32_t MT = 2, RT = 4;
+    __shared__ f4v_t part[4][MT][RT][64];
+    uint32_t tm, tn;
+    if (!tile_place(a, blockIdx.x, tm, tn)) return;
+    const RowTile t = find_tile(a.offsets, a.groups, a.rows, 16u * MT, tm);
+    if (!t.any) return;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4, n0 = tn * 16u * RT;
+    const TW* w[RT];
+#pragma unroll
+    for (uint32_t f = 0; f < RT; f++)  // columns past the last read it again; their results are not stored
+        w[f] = reinterpret_cast<const TW*>(a.w) + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.k +
+               8u * q;
+    const uint32_t quarter = ((a.k + 3u) / 4u + 63u) & ~63u, k0 = min(wave * quarter, a.k);
+    int64_t src[MT];
+    f4v_t acc[MT][RT] = {};
+    k_range<TX, TW, MT, RT>(
+        w,
+        [&](const TX*(&x)[MT]) {
+#pragma unroll
+            for (uint32_t m = 0; m < MT; m++) {
+                const uint32_t p = t.beg + 16u * m + l;
+                const int64_t found = src_row(a, min(p, t.end - 1u));
+                src[m] = p < t.end ? found : -1;
+                x[m] = static_cast<const TX*>(a.x) + (src[m] < 0 ? 0 : (uint64_t)src[m] * a.ldx) + 8u * q;
+            }
+        },
+        k0, min(k0 + quarter, a.k), acc);
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++)
+#pragma unroll
+        for (uint32_t f = 0; f < RT; f++) part[wave][m][f][lane] = acc[m][f];
+    __syncthreads();
+#pragma unroll
+    for (uint32_t m = 0; m < MT; m++) {  // a wave stores 16 of the columns
+        const f4v_t s = ((part[0][m][wave][lane] + part[1][m][wave][lane]) + part[2][m][wave][lane]) + part[3][m][wave][lane];
+        if (src[m] < 0) continue;
+        const int64_t dst = dst_row(a, t.beg + 16u * m + l);
+        if (dst >= 0) st_four<TW>(a, dst, n0 + 16u * wave + 4u * q, s);
+    }
+}
+
+#define RFXQ_GROUPED_QUARTERS(name, TX, TW) \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_grouped_quarters_##name(GroupedArgs a) { grouped_quarters<TX, TW>(a); }
+RFXQ_GROUPED_QUARTERS(f32_f16, float, half_t)
+RFXQ_GROUPED_QUARTERS(f32_bf16, float, __bf16)
+
 // ---------------------------------------------------------------- few rows a group
 
 // Decode: what a group's matrix weighs is all that counts, so its rows go from
@@ -599,7 +734,6 @@ RFXQ_GROUPED_TILE(256_bf16, __bf16, 256, 256, 2, 4, 2, run_turns)
 template <typename TX, typename TW, uint32_t NT, uint32_t WK>
 RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     constexpr bool F32 = __is_same(TX, float);
-    constexpr uint32_t XV = F32 ? 2u : 1u;  // 16-byte loads of 8 activations
     __shared__ f4v_t part[WK > 1 ? (WK - 1) * NT * 64u : 1u];
     constexpr uint32_t COLS = 16u * NT * 4u / WK;  // a workgroup's
     const uint32_t tn = blockIdx.x % a.tiles_n;
@@ -616,11 +750,12 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     for (uint32_t f = 0; f < NT; f++)
         w[f] = reinterpret_cast<const TW*>(a.w) + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.k;
     f4v_t acc[NT] = {};
-    u4_t wv[2][4][NT], xv[2][4][XV];
+    Eight<TW> wv[2][4][NT];
+    Eight<TX> xv[2][4];
     // blocks of 128 that are whole, without conditions; then the last values of K
     const auto load_w = [&](uint32_t s, uint32_t b, uint32_t i) {
 #pragma unroll
-        for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = ld16(w[f] + 128u * b + 32u * i + 8u * q);
+        for (uint32_t f = 0; f < NT; f++) wv[s][i][f] = ld_eight(w[f] + 128u * b + 32u * i + 8u * q);
     };
     const uint32_t whole = min(b1, a.k / 128u);
     if (b0 < whole) {  // on their way while the rows are looked up
@@ -629,10 +764,7 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     }
     const int64_t found = src_row(a, min(p, t.end - 1u)), src = p < t.end ? found : -1;
     const TX* x = static_cast<const TX*>(a.x) + (src < 0 ? 0 : (uint64_t)src * a.ldx);
-    const auto load_x = [&](uint32_t s, uint32_t b, uint32_t i) {
-#pragma unroll
-        for (uint32_t v = 0; v < XV; v++) xv[s][i][v] = ld16(x + 128u * b + 32u * i + 8u * q + 4u * v);
-    };
+    const auto load_x = [&](uint32_t s, uint32_t b, uint32_t i) { xv[s][i] = ld_eight(x + 128u * b + 32u * i + 8u * q); };
     const auto load = [&](uint32_t s, uint32_t b) {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
@@ -643,12 +775,10 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     const auto load_tail = [&](uint32_t b) {
 #pragma unroll
         for (uint32_t i = 0; i < 4u; i++) {
-            const uint32_t k = 128u * b + 32u * i + 8u * q;
-            const bool have = k < a.k;
+            const uint32_t k = 128u * b + 32u * i + 8u * q, have = a.k > k ? a.k - k : 0u;
 #pragma unroll
-            for (uint32_t f = 0; f < NT; f++) wv[0][i][f] = have ? ld16(w[f] + k) : u4_t{0, 0, 0, 0};
-#pragma unroll
-            for (uint32_t v = 0; v < XV; v++) xv[0][i][v] = have ? ld16(x + k + 4u * v) : u4_t{0, 0, 0, 0};
+            for (uint32_t f = 0; f < NT; f++) wv[0][i][f] = ld_eight(w[f] + k, have);
+            xv[0][i] = ld_eight(x + k, have);
         }
     };
     const auto multiply = [&](uint32_t s) {
@@ -657,13 +787,11 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
 #pragma unroll
             for (uint32_t f = 0; f < NT; f++) {
                 if constexpr (F32) {
-                    typedef TW t8_t __attribute__((ext_vector_type(8)));
-                    const t8_t w8 = __builtin_bit_cast(t8_t, wv[s][i][f]);
 #pragma unroll
                     for (uint32_t j = 0; j < 8u; j++)
-                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)w8[j], as_f32(xv[s][i][j >> 2][j & 3u]), acc[f], 0, 0, 0);
+                        acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[s][i][f].at(j), xv[s][i].at(j), acc[f], 0, 0, 0);
                 } else {
-                    acc[f] = mfma32<TW>(wv[s][i][f], xv[s][i][0], acc[f]);
+                    acc[f] = mfma32<TW>(wv[s][i][f].v, xv[s][i].v, acc[f]);
                 }
             }
     };

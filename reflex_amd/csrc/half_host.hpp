@@ -139,39 +139,55 @@ GroupPlan group_plan(uint32_t n, uint32_t groups) {
 
 constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offsets reach
 
-// The kernel of a grouped product, by the mean rows of the groups that can have
-// any, measured with stacks of 128 matrices of 768 x 2048 and 2048 x 768 and of 8 of
-// 14336 x 4096 and 4096 x 14336 (N x K; us, bf16):
-//   few rows  16 rows, weights straight from memory: up to 4 rows (64 against 72 on
-//             128 x 768 x 2048 at 4 rows, 88 against 88 at 8); f32 activations, whose
-//             pieces the tiles have to multiply one by one, up to 8 (121 against 128);
-//             short K up to 2, where the tiles keep more loads in flight (54 against
-//             51 at 2 rows, 61 against 66 at 4)
+// The kernel of a grouped product, by the mean rows of the groups that can have any and
+// the tiles that makes, measured (us) over groups 1..128, rows of 1..2048, N and K of
+// 64..14336:
+//   few4      16 x 16, K in quarters, weights straight from memory: where its tiles are
+//             at most 3 a CU. There a tile's own time is all: smaller ones on more CUs win
+//             (f16, 8 groups of 16 rows, N x K 1024 x 4096: 18 against 32 with 64 x 128
+//             tiles; 8 x 64 rows, 320 x 1000: 6.4 against 9.4; 1024 of them lose, 115
+//             against 51 at 32 x 32 x 1024 x 4096). Rows that do not start at 16 bytes: 2
+//             a CU (8 x 64 x 320 x 3149 at 2.5: 48 against 41)
+//   few rows  for decode, where every weight is read once: few4 up to 4 rows (64 against
+//             72 on 128 x 768 x 2048 at 4 rows), long K up to 6 (60 x 1024 x 4096 at 6: 96
+//             against 114; 60 x 4096 x 1024: 104 against 96); with short K, up to 2
+//             rows, all of K in a wave (51 against 54 at 2 rows, 66 against 61 at 4), for
+//             f32 activations up to 8 from 6 tiles of 128 columns a CU on (128 x 2048 x 768 at 8:
+//             96 against 105; 768 such tiles, 128 x 768 x 2048: 100 against 91)
+//   quarters  32 x 64, K in quarters, f32 activations: few tiles (8 x 64 x 1024 x 4096: 38
+//             against 95; 8 x 64 x 2048 x 768: 17 against 23; from 4 a CU on 36
+//             against 32), and up to 16 rows, long K up to 32 (128 x 768 x 2048 at 16: 96
+//             against 110; 60 x 1024 x 4096 at 20: 115 against 132; short K 60 x 2816 x 704
+//             at 6: 56 against 50)
+//   large     256 x 256: from where its steps pay (8 x 14336 x 4096: 327 against
+//             324 at 128 rows, 358 against 395 at 200) and its tiles fill over half of
+//             the CUs (8 x 4096 x 4096, 256 rows, 128 tiles: 111 against 111; 64 tiles,
+//             8 x 512 x 1024 x 4096: 85 against 53)
+//   pipelined 64 x 128 copied ahead into three buffers: up to 2 tiles a CU, where each
+//             workgroup has to hide its own latency (8 x 4096 x 14336 at 32 rows: 186
+//             against 247; 8 x 512 x 1024 x 4096: 53 against 57); beyond, faster
+//             without (8 x 192 x 4096 x 4096: 105 against 88)
 //   tiles     64 x 128 through registers: the rest
-//   pipelined 64 x 128 copied ahead into three buffers: where the tiles do not fill the
-//             CUs twice, each workgroup has to hide its own latency (8 x 4096 x 14336 at
-//             32 rows: 186 against 247); 896 tiles are faster without (176 against 163)
-//   large     256 x 256: from where its larger steps pay (8 x 14336 x 4096: 327 against
-//             324 at 128 rows, 358 against 395 at 200); for f32 activations it goes
-//             through the pieces, reading the weights again (1372 against 1289 at 400)
 struct GroupedVariant {
     hipFunction_t f;
     uint32_t bm, bn, threads;
     bool few;
 };
 GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n,
-                               bool direct, bool copies) {
+                               bool aligned, bool copies) {
     const uint32_t used = std::min(rows, groups), mean = rows / used, xt = f32 ? 0u : 1u;
-    const uint64_t fill = 2ull * c->cus;
-    if (direct && mean <= (k < 1024u ? 2u : f32 ? 8u : 4u)) {
-        // a wave's columns over all of K, unless that leaves CUs without work or long K
-        // to one wave (128 x 768 x 2048, 8 rows in 8 groups: 20 against 8 us)
-        if (k < 1024u && (uint64_t)used * ((n + 127u) / 128u) >= fill) return {c->half.few[xt][t], 16, 128, 256, true};
-        return {c->half.few4[xt][t], 16, 16, 256, true};
-    }
-    if (copies && mean > 160u) return {c->half.t256[t], 256, 256, 512, false};
-    if (copies && mean <= 64u && (uint64_t)max_tiles(rows, groups, 64u) * ((n + 127u) / 128u) < fill)
-        return {c->half.t64[t], 64, 128, 256, false};
+    const uint64_t cus = (uint64_t)c->cus;
+    const auto tiles = [&](uint32_t bm, uint32_t bn) {
+        return (uint64_t)used * ((mean + bm - 1u) / bm) * (((uint64_t)n + bn - 1u) / bn);
+    };
+    const GroupedVariant few4 = {c->half.few4[xt][t], 16, 16, 256, true}, few = {c->half.few[xt][t], 16, 128, 256, true};
+    if (tiles(16, 16) <= (aligned ? 3u : 2u) * cus) return few4;
+    if (aligned && f32 && mean <= 8u && tiles(16, 128) >= 6u * cus) return few;
+    if (aligned && !f32 && k < 1024u && mean <= 2u && tiles(16, 128) >= 2u * cus) return few;
+    if (aligned && !f32 && k >= 1024u && mean <= (k >= 2048u ? 6u : 4u)) return few4;
+    if (f32 && ((aligned && mean <= (k >= 2048u ? 32u : k >= 1024u ? 16u : 0u)) || tiles(32, 64) <= 3u * cus)) return {c->half.quarters[t], 32, 64, 256, false};
+    if (copies && mean > 160u && 8u * tiles(256, 256) >= 5u * cus) return {c->half.t256[t], 256, 256, 512, false};
+    if (copies && tiles(64, 128) <= 2u * cus) return {c->half.t64[t], 64, 128, 256, false};
     return {c->half.any[xt][t], 64, 128, 256, false};
 }
 
@@ -279,12 +295,11 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.n = n;
     a.groups = groups;
     a.y_f32 = y->type == RFXQ_TYPE_F32 ? 1u : 0u;
-    // asynchronous copies: rows at whole 16 bytes, 32-bit offsets
     const bool f32 = x->type == RFXQ_TYPE_F32;
-    const bool direct = aligned16(x->data) && x->stride % (f32 ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
-    // asynchronous copies: 32-bit offsets
-    const bool copies = direct && !f32 && rows_span(x, k) < kMaxOffset && 2ull * k * n < kMaxOffset;
-    const GroupedVariant v = grouped_variant(c, t, f32, rows, groups, k, n, direct, copies);
+    const bool aligned = aligned16(x->data) && x->stride % (f32 ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
+    // asynchronous copies: half types, rows at whole 16 bytes, 32-bit offsets
+    const bool copies = aligned && !f32 && rows_span(x, k) < kMaxOffset && 2ull * k * n < kMaxOffset;
+    const GroupedVariant v = grouped_variant(c, t, f32, rows, groups, k, n, aligned, copies);
     a.tiles_m = max_tiles(rows, groups, v.bm);
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of up to 4 row tiles and 4 column tiles, evenly cut, small enough that every XCD has several

@@ -110,7 +110,6 @@ struct LoraDown {
     template <uint32_t RT>
     __device__ __forceinline__ void pass(const LoraArgs& a, uint32_t r0, f4v_t (*part)[MT][4][64]) const {
         const uint32_t l = lane & 15u, q = lane >> 4;
-        const uint32_t full = (k1 - k0) / 32u, tail = (k1 - k0) % 32u;
         f4v_t acc[MT][RT] = {};
         const TW* w[RT];
 #pragma unroll
@@ -118,70 +117,14 @@ struct LoraDown {
             // rows past the rank read the last one; their results are dropped below
             w[f] = static_cast<const TW*>(a.a) + ((uint64_t)t.group * a.rank + min(r0 + 16u * f + l, rank - 1u)) * a.k + 8u * q;
         }
-        Eight<TX> xv[2][MT];
-        Eight<TW> wv[2][RT];
-        const auto load_w = [&](uint32_t s, uint32_t k) {
+        k_range<TX, TW, MT, RT>(
+            w,
+            [&](const TX*(&x)[MT]) {
 #pragma unroll
-            for (uint32_t f = 0; f < RT; f++) wv[s][f] = ld_eight(w[f] + k);
-        };
-        if (full) load_w(0, k0);  // on their way while the rows are looked up
-        const TX* x[MT];
-#pragma unroll
-        for (uint32_t m = 0; m < MT; m++)  // places without a row read the first one: what comes of it is not used
-            x[m] = static_cast<const TX*>(a.x) + (row[m] < 0 ? 0 : (uint64_t)row[m] * a.ldx) + 8u * q;
-        const auto load_x = [&](uint32_t s, uint32_t k) {
-#pragma unroll
-            for (uint32_t m = 0; m < MT; m++) xv[s][m] = ld_eight(x[m] + k);
-        };
-        const auto load = [&](uint32_t s, uint32_t k) {
-            load_w(s, k);
-            load_x(s, k);
-        };
-        const auto multiply = [&](uint32_t s) {
-#pragma unroll
-            for (uint32_t m = 0; m < MT; m++) {
-                if constexpr (__is_same(TW, float)) {
-#pragma unroll
-                    for (uint32_t f = 0; f < RT; f++)
-#pragma unroll
-                        for (uint32_t j = 0; j < 8u; j++)
-                            acc[m][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[s][f].at(j), xv[s][m].at(j), acc[m][f], 0, 0, 0);
-                } else if constexpr (__is_same(TX, TW)) {
-#pragma unroll
-                    for (uint32_t f = 0; f < RT; f++) acc[m][f] = mfma32<TW>(wv[s][f].v, xv[s][m].v, acc[m][f]);
-                } else {
-                    constexpr uint32_t NP = __is_same(TW, half_t) ? 2u : 3u;
-                    const uint32_t top = top_over_q(top_of_eight(xv[s][m]));
-                    const StepScale scale = step_scale(top);
-                    const float back = scale.back;
-                    u4_t xp[NP];
-                    split_eight<TW, NP>(xv[s][m], scale.up, top, xp);
-#pragma unroll
-                    for (uint32_t f = 0; f < RT; f++) {
-                        f4v_t d = {0, 0, 0, 0};
-#pragma unroll
-                        for (uint32_t n = 0; n < NP; n++) d = mfma32<TW>(wv[s][f].v, xp[NP - 1u - n], d);
-                        acc[m][f] += d * back;
-                    }
-                }
-            }
-        };
-        if (full) load_x(0, k0);
-        for (uint32_t i = 0; i < full; i += 2u) {
-            if (i + 1u < full) load(1, k0 + 32u * (i + 1u));
-            multiply(0);
-            if (i + 2u < full) load(0, k0 + 32u * (i + 2u));
-            if (i + 1u < full) multiply(1);
-        }
-        if (tail) {
-            const uint32_t k = k0 + 32u * full, have = tail > 8u * q ? tail - 8u * q : 0u;
-#pragma unroll
-            for (uint32_t f = 0; f < RT; f++) wv[0][f] = ld_eight(w[f] + k, have);
-#pragma unroll
-            for (uint32_t m = 0; m < MT; m++) xv[0][m] = ld_eight(x[m] + k, have);
-            multiply(0);
-        }
-        mfma_settle();
+                for (uint32_t m = 0; m < MT; m++)  // places without a row read the first one: what comes of it is not used
+                    x[m] = static_cast<const TX*>(a.x) + (row[m] < 0 ? 0 : (uint64_t)row[m] * a.ldx) + 8u * q;
+            },
+            k0, k1, acc);
         __syncthreads();
         if (wave) {
 #pragma unroll
@@ -228,7 +171,7 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
         const int64_t found = lora_row(a, min(p, d.t.end - 1u));
         d.row[m] = p < d.t.end ? found : -1;
     }
-    const uint32_t quarter = (a.k_split / 4u + 31u) & ~31u;
+    const uint32_t quarter = (a.k_split / 4u + 63u) & ~63u;
     const uint32_t end = min(a.k, (d.split + 1u) * a.k_split);
     d.k0 = min(d.split * a.k_split + d.wave * quarter, end);
     d.k1 = min(d.k0 + quarter, end);

@@ -148,7 +148,7 @@ constexpr uint32_t kNormRowsPerWg = 4;  // rows per rfxq_rmsnorm_q8_1 workgroup 
 // kernels of the second code object (half_host.hpp)
 struct HalfKernels {
     hipFunction_t group_rows = nullptr, group_count = nullptr, moe_order = nullptr;
-    hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {};  // [f32 activations, the weights' type][F16, BF16]
+    hipFunction_t any[2][2] = {}, few[2][2] = {}, few4[2][2] = {}, quarters[2] = {};  // [f32 activations, the weights' type][F16, BF16]
     hipFunction_t t64[2] = {}, t256[2] = {};                       // activations of the weights' type
     // [f32 x F32, f32 x F16, f32 x BF16, F16, BF16]
     hipFunction_t lora_down[5][2] = {}, lora_up[5][3] = {};  // [16, 32 rows, 16 rows of any rank and columns]
@@ -218,6 +218,8 @@ int load_half(hipModule_t mod, HalfKernels* h) {
         {&h->few[0][1], "rfxq_grouped_few_f32_bf16"},
         {&h->few[1][0], "rfxq_grouped_few_f16"},
         {&h->few[1][1], "rfxq_grouped_few_bf16"},
+        {&h->quarters[0], "rfxq_grouped_quarters_f32_f16"},
+        {&h->quarters[1], "rfxq_grouped_quarters_f32_bf16"},
         {&h->few4[0][0], "rfxq_grouped_few4_f32_f16"},
         {&h->few4[0][1], "rfxq_grouped_few4_f32_bf16"},
         {&h->few4[1][0], "rfxq_grouped_few4_f16"},

@@ -175,12 +175,14 @@ def test_grouped_gemm(rq, rows, groups, k, n, x_type, w_type, y_type):
     assert kept
 
 
-# sizes at which each kernel is chosen, whole and ragged: few rows over short K with many columns,
-# few rows, tiles copied ahead, tiles through registers, large tiles (f32: above 512 rows a group)
+# sizes at which each kernel is chosen, whole and ragged: few tiles, few rows over short K with many columns
+# (half types, then f32), quarters of K (f32) or tiles copied ahead, tiles through registers, large tiles
 @pytest.mark.parametrize("x_type,w_type,y_type", TYPES)
 @pytest.mark.parametrize("rows,groups,k,n", [
     (150, 128, 128, 520), (70, 64, 1160, 200), (40, 9, 1152, 48), (64, 3, 640, 1032), (20, 1, 264, 24),
-    (400, 4, 200, 136), (1000, 3, 328, 520), (1030, 4, 64, 272), (1500, 2, 136, 264), (1200, 1, 8, 256)])
+    (400, 4, 200, 136), (1000, 3, 328, 520), (1030, 4, 64, 272), (1500, 2, 136, 264), (1200, 1, 8, 256),
+    (128, 64, 520, 1024), (512, 256, 72, 768), (300, 4, 200, 700), (300, 4, 201, 700), (260, 20, 1000, 640),
+    (2000, 4, 72, 2104), (2000, 2, 136, 5200), (1999, 2, 72, 5121)])
 def test_grouped_gemm_each_kernel(rq, rows, groups, k, n, x_type, w_type, y_type):
     _say("grouped_gemm kernels", rows, groups, k, n, x_type, w_type, y_type)
     x, w = _case(rows, groups, k, n, x_type, w_type, rows + k)
@@ -190,7 +192,7 @@ def test_grouped_gemm_each_kernel(rq, rows, groups, k, n, x_type, w_type, y_type
     assert kept
 
 
-@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("rows", [3, 300, 6000])
 def test_grouped_gemm_rows_past_4_gib(rq, rows):
     """Rows of x, y and matrices of a stack whose bytes lie past 32-bit offsets."""
     _say("grouped_gemm past 4 GiB", rows)
