@@ -2,12 +2,12 @@
 // (rfxq_grouped_gemm): y[dst_p][n] = sum_k x[src_p][k] W_g[n][k] for the rows p
 // of group g, f32 accumulation, one rounding to the type of y.
 //
-// f32 activations keep their accuracy: few rows go through f32 matrix
-// instructions, more are split, as a tile is staged, into pieces of the weights'
-// type that add up to them and multiply the same weights. A row's 64 values of a
-// step are scaled by a power of two first, so that the largest lies in [2^14,
-// 2^15) (the matrix instructions take subnormal bf16 operands as 0), and the
-// step's sum is scaled back as it is added:
+// f32 activations keep their accuracy: they are split into pieces of the weights'
+// type that add up to them and multiply the same weights (where a wave has one
+// operand of weights, they go through f32 matrix instructions as they are). A
+// row's 32 or 64 values of a step are scaled by a power of two first, so that the
+// largest lies in [2^14, 2^15) (the matrix instructions take subnormal bf16
+// operands as 0), and the step's sum is scaled back as it is added:
 //   f16:  x = RN16(x) + RN16(the rest): 22 bits or more of every value above
 //         2^-17 of the step's largest, 2^-39 of the largest of every other
 //   bf16: three truncations of 8 bits each: exact
@@ -728,9 +728,10 @@ RFXQ_GROUPED_QUARTERS(f32_bf16, float, __bf16)
 // columns and all of K (WK = 1) or, where that makes too few waves, a quarter of K
 // (WK = 4, the workgroup's waves add their parts in LDS). Loads run a block of 128 of K
 // ahead of the products.
-// f32 activations are multiplied as they are (f32 matrix instructions, the weights
-// widened): 32 cycles for 4 of K, which stays below the time of the weights'
-// memory reads.
+// f32 activations: in pieces where a wave has two operands of weights for them (128
+// experts, 32 tokens over 8 of them, 2048 x 768 f16: 54 us, 5.9 TB/s of weights; 61 with
+// f32 matrix instructions, 256 cycles for 8 x 4 of K and an operand, which the memory
+// reads no longer hid), as they are where it has one (60 x 1024 x 4096: 111 against 127 us).
 template <typename TX, typename TW, uint32_t NT, uint32_t WK>
 RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     constexpr bool F32 = __is_same(TX, float);
@@ -783,17 +784,32 @@ RFXQ_DEV void grouped_few(const GroupedArgs& a) {
     };
     const auto multiply = [&](uint32_t s) {
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; i++)
+        for (uint32_t i = 0; i < 4u; i++) {
+            if constexpr (F32 && WK > 1) {
 #pragma unroll
-            for (uint32_t f = 0; f < NT; f++) {
-                if constexpr (F32) {
+                for (uint32_t f = 0; f < NT; f++)
 #pragma unroll
                     for (uint32_t j = 0; j < 8u; j++)
                         acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(wv[s][i][f].at(j), xv[s][i].at(j), acc[f], 0, 0, 0);
-                } else {
-                    acc[f] = mfma32<TW>(wv[s][i][f].v, xv[s][i].v, acc[f]);
+            } else if constexpr (F32) {
+                constexpr uint32_t NP = __is_same(TW, half_t) ? 2u : 3u;
+                const uint32_t top = top_over_q(top_of_eight(xv[s][i]));
+                const StepScale scale = step_scale(top);
+                const float back = scale.back;
+                u4_t xp[NP];
+                split_eight<TW, NP>(xv[s][i], scale.up, top, xp);
+#pragma unroll
+                for (uint32_t f = 0; f < NT; f++) {
+                    f4v_t d = {0, 0, 0, 0};
+#pragma unroll
+                    for (uint32_t n = 0; n < NP; n++) d = mfma32<TW>(wv[s][i][f].v, xp[NP - 1u - n], d);
+                    acc[f] += d * back;
                 }
+            } else {
+#pragma unroll
+                for (uint32_t f = 0; f < NT; f++) acc[f] = mfma32<TW>(wv[s][i][f].v, xv[s][i].v, acc[f]);
             }
+        }
     };
     if (b0 < whole) {
 #pragma unroll

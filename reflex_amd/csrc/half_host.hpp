@@ -145,15 +145,16 @@ constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offse
 //   few4      16 x 16, K in quarters, weights straight from memory: where its tiles are
 //             at most 3 a CU. There a tile's own time is all: smaller ones on more CUs win
 //             (f16, 8 groups of 16 rows, N x K 1024 x 4096: 18 against 32 with 64 x 128
-//             tiles; 8 x 64 rows, 320 x 1000: 6.4 against 9.4; 1024 of them lose, 115
+//             tiles; 8 x 64 rows, 320 x 1000: 6.4 against 9.4; 16 a CU lose, 115
 //             against 51 at 32 x 32 x 1024 x 4096). Rows that do not start at 16 bytes: 2
 //             a CU (8 x 64 x 320 x 3149 at 2.5: 48 against 41)
 //   few rows  for decode, where every weight is read once: few4 up to 4 rows (64 against
 //             72 on 128 x 768 x 2048 at 4 rows), long K up to 6 (60 x 1024 x 4096 at 6: 96
 //             against 114; 60 x 4096 x 1024: 104 against 96); with short K, up to 2
 //             rows, all of K in a wave (51 against 54 at 2 rows, 66 against 61 at 4), for
-//             f32 activations up to 8 from 6 tiles of 128 columns a CU on (128 x 2048 x 768 at 8:
-//             96 against 105; 768 such tiles, 128 x 768 x 2048: 100 against 91)
+//             f32 activations up to 8 where a CU has a tile of 128 columns, for long K six
+//             (quarters in its place: 128 x 2048 x 768 at 8 105 against 91, 128 x 320 x 1000
+//             33 against 27; 60 x 1024 x 4096 104 against 109)
 //   quarters  32 x 64, K in quarters, f32 activations: few tiles (8 x 64 x 1024 x 4096: 38
 //             against 95; 8 x 64 x 2048 x 768: 17 against 23; from 4 a CU on 36
 //             against 32), and up to 16 rows, long K up to 32 (128 x 768 x 2048 at 16: 96
@@ -182,7 +183,7 @@ GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows
     };
     const GroupedVariant few4 = {c->half.few4[xt][t], 16, 16, 256, true}, few = {c->half.few[xt][t], 16, 128, 256, true};
     if (tiles(16, 16) <= (aligned ? 3u : 2u) * cus) return few4;
-    if (aligned && f32 && mean <= 8u && tiles(16, 128) >= 6u * cus) return few;
+    if (aligned && f32 && mean <= 8u && tiles(16, 128) >= (k < 2048u ? 1u : 6u) * cus) return few;
     if (aligned && !f32 && k < 1024u && mean <= 2u && tiles(16, 128) >= 2u * cus) return few;
     if (aligned && !f32 && k >= 1024u && mean <= (k >= 2048u ? 6u : 4u)) return few4;
     if (f32 && ((aligned && mean <= (k >= 2048u ? 32u : k >= 1024u ? 16u : 0u)) || tiles(32, 64) <= 3u * cus)) return {c->half.quarters[t], 32, 64, 256, false};
