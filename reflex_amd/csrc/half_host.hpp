@@ -74,6 +74,8 @@ int check_stack(const rfxq_weight* w, bool f32_too, const char* what) {
         return fail(RFXQ_ERR_OTHER, "%s: weight of %llu bytes, shape [%u, %u, %u] needs %llu", what,
                     (unsigned long long)w->len, w->in_features, w->out_features, std::max(w->expert_count, 1u),
                     (unsigned long long)need);
+    if (std::max(w->in_features, w->out_features) > 0x7FFFFFFFu)  // sums of these and a tile's size do not wrap
+        return fail(RFXQ_ERR_OTHER, "%s: shape [%u, %u] (each below 2^31)", what, w->in_features, w->out_features);
     if (!w->data) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight data is NULL", what);
     if (reinterpret_cast<uintptr_t>(w->data) % elem_bytes(w->ggml_type))
         return fail(RFXQ_ERR_OTHER, "%s: weight data at %p is not %u-byte aligned", what, w->data,
@@ -86,8 +88,10 @@ int check_rows(const rfxq_rows* r, uint32_t columns, const char* what, const cha
     if (!float_type(r->type)) return fail(RFXQ_ERR_GGUF, "%s: %s of type %u (F32, F16 or BF16)", what, name, r->type);
     if (r->rows == 0) return RFXQ_OK;
     if (!r->data) return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s data is NULL", what, name);
-    if (r->rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "%s: %u rows of %s", what, r->rows, name);
-    if (r->stride < columns || r->stride > (1ull << 40))
+    // as many bytes as an address space holds: products of these do not wrap
+    if (r->rows > 0x7FFFFFFFu || (unsigned __int128)r->rows * r->stride >> 47)
+        return fail(RFXQ_ERR_OTHER, "%s: %u rows of %s, stride=%llu", what, r->rows, name, (unsigned long long)r->stride);
+    if (r->stride < columns)
         return fail(RFXQ_ERR_OTHER, "%s: %s stride=%llu (at least %u columns)", what, name,
                     (unsigned long long)r->stride, columns);
     if (reinterpret_cast<uintptr_t>(r->data) % elem_bytes(r->type))

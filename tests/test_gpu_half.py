@@ -295,6 +295,34 @@ def test_grouped_gemm_not_finite_rows(rq, w_type, k):
         assert (np.abs(y[r].double().numpy() - want[r]) <= b).all(), r
 
 
+# quarters of K (whole and ragged), few rows over short K, tiles through registers
+@pytest.mark.parametrize("w_type", [F16, BF16])
+@pytest.mark.parametrize("rows,groups,k,n", [(300, 4, 136, 700), (300, 4, 203, 700), (512, 256, 72, 768), (2000, 4, 72, 1000),
+                                              (2000, 4, 75, 1000)])
+def test_grouped_gemm_not_finite_rows_each_kernel(rq, rows, groups, k, n, w_type):
+    _say("grouped_gemm not finite", rows, groups, k, n, w_type)
+    x, w = _case(rows, groups, k, n, F32, w_type, 12)
+    at = np.arange(0, 240, 30)
+    x[at[0], 5], x[at[1], 0], x[at[2]] = float("inf"), float("nan"), 0.0
+    x[at[3]] *= 1e37
+    x[at[4]] *= 1e-37
+    x[at[5]], x[at[5], 1] = 0.0, 3e38
+    x[at[6], k - 1], x[at[7], k - 1] = float("-inf"), float("nan")
+    offsets, _ = _grouped(_ids(rows, groups, "all"), groups)
+    y, _ = _run_grouped(rq, x, w, offsets, rows, None, 1, None, F32, rows)
+    x64, w64 = x.double().numpy(), w.double().numpy()
+    lost = at[[0, 1, 6, 7]]
+    assert not torch.isfinite(y[lost]).any() and torch.isnan(y[at[[1, 7]]]).all() and (y[at[2]] == 0).all()
+    got = y.double().numpy()
+    for g in range(groups):
+        r = np.array([p for p in range(offsets[g], offsets[g + 1]) if p not in lost], int)
+        if r.size == 0:
+            continue
+        want = x64[r] @ w64[g].T
+        b = _product_bound(x64[r], w64[g], want, F32, w_type, F32) + k * 2.0 ** -149 * (1 + np.abs(w64[g]).max())
+        assert (np.abs(got[r] - want) <= b).all(), g
+
+
 def test_grouped_gemm_2d_weight_and_new_output(rq):
     x, w = _case(50, 1, 100, 40, F32, F16, 2)
     weight = rq.Weight.from_tensor(w[0].contiguous().to(DEV))

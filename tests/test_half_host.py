@@ -78,6 +78,10 @@ def _grouped(L, x=None, w=None, offsets=5 * P, rows=8, x_index=None, x_div=1, y_
     ({"y": {"stride": 31}}, 12, "stride=31"),
     ({"y": {"data": 2 * P + 64}}, 11, "overlap"),
     ({"rows": 1 << 31}, 12, "rows="),
+    ({"w": {"k": 1 << 31, "n": 1, "length": 1 << 40}}, 12, "shape"),
+    ({"w": {"k": 1, "n": 1 << 31, "length": 1 << 40}}, 12, "shape"),
+    ({"x": {"rows": 1 << 30, "stride": 1 << 40}}, 12, "rows of x"),
+    ({"y": {"rows": 1 << 30, "stride": 1 << 20}}, 12, "rows of y"),
     ({"x_div": 0}, 11, "x_div=0"),
     ({"x_div": 2}, 11, "without x_index"),
     ({"offsets": None}, 11, "offsets is NULL"),
