@@ -128,11 +128,11 @@ struct GroupPlan {
 GroupPlan group_plan(uint32_t n, uint32_t groups) {
     GroupPlan p;
     // One launch, in which every workgroup counts all ids, or a launch of counts before
-    // it (us, 128 groups: 7.4 against 8.0 at 32768 rows, 9.9 against 9.2 at 65536, 15.4
-    // against 10.5 at 131072; 1024 groups, whose counts are longer to add up: 14.8 against
-    // 24 at 131072). 2 rows a thread there (12.0 with 1, 11.4 with 4), 4 from a million on
-    // (33 against 23).
-    const bool many = n > (groups > 256u ? 262144u : 65536u);
+    // it (us, 128 groups: 7.6 against 8.8 at 32768 rows, 10.2 against 8.8 at 65536, 15.6
+    // against 9.7 at 131072; 1024 groups, whose counts are longer to add up: 14.6 against
+    // 16.5 at 131072, 43 against 21 at 300000). 2 rows a thread there (131072: 9.6 with
+    // 1, 11.1 with 4), 4 from 262144 on (a million: 17 against 27).
+    const bool many = n > (groups > 256u ? 131072u : 32768u);
     p.rounds = !many ? 1u : n <= 262144u ? 2u : 4u;
     p.grid = std::max(1u, (n + kGroupThreads * p.rounds - 1u) / (kGroupThreads * p.rounds));
     p.counts = many ? align256(4ull * p.grid * (groups + 1u)) : 0u;

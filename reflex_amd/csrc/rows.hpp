@@ -135,8 +135,8 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_count(GroupRowsArg
 // Workgroup b places rows [b c, (b + 1) c), c = 1024 rounds. It needs each key's
 // rows before its own and in all: up to some ten thousand rows it counts
 // them itself (one launch, no scratch memory; the ids come from L2, the LDS
-// atomics bound it: 15.4 us for 131072 rows, 128 groups), for more it adds up what
-// rfxq_group_count left (10.5 us).
+// atomics bound it: 15.6 us for 131072 rows, 128 groups), for more it adds up what
+// rfxq_group_count left (9.7 us: 2.6 there, 7.2 here, trips to memory and barriers).
 //
 // Dynamic LDS: before[groups + 1], rest[groups + 1] (rows before the
 // workgroup's own; the others), then wcnt[16][groups + 1] (16 bits: a wave's own rows).
@@ -147,22 +147,35 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
     uint32_t* rest = lds + keys;
     uint16_t* wcnt = reinterpret_cast<uint16_t*>(lds + 2u * keys);
     __shared__ uint32_t part[kGroupWaves];
+    const uint32_t chunk = kGroupThreads * a.rounds, begin = blockIdx.x * chunk;
+    // a wave takes 64 neighbouring rows a round; their ids are on their way meanwhile
+    int32_t id[kGroupRounds] = {};
+    if (a.n) {
+#pragma unroll
+        for (uint32_t r = 0; r < kGroupRounds; r++)
+            id[r] = ((const RFXQ_GLOBAL int32_t*)a.ids)[min(begin + (wave * a.rounds + r) * 64u + lane, a.n - 1u)];
+    }
     const uint32_t words = 2u * keys + (kGroupWaves * keys + 1u) / 2u;
     for (uint32_t i = tid; i < words; i += kGroupThreads) lds[i] = 0;
     __syncthreads();
 
-    const uint32_t chunk = kGroupThreads * a.rounds, begin = blockIdx.x * chunk;
     if (a.counts) {
         // the threads of one key take every `parts`th workgroup's counts
         const uint32_t parts = max(kGroupThreads / keys, 1u);
         for (uint32_t j = tid; j < parts * keys; j += kGroupThreads) {
             const uint32_t k = j % keys;
             uint32_t ahead = 0, behind = 0;
-#pragma unroll 8
-            for (uint32_t w = j / keys; w < gridDim.x; w += parts) {
-                const uint32_t c = a.counts[(uint64_t)w * keys + k];
-                ahead += w < blockIdx.x ? c : 0u;
-                behind += w < blockIdx.x ? 0u : c;
+            for (uint32_t w = j / keys; w < gridDim.x; w += 8u * parts) {
+                uint32_t c[8];  // loads without a condition: all on their way at once
+#pragma unroll
+                for (uint32_t u = 0; u < 8u; u++)
+                    c[u] = ((const RFXQ_GLOBAL uint32_t*)a.counts)[(uint64_t)min(w + u * parts, gridDim.x - 1u) * keys + k];
+#pragma unroll
+                for (uint32_t u = 0; u < 8u; u++) {
+                    const uint32_t at = w + u * parts, n = at < gridDim.x ? c[u] : 0u;
+                    ahead += at < blockIdx.x ? n : 0u;
+                    behind += at < blockIdx.x ? 0u : n;
+                }
             }
             atomicAdd(before + k, ahead);
             atomicAdd(rest + k, behind);
@@ -192,8 +205,7 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
     if (tid < a.groups) before[tid] += base;
     if (tid == 0) before[a.groups] += total;
 
-    // the own rows: a wave takes 64 neighbouring rows a round; lanes of one
-    // key find each other by ballots over the key's bits
+    // the own rows: lanes of one key find each other by ballots over the key's bits
     const uint32_t bits = 32u - (uint32_t)__builtin_clz(a.groups);
     const uint64_t below = ((uint64_t)1 << lane) - 1u;
     uint32_t key[kGroupRounds], rank[kGroupRounds];
@@ -202,7 +214,7 @@ extern "C" __global__ __launch_bounds__(1024) void rfxq_group_rows(GroupRowsArgs
         if (r >= a.rounds) break;
         const uint32_t i = begin + (wave * a.rounds + r) * 64u + lane;
         const bool own = i < a.n;
-        key[r] = own ? group_key(a, i) : 0u;
+        key[r] = own ? min((uint32_t)id[r], a.groups) : 0u;
         uint64_t same = __builtin_amdgcn_ballot_w64(own);
         for (uint32_t b = 0; b < bits; b++) {
             const uint64_t set = __builtin_amdgcn_ballot_w64((key[r] >> b) & 1u);
