@@ -308,7 +308,7 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.tiles_m = max_tiles(rows, groups, v.bm);
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of up to 4 row tiles and 4 column tiles, evenly cut, small enough that every XCD has several
-    // (47 x 12 tiles: 76 us with 2 row tiles, 86 with 4)
+    // (47 x 12 tiles: 12% less time with 2 row tiles than with 4)
     const uint32_t across = (a.tiles_n + 3u) / 4u;
     const uint64_t each = (uint64_t)a.tiles_m * across / 64u;
     a.sm = each >= 4u ? 4u : each >= 2u ? 2u : 1u;

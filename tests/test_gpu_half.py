@@ -47,7 +47,8 @@ def _ids(n, groups, how, seed=0):
 
 @pytest.mark.parametrize("how", ["any", "one", "none", "rising", "all"])
 @pytest.mark.parametrize("n,groups", [(0, 5), (1, 1), (2, 3), (63, 2), (64, 128), (65, 1024), (300, 37), (1000, 128),
-                                      (1024, 7), (1025, 1023), (4096, 128), (32768, 3), (32769, 256), (65536, 64), (65537, 1024), (131072, 257), (131073, 900),
+                                      (1024, 7), (1025, 1023), (4096, 128), (32768, 3), (32769, 256), (65536, 64),
+                                      (65537, 1024), (131072, 257), (131073, 900),
                                       (131077, 129), (270001, 256), (300007, 1000)])
 def test_group_rows(rq, n, groups, how):
     _say("group_rows", n, groups, how)
