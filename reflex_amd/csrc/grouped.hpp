@@ -521,7 +521,8 @@ struct GroupedTile {
     // The lower and the upper waves take every other 16 rows of the tile, and leave
     // out those behind the group's last row: FULL has none.
     // 8192 rows over 8 matrices of 14336 x 4096 f16: 0.90 ms, 1.07 PFLOP/s, matrix
-    // pipes 58% busy (64 x 128 tiles: 1.46 ms); without copies 0.66 ms, so LDS bounds it.
+    // pipes 58% busy (64 x 128 tiles: 1.46 ms); without copies 0.66 ms, with all of
+    // them from L2 0.77: their traffic and the clock it costs bound it.
     template <bool FULL>
     __device__ __forceinline__ void turns(u4_t* xs0, u4_t* xs1, u4_t* ws0, u4_t* ws1, f4v_t (&acc)[MF][4]) {
         const uint32_t upper = wave >> 2, l = lane & 15u, q = lane >> 4, row0 = upper * 16u, col0 = (wave & 3u) * 64u;
