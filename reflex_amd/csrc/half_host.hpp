@@ -397,7 +397,7 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
     const uint32_t t = x->type == RFXQ_TYPE_F32 ? (a->ggml_type == RFXQ_TYPE_F32 ? 0u : a->ggml_type == RFXQ_TYPE_F16 ? 1u : 2u)
                        : x->type == RFXQ_TYPE_F16 ? 3u : 4u;
     const uint32_t wide = p.bm == 32u ? 1u : 0u, form = lora_vec(rank, n) ? wide : 2u, ldl = (rank + 31u) & ~31u;
-    const uint32_t pieces = x->type == RFXQ_TYPE_F32 && a->ggml_type == RFXQ_TYPE_BF16 ? 3u : 2u;
+    const uint32_t pieces = a->ggml_type == RFXQ_TYPE_BF16 ? 3u : 2u;
     const uint32_t lds = a->ggml_type == RFXQ_TYPE_F32 ? 4u * p.bm * (ldl + 4u)
                                                        : 2u * pieces * p.bm * (ldl + 8u) + 4u * p.bm * (ldl / 32u);
     if (int rc = launch(c->half.lora_down[t][wide], p.tiles * p.splits, 0, stream, &l, sizeof l, "rfxq_lora_down launch"))

@@ -12,10 +12,11 @@
 // it). Activations and adapters of one half type multiply exactly. f32 values (x,
 // and v always) beside half-typed adapters are split for each step into pieces of
 // the adapters' type, scaled by a power of two per row and step so that the row's
-// largest lies in [2^14, 2^15): 2 pieces of f16 (2^-22 of a value), 3 of bf16
-// (exact; 2 for bf16 results, 2^-15 of v). f32 matrix instructions take 256 cycles for
-// what 2 or 3 half-typed ones and four multiply-adds take about 50 for; they are left
-// for f32 adapters.
+// largest lies in [2^14, 2^15): 2 pieces of f16 (2^-22 of a value, 2^-39 of the
+// largest for values below 2^-17 of it), 3 of bf16 (exact; for bf16 results too: where y
+// and the adapter cancel, what 2 of them lose, 2^-15 of v, is more than the result's
+// rounding). f32 matrix instructions take 256 cycles for what 2 or 3 half-typed ones
+// and four multiply-adds take about 50 for; they are left for f32 adapters.
 #pragma once
 #include "common.hpp"
 #include "grouped.hpp"
@@ -204,7 +205,7 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
 template <typename TX, typename TW, uint32_t MT, uint32_t NF, bool VEC>
 RFXQ_DEV void lora_up(const LoraArgs& a) {
     constexpr bool F32 = __is_same(TW, float);
-    constexpr uint32_t BM = 16u * MT, NP = __is_same(TW, __bf16) && __is_same(TX, float) ? 3u : 2u;
+    constexpr uint32_t BM = 16u * MT, NP = __is_same(TW, __bf16) ? 3u : 2u;
     extern __shared__ uint32_t lds[];
     RowTile t = find_tile(a.offsets, a.groups, a.rows, BM, blockIdx.x / a.across, a.ranks);
     if (!t.any) {  // rows in no group

@@ -713,3 +713,40 @@ def test_same_results_every_time(rq):
     first = _run_lora(rq, x, a, b, ids, ranks, scales, y, False)
     for _ in range(3):
         assert torch.equal(_run_lora(rq, x, a, b, ids, ranks, scales, y, False), first)
+
+
+# ------------------------------------------------------------------ v = A x to its last bit
+
+def _whole_v(rows, count, rank, k, n, x_type, w_type):
+    """A case in which every sum is exact in f32, whatever its order. v is 1.something times a power of two a row,
+    of all the bits that are kept: 24 (F32 adapters: in one value of A; BF16: in three), 22 (F16: in two). Each
+    value of A that counts lies in 32 of K of its own, and a row of B has a single power of two. y is the
+    adapter's part rounded to 8 bits and negated: what is left of their sum is the lower bits of v alone."""
+    gen = torch.Generator().manual_seed(rows + rank)
+    pieces, bits = {F32: (1, 24), F16: (2, 11), BF16: (3, 8)}[w_type]
+    a = torch.randn(count, rank, k, generator=gen).to(w_type)
+    x = torch.zeros(rows, k)
+    sign = torch.where(torch.arange(rows) % 3 == 1, -1.0, 1.0) * 2.0 ** (torch.arange(rows) % 7 - 3)
+    for p in range(pieces):
+        a[:, :, 37 * p + 5] = (1 + 0.9 * torch.rand(count, rank, generator=gen)).to(w_type)
+        x[:, 37 * p + 5] = sign * 2.0 ** (-bits * p)
+    b = torch.zeros(count, n, rank)
+    b[:, torch.arange(n), torch.arange(n) % rank] = 2.0 ** (torch.arange(n) % 3)
+    ids = (torch.arange(rows) * 7 % count).to(torch.int32)
+    v = torch.stack([a[g].double() @ x[r].double() for r, g in enumerate(ids.tolist())])
+    assert torch.equal(v.float().double(), v) and (v.abs() >= 2.0 ** -3).all()
+    delta = 2.0 * v @ b[0].double().t()
+    y = -delta.to(BF16).to(x_type)
+    want = (delta + y.double()).to(x_type)
+    return x.to(x_type), a, b.to(w_type), ids.numpy(), y, want
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,n", [(3, 2, 16, 48), (40, 2, 40, 52), (9, 3, 13, 51), (20, 2, 264, 300)])
+def test_lora_add_keeps_v(rq, rows, count, rank, n, x_type, w_type):
+    """A x is kept to 22 bits beside F16 adapters and to all of f32's 24 beside the others: where y and the
+    adapter cancel, only the result's own rounding is left."""
+    _say("lora_add keeps v", rows, count, rank, n, x_type, w_type)
+    x, a, b, ids, y, want = _whole_v(rows, count, rank, 128, n, x_type, w_type)
+    got = _run_lora(rq, x, a, b, ids, None, [2.0] * count, y, False)
+    assert torch.equal(got, want), (got.double() - want.double()).abs().max()
