@@ -343,9 +343,10 @@ int rfxq_silu_and_mul(const float* gate, const float* up, float* out, uint64_t n
  * host-to-device copy of the routing table; no per-expert launches. Up to 4
  * rows (with 4 <= expert_count <= 1024 and top_k <= 64) run every routed pair
  * as GEMVs planned on the device from the copied routing, the launches of
- * rfxq_moe_ffn_grouped_device. F16 or BF16 stacks (any sizes, up to 1024
- * experts) run as rfxq_group_rows and rfxq_grouped_gemm with f32 activations
- * kept to f32 accuracy; out must not overlap x then. */
+ * rfxq_moe_ffn_grouped_device. F16 or BF16 stacks (each of either type, any
+ * sizes and alignment of whole elements, up to 1024 experts, top_k <= 64,
+ * rows * top_k <= 2^24) run as rfxq_group_rows and rfxq_grouped_gemm with f32
+ * activations (its accuracy, and its limits); out must not overlap x then. */
 int rfxq_moe_ffn_grouped(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits_host,
                          uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
                          const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out,
@@ -371,8 +372,8 @@ int rfxq_moe_route_device(const float* logits, uint32_t tokens, uint32_t expert_
  * rows and the waves of workgroups their tiles need). Requires
  * 4 <= expert_count <= 1024, top_k <= 64 and rows * top_k <= 16384.
  * Routing errors of the host path (non-finite softmax sums) are not
- * reported: such tokens get non-finite outputs. F16 or BF16 stacks: as
- * rfxq_moe_ffn_grouped, with 1 <= expert_count <= 1024 and rows * top_k <= 2^24. */
+ * reported: such tokens get non-finite outputs. F16 or BF16 stacks: what
+ * rfxq_moe_ffn_grouped takes, with 1 <= expert_count <= 1024. */
 int rfxq_moe_ffn_grouped_device(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits,
                                 uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
                                 const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out,

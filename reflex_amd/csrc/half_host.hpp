@@ -414,14 +414,11 @@ bool half_layer(const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weigh
     return gate && up && down && half_type(gate->ggml_type) && half_type(up->ggml_type) && half_type(down->ggml_type);
 }
 
-// rfxq_moe_ffn_grouped(_device) over F16 or BF16 stacks: the routing (from the
-// device's logits, or the host's, copied up), rfxq_group_rows, three grouped
-// products of f32 activations and the combine in increasing expert order.
-int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits, const uint32_t* host_idx,
-             const float* host_w, uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
-             const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out, hipStream_t stream) {
-    if (!x || !out) return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped: NULL argument");
-    if (rows == 0) return ok();
+// What rfxq_moe_ffn_grouped(_device) refuse of a layer with such stacks, before any
+// routing. Of its own: gate and up may be of two half types, and x and the stacks
+// start at any element.
+int check_moe_half(const float* x, uint32_t rows, uint32_t hidden, uint32_t expert_count, uint32_t top_k,
+                   const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, const float* out) {
     if (gate->expert_count != expert_count || up->expert_count != expert_count || down->expert_count != expert_count)
         return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: expert tensors must have expert_count=%u", expert_count);
     if (gate->in_features != hidden || up->in_features != hidden || down->out_features != hidden ||
@@ -441,9 +438,23 @@ int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router
     if (P64 > kMaxGroupRows)
         return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: %llu routed pairs (at most %u)", (unsigned long long)P64,
                     kMaxGroupRows);
-    const uint32_t P = (uint32_t)P64, ffn = gate->out_features;
+    if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % 4u)
+        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: x or out not 4-byte aligned");
     if (overlap(x, 4ull * rows * hidden, out, 4ull * rows * hidden))
         return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped: x and out overlap");
+    return RFXQ_OK;
+}
+
+// rfxq_moe_ffn_grouped(_device) over F16 or BF16 stacks: the routing (from the
+// device's logits, or the host's, copied up), rfxq_group_rows, three grouped
+// products of f32 activations and the combine in increasing expert order.
+int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits, const uint32_t* host_idx,
+             const float* host_w, uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
+             const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out, hipStream_t stream) {
+    if (!x || !out) return fail(RFXQ_ERR_INVALID_INPUT, "moe_ffn_grouped: NULL argument");
+    if (rows == 0) return ok();
+    if (int rc = check_moe_half(x, rows, hidden, expert_count, top_k, gate, up, down, out)) return rc;
+    const uint32_t P = rows * top_k, ffn = gate->out_features;
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
     const uint64_t pairs = align256(4ull * P), wide = align256(4ull * P * ffn);

@@ -2978,6 +2978,8 @@ int moe_grouped_device(const float* x, uint32_t rows, uint32_t hidden, const flo
                        const rfxq_weight* down, float* out, hipStream_t stream);
 // the same layer with F16 or BF16 stacks (half_host.hpp)
 bool half_layer(const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down);
+int check_moe_half(const float* x, uint32_t rows, uint32_t hidden, uint32_t expert_count, uint32_t top_k,
+                   const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, const float* out);
 int moe_half(const float* x, uint32_t rows, uint32_t hidden, const float* router_logits, const uint32_t* host_idx,
              const float* host_w, uint32_t expert_count, uint32_t top_k, int normalize, float weight_scale,
              const rfxq_weight* gate, const rfxq_weight* up, const rfxq_weight* down, float* out, hipStream_t stream);
@@ -3001,18 +3003,20 @@ int rfxq_moe_ffn_grouped(const float* x, uint32_t rows, uint32_t hidden, const f
                     down->out_features, hidden);
     const uint32_t ffn = gate->out_features;
     const bool half = half_layer(gate, up, down);
-    rfxq_weight g0, u0, d0;
-    if (int rc = expert_slice(gate, 0, &g0, "moe_ffn_grouped gate")) return rc;
-    if (int rc = expert_slice(up, 0, &u0, "moe_ffn_grouped up")) return rc;
-    if (int rc = expert_slice(down, 0, &d0, "moe_ffn_grouped down")) return rc;
-    if (!half) {
+    rfxq_weight g0, u0, d0;  // of the first expert
+    if (half) {
+        if (int rc = check_moe_half(x, rows, hidden, expert_count, top_k, gate, up, down, out)) return rc;
+    } else {
+        if (int rc = expert_slice(gate, 0, &g0, "moe_ffn_grouped gate")) return rc;
+        if (int rc = expert_slice(up, 0, &u0, "moe_ffn_grouped up")) return rc;
+        if (int rc = expert_slice(down, 0, &d0, "moe_ffn_grouped down")) return rc;
         if (int rc = check_mmq_weight(&g0, "moe_ffn_grouped gate")) return rc;
         if (int rc = check_mmq_weight(&u0, "moe_ffn_grouped up")) return rc;
         if (int rc = check_mmq_weight(&d0, "moe_ffn_grouped down")) return rc;
+        if (gate->ggml_type != up->ggml_type)
+            return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: gate and up must share a type");
+        if (reinterpret_cast<uintptr_t>(x) % 16u) return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: x not 16-byte aligned");
     }
-    if (gate->ggml_type != up->ggml_type)
-        return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: gate and up must share a type");
-    if (reinterpret_cast<uintptr_t>(x) % 16u) return fail(RFXQ_ERR_OTHER, "moe_ffn_grouped: x not 16-byte aligned");
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
 

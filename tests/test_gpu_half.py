@@ -750,3 +750,27 @@ def test_lora_add_keeps_v(rq, rows, count, rank, n, x_type, w_type):
     x, a, b, ids, y, want = _whole_v(rows, count, rank, 128, n, x_type, w_type)
     got = _run_lora(rq, x, a, b, ids, None, [2.0] * count, y, False)
     assert torch.equal(got, want), (got.double() - want.double()).abs().max()
+
+
+def test_moe_ffn_grouped_half_one_rule_for_both_entries(rq):
+    """Gate and up of two half types, x at any element, stacks in memory that is longer than they are: layers that
+    the device-routed entry runs, the host-routed one runs too. Bound: see test_expert_layer_and_adapters."""
+    tokens, groups, hidden, ffn, top_k = 6, 5, 72, 40, 2
+    x, logits, w = _layer_inputs(tokens, groups, hidden, ffn, F16, 9)
+    w[1] = w[1].to(BF16)
+    weights = []
+    for t in w:
+        memory = torch.cat([t.reshape(-1), torch.full((3,), float("nan"), dtype=t.dtype)]).to(DEV)
+        weights.append(rq.Weight(rq.GgmlType.F16 if t.dtype == F16 else rq.GgmlType.BF16, memory,
+                                 list(reversed(t.shape)), len=memory.numel() * 2))
+    memory = torch.full((1 + tokens * hidden,), float("nan"), device=DEV)
+    xd = memory[1:]
+    xd.copy_(x.reshape(-1))
+    ld = logits.to(DEV).reshape(-1)
+    ids, share = rq.moe_route_device(ld, tokens, groups, top_k, True, 1.0)
+    want = _layer_64(x, ids.cpu(), share.cpu(), w)
+    for entry, lg in ((rq.moe_ffn_grouped_device, ld), (rq.moe_ffn_grouped, logits.numpy())):
+        _say("moe_ffn_grouped", entry.__name__)
+        out = torch.full((tokens * hidden,), float("nan"), device=DEV)
+        entry(xd, tokens, hidden, lg, groups, top_k, True, 1.0, *weights, out)
+        assert (out.cpu().view(tokens, hidden).double() - want).norm() <= 2.0 ** -17 * want.norm()

@@ -140,6 +140,43 @@ def test_lora_add_refusals(L, change, code, text):
     _expect(L, _lora(L, **a), code, text)
 
 
+def _layer(L, entry, rows=4, experts=16, top_k=2, logits=None, x=2 * P, out=8 * P, gate=None, up=None, down=None):
+    logits = logits or (ctypes.c_float * (rows * experts))()
+    w = [_weight(**{"k": 32, "n": 48, "e": experts, **(gate or {})}), _weight(**{"k": 32, "n": 48, "e": experts, **(up or {})}),
+         _weight(**{"k": 48, "n": 32, "e": experts, **(down or {})})]
+    return getattr(L, entry)(x, rows, 32, logits, experts, top_k, 1, 1.0, *map(ctypes.byref, w), out, None)
+
+
+@pytest.mark.parametrize("entry", ["rfxq_moe_ffn_grouped", "rfxq_moe_ffn_grouped_device"])
+@pytest.mark.parametrize("change,code,text", [
+    ({"rows": 1 << 21, "top_k": 16, "logits": 3 * P}, 12, "33554432 routed pairs"),  # before any logit is read
+    ({"top_k": 17}, 12, "route_top_k: k (17)"),
+    ({"experts": 128, "top_k": 65}, 12, "route_top_k: k (65)"),
+    ({"experts": 1025, "logits": 3 * P}, 12, "expert_count=1025"),
+    ({"up": {"k": 31}}, 12, "shapes"),
+    ({"up": {"e": 15}}, 12, "expert_count=16"),
+    ({"down": {"length": 100}}, 12, "weight of 100 bytes"),
+    ({"gate": {"data": P + 1}}, 12, "aligned"),
+    ({"out": 2 * P + 64}, 11, "overlap"),
+    ({"x": 2 * P + 2}, 12, "4-byte aligned"),
+    ({"x": None}, 11, "NULL"),
+])
+def test_half_layer_refusals(L, entry, change, code, text):
+    """Both entry points refuse the same layers of F16 / BF16 stacks, before any routing."""
+    _expect(L, _layer(L, entry, **change), code, text)
+
+
+@pytest.mark.parametrize("entry", ["rfxq_moe_ffn_grouped", "rfxq_moe_ffn_grouped_device"])
+@pytest.mark.parametrize("change", [{"up": {"ty": BF16}}, {"x": 2 * P + 4}, {"down": {"length": 48 * 32 * 16 * 2 + 2}}])
+def test_half_layers_of_any_half_types_and_alignment(L, entry, change):
+    """What the device-routed entry takes, the host-routed one takes too: no refusal of the layer itself (none at
+    rows = 0; with rows, on a machine without a GPU, the missing device is what fails)."""
+    if not torch.cuda.is_available():
+        rc = _layer(L, entry, **change)
+        assert rc not in (0, 1, 11, 12), L.rfxq_last_error()
+    assert _layer(L, entry, **{**change, "rows": 0}) == 0
+
+
 def test_workspace_sizes(L):
     # a buffer for the most rows holds any fewer rows' needs
     a = _weight(k=4096, n=64, e=64)
