@@ -425,7 +425,7 @@ struct GroupedTile {
     static constexpr uint32_t THREADS = 64u * WM * WN, MF = BM / WM / 16;
     static constexpr uint32_t NX = BM * 8u / THREADS, NW = BN * 8u / THREADS, LOADS = NX + NW;
     static constexpr uint32_t PAST = 0xFFFFFFF0u;
-    static_assert(BN == 64 * WN && NX >= 1 && NW >= 1 && STAGES >= 2 && STAGES <= 4 && (STAGES - 2) * LOADS < 64);
+    static_assert(BN == 64 * WN && NX >= 1 && NW >= 1 && LOADS < 64);
 
     RowTile t;
     rsrc_t xr, wr;
@@ -478,35 +478,23 @@ struct GroupedTile {
     }
 
     __device__ __forceinline__ void run(const GroupedArgs& a) {
-        __shared__ u4_t xs0[BM * 8], xs1[BM * 8], xs2[STAGES > 2 ? BM * 8 : 1], xs3[STAGES > 3 ? BM * 8 : 1];
-        __shared__ u4_t ws0[BN * 8], ws1[BN * 8], ws2[STAGES > 2 ? BN * 8 : 1], ws3[STAGES > 3 ? BN * 8 : 1];
+        static_assert(STAGES == 3);
+        __shared__ u4_t xs0[BM * 8], xs1[BM * 8], xs2[BM * 8], ws0[BN * 8], ws1[BN * 8], ws2[BN * 8];
         if (!begin(a)) return;
         f4v_t acc[MF][4] = {};
         const uint32_t row0 = (wave / WN) * (BM / WM), col0 = (wave % WN) * 64u;
         issue(xs0, ws0);
-        if constexpr (STAGES > 2) issue(xs1, ws1);
-        if constexpr (STAGES > 3) issue(xs2, ws2);
+        issue(xs1, ws1);
         const auto step = [&](const u4_t* xs, const u4_t* ws, u4_t* nx, u4_t* nw) {
-            constexpr uint32_t left = (STAGES - 2) * LOADS;  // copies of later steps
-            __builtin_amdgcn_s_waitcnt(0x0F70 | (left & 15u) | (left >> 4) << 14);
+            __builtin_amdgcn_s_waitcnt(0x0F70 | (LOADS & 15u) | (LOADS >> 4) << 14);  // all but the next step's copies
             lds_barrier();
             issue(nx, nw);
             tile_step<T, MF, 1, 0>(xs, ws, row0, col0, acc);
         };
-        for (uint32_t s = 0; s < steps; s += STAGES) {
-            if constexpr (STAGES == 2) {
-                step(xs0, ws0, xs1, ws1);
-                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
-            } else if constexpr (STAGES == 3) {
-                step(xs0, ws0, xs2, ws2);
-                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
-                if (s + 2u < steps) step(xs2, ws2, xs1, ws1);
-            } else {
-                step(xs0, ws0, xs3, ws3);
-                if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
-                if (s + 2u < steps) step(xs2, ws2, xs1, ws1);
-                if (s + 3u < steps) step(xs3, ws3, xs2, ws2);
-            }
+        for (uint32_t s = 0; s < steps; s += 3u) {
+            step(xs0, ws0, xs2, ws2);
+            if (s + 1u < steps) step(xs1, ws1, xs0, ws0);
+            if (s + 2u < steps) step(xs2, ws2, xs1, ws1);
         }
         __builtin_amdgcn_s_waitcnt(0x0F70);  // no copy outlives the workgroup
         tile_out<T, MF>(a, t, row0, n0 + col0, acc);
