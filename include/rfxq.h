@@ -428,6 +428,21 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
                       const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
                       hipStream_t stream);
 
+/* Test hook: the kernel and row tile that rfxq_grouped_gemm runs on the current
+ * device (256 compute units before rfxq_init) for `rows` places of x and w; no
+ * memory is read. */
+#define RFXQ_GROUPED_FEW4 0     /* weights straight from memory, K in quarters */
+#define RFXQ_GROUPED_FEW 1      /* weights straight from memory, all of K in a wave */
+#define RFXQ_GROUPED_QUARTERS 2 /* f32 activations, K in quarters */
+#define RFXQ_GROUPED_LARGE 3    /* 256 x 256 tiles */
+#define RFXQ_GROUPED_COPIED 4   /* 64 x 128 tiles, copies into three buffers */
+#define RFXQ_GROUPED_TILES 5    /* 64 x 128 tiles through registers */
+typedef struct rfxq_grouped_policy {
+    uint32_t kernel; /* RFXQ_GROUPED_* */
+    uint32_t tile_m, tile_n;
+} rfxq_grouped_policy;
+int rfxq_grouped_gemm_policy(const rfxq_rows* x, const rfxq_weight* w, uint32_t rows, rfxq_grouped_policy* out);
+
 /* Low-rank adapters of many requests beside a projection that all rows share:
  * for the rows r = order[p] (NULL: p) of group g, offsets[g] <= p < offsets[g + 1],
  *   out[r] = y[r] + scales[g] * B_g (A_g x[r])

@@ -42,6 +42,12 @@ class RfxqRows(ctypes.Structure):
                 ("stride", ctypes.c_uint64)]
 
 
+class RfxqGroupedPolicy(ctypes.Structure):
+    """``rfxq_grouped_policy`` (include/rfxq.h)."""
+
+    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32)]
+
+
 class RfxqOptions(ctypes.Structure):
     """``rfxq_options`` (include/rfxq.h)."""
 
@@ -127,6 +133,7 @@ SIGNATURES = {
     "rfxq_group_rows": (_I, [_P, _U32, _U32, _P, _P, _P, _U64, _P]),
     "rfxq_group_rows_workspace_size": (_U64, [_U32, _U32]),
     "rfxq_grouped_gemm": (_I, [_RP, _WP, _P, _U32, _P, _U32, _P, _RP, _P]),
+    "rfxq_grouped_gemm_policy": (_I, [_RP, _WP, _U32, ctypes.POINTER(RfxqGroupedPolicy)]),
     "rfxq_lora_add": (_I, [_RP, _WP, _WP, _P, _P, _P, _P, _RP, _RP, _P, _U64, _P]),
     "rfxq_lora_add_workspace_size": (_U64, [_WP, _U32]),
 }

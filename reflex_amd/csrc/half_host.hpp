@@ -174,26 +174,45 @@ constexpr uint64_t kMaxOffset = 0xFFFFFFF0ull;  // bytes a buffer's 32-bit offse
 //             without (8 x 192 x 4096 x 4096: 105 against 88)
 //   tiles     64 x 128 through registers: the rest
 struct GroupedVariant {
-    hipFunction_t f;
+    uint32_t kernel;  // RFXQ_GROUPED_*
     uint32_t bm, bn, threads;
-    bool few;
 };
-GroupedVariant grouped_variant(const Ctx* c, uint32_t t, bool f32, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n,
-                               bool aligned, bool copies) {
-    const uint32_t used = std::min(rows, groups), mean = rows / used, xt = f32 ? 0u : 1u;
-    const uint64_t cus = (uint64_t)c->cus;
+GroupedVariant grouped_variant(uint64_t cus, bool f32, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n, bool aligned,
+                               bool copies) {
+    const uint32_t used = std::min(rows, groups), mean = rows / used;
     const auto tiles = [&](uint32_t bm, uint32_t bn) {
         return (uint64_t)used * ((mean + bm - 1u) / bm) * (((uint64_t)n + bn - 1u) / bn);
     };
-    const GroupedVariant few4 = {c->half.few4[xt][t], 16, 16, 256, true}, few = {c->half.few[xt][t], 16, 128, 256, true};
+    const GroupedVariant few4 = {RFXQ_GROUPED_FEW4, 16, 16, 256}, few = {RFXQ_GROUPED_FEW, 16, 128, 256};
     if (tiles(16, 16) <= (aligned ? 3u : 2u) * cus) return few4;
     if (aligned && f32 && mean <= 8u && tiles(16, 128) >= (k < 2048u ? 1u : 6u) * cus) return few;
     if (aligned && !f32 && k < 1024u && mean <= 2u && tiles(16, 128) >= 2u * cus) return few;
     if (aligned && !f32 && k >= 1024u && mean <= (k >= 2048u ? 6u : 4u)) return few4;
-    if (f32 && ((aligned && mean <= (k >= 2048u ? 32u : k >= 1024u ? 16u : 0u)) || tiles(32, 64) <= 3u * cus)) return {c->half.quarters[t], 32, 64, 256, false};
-    if (copies && mean > 160u && 8u * tiles(256, 256) >= 5u * cus) return {c->half.t256[t], 256, 256, 512, false};
-    if (copies && tiles(64, 128) <= 2u * cus) return {c->half.t64[t], 64, 128, 256, false};
-    return {c->half.any[xt][t], 64, 128, 256, false};
+    if (f32 && ((aligned && mean <= (k >= 2048u ? 32u : k >= 1024u ? 16u : 0u)) || tiles(32, 64) <= 3u * cus))
+        return {RFXQ_GROUPED_QUARTERS, 32, 64, 256};
+    if (copies && mean > 160u && 8u * tiles(256, 256) >= 5u * cus) return {RFXQ_GROUPED_LARGE, 256, 256, 512};
+    if (copies && tiles(64, 128) <= 2u * cus) return {RFXQ_GROUPED_COPIED, 64, 128, 256};
+    return {RFXQ_GROUPED_TILES, 64, 128, 256};
+}
+// the kernel for `rows` (> 0) places of checked x and w (x->rows > 0)
+GroupedVariant grouped_variant(uint64_t cus, const rfxq_rows* x, const rfxq_weight* w, uint32_t rows) {
+    const uint32_t k = w->in_features, n = w->out_features;
+    const bool f32 = x->type == RFXQ_TYPE_F32;
+    const bool aligned = aligned16(x->data) && x->stride % (f32 ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
+    // asynchronous copies: half types, rows at whole 16 bytes, 32-bit offsets
+    const bool copies = aligned && !f32 && rows_span(x, k) < kMaxOffset && 2ull * k * n < kMaxOffset;
+    return grouped_variant(cus, f32, rows, std::max(w->expert_count, 1u), k, n, aligned, copies);
+}
+hipFunction_t grouped_function(const HalfKernels& h, uint32_t kernel, bool f32, uint32_t w_type) {
+    const uint32_t t = w_type == RFXQ_TYPE_F16 ? 0u : 1u, xt = f32 ? 0u : 1u;
+    switch (kernel) {
+        case RFXQ_GROUPED_FEW4: return h.few4[xt][t];
+        case RFXQ_GROUPED_FEW: return h.few[xt][t];
+        case RFXQ_GROUPED_QUARTERS: return h.quarters[t];
+        case RFXQ_GROUPED_LARGE: return h.t256[t];
+        case RFXQ_GROUPED_COPIED: return h.t64[t];
+        default: return h.any[xt][t];
+    }
 }
 
 // ------------------------------------------------------------------ adapters
@@ -258,6 +277,18 @@ int rfxq_group_rows(const int32_t* ids, uint32_t n, uint32_t groups, int32_t* of
     return ok();
 }
 
+int rfxq_grouped_gemm_policy(const rfxq_rows* x, const rfxq_weight* w, uint32_t rows, rfxq_grouped_policy* out) {
+    if (!out) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_policy: NULL output");
+    if (int rc = check_stack(w, false, "grouped_gemm_policy")) return rc;
+    if (int rc = check_rows(x, w->in_features, "grouped_gemm_policy", "x")) return rc;
+    if (rows == 0 || rows > 0x7FFFFFFFu || x->rows == 0)
+        return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_policy: rows=%u of %u", rows, x->rows);
+    const Ctx* c = loaded_ctx();
+    const GroupedVariant v = grouped_variant(c ? (uint64_t)c->cus : 256u, x, w, rows);
+    *out = {v.kernel, v.bm, v.bn};
+    return ok();
+}
+
 int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
                       const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
                       hipStream_t stream) {
@@ -280,7 +311,7 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
         return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm: x and y overlap");
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
-    const uint32_t t = ty == RFXQ_TYPE_F16 ? 0u : 1u, groups = std::max(w->expert_count, 1u);
+    const uint32_t groups = std::max(w->expert_count, 1u);
     GroupedArgs a;
     std::memset(&a, 0, sizeof a);
     a.x = x->data;
@@ -300,11 +331,8 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.n = n;
     a.groups = groups;
     a.y_f32 = y->type == RFXQ_TYPE_F32 ? 1u : 0u;
-    const bool f32 = x->type == RFXQ_TYPE_F32;
-    const bool aligned = aligned16(x->data) && x->stride % (f32 ? 4u : 8u) == 0 && aligned16(w->data) && k % 8u == 0;
-    // asynchronous copies: half types, rows at whole 16 bytes, 32-bit offsets
-    const bool copies = aligned && !f32 && rows_span(x, k) < kMaxOffset && 2ull * k * n < kMaxOffset;
-    const GroupedVariant v = grouped_variant(c, t, f32, rows, groups, k, n, aligned, copies);
+    const GroupedVariant v = grouped_variant((uint64_t)c->cus, x, w, rows);
+    const bool few = v.kernel == RFXQ_GROUPED_FEW4 || v.kernel == RFXQ_GROUPED_FEW;
     a.tiles_m = max_tiles(rows, groups, v.bm);
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of up to 4 row tiles and 4 column tiles, evenly cut, small enough that every XCD has several
@@ -314,11 +342,13 @@ int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* o
     a.sm = each >= 4u ? 4u : each >= 2u ? 2u : 1u;
     a.sn = (a.tiles_n + across - 1u) / across;
     const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
-    const uint64_t grid = v.few ? (uint64_t)a.tiles_m * a.tiles_n : (blocks + 7u) / 8u * 8u * a.sm * a.sn;
+    const uint64_t grid = few ? (uint64_t)a.tiles_m * a.tiles_n : (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
         return fail(RFXQ_ERR_OTHER, "grouped_gemm: %u rows x %u columns need %llu workgroups", rows, n,
                     (unsigned long long)grid);
-    if (int rc = launch(v.f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_grouped launch", v.threads)) return rc;
+    if (int rc = launch(grouped_function(c->half, v.kernel, x->type == RFXQ_TYPE_F32, ty), (uint32_t)grid, 0, stream, &a,
+                        sizeof a, "rfxq_grouped launch", v.threads))
+        return rc;
     return ok();
 }
 

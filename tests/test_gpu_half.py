@@ -774,3 +774,34 @@ def test_moe_ffn_grouped_half_one_rule_for_both_entries(rq):
         out = torch.full((tokens * hidden,), float("nan"), device=DEV)
         entry(xd, tokens, hidden, lg, groups, top_k, True, 1.0, *weights, out)
         assert (out.cpu().view(tokens, hidden).double() - want).norm() <= 2.0 ** -17 * want.norm()
+
+
+FEW4, FEW, QUARTERS, LARGE, COPIED, TILES = range(6)  # rfxq_grouped_policy.kernel
+
+
+# (kernel of half-typed, of f32 activations): ten steps of 64 of K and more, so that every buffer is filled
+# again several times; odd and even numbers of steps, whole and with a tail
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES)
+@pytest.mark.parametrize("rows,groups,k,n,shift,half_kernel,f32_kernel", [
+    (1500, 2, 704, 7168, 0, LARGE, TILES), (1500, 2, 776, 7161, 0, LARGE, TILES), (1536, 2, 640, 7168, 0, LARGE, TILES),
+    (1000, 3, 704, 520, 0, COPIED, QUARTERS), (1000, 3, 776, 520, 0, COPIED, QUARTERS), (999, 3, 648, 513, 0, COPIED, QUARTERS),
+    (2000, 4, 704, 2104, 0, TILES, TILES), (2000, 4, 776, 2104, 0, TILES, TILES), (2000, 4, 649, 2103, 1, TILES, TILES),
+    (600, 4, 771, 1400, 3, TILES, QUARTERS), (400, 4, 2888, 1000, 0, COPIED, QUARTERS), (400, 4, 2891, 1001, 1, TILES, QUARTERS),
+    (150, 40, 1160, 1032, 0, FEW4, FEW), (60, 32, 1992, 1024, 0, FEW4, FEW), (40, 9, 1355, 48, 1, FEW4, FEW4),
+    (70, 64, 904, 1032, 0, FEW, FEW)])
+def test_grouped_gemm_many_steps(rq, rows, groups, k, n, shift, half_kernel, f32_kernel, x_type, w_type, y_type):
+    import ctypes
+
+    want = f32_kernel if x_type == F32 else half_kernel
+    _say("grouped_gemm many steps", rows, groups, k, n, shift, x_type, w_type, y_type)
+    x, w = _case(rows, groups, k, n, x_type, w_type, rows + k)
+    p = rq.RfxqGroupedPolicy()
+    xr = rq.RfxqRows(1 << 20 | x.element_size() * shift, {F32: 0, F16: 1, BF16: 30}[x_type], rows, k + 8 - k % 8)
+    wt = rq.Weight.from_tensor(w)
+    rq.lib().rfxq_grouped_gemm_policy(ctypes.byref(xr), wt.cref(), rows, ctypes.byref(p))
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert p.kernel == want
+    offsets, order = _grouped(_ids(rows, groups, "all"), groups)
+    y, kept = _run_grouped(rq, x, w, offsets, rows, order, 1, order, y_type, rows, (8 - k % 8, shift), (8, 0), 8 * (shift == 0))
+    _check_grouped(x, w, offsets, order, 1, order, y)
+    assert kept

@@ -104,6 +104,52 @@ def test_grouped_gemm_of_nothing(L, empty):
     assert _grouped(L, **a) == 0
 
 
+FEW4, FEW, QUARTERS, LARGE, COPIED, TILES = range(6)
+
+
+@pytest.mark.parametrize("rows,groups,k,n,f32,shift,kernel", [
+    # few tiles, of either kind; rows that do not start at 16 bytes up to a lower limit
+    (20, 1, 264, 24, True, 0, FEW4), (48, 3, 640, 4096, False, 0, FEW4), (48, 3, 640, 4112, False, 0, COPIED),
+    (32, 2, 640, 4096, False, 2, FEW4), (32, 2, 640, 4112, False, 2, TILES),
+    # few rows a group
+    (256, 128, 768, 2048, True, 0, FEW), (512, 256, 72, 768, False, 0, FEW), (768, 256, 72, 768, False, 0, TILES),
+    (512, 128, 1024, 2048, False, 0, FEW4), (640, 128, 1024, 2048, False, 0, TILES),
+    (60, 32, 1992, 1024, True, 0, FEW), (60, 32, 1992, 1016, True, 0, FEW), (60, 32, 1992, 896, True, 0, QUARTERS),
+    # f32 in quarters of K: long K, or few tiles
+    (4096, 128, 2048, 768, True, 0, QUARTERS), (4224, 128, 2048, 768, True, 0, TILES), (512, 8, 4096, 1024, True, 0, QUARTERS),
+    (1000, 4, 203, 700, True, 1, QUARTERS), (2000, 4, 72, 2104, True, 0, TILES),
+    # large tiles, tiles copied ahead, tiles through registers
+    (1500, 2, 704, 7168, False, 0, LARGE), (1500, 2, 704, 6400, False, 0, TILES), (1500, 2, 704, 7168, False, 2, TILES),
+    (1500, 2, 708, 7168, False, 0, TILES), (1000, 3, 704, 520, False, 0, COPIED), (2000, 4, 776, 2104, False, 0, TILES),
+])
+def test_grouped_gemm_kernel(L, rows, groups, k, n, f32, shift, kernel):
+    """The kernel that the rule takes for 256 compute units."""
+    import reflex_amd as rq
+
+    if torch.cuda.is_available():
+        pytest.skip("the rule for the device's own compute units")
+    p = rq.RfxqGroupedPolicy()
+    x = _rows(F32 if f32 else F16, rows, k + 8 - k % 8, 2 * P + (4 if f32 else 1) * shift)
+    w = _weight(F16, k, n, groups)
+    assert L.rfxq_grouped_gemm_policy(ctypes.byref(x), ctypes.byref(w), rows, ctypes.byref(p)) == 0
+    tile = {FEW4: (16, 16), FEW: (16, 128), QUARTERS: (32, 64), LARGE: (256, 256)}.get(kernel, (64, 128))
+    assert (p.kernel, (p.tile_m, p.tile_n)) == (kernel, tile)
+
+
+def test_grouped_gemm_kernel_refusals(L):
+    import reflex_amd as rq
+
+    p, x, w = rq.RfxqGroupedPolicy(), _rows(), _weight()
+    ask = lambda x, w, rows, out: L.rfxq_grouped_gemm_policy(  # noqa: E731
+        *(None if v is None else ctypes.byref(v) for v in (x, w)), rows, None if out is None else ctypes.byref(out))
+    _expect(L, ask(x, w, 8, None), 11, "NULL output")
+    _expect(L, ask(None, w, 8, p), 11, "x is NULL")
+    _expect(L, ask(x, None, 8, p), 11, "weight is NULL")
+    _expect(L, ask(x, w, 0, p), 11, "rows=0")
+    _expect(L, ask(_rows(rows=0), w, 8, p), 11, "of 0")
+    _expect(L, ask(x, _weight(ty=Q4K), 8, p), 1, "F16 or BF16")
+
+
 def _lora(L, x=None, a=None, b=None, y=None, out=None, offsets=9 * P, ws=None, ws_bytes=0):
     ref = lambda v: None if v is None else ctypes.byref(v)  # noqa: E731
     return L.rfxq_lora_add(ref(x), ref(a), ref(b), None, None, offsets, None, ref(y), ref(out), ws, ws_bytes, None)
