@@ -805,3 +805,63 @@ def test_grouped_gemm_many_steps(rq, rows, groups, k, n, shift, half_kernel, f32
     y, kept = _run_grouped(rq, x, w, offsets, rows, order, 1, order, y_type, rows, (8 - k % 8, shift), (8, 0), 8 * (shift == 0))
     _check_grouped(x, w, offsets, order, 1, order, y)
     assert kept
+
+
+# ------------------------------------------------------------------ adapters: orders and offsets of any values
+
+def _lora_ordered(rq, c, offsets, order):
+    """lora_add on given offsets and order (out apart from y): the result, what lies around it unchanged."""
+    x, a, b, _, ranks, scales, y = c
+    dev = lambda v, t=torch.int32: None if v is None else torch.tensor(v, dtype=t, device=DEV)  # noqa: E731
+    out, memory = _strided(torch.full(y.shape, 123.0, dtype=y.dtype), y.shape[1] + 8, 8, 99.0)
+    rq.lora_add(x.to(DEV), *(rq.Weight.from_tensor(t.to(DEV)) for t in (a, b)), rq.RowGroups(dev(offsets), dev(order)),
+                y.to(DEV), ranks=dev(ranks), scales=dev(scales, F32), out=out)
+    torch.cuda.synchronize()
+    got, around = out.cpu(), memory.clone()
+    around[8:8 + y.shape[0] * (y.shape[1] + 8)].view(y.shape[0], -1)[:, :y.shape[1]] = 99.0
+    assert bool((around == 99.0).all())
+    return got
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,k,n", [(1, 1, 8, 40, 16), (50, 4, 24, 136, 144), (200, 3, 13, 72, 33)])
+def test_lora_add_without_an_order(rq, rows, count, rank, k, n, x_type, w_type):
+    """order = None: the rows themselves are grouped; rows behind the last group are copied."""
+    _say("lora_add without an order", rows, count, rank, k, n, x_type, w_type)
+    c = _lora_case(rows, count, rank, k, n, x_type, w_type, rows)
+    ids = np.sort(np.where((c[3] < 0) | (c[3] >= count), count, c[3])).astype(np.int32)
+    offsets, _ = _grouped(ids, count)
+    got = _lora_ordered(rq, c, offsets.tolist(), None)
+    _check_lora(*c[:3], ids, *c[4:], got)
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,k,n", [(70, 3, 16, 64, 72), (140, 3, 11, 200, 45)])
+def test_lora_add_order_out_of_range(rq, rows, count, rank, k, n, x_type, w_type):
+    """Places that name no row compute nothing; a row that the order does not list keeps what out held."""
+    _say("lora_add order out of range", rows, count, rank, k, n, x_type, w_type)
+    c = _lora_case(rows, count, rank, k, n, x_type, w_type, rows)
+    offsets, order = _grouped(c[3], count)
+    at = [0, 5, 31, rows - 1]
+    left = order[at].copy()
+    order[at] = [-1, rows, -(1 << 31), (1 << 31) - 1]
+    got = _lora_ordered(rq, c, offsets.tolist(), order.tolist())
+    assert bool((got[left] == 123.0).all())
+    keep = np.setdiff1d(np.arange(rows), left)
+    _check_lora(c[0][keep], *c[1:3], c[3][keep], *c[4:6], c[6][keep], got[keep])
+
+
+@pytest.mark.parametrize("rank,n", [(16, 72), (11, 45)])
+@pytest.mark.parametrize("offsets", [[5, 9, 9, 20], [0, 40, 10, 50], [-7, 3, 1 << 30, 50], [50, 50, 0, 0],
+                                     [0, -(1 << 31), (1 << 31) - 1, -5], [0, 0, 0, 1 << 30]])
+def test_lora_add_odd_offsets(rq, offsets, rank, n):
+    """Offsets that do not rise from 0 to the rows stay inside the arrays: every row is what it was, or y's, with
+    or without an adapter's part."""
+    _say("lora_add odd offsets", offsets, rank, n)
+    x, a, b, _, _, _, y = _lora_case(50, 3, rank, 64, n, F16, F16, 9)
+    a, b = (torch.where(torch.isfinite(t), t, 0.25) for t in (a, b))
+    got = _lora_ordered(rq, (x, a, b, None, None, None, y), offsets, list(range(50)))
+    one = [_run_lora(rq, x, a, b, np.full(50, g, np.int32), None, None, y, False) for g in range(3)]
+    for r in range(50):
+        assert any(torch.equal(got[r], t[r]) for t in [torch.full_like(y, 123.0), y] + one) or \
+            sum(b <= r < e for b, e in zip(offsets, offsets[1:])) + (r >= offsets[-1]) > 1, r
