@@ -416,14 +416,19 @@ uint64_t rfxq_group_rows_workspace_size(uint32_t n, uint32_t groups);
  * names, and places in no group, with an index out of range or behind
  * x->rows, leave y as it was; a destination named twice holds one of its results.
  * x: f32, or the weights' type; y: f32, or the weights' type (the memory from its
- * first element to its last must not overlap x's). Accumulation is f32, each result is rounded once; f32 activations
- * keep f32 accuracy (they are split into 2 (F16) or 3 (BF16) pieces of the
- * weights' type; a weight that is infinite, or of 2^100 and more, can give a
- * result that is not finite, of either kind). Any in_features, stride and alignment of whole elements; rows of x
- * and W that start at multiples of 16 bytes (in_features and strides multiples of
- * 8) are faster. One launch, no workspace, no host synchronisation: it can be
- * captured. The counterpart of rfxq_expert_gemm for all experts at once
- * (src/model/dense.rs:1086-1115, 1531-1548). */
+ * first element to its last must not overlap x's). Accumulation is f32, each
+ * result is rounded once. f32 activations are multiplied in pieces of the weights'
+ * type: three of BF16, which hold all bits of a value, or two of F16, which hold 22
+ * of its 24 bits (values below 2^-17 of the largest of the 32 or 64 neighbours that
+ * are scaled together: 2^-39 of that one). Where a call's rows are few they are
+ * multiplied as they are, in all bits: the last bits of a row's results can change
+ * with the rows beside it. Beside f32 activations, a weight that is infinite, or of
+ * 2^100 and more, can give a result that is not finite, of either kind; subnormal
+ * BF16 values (below 2^-126) may count as 0. Any in_features, stride and alignment of
+ * whole elements; rows of x and W that start at multiples of 16 bytes (in_features
+ * and strides multiples of 8) are faster. One launch, no workspace, no host
+ * synchronisation: it can be captured. The counterpart of rfxq_expert_gemm for all
+ * experts at once (src/model/dense.rs:1086-1115, 1531-1548). */
 int rfxq_grouped_gemm(const rfxq_rows* x, const rfxq_weight* w, const int32_t* offsets, uint32_t rows,
                       const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
                       hipStream_t stream);
@@ -458,7 +463,11 @@ int rfxq_grouped_gemm_policy(const rfxq_rows* x, const rfxq_weight* w, uint32_t 
  * of x once (a row that it does not list keeps what out held), and offsets rise
  * from 0. x, y and out have
  * one type: f32 (any adapters), or the adapters' F16 / BF16; as many rows each.
- * A x is kept in f32, accumulation is f32, each result is rounded once.
+ * A x is summed and kept in f32, and multiplied with B in pieces as f32 activations
+ * are by rfxq_grouped_gemm: in all bits beside F32 and BF16 adapters, in 22 beside
+ * F16; so are f32 rows x with A. Accumulation is f32, each result is rounded once.
+ * What rfxq_grouped_gemm says of infinite, huge and subnormal weights holds here for
+ * A beside f32 rows and for B beside all, in F16 and BF16 adapters.
  * `workspace`: rfxq_lora_add_workspace_size bytes for up to `rows` rows, 16-byte
  * aligned, or NULL for the library's own (see rfxq_gemm). No counterpart in the
  * reference. */

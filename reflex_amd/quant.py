@@ -705,7 +705,8 @@ def grouped_gemm(x: torch.Tensor, w: Weight, offsets: torch.Tensor, rows: int, x
     """Products of grouped rows with a stack of F16 / BF16 matrices: for the places p of group g,
     ``out[y_index[p]] = x[x_index[p] // x_div] @ W[g].T`` (either index may be left out: place p itself).
     The counterpart of ``expert_gemm`` for all experts at once. Without ``out``, a new tensor of x's type with
-    ``rows`` rows, zero where no place of a group writes."""
+    ``rows`` rows, zero where no place of a group writes. f32 activations keep all their bits beside BF16 weights
+    and 22 beside F16; infinite or huge (2^100) weights beside them can give either kind of non-finite result."""
     dev = _on(x, "grouped_gemm: x")
     count = _stack(w, dev, "grouped_gemm")
     _count(rows, 0, "grouped_gemm: rows")
@@ -732,7 +733,8 @@ def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.
     """Low-rank adapters of many requests beside a shared projection: ``out[r] = y[r] + scales[g] * B[g] (A[g] x[r])``
     for the rows r of group g, ``out[r] = y[r]`` for rows in no group. a [count, rank, in] and b [count, out, rank]
     are stacks; adapter g is their first ``ranks[g]`` rows and columns. ``groups``: the rows grouped by their adapter
-    ids (``group_rows``). Without ``out``, y itself is updated."""
+    ids (``group_rows``). Without ``out``, y itself is updated. A x is kept in f32 and meets B in all its bits, or
+    in 22 beside F16 adapters; infinite or huge (2^100) values of B can give either kind of non-finite result."""
     dev = _on(x, "lora_add: x")
     count = _stack(a, dev, "lora_add a")
     _stack(b, dev, "lora_add b")

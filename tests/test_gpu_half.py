@@ -865,3 +865,49 @@ def test_lora_add_odd_offsets(rq, offsets, rank, n):
     for r in range(50):
         assert any(torch.equal(got[r], t[r]) for t in [torch.full_like(y, 123.0), y] + one) or \
             sum(b <= r < e for b, e in zip(offsets, offsets[1:])) + (r >= offsets[-1]) > 1, r
+
+
+# ------------------------------------------------------------------ weights that are not finite
+
+@pytest.mark.parametrize("x_type,w_type,y_type", TYPES[:4])
+@pytest.mark.parametrize("rows,groups,k,n", [(30, 3, 72, 40), (1000, 3, 136, 520), (2000, 4, 72, 2104)])
+def test_grouped_gemm_weights_not_finite(rq, rows, groups, k, n, x_type, w_type, y_type):
+    """An infinite or NaN weight leaves its own column of its own group without a finite result, and no other."""
+    _say("grouped_gemm weights not finite", rows, groups, k, n, x_type, w_type)
+    x, w = _case(rows, groups, k, n, x_type, w_type, 21)
+    offsets, _ = _grouped(_ids(rows, groups, "all"), groups)
+    lost = {(0, 3): float("inf"), (1, n - 1): float("-inf"), (2, 17): float("nan")}
+    clean = w.clone()
+    for i, ((g, c), v) in enumerate(lost.items()):
+        w[g, c, (5 + 30 * i) % k] = v
+    y, kept = _run_grouped(rq, x, w, offsets, rows, None, 1, None, y_type, rows)
+    assert kept
+    for g, c in lost:
+        part = y[offsets[g]:offsets[g + 1], c]
+        assert part.numel() and not torch.isfinite(part).any()
+        # the column's own results are checked above; the others against the weights without it
+        x64 = x[offsets[g]:offsets[g + 1]].double().numpy()
+        y[offsets[g]:offsets[g + 1], c] = torch.from_numpy(x64 @ clean[g, c].double().numpy()).to(y_type)
+    _check_grouped(x, clean, offsets, None, 1, None, y)
+
+
+@pytest.mark.parametrize("x_type,w_type", LORA_TYPES)
+@pytest.mark.parametrize("rows,count,rank,k,n", [(20, 2, 16, 72, 40), (90, 2, 24, 136, 144), (33, 2, 13, 75, 51)])
+def test_lora_add_weights_not_finite(rq, rows, count, rank, k, n, x_type, w_type):
+    """An infinite value of B leaves its column of its adapter's rows without a finite result, one of A all of them;
+    the other adapter's rows keep theirs."""
+    _say("lora_add weights not finite", rows, count, rank, k, n, x_type, w_type)
+    x, a, b, _, _, scales, y = _lora_case(rows, count, rank, k, n, x_type, w_type, 5)
+    a, b = (torch.where(torch.isfinite(t), t, 0.25) for t in (a, b))
+    ids = (np.arange(rows) % 2).astype(np.int32)
+    bad = b.clone()
+    bad[0, n // 2, rank - 2] = float("inf")
+    got = _run_lora(rq, x, a, bad, ids, None, scales, y, False)
+    assert not torch.isfinite(got[0::2, n // 2]).any()
+    keep = [c for c in range(n) if c != n // 2]
+    _check_lora(x, a, b[:, keep], ids, None, scales, y[:, keep], got[:, keep])
+    bad = a.clone()
+    bad[0, rank - 2, k // 3] = float("-inf")
+    got = _run_lora(rq, x, bad, b, ids, None, scales, y, False)
+    assert not torch.isfinite(got[0::2]).any()
+    _check_lora(x[1::2], a, b, ids[1::2], None, scales, y[1::2], got[1::2])
