@@ -2,8 +2,8 @@
 // (rfxq_grouped_gemm): y[dst_p][n] = sum_k x[src_p][k] W_g[n][k] for the rows p
 // of group g, f32 accumulation, one rounding to the type of y.
 //
-// f32 activations keep their accuracy: they are split into pieces of the weights'
-// type that add up to them and multiply the same weights (where a wave has one
+// f32 activations keep 22 (f16) or all (bf16) of their bits: they are split into pieces of the
+// weights' type that add up to them and multiply the same weights (where a wave has one
 // operand of weights, they go through f32 matrix instructions as they are). A
 // row's 32 or 64 values of a step are scaled by a power of two first, so that the
 // largest lies in [2^14, 2^15) (the matrix instructions take subnormal bf16
@@ -413,13 +413,15 @@ extern "C" __global__ __launch_bounds__(256, 3) void rfxq_grouped_any_f32_bf16(G
 // ---------------------------------------------------------------- tiles filled by asynchronous copies
 
 // BM x BN tiles of WM x WN waves (each BM / WM rows x 64 columns), 64-wide
-// steps of K in STAGES buffers: copies global -> LDS run STAGES - 1 steps
+// steps of K in STAGES buffers: copies global -> LDS are issued STAGES - 1 steps
 // ahead of the products, without registers between. Rows of x and W start at
 // whole 16 bytes; what lies past a row's end or the tile's last row is copied
 // from past the buffer's end, which fills it with zeros. Offsets within x and
 // within one matrix stay below 4 GiB (the host's rule). 64 x 128, 3 buffers: one
 // or two workgroups a CU reach memory's rate (8 x 4096 x 14336, 32 rows each, bf16:
-// 186 us, 5.0 TB/s; 247 through registers).
+// 186 us, 5.0 TB/s; 247 through registers). In two of the loop's three steps the
+// compiler has the first LDS read wait for every copy in flight (it cannot tell the
+// buffers that they go to from the one it reads): there the copies are one step ahead only.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 struct GroupedTile {
     static constexpr uint32_t THREADS = 64u * WM * WN, MF = BM / WM / 16;
@@ -508,9 +510,9 @@ struct GroupedTile {
     // end of that step's last turn (the upper waves' last reading turn).
     // The lower and the upper waves take every other 16 rows of the tile, and leave
     // out those behind the group's last row: FULL has none.
-    // 8192 rows over 8 matrices of 14336 x 4096 f16: 0.90 ms, 1.07 PFLOP/s, matrix
-    // pipes 58% busy (64 x 128 tiles: 1.46 ms); without copies 0.66 ms, with all of
-    // them from L2 0.77: their traffic and the clock it costs bound it.
+    // 8192 rows over 8 matrices of 14336 x 4096 f16: 0.90 to 0.94 ms, 1.02 to 1.07
+    // PFLOP/s, matrix pipes 58% busy (64 x 128 tiles: 1.46 ms); without copies 0.66 ms,
+    // with all of them from L2 0.77: their traffic and the clock it costs bound it.
     template <bool FULL>
     __device__ __forceinline__ void turns(u4_t* xs0, u4_t* xs1, u4_t* ws0, u4_t* ws1, f4v_t (&acc)[MF][4]) {
         const uint32_t upper = wave >> 2, l = lane & 15u, q = lane >> 4, row0 = upper * 16u, col0 = (wave & 3u) * 64u;

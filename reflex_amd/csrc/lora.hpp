@@ -194,7 +194,8 @@ RFXQ_DEV void lora_down(const LoraArgs& a) {
 // all of them; B's values and y of the next strip are loaded during a strip.
 //
 // y, out and B bound it: 4096 rows of 4096 f32 values 32 us, 4.6 TB/s; 256 rows, 64
-// adapters of ranks to 64, 14336 values, bf16: 28 us, 4.5 TB/s of whole lines of B and y.
+// adapters of ranks to 64, 14336 values, bf16: 28 us, 4.5 TB/s of whole lines of B and y
+// (939 of 940 thousand requests are of 128 bytes).
 //
 // VEC: rank is a multiple of 8 and n of 4. Then no load has a condition: what does not
 // exist reads the row's first values and is left out where it is used, so loads
