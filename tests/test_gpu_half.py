@@ -911,3 +911,96 @@ def test_lora_add_weights_not_finite(rq, rows, count, rank, k, n, x_type, w_type
     got = _run_lora(rq, x, bad, b, ids, None, scales, y, False)
     assert not torch.isfinite(got[0::2]).any()
     _check_lora(x[1::2], a, b, ids[1::2], None, scales, y[1::2], got[1::2])
+
+
+# ------------------------------------------------------------------ the largest calls, and calls side by side
+
+@pytest.mark.parametrize("groups", [1, 300, 1024])
+def test_group_rows_of_the_most_rows(rq, groups):
+    n = 1 << 24
+    _say("group_rows", n, groups)
+    ids = _ids(n, groups, "any")
+    g = rq.group_rows(torch.from_numpy(ids).to(DEV), groups)
+    want_offsets, want_order = _grouped(ids, groups)
+    assert np.array_equal(g.offsets.cpu().numpy(), want_offsets) and np.array_equal(g.order.cpu().numpy(), want_order)
+
+
+def test_lora_add_rows_past_4_gib(rq):
+    """Rows of x, y and out whose bytes lie past 32-bit offsets; the first, some and the last are looked at."""
+    _say("lora_add past 4 GiB")
+    rows, count, rank, k, n = 2_200_001, 3, 8, 1024, 1024
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x, y = (torch.empty(rows, m, dtype=F16, device=DEV) for m in (k, n))
+    for t in (x, y):
+        for b in range(0, rows, 1 << 18):
+            t[b:b + (1 << 18)].normal_(generator=gen)
+    a, b = ((torch.randn(*s, generator=torch.Generator().manual_seed(4)) * 0.05).half() for s in ((count, rank, k), (count, n, rank)))
+    ids = (torch.arange(rows, dtype=torch.int32, device=DEV) * 7 % (count + 1))
+    out = torch.full((rows, n), 123.0, dtype=F16, device=DEV)
+    rq.lora_add(x, rq.Weight.from_tensor(a.to(DEV)), rq.Weight.from_tensor(b.to(DEV)), rq.group_rows(ids, count), y, out=out)
+    at = torch.cat([torch.arange(0, 40), torch.arange(rows // 2, rows // 2 + 40), torch.arange(rows - 200, rows)])
+    d = at.to(DEV)
+    _check_lora(x[d].cpu(), a, b, ids[d].cpu().numpy(), None, None, y[d].cpu(), out[d].cpu())
+    none = ids == count
+    assert torch.equal(out[none], y[none]) and not bool((out[~none] == 123.0).all(1).any())
+
+
+def test_lora_add_stacks_past_4_gib(rq):
+    """Adapters whose bytes lie past 32-bit offsets in their stacks."""
+    _say("lora_add stacks past 4 GiB")
+    rows, count, rank, k, n = 70, 1000, 256, 8256, 8320
+    a, b = (torch.zeros(count, *s, dtype=F16, device=DEV) for s in ((rank, k), (n, rank)))
+    c = _lora_case(rows, 2, rank, k, n, F16, F16, 8)
+    a[-2:], b[-2:] = c[1].to(DEV), c[2].to(DEV)
+    far = torch.from_numpy(np.where((c[3] == 0) | (c[3] == 1), c[3] + count - 2, -1).astype(np.int32)).to(DEV)
+    full = lambda v, t: torch.cat([torch.zeros(count - 2, dtype=t), torch.tensor(v, dtype=t)]).to(DEV)  # noqa: E731
+    got = rq.lora_add(c[0].to(DEV), rq.Weight.from_tensor(a), rq.Weight.from_tensor(b), rq.group_rows(far, count), c[6].to(DEV),
+                      ranks=full(c[4], torch.int32), scales=full(c[5], F32))
+    _check_lora(*c, got.cpu())
+
+
+def test_two_streams_at_once(rq):
+    """Calls on two streams that overlap, each with its own workspace."""
+    cases = [_lora_case(300, 5, 40, 4096, 264, F32, BF16, s) for s in (1, 2)]
+    ids = [torch.from_numpy(_ids(70_001, 300, "any", s)).to(DEV) for s in (1, 2)]
+    want = [rq.group_rows(i, 300) for i in ids]
+    dev = [(x.to(DEV), rq.Weight.from_tensor(a.to(DEV)), rq.Weight.from_tensor(b.to(DEV)),
+            rq.group_rows(torch.from_numpy(i).to(DEV), 5), torch.tensor(r, dtype=torch.int32, device=DEV),
+            torch.tensor(s, device=DEV), y.to(DEV)) for x, a, b, i, r, s, y in cases]
+    lws = [torch.empty(rq.lora_add_workspace_size(d[1], 300), dtype=torch.uint8, device=DEV) for d in dev]
+    gws = [torch.empty(rq.group_rows_workspace_size(70_001, 300), dtype=torch.uint8, device=DEV) for _ in dev]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs, groups = [[], []], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, a, b, g, r, sc, y = dev[i]
+                outs[i].append(rq.lora_add(x, a, b, g, y, ranks=r, scales=sc, out=torch.empty_like(y), workspace=lws[i]))
+                groups[i].append(rq.group_rows(ids[i], 300, workspace=gws[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        _check_lora(*cases[i], outs[i][0].cpu())
+        assert all(torch.equal(o, outs[i][0]) for o in outs[i])
+        assert all(torch.equal(g.order, want[i].order) and torch.equal(g.offsets, want[i].offsets) for g in groups[i])
+
+
+def test_moe_ffn_grouped_half_host_routing_is_not_captured(rq):
+    """The host-routed layer copies its routing up, which a graph would not repeat: refused while capturing, and
+    the graph of what came before it is whole."""
+    x, logits, w = _layer_inputs(4, 4, 64, 48, F16, 1)
+    weights = [rq.Weight.from_tensor(t.to(DEV)) for t in w]
+    xd, out, seen = x.to(DEV), torch.full((4 * 64,), 5.0, device=DEV), torch.zeros(8, device=DEV)
+    run = lambda: rq.moe_ffn_grouped(xd, 4, 64, logits.numpy(), 4, 2, True, 1.0, *weights, out)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    out.fill_(5.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        seen.add_(1.0)
+        with pytest.raises(rq.InvalidInputError, match="captured"):
+            run()
+    for r in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((seen == r + 1.0).all()) and bool((out == 5.0).all())
