@@ -17,10 +17,8 @@
 #pragma once
 #include "common.hpp"
 #include "rows.hpp"
+#include "tiles.hpp"
 
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
-typedef u4_t u4a2_t __attribute__((aligned(2)));
 
 template <typename T>
 RFXQ_DEV f4v_t mfma32(u4_t a, u4_t b, f4v_t c) {
@@ -28,16 +26,6 @@ RFXQ_DEV f4v_t mfma32(u4_t a, u4_t b, f4v_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
-}
-
-// Between a run of matrix instructions that ends at a branch and the first reads
-// of their results. The compiler's own wait states have come out short there: a
-// result read as the first instruction behind a branch was read too early.
-// 32 wait states, more than the longest of the instructions used here needs.
-RFXQ_DEV void mfma_settle() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
 }
 
 struct GroupedArgs {
@@ -53,79 +41,6 @@ struct GroupedArgs {
     uint32_t tiles_m, tiles_n, sm, sn;
 };
 
-// Row p's source and destination; -1 where an index is out of range (such a row
-// is not computed). The load has no condition (without an index it reads the first
-// offset), so that nothing waits for it where it is issued.
-RFXQ_DEV int64_t src_row(const GroupedArgs& a, uint32_t p) {
-    const int32_t i = ((const RFXQ_GLOBAL int32_t*)(a.x_index ? a.x_index : a.offsets))[a.x_index ? p : 0u];
-    const uint32_t s = a.x_index ? (uint32_t)i / a.x_div : p;
-    return (i >= 0 || !a.x_index) && s < a.x_rows ? (int64_t)s : -1;
-}
-RFXQ_DEV int64_t dst_row(const GroupedArgs& a, uint32_t p) {
-    const int32_t i = a.y_index ? a.y_index[p] : (int32_t)p;
-    return i >= 0 && (uint32_t)i < a.y_rows ? (int64_t)i : -1;
-}
-
-// Vectors that may start at any element.
-typedef float f4a4_t __attribute__((ext_vector_type(4), aligned(4)));
-
-// 8 neighbouring values of a row as they lie in memory.
-template <typename T>
-struct Eight {
-    u4_t v;
-    __device__ __forceinline__ float at(uint32_t j) const {
-        if constexpr (__is_same(T, half_t))
-            return (float)__builtin_bit_cast(h8_t, v)[j];
-        else
-            return (float)__builtin_bit_cast(b8_t, v)[j];
-    }
-};
-template <>
-struct Eight<float> {
-    f4v_t v[2];
-    __device__ __forceinline__ float at(uint32_t j) const { return v[j >> 2][j & 3u]; }
-};
-
-// The 8 values at p.
-template <typename T>
-RFXQ_DEV Eight<T> ld_eight(const T* p) {
-    Eight<T> r;
-    if constexpr (__is_same(T, float)) {
-        r.v[0] = *(const RFXQ_GLOBAL f4a4_t*)p;
-        r.v[1] = *(const RFXQ_GLOBAL f4a4_t*)(p + 4);
-    } else {
-        r.v = *(const RFXQ_GLOBAL u4a2_t*)p;
-    }
-    return r;
-}
-// The first `have` of the 8 values at p, one by one, then zeros.
-template <typename T>
-RFXQ_DEV Eight<T> ld_eight(const T* p, uint32_t have) {
-    if (have >= 8u) return ld_eight(p);
-    T t[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) t[i] = i < have ? ((const RFXQ_GLOBAL T*)p)[i] : (T)0.0f;
-    Eight<T> r;
-    __builtin_memcpy(&r, t, sizeof t);
-    return r;
-}
-
-// The largest of 8 values' sizes, as bits: sizes order like their bits, and
-// infinities and NaN lie above every finite one.
-constexpr uint32_t kInfBits = 0x7F800000u;
-RFXQ_DEV uint32_t top_of_eight(const Eight<float>& x) {
-    uint32_t t = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; i++) t = max(t, __builtin_bit_cast(uint32_t, x.at(i)) & 0x7FFFFFFFu);
-    return t;
-}
-#define RFXQ_DPP_U32(v, ctrl) (uint32_t) __builtin_amdgcn_update_dpp(0, (int)(v), (ctrl), 0xF, 0xF, false)
-// the largest of 8 neighbouring lanes
-RFXQ_DEV uint32_t top_over_8(uint32_t v) {
-    v = max(v, RFXQ_DPP_U32(v, 0xB1));
-    v = max(v, RFXQ_DPP_U32(v, 0x4E));
-    return max(v, RFXQ_DPP_U32(v, 0x141));
-}
 // the largest of the four lanes (l, 0..3)
 RFXQ_DEV uint32_t top_over_q(uint32_t v) {
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
@@ -186,17 +101,6 @@ RFXQ_DEV void split_eight(const Eight<float>& x, float scale, uint32_t top, u4_t
         pieces(false);
     else
         pieces(true);
-}
-
-// Workgroup b's place in the grid of tiles: workgroups go round-robin to the 8
-// XCDs, and each XCD takes blocks of sm x sn neighbouring tiles, whose rows
-// and columns meet in its L2.
-RFXQ_DEV bool tile_place(const GroupedArgs& a, uint32_t b, uint32_t& tm, uint32_t& tn) {
-    const uint32_t j = b >> 3, per = a.sm * a.sn;
-    const uint32_t block = (j / per) * 8u + (b & 7u), r = j % per, across = (a.tiles_n + a.sn - 1u) / a.sn;
-    tm = (block / across) * a.sm + r % a.sm;
-    tn = (block % across) * a.sn + r / a.sm;
-    return tm < a.tiles_m && tn < a.tiles_n;
 }
 
 // 16 neighbouring results of one row, of which the first `have` are there. Whole
@@ -265,15 +169,6 @@ RFXQ_DEV void st_four(const GroupedArgs& a, int64_t row, uint32_t n, f4v_t v) {
             if (i < have) ((RFXQ_GLOBAL T*)y)[i] = r[i];
     }
 }
-
-// Place of 16-byte piece c (of 8) of LDS row r: rows of 128 bytes, pieces
-// xor'ed with the row so that 8 rows' pieces of one column lie in 8 banks' groups.
-RFXQ_DEV uint32_t lds_piece(uint32_t r, uint32_t c) { return r * 8u + (c ^ (r & 7u)); }
-
-// The column of a tile that LDS row j of the weights holds. A lane's results
-// are rows 4q..4q+3 of each 16-row operand (q = lane / 16): with this order the
-// four operands of a wave's 64 columns give it 16 neighbouring ones.
-RFXQ_DEV uint32_t col_of(uint32_t j) { return (j & ~63u) + ((j >> 2) & 3u) * 16u + ((j >> 4) & 3u) * 4u + (j & 3u); }
 
 // The wave's 16 MF x 64 tile of one 64-wide step of K, both operands in LDS
 // (the activations' pieces XS apart, the last ones first).

@@ -1,5 +1,4 @@
-// Rows grouped by an id (rfxq_group_rows), and the search of the products that
-// work on such groups for the tile a workgroup computes.
+// Rows grouped by an id (rfxq_group_rows).
 //
 // key_i = id_i, or `groups` for an id outside [0, groups);
 //   offsets[g] = #{ i : key_i < g }, g = 0..groups
@@ -8,88 +7,9 @@
 //   offsets[key_i] + #{ j < i : key_j = key_i }.
 #pragma once
 #include "common.hpp"
+#include "tiles.hpp"
 
 constexpr uint32_t kMaxGroups = 1024;
-
-// Inclusive sum over the wave's lanes: within 16-lane rows by row shifts, then
-// the rows' last lanes carried over (row_bcast 15 and 31).
-RFXQ_DEV uint32_t wave_scan(uint32_t v) {
-#define RFXQ_SCAN(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, (ctrl), (rows), 0xF, false)
-    RFXQ_SCAN(0x111, 0xF);
-    RFXQ_SCAN(0x112, 0xF);
-    RFXQ_SCAN(0x114, 0xF);
-    RFXQ_SCAN(0x118, 0xF);
-    RFXQ_SCAN(0x142, 0xA);
-    RFXQ_SCAN(0x143, 0xC);
-#undef RFXQ_SCAN
-    return v;
-}
-
-// The rows [beg, end) of one tile of at most `bm` rows, all of one group; where
-// there is none (any = false), `beg` is the tile's number behind the last one.
-struct RowTile {
-    uint32_t group, beg, end;
-    int32_t extra;
-    bool any;
-};
-
-template <uint32_t N>
-struct Count {
-    static constexpr uint32_t value = N;
-};
-
-// Tile t of the grouped rows: the groups' tiles counted in order, each group
-// starting a tile of its own. Every wave searches by itself (no LDS, no
-// barrier), a group a lane: the offsets of up to 256 groups are one trip to memory,
-// which every kernel here waits for before it knows what to read (with neighbouring
-// groups in a lane it is two and more: a token over 8 of 128 experts, 768 x 2048, 8.4 us
-// against 7.5).
-// Offsets are taken as they are found: clamped to [0, rows], and a group
-// whose end lies before its start has no tiles, so that no value there leads
-// outside the arrays. `extra`: a value per group, returned for the tile's.
-RFXQ_DEV RowTile find_tile(const int32_t* offsets, uint32_t groups, uint32_t rows, uint32_t bm, uint32_t t,
-                           const int32_t* extra = nullptr) {
-    const uint32_t lane = threadIdx.x & 63u;
-    uint32_t before = 0;  // tiles of the groups looked at
-    RowTile r = {0, 0, 0, 0, false};
-    const auto look = [&](auto n, uint32_t g0) {
-        constexpr uint32_t N = decltype(n)::value;
-        int32_t b[N], e[N], x[N];
-#pragma unroll
-        for (uint32_t i = 0; i < N; i++) {
-            const uint32_t g = g0 + 64u * i + lane;
-            b[i] = ((const RFXQ_GLOBAL int32_t*)offsets)[min(g, groups)];
-            e[i] = ((const RFXQ_GLOBAL int32_t*)offsets)[min(g + 1u, groups)];
-            x[i] = extra ? ((const RFXQ_GLOBAL int32_t*)extra)[min(g, groups - 1u)] : 0;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < N; i++) {
-            const uint32_t bi = min((uint32_t)max(b[i], 0), rows), ei = min((uint32_t)max(e[i], 0), rows);
-            const uint32_t mine = ei > bi ? (ei - bi + bm - 1u) / bm : 0u;
-            const uint32_t upto = before + wave_scan(mine);
-            const uint64_t has = __builtin_amdgcn_ballot_w64(upto > t);
-            if (has) {
-                const int l = __builtin_ctzll(has);
-                const uint32_t left = t - (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), l);
-                if (left >= (uint32_t)__builtin_amdgcn_readlane((int)mine, l)) return;  // a sum that wrapped
-                const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)ei, l);
-                r.group = g0 + 64u * i + (uint32_t)l;
-                r.beg = (uint32_t)__builtin_amdgcn_readlane((int)bi, l) + left * bm;
-                r.end = min(r.beg + bm, end);
-                r.extra = __builtin_amdgcn_readlane(x[i], l);
-                r.any = true;
-                return;
-            }
-            before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-        }
-    };
-    if (groups <= 64u)
-        look(Count<1>{}, 0);
-    else
-        for (uint32_t g0 = 0; g0 < groups && !r.any; g0 += 256u) look(Count<4>{}, g0);
-    if (!r.any) r.beg = t - before;
-    return r;
-}
 
 struct GroupRowsArgs {
     const int32_t* ids;
