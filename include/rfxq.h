@@ -476,6 +476,96 @@ int rfxq_lora_add(const rfxq_rows* x, const rfxq_weight* a, const rfxq_weight* b
                   const rfxq_rows* out, void* workspace, uint64_t workspace_bytes, hipStream_t stream);
 uint64_t rfxq_lora_add_workspace_size(const rfxq_weight* a, uint32_t rows);
 
+/* ---- 8-bit floating point with a scale for each 128 ------------------------- */
+
+/* Rows in e4m3 (OCP: 1 sign, 4 exponent and 3 fraction bits, no infinities, largest
+ * 448) with an f32 scale for each 128 values of a row, the last group of a row as
+ * short as it is. In device memory; value (r, c) is
+ *   e4m3(data[r * stride + c]) * scales[r * scale_stride + c / 128] */
+typedef struct rfxq_f8_rows {
+    void* data;
+    float* scales;
+    uint32_t rows;
+    uint64_t stride;       /* codes (bytes) between rows, at least the row's columns */
+    uint64_t scale_stride; /* scales between rows, at least ceil(columns / 128) */
+} rfxq_f8_rows;
+
+/* A matrix, or a stack of them, in e4m3 with an f32 scale for each block of 128 x 128
+ * (short at the ends), as checkpoints hold them: codes [expert_count][out][in], scales
+ * [expert_count][ceil(out / 128)][ceil(in / 128)], both contiguous, in device memory. */
+typedef struct rfxq_f8_weight {
+    uint32_t in_features;  /* K */
+    uint32_t out_features; /* N */
+    uint32_t expert_count; /* 0 for a 2-D weight */
+    const void* data;
+    const float* scales;
+    uint64_t len;        /* bytes of data */
+    uint64_t scales_len; /* bytes of scales */
+} rfxq_f8_weight;
+
+/* What writes such rows. Of a group's values v (of 128, in f32)
+ *   scale = max(amax, 448 * 2^-120) / 448, amax = max |v|;  code = e4m3(v / scale)
+ * rounded to nearest even (scale and quotient in f32, within its last bits); a group
+ * with a value that is not finite has NaN for its scale. Rows of x, gate, up, residual,
+ * sum and y are f32, f16 or bf16, all of one call of one type and count, any
+ * alignment of whole elements; out's codes and scales, sum and y must not overlap
+ * each other nor an input, from the first element to the last, but where
+ * allowed below. k up to 2^31 - 1; no rows: nothing is done. One launch, no
+ * workspace, no host synchronisation: they can be captured. Stand beside
+ * rfxq_quantize_act_q8_1, rfxq_silu_and_mul_q8_1 and rfxq_rmsnorm_q8_1; no
+ * counterpart in the reference, which has no 8-bit floating point. */
+
+/* out = x [rows][k]. */
+int rfxq_quantize_f8(const rfxq_rows* x, uint32_t k, const rfxq_f8_rows* out, hipStream_t stream);
+
+/* out = gate / (1 + exp(-gate)) * up: Model::silu_and_mul (silu_and_mul.cu:7-23). gate
+ * and up may be columns of one matrix. */
+int rfxq_silu_and_mul_f8(const rfxq_rows* gate, const rfxq_rows* up, uint32_t k, const rfxq_f8_rows* out,
+                         hipStream_t stream);
+
+/* The residual stream's addition and the norm behind it:
+ *   t = x + residual (NULL: x);  sum = t (NULL: not stored);
+ *   v = t / sqrt(mean(t^2) + eps) * weight;  y = v (NULL: not stored);  out = v
+ * in f32 throughout: the norm takes t as it was summed, not as `sum` rounds it.
+ * sum may be x or residual (the same data and stride). weight: k f32 values. eps is
+ * finite and not negative. Squares are summed in an order of this kernel's, the same on every
+ * call (rfxq_rmsnorm_q8_1 keeps the reference's). */
+int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const float* weight, uint32_t k, float eps,
+                        const rfxq_rows* sum, const rfxq_f8_rows* out, const rfxq_rows* y, hipStream_t stream);
+
+/* y[m][n] = sum_k x[m][k] w[n][k] of both with their scales (Model::gemm's counterpart
+ * for such weights). Each block's sum times the product of its two scales (an f32
+ * value: where that is out of f32's range, so is the result) is added in f32, and each
+ * result rounded once to y's type (f32, f16 or bf16). Within a block of 128, f32
+ * results have exact products summed in f32; for f16 and bf16 ones the matrix
+ * instructions may cut each product to a multiple of 2^-13 of the largest of the eight
+ * neighbours that are added first (by the exponents of their codes, subnormal codes
+ * and zeros counted as 2^-6), which costs 1.5e-5 of a result for normal values. NaN codes and scales give NaN in the results that they
+ * belong to. Any sizes, strides and alignment of whole elements (scales and
+ * y); rows of x and w that start at multiples of 16 bytes are faster. y must not overlap x. One
+ * launch, no workspace, no host synchronisation: it can be captured. The order of a sum depends
+ * on the call's sizes and alignment, not on anything else: equal calls give equal bits. */
+int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream);
+
+/* rfxq_gemm_f8 of grouped rows with a stack: rows, offsets, x_index, x_div and
+ * y_index as rfxq_grouped_gemm takes them (rfxq_group_rows writes them), and as there
+ * rows that no place names, and places in no group or with an index out of range,
+ * leave y as it was. Up to 1024 matrices. */
+int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
+                         const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
+                         hipStream_t stream);
+
+/* Test hook: the kernel and tile that rfxq_gemm_f8 (grouped = 0) or
+ * rfxq_grouped_gemm_f8 runs on the current device (256 compute units before
+ * rfxq_init) for `rows` rows or places of x and w; no memory is read. */
+#define RFXQ_F8_ANY 0 /* 64 x 128 tiles through registers, any alignment */
+#define RFXQ_F8_FEW 1 /* weights straight from memory, K among a workgroup's waves */
+typedef struct rfxq_f8_policy {
+    uint32_t kernel; /* RFXQ_F8_* */
+    uint32_t tile_m, tile_n;
+} rfxq_f8_policy;
+int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, rfxq_f8_policy* out);
+
 /* ---- GGUF files (the on-disk path) ---------------------------------------- */
 
 /* GgufFile (src/gguf.rs:183-334): the file memory-mapped and parsed (magic,

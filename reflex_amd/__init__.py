@@ -48,6 +48,27 @@ class RfxqGroupedPolicy(ctypes.Structure):
     _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32)]
 
 
+class RfxqF8Rows(ctypes.Structure):
+    """``rfxq_f8_rows`` (include/rfxq.h)."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_uint32),
+                ("stride", ctypes.c_uint64), ("scale_stride", ctypes.c_uint64)]
+
+
+class RfxqF8Weight(ctypes.Structure):
+    """``rfxq_f8_weight`` (include/rfxq.h)."""
+
+    _fields_ = [("in_features", ctypes.c_uint32), ("out_features", ctypes.c_uint32), ("expert_count", ctypes.c_uint32),
+                ("data", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("len", ctypes.c_uint64),
+                ("scales_len", ctypes.c_uint64)]
+
+
+class RfxqF8Policy(ctypes.Structure):
+    """``rfxq_f8_policy`` (include/rfxq.h)."""
+
+    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32)]
+
+
 class RfxqOptions(ctypes.Structure):
     """``rfxq_options`` (include/rfxq.h)."""
 
@@ -71,6 +92,7 @@ class RfxqGemmPolicy(ctypes.Structure):
 _P, _U32, _U64, _I = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int
 _WP = ctypes.POINTER(RfxqWeight)
 _RP = ctypes.POINTER(RfxqRows)
+_F8R, _F8W = ctypes.POINTER(RfxqF8Rows), ctypes.POINTER(RfxqF8Weight)
 SIGNATURES = {
     "rfxq_last_error": (ctypes.c_char_p, []),
     "rfxq_last_error_code": (_I, []),
@@ -136,6 +158,12 @@ SIGNATURES = {
     "rfxq_grouped_gemm_policy": (_I, [_RP, _WP, _U32, ctypes.POINTER(RfxqGroupedPolicy)]),
     "rfxq_lora_add": (_I, [_RP, _WP, _WP, _P, _P, _P, _P, _RP, _RP, _P, _U64, _P]),
     "rfxq_lora_add_workspace_size": (_U64, [_WP, _U32]),
+    "rfxq_quantize_f8": (_I, [_RP, _U32, _F8R, _P]),
+    "rfxq_silu_and_mul_f8": (_I, [_RP, _RP, _U32, _F8R, _P]),
+    "rfxq_add_rmsnorm_f8": (_I, [_RP, _RP, _P, _U32, ctypes.c_float, _RP, _F8R, _RP, _P]),
+    "rfxq_gemm_f8": (_I, [_F8R, _F8W, _RP, _P]),
+    "rfxq_grouped_gemm_f8": (_I, [_F8R, _F8W, _P, _U32, _P, _U32, _P, _RP, _P]),
+    "rfxq_gemm_f8_policy": (_I, [_F8R, _F8W, _U32, _I, ctypes.POINTER(RfxqF8Policy)]),
 }
 
 

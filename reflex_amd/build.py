@@ -3,9 +3,10 @@
 Steps (the counterpart of the reference's build.rs:199-252 + src/aot.rs, which
 run nvcc per .cu file and embed the images as bytes):
   1. hipcc --offload-arch=gfx950 --cuda-device-only --no-gpu-bundle-output
-     compiles csrc/kernels.hip (the quantized path) and csrc/half.hip (grouped
-     rows, half-typed stacks, adapters) side by side to raw code objects
-     (_build/rfxq_gfx950.co, _build/half_gfx950.co).
+     compiles csrc/kernels.hip (the quantized path), csrc/half.hip (grouped
+     rows, half-typed stacks, adapters) and csrc/f8.hip (8-bit floating point) side
+     by side to raw code objects (_build/rfxq_gfx950.co, _build/half_gfx950.co,
+     _build/f8_gfx950.co).
   2. An assembler stub .incbin's those files into .rodata (_build/embed.o).
   3. hipcc compiles csrc/scratch.hip (host code plus the fixed device scratch
      array of rfxq_gemm_no_alloc) to an ordinary object.
@@ -29,7 +30,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 LIB = os.path.join(HERE, "librfxq.so")
 ARCH = "gfx950"
 # device sources and the symbols their images are embedded under
-IMAGES = [("kernels", "rfxq_code_object"), ("half", "rfxq_half_code_object")]
+IMAGES = [("kernels", "rfxq_code_object"), ("half", "rfxq_half_code_object"), ("f8", "rfxq_f8_code_object")]
 
 DEVICE_FLAGS = [
     "-O3", "-std=c++17", f"--offload-arch={ARCH}", "--cuda-device-only", "--no-gpu-bundle-output",

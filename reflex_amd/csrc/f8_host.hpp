@@ -1,0 +1,347 @@
+// Host side of the entry points in 8-bit floating point: rfxq_quantize_f8,
+// rfxq_silu_and_mul_f8, rfxq_add_rmsnorm_f8 (kernels: f8_rows.hpp), rfxq_gemm_f8 and
+// rfxq_grouped_gemm_f8 (f8_gemm.hpp). Included by rfxq.cpp behind half_host.hpp, whose
+// checks of rows it uses.
+#pragma once
+
+namespace {
+
+constexpr uint32_t kF8Block = 128;  // f8_rows.hpp
+
+// Mirrors of the device structs.
+struct F8RowsArgs {
+    const void* x;
+    const void* x2;
+    const float* weight;
+    void* sum;
+    void* y;
+    uint8_t* out;
+    float* scales;
+    uint64_t ldx, ldx2, ldsum, ldy, ldo, lds;
+    uint32_t rows, k, groups;
+    float eps;
+    uint32_t by_rows, by_groups;
+};
+static_assert(sizeof(F8RowsArgs) == 128, "F8RowsArgs layout");
+
+struct F8Args {
+    const uint8_t* x;
+    const float* xs;
+    const uint8_t* w;
+    const float* ws;
+    void* y;
+    const int32_t* offsets;
+    const int32_t* x_index;
+    const int32_t* y_index;
+    uint64_t ldx, ldxs, ldy, w_stride, ws_stride;
+    uint32_t rows, x_rows, y_rows, x_div;
+    uint32_t k, n, groups, y_type;
+    uint32_t tiles_m, tiles_n, sm, sn;
+};
+static_assert(sizeof(F8Args) == 152, "F8Args layout");
+
+uint32_t f8_groups(uint32_t k) { return (k + kF8Block - 1u) / kF8Block; }
+uint32_t float_index(uint32_t ty) { return ty == RFXQ_TYPE_F32 ? 0u : ty == RFXQ_TYPE_F16 ? 1u : 2u; }
+
+int check_f8_rows(const rfxq_f8_rows* r, uint32_t columns, const char* what, const char* name) {
+    if (!r) return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s is NULL", what, name);
+    if (r->rows == 0) return RFXQ_OK;
+    if (!r->data || !r->scales) return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s data or scales is NULL", what, name);
+    // as many bytes as an address space holds: products of these do not wrap
+    if (r->rows > 0x7FFFFFFFu || (unsigned __int128)r->rows * r->stride >> 47 ||
+        (unsigned __int128)r->rows * r->scale_stride >> 45)
+        return fail(RFXQ_ERR_OTHER, "%s: %u rows of %s, stride=%llu, scale_stride=%llu", what, r->rows, name,
+                    (unsigned long long)r->stride, (unsigned long long)r->scale_stride);
+    if (r->stride < columns || r->scale_stride < f8_groups(columns))
+        return fail(RFXQ_ERR_OTHER, "%s: %s stride=%llu, scale_stride=%llu (at least %u columns, %u scales)", what, name,
+                    (unsigned long long)r->stride, (unsigned long long)r->scale_stride, columns, f8_groups(columns));
+    if (reinterpret_cast<uintptr_t>(r->scales) % 4u)
+        return fail(RFXQ_ERR_OTHER, "%s: %s scales at %p are not 4-byte aligned", what, name, (void*)r->scales);
+    return RFXQ_OK;
+}
+
+int check_f8_weight(const rfxq_f8_weight* w, const char* what) {
+    if (!w) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight is NULL", what);
+    const uint32_t k = w->in_features, n = w->out_features;
+    if (k == 0 || n == 0 || k > 0x7FFFFFFFu || n > 0x7FFFFFFFu)
+        return fail(RFXQ_ERR_OTHER, "%s: shape [%u, %u] (each 1..2^31 - 1)", what, k, n);
+    if (w->expert_count > kMaxGroups)
+        return fail(RFXQ_ERR_OTHER, "%s: expert_count=%u (at most %u)", what, w->expert_count, kMaxGroups);
+    const uint32_t count = std::max(w->expert_count, 1u);
+    const unsigned __int128 need = (unsigned __int128)count * k * n;
+    const unsigned __int128 scales = (unsigned __int128)count * f8_groups(k) * f8_groups(n) * 4u;
+    if (w->len < need || w->scales_len < scales)
+        return fail(RFXQ_ERR_OTHER, "%s: weight of %llu bytes and %llu of scales, shape [%u, %u, %u] needs %llu and %llu", what,
+                    (unsigned long long)w->len, (unsigned long long)w->scales_len, k, n, count, (unsigned long long)need,
+                    (unsigned long long)scales);
+    if (!w->data || !w->scales) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight data or scales is NULL", what);
+    if (reinterpret_cast<uintptr_t>(w->scales) % 4u)
+        return fail(RFXQ_ERR_OTHER, "%s: weight scales at %p are not 4-byte aligned", what, (const void*)w->scales);
+    return RFXQ_OK;
+}
+
+// A piece of memory from its first byte to its last.
+struct Span {
+    const void* p;
+    uint64_t bytes;
+    const char* name;
+};
+Span span_of(const rfxq_rows* r, uint32_t columns, const char* name) { return {r->data, rows_span(r, columns), name}; }
+Span codes_of(const rfxq_f8_rows* r, uint32_t columns, const char* name) {
+    return {r->data, r->rows ? (uint64_t)(r->rows - 1u) * r->stride + columns : 0u, name};
+}
+Span scales_of(const rfxq_f8_rows* r, uint32_t columns, const char* name) {
+    return {r->scales, r->rows ? 4u * ((uint64_t)(r->rows - 1u) * r->scale_stride + f8_groups(columns)) : 0u, name};
+}
+int check_apart(const Span& a, const Span& b, const char* what) {
+    if (a.p && b.p && overlap(a.p, a.bytes, b.p, b.bytes))
+        return fail(RFXQ_ERR_INVALID_INPUT, "%s: %s and %s overlap", what, a.name, b.name);
+    return RFXQ_OK;
+}
+
+// What rfxq_quantize_f8 and rfxq_silu_and_mul_f8 share: a group of 128 for 16 lanes.
+int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows* up, uint32_t k, const rfxq_f8_rows* out,
+                   hipStream_t stream, const char* what) {
+    F8RowsArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.x = x->data;
+    a.ldx = x->stride;
+    if (up) {
+        a.x2 = up->data;
+        a.ldx2 = up->stride;
+    }
+    a.out = static_cast<uint8_t*>(out->data);
+    a.scales = out->scales;
+    a.ldo = out->stride;
+    a.lds = out->scale_stride;
+    a.rows = x->rows;
+    a.k = k;
+    a.groups = f8_groups(k);
+    const uint64_t grid = std::min<uint64_t>(((uint64_t)a.rows * a.groups + 15u) / 16u, 1u << 20);
+    a.by_rows = (uint32_t)(grid * 16u / a.groups);
+    a.by_groups = (uint32_t)(grid * 16u % a.groups);
+    return launch(fns[float_index(x->type)], (uint32_t)grid, 0, stream, &a, sizeof a, what);
+}
+
+// The kernel and tile of a product.
+struct F8Variant {
+    uint32_t kernel;  // RFXQ_F8_*
+    uint32_t bm, bn, threads;
+};
+F8Variant f8_variant(uint64_t cus, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n, bool aligned) {
+    const uint32_t used = std::min(rows, groups), mean = rows / used;
+    if (mean <= 16u) return {RFXQ_F8_FEW, 16, 16, 512};
+    return {RFXQ_F8_ANY, 64, 128, 256};
+}
+
+// the kernel for `rows` (> 0) places of checked x and w
+F8Variant f8_variant(uint64_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped) {
+    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, w->in_features, w->out_features, false);
+}
+
+int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows, const int32_t* x_index,
+               uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, hipStream_t stream, const char* what) {
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    const uint32_t k = w->in_features, n = w->out_features, groups = std::max(w->expert_count, 1u);
+    F8Args a;
+    std::memset(&a, 0, sizeof a);
+    a.x = static_cast<const uint8_t*>(x->data);
+    a.xs = x->scales;
+    a.w = static_cast<const uint8_t*>(w->data);
+    a.ws = w->scales;
+    a.y = y->data;
+    a.offsets = offsets;
+    a.x_index = x_index;
+    a.y_index = y_index;
+    a.ldx = x->stride;
+    a.ldxs = x->scale_stride;
+    a.ldy = y->stride;
+    a.w_stride = (uint64_t)k * n;
+    a.ws_stride = (uint64_t)f8_groups(k) * f8_groups(n);
+    a.rows = rows;
+    a.x_rows = x->rows;
+    a.y_rows = y->rows;
+    a.x_div = x_div;
+    a.k = k;
+    a.n = n;
+    a.groups = groups;
+    a.y_type = float_index(y->type);
+    const F8Variant v = f8_variant((uint64_t)c->cus, x, w, rows, offsets != nullptr);
+    a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
+    a.tiles_n = (n + v.bn - 1u) / v.bn;
+    // XCD blocks as rfxq_grouped_gemm's
+    const uint32_t across = (a.tiles_n + 3u) / 4u;
+    const uint64_t each = (uint64_t)a.tiles_m * across / 64u;
+    a.sm = each >= 4u ? 4u : each >= 2u ? 2u : 1u;
+    a.sn = (a.tiles_n + across - 1u) / across;
+    const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
+    const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
+    if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
+        return fail(RFXQ_ERR_OTHER, "%s: %u rows x %u columns need %llu workgroups", what, rows, n, (unsigned long long)grid);
+    const uint32_t g = offsets ? 1u : 0u;
+    const hipFunction_t f = v.kernel == RFXQ_F8_FEW ? c->f8.few[g] : c->f8.any[a.y_type == 0 ? 1u : 0u][g];
+    return launch(f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_f8 product launch",
+                  v.threads);
+}
+
+}  // namespace
+
+extern "C" {
+
+int rfxq_quantize_f8(const rfxq_rows* x, uint32_t k, const rfxq_f8_rows* out, hipStream_t stream) {
+    if (k == 0 || k > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "quantize_f8: k=%u", k);
+    if (int rc = check_rows(x, k, "quantize_f8", "x")) return rc;
+    if (int rc = check_f8_rows(out, k, "quantize_f8", "out")) return rc;
+    if (x->rows != out->rows) return fail(RFXQ_ERR_OTHER, "quantize_f8: %u rows of x, %u of out", x->rows, out->rows);
+    if (x->rows == 0) return ok();
+    const Span sx = span_of(x, k, "x"), sc = codes_of(out, k, "out"), ss = scales_of(out, k, "out's scales");
+    for (auto& [a, b] : {std::pair{sx, sc}, std::pair{sx, ss}, std::pair{sc, ss}})
+        if (int rc = check_apart(a, b, "quantize_f8")) return rc;
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    if (int rc = f8_rows_launch(c->f8.quantize, x, nullptr, k, out, stream, "rfxq_f8_quantize launch")) return rc;
+    return ok();
+}
+
+int rfxq_silu_and_mul_f8(const rfxq_rows* gate, const rfxq_rows* up, uint32_t k, const rfxq_f8_rows* out,
+                         hipStream_t stream) {
+    if (k == 0 || k > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "silu_and_mul_f8: k=%u", k);
+    if (int rc = check_rows(gate, k, "silu_and_mul_f8", "gate")) return rc;
+    if (int rc = check_rows(up, k, "silu_and_mul_f8", "up")) return rc;
+    if (int rc = check_f8_rows(out, k, "silu_and_mul_f8", "out")) return rc;
+    if (gate->type != up->type)
+        return fail(RFXQ_ERR_INVALID_INPUT, "silu_and_mul_f8: gate of type %u, up %u", gate->type, up->type);
+    if (gate->rows != up->rows || gate->rows != out->rows)
+        return fail(RFXQ_ERR_OTHER, "silu_and_mul_f8: %u rows of gate, %u of up, %u of out", gate->rows, up->rows, out->rows);
+    if (gate->rows == 0) return ok();
+    const Span sg = span_of(gate, k, "gate"), su = span_of(up, k, "up"), sc = codes_of(out, k, "out");
+    const Span ss = scales_of(out, k, "out's scales");
+    for (auto& [a, b] : {std::pair{sg, sc}, std::pair{su, sc}, std::pair{sg, ss}, std::pair{su, ss}, std::pair{sc, ss}})
+        if (int rc = check_apart(a, b, "silu_and_mul_f8")) return rc;
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    if (int rc = f8_rows_launch(c->f8.silu, gate, up, k, out, stream, "rfxq_f8_silu launch")) return rc;
+    return ok();
+}
+
+int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const float* weight, uint32_t k, float eps,
+                        const rfxq_rows* sum, const rfxq_f8_rows* out, const rfxq_rows* y, hipStream_t stream) {
+    const char* const what = "add_rmsnorm_f8";
+    if (k == 0 || k > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "add_rmsnorm_f8: k=%u", k);
+    if (!(eps >= 0.0f) || std::isinf(eps)) return fail(RFXQ_ERR_INVALID_INPUT, "add_rmsnorm_f8: eps=%g", (double)eps);
+    if (int rc = check_rows(x, k, what, "x")) return rc;
+    if (residual)
+        if (int rc = check_rows(residual, k, what, "residual")) return rc;
+    if (sum)
+        if (int rc = check_rows(sum, k, what, "sum")) return rc;
+    if (y)
+        if (int rc = check_rows(y, k, what, "y")) return rc;
+    if (int rc = check_f8_rows(out, k, what, "out")) return rc;
+    const rfxq_rows* const rows[] = {residual, sum, y};
+    for (const rfxq_rows* r : rows) {
+        if (!r) continue;
+        if (r->type != x->type)
+            return fail(RFXQ_ERR_INVALID_INPUT, "add_rmsnorm_f8: rows of types %u and %u (one type)", x->type, r->type);
+        if (r->rows != x->rows) return fail(RFXQ_ERR_OTHER, "add_rmsnorm_f8: %u and %u rows", x->rows, r->rows);
+    }
+    if (out->rows != x->rows) return fail(RFXQ_ERR_OTHER, "add_rmsnorm_f8: %u rows of x, %u of out", x->rows, out->rows);
+    if (x->rows == 0) return ok();
+    if (!weight || reinterpret_cast<uintptr_t>(weight) % 4u)
+        return fail(RFXQ_ERR_INVALID_INPUT, "add_rmsnorm_f8: weight is NULL or not 4-byte aligned");
+    const Span none = {nullptr, 0, ""};
+    const Span in[] = {span_of(x, k, "x"), residual ? span_of(residual, k, "residual") : none, {weight, 4ull * k, "weight"}};
+    const Span results[] = {codes_of(out, k, "out"), scales_of(out, k, "out's scales"), sum ? span_of(sum, k, "sum") : none,
+                            y ? span_of(y, k, "y") : none};
+    for (size_t i = 0; i < 4; i++) {
+        for (size_t j = 0; j < 3; j++) {
+            const rfxq_rows* r = j == 0 ? x : j == 1 ? residual : nullptr;
+            if (i == 2 && r && sum && sum->data == r->data && sum->stride == r->stride) continue;  // in place
+            if (int rc = check_apart(in[j], results[i], what)) return rc;
+        }
+        for (size_t j = 0; j < i; j++)
+            if (int rc = check_apart(results[j], results[i], what)) return rc;
+    }
+    Ctx* c;
+    if (int rc = current_ctx(&c)) return rc;
+    F8RowsArgs a;
+    std::memset(&a, 0, sizeof a);
+    a.x = x->data;
+    a.ldx = x->stride;
+    if (residual) {
+        a.x2 = residual->data;
+        a.ldx2 = residual->stride;
+    }
+    a.weight = weight;
+    if (sum) {
+        a.sum = sum->data;
+        a.ldsum = sum->stride;
+    }
+    if (y) {
+        a.y = y->data;
+        a.ldy = y->stride;
+    }
+    a.out = static_cast<uint8_t*>(out->data);
+    a.scales = out->scales;
+    a.ldo = out->stride;
+    a.lds = out->scale_stride;
+    a.rows = x->rows;
+    a.k = k;
+    a.groups = f8_groups(k);
+    a.eps = eps;
+    const uint32_t form = k <= 8192u ? 0u : k <= 32768u ? 1u : 2u, each = form == 1u ? 32u : 8u;
+    const uint32_t threads = std::min(1024u, ((k + each - 1u) / each + 63u) / 64u * 64u);
+    if (int rc = launch(c->f8.norm[float_index(x->type)][form], std::min(a.rows, 1u << 20), 0, stream, &a, sizeof a,
+                        "rfxq_f8_norm launch", threads))
+        return rc;
+    return ok();
+}
+
+int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream) {
+    if (int rc = check_f8_weight(w, "gemm_f8")) return rc;
+    if (w->expert_count > 1u)
+        return fail(RFXQ_ERR_OTHER, "gemm_f8: a stack of %u matrices (rfxq_grouped_gemm_f8 takes stacks)", w->expert_count);
+    const uint32_t k = w->in_features, n = w->out_features;
+    if (int rc = check_f8_rows(x, k, "gemm_f8", "x")) return rc;
+    if (int rc = check_rows(y, n, "gemm_f8", "y")) return rc;
+    if (x->rows != y->rows) return fail(RFXQ_ERR_OTHER, "gemm_f8: %u rows of x, %u of y", x->rows, y->rows);
+    if (x->rows == 0) return ok();
+    const Span sy = span_of(y, n, "y");
+    if (int rc = check_apart(codes_of(x, k, "x"), sy, "gemm_f8")) return rc;
+    if (int rc = check_apart(scales_of(x, k, "x's scales"), sy, "gemm_f8")) return rc;
+    if (int rc = f8_product(x, w, nullptr, x->rows, nullptr, 1, nullptr, y, stream, "gemm_f8")) return rc;
+    return ok();
+}
+
+int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
+                         const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
+                         hipStream_t stream) {
+    if (int rc = check_f8_weight(w, "grouped_gemm_f8")) return rc;
+    const uint32_t k = w->in_features, n = w->out_features;
+    if (int rc = check_f8_rows(x, k, "grouped_gemm_f8", "x")) return rc;
+    if (int rc = check_rows(y, n, "grouped_gemm_f8", "y")) return rc;
+    if (rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "grouped_gemm_f8: rows=%u", rows);
+    if (x_div == 0) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: x_div=0");
+    if (!x_index && x_div != 1) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: x_div=%u without x_index", x_div);
+    if (rows == 0 || x->rows == 0 || y->rows == 0) return ok();
+    if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: offsets is NULL");
+    const Span sy = span_of(y, n, "y");
+    if (int rc = check_apart(codes_of(x, k, "x"), sy, "grouped_gemm_f8")) return rc;
+    if (int rc = check_apart(scales_of(x, k, "x's scales"), sy, "grouped_gemm_f8")) return rc;
+    if (int rc = f8_product(x, w, offsets, rows, x_index, x_div, y_index, y, stream, "grouped_gemm_f8")) return rc;
+    return ok();
+}
+
+int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, rfxq_f8_policy* out) {
+    if (!out) return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: NULL output");
+    if (int rc = check_f8_weight(w, "gemm_f8_policy")) return rc;
+    if (int rc = check_f8_rows(x, w->in_features, "gemm_f8_policy", "x")) return rc;
+    if (rows == 0 || rows > 0x7FFFFFFFu || x->rows == 0)
+        return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: rows=%u of %u", rows, x->rows);
+    const Ctx* c = loaded_ctx();
+    const F8Variant v = f8_variant(c ? (uint64_t)c->cus : 256u, x, w, rows, grouped != 0);
+    *out = {v.kernel, v.bm, v.bn};
+    return ok();
+}
+
+}  // extern "C"

@@ -1,0 +1,225 @@
+// Rows in 8-bit floating point (e4m3: 4 bits of exponent, 3 of fraction, no
+// infinities, largest 448) with an f32 scale for each 128 of a row, written by what
+// produces them: plain rows, SiLU(gate) * up, and the RMS norm with the residual's
+// addition. Of a group's 128 values v
+//   amax = max |v|,  scale = max(amax, 448 * 2^-120) / 448,  code = RN_e4m3(v / scale)
+// A group with a value that is not finite has NaN for its scale. The smallest scale
+// keeps 1 / scale an f32 value; groups of zeros have it.
+//
+// 16 lanes (a DPP row) hold a group, 8 values each: amax is four lane moves, and the
+// group's codes one 128-byte line. All three kernels are bound by memory: each input
+// is read once, each output written once.
+#pragma once
+#include "common.hpp"
+#include "tiles.hpp"
+
+constexpr uint32_t kF8Block = 128;
+constexpr float kF8Top = 448.0f, kF8Least = 0x1p-120f;
+typedef u2_t u2a1_t __attribute__((aligned(1)));
+
+struct F8RowsArgs {
+    const void* x;
+    const void* x2;       // SiLU: up; norm: the residual, or NULL
+    const float* weight;  // norm
+    void* sum;            // norm: x + residual, or NULL
+    void* y;              // norm: the values before they are quantized, or NULL
+    uint8_t* out;
+    float* scales;
+    uint64_t ldx, ldx2, ldsum, ldy, ldo, lds;
+    uint32_t rows, k, groups;  // groups = ceil(k / 128)
+    float eps;
+    uint32_t by_rows, by_groups;  // the launch's groups, in rows and groups (quantize, SiLU)
+};
+
+// 8 values starting at v of the group that the 16 lanes of this DPP row hold, as codes
+// and the group's scale.
+RFXQ_DEV u2_t to_f8(const float (&v)[8], float& scale) {
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+    top = top_over_8(top);
+    top = max(top, RFXQ_DPP_U32(top, 0x140));
+    scale = fmaxf(as_f32(top) * (1.0f / kF8Top), kF8Least);
+    float inv = __builtin_amdgcn_rcpf(scale);
+    if (top >= kInfBits) {
+        scale = __builtin_nanf("");
+        inv = 0.0f;
+    }
+    u2_t codes;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; i++) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, 0, false);
+        codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, c, true);
+    }
+    return codes;
+}
+
+// The first `have` of 8 codes, at any byte.
+RFXQ_DEV void st_codes(uint8_t* p, u2_t codes, uint32_t have) {
+    if (have >= 8u) {
+        *(RFXQ_GLOBAL u2a1_t*)p = codes;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++)
+            if (i < have) ((RFXQ_GLOBAL uint8_t*)p)[i] = (uint8_t)(codes[i >> 2] >> (8u * (i & 3u)));
+    }
+}
+
+// The first `have` of 8 values, rounded to T.
+template <typename T>
+RFXQ_DEV void st_eight(T* p, const float (&v)[8], uint32_t have) {
+    if (have >= 8u) {
+        if constexpr (__is_same(T, float)) {
+            *(RFXQ_GLOBAL f4a4_t*)p = f4v_t{v[0], v[1], v[2], v[3]};
+            *(RFXQ_GLOBAL f4a4_t*)(p + 4) = f4v_t{v[4], v[5], v[6], v[7]};
+        } else {
+            u4_t r;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; i++)
+                r[i] = (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * i]) |
+                       (uint32_t)__builtin_bit_cast(uint16_t, (T)v[2 * i + 1]) << 16;
+            *(RFXQ_GLOBAL u4a2_t*)p = r;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++)
+            if (i < have) ((RFXQ_GLOBAL T*)p)[i] = (T)v[i];
+    }
+}
+
+// g / (1 + exp(-g)) * u, by p = exp(-|g|): 1 / (1 + p) or p / (1 + p), which do not overflow.
+// exp by 2^(t + r) with t = RN(-|g| log2 e) and r what the rounding and log2 e's own bits
+// left, so that far values keep f32's bits (below -87 p is under f32's normal range: 0).
+RFXQ_DEV float silu_mul(float g, float u) {
+    constexpr float kLog2e = 1.44269504088896340736f, kLog2eRest = 1.92596299112661746887e-8f;
+    const float n = fmaxf(-__builtin_fabsf(g), -128.0f), t = n * kLog2e, r = __builtin_fmaf(n, kLog2e, -t) + n * kLog2eRest;
+    const float e = __builtin_amdgcn_exp2f(t), p = __builtin_fmaf(e, r * 0.69314718055994530942f, e);
+    return g * ((g < 0.0f ? p : 1.0f) * __builtin_amdgcn_rcpf(1.0f + p)) * u;
+}
+
+// Plain rows, and SiLU(gate) * up: a group is 16 lanes' work, N of them at once so
+// that their loads are in flight together, the launch's other groups between them.
+template <typename T, bool SILU, uint32_t N>
+RFXQ_DEV void f8_rows(const F8RowsArgs& a) {
+    const uint32_t first = (blockIdx.x * 256u + threadIdx.x) >> 4, c = (threadIdx.x & 15u) * 8u;
+    uint32_t row = first / a.groups, group = first % a.groups;
+    while (row < a.rows) {
+        uint32_t at_row[N], at_k[N], have[N];
+        Eight<T> x[N], up[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            at_row[i] = row;
+            at_k[i] = group * kF8Block + c;
+            have[i] = row < a.rows && at_k[i] < a.k ? a.k - at_k[i] : 0u;
+            group += a.by_groups;
+            const uint32_t over = group >= a.groups ? 1u : 0u;
+            group -= over ? a.groups : 0u;
+            row += a.by_rows + over;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            x[i] = ld_eight(static_cast<const T*>(a.x) + (uint64_t)at_row[i] * a.ldx + at_k[i], have[i]);
+            if constexpr (SILU) up[i] = ld_eight(static_cast<const T*>(a.x2) + (uint64_t)at_row[i] * a.ldx2 + at_k[i], have[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            float v[8], scale;
+#pragma unroll
+            for (uint32_t j = 0; j < 8u; j++) {
+                if constexpr (SILU)
+                    v[j] = silu_mul(x[i].at(j), up[i].at(j));
+                else
+                    v[j] = x[i].at(j);
+            }
+            const u2_t codes = to_f8(v, scale);
+            if (at_row[i] >= a.rows) continue;
+            st_codes(a.out + (uint64_t)at_row[i] * a.ldo + at_k[i], codes, have[i]);
+            if (c == 0) stf(a.scales + (uint64_t)at_row[i] * a.lds + at_k[i] / kF8Block, scale);
+        }
+    }
+}
+
+#define RFXQ_F8_ROWS(name, T)                                                                                                  \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_f8_quantize_##name(F8RowsArgs a) { f8_rows<T, false, 1>(a); }       \
+    extern "C" __global__ __launch_bounds__(256) void rfxq_f8_silu_##name(F8RowsArgs a) { f8_rows<T, true, 1>(a); }
+RFXQ_F8_ROWS(f32, float)
+RFXQ_F8_ROWS(f16, half_t)
+RFXQ_F8_ROWS(bf16, __bf16)
+
+// t = x + residual, y = t / sqrt(mean t^2 + eps) * weight: a row a workgroup, its values
+// in registers between the two (N pieces of 8 a thread), in f32 throughout (the sum that
+// is stored is rounded, the norm's is not). N = 0: rows of any length, read
+// twice; a thread reads its values for the second time before it writes over them.
+template <typename T, uint32_t N>
+RFXQ_DEV void f8_norm(const F8RowsArgs& a) {
+    __shared__ float part[16];
+    const uint32_t tid = threadIdx.x, waves = blockDim.x >> 6, by = blockDim.x * 8u;
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + (uint64_t)row * a.ldx;
+        const T* r = static_cast<const T*>(a.x2) + (uint64_t)row * a.ldx2;
+        const auto load = [&](uint32_t k, float(&v)[8]) {
+            const uint32_t have = k < a.k ? a.k - k : 0u;
+            const Eight<T> p = ld_eight(x + k, have);
+            if (a.x2) {
+                const Eight<T> q = ld_eight(r + k, have);
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++) v[j] = p.at(j) + q.at(j);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++) v[j] = p.at(j);
+            }
+        };
+        float t[N ? N : 1u][8], sum = 0.0f;
+        if constexpr (N > 0) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) load((tid + blockDim.x * i) * 8u, t[i]);
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++) sum = __builtin_fmaf(t[i][j], t[i][j], sum);
+        } else {
+            for (uint32_t k = tid * 8u; k < a.k; k += by) {
+                load(k, t[0]);
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++) sum = __builtin_fmaf(t[0][j], t[0][j], sum);
+            }
+        }
+        sum = group_sum<64>(sum);
+        __syncthreads();  // the last row's parts have been read
+        if ((tid & 63u) == 0) part[tid >> 6] = sum;
+        __syncthreads();
+        float all = 0.0f;
+        for (uint32_t w = 0; w < waves; w++) all += part[w];
+        const float rinv = 1.0f / sqrtf(all / (float)a.k + a.eps);
+        const auto write = [&](uint32_t k, const float(&v)[8]) {
+            const uint32_t have = k < a.k ? a.k - k : 0u;
+            if (a.sum) st_eight(static_cast<T*>(a.sum) + (uint64_t)row * a.ldsum + k, v, have);
+            const Eight<float> w = ld_eight(a.weight + k, have);
+            float y[8], scale;
+#pragma unroll
+            for (uint32_t j = 0; j < 8u; j++) y[j] = v[j] * rinv * w.at(j);
+            if (a.y) st_eight(static_cast<T*>(a.y) + (uint64_t)row * a.ldy + k, y, have);
+            const u2_t codes = to_f8(y, scale);
+            st_codes(a.out + (uint64_t)row * a.ldo + k, codes, have);
+            if ((tid & 15u) == 0 && have) stf(a.scales + (uint64_t)row * a.lds + k / kF8Block, scale);
+        };
+        if constexpr (N > 0) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) write((tid + blockDim.x * i) * 8u, t[i]);
+        } else {
+            // whole groups of 16 lanes: the lanes behind the row's end hold zeros
+            for (uint32_t k = tid * 8u; k < (a.k + kF8Block - 1u) / kF8Block * kF8Block; k += by) {
+                load(k, t[0]);
+                write(k, t[0]);
+            }
+        }
+    }
+}
+
+#define RFXQ_F8_NORM(name, T)                                                                                         \
+    extern "C" __global__ __launch_bounds__(1024) void rfxq_f8_norm_##name##_1(F8RowsArgs a) { f8_norm<T, 1>(a); }    \
+    extern "C" __global__ __launch_bounds__(1024) void rfxq_f8_norm_##name##_4(F8RowsArgs a) { f8_norm<T, 4>(a); }    \
+    extern "C" __global__ __launch_bounds__(1024) void rfxq_f8_norm_##name##_any(F8RowsArgs a) { f8_norm<T, 0>(a); }
+RFXQ_F8_NORM(f32, float)
+RFXQ_F8_NORM(f16, half_t)
+RFXQ_F8_NORM(bf16, __bf16)

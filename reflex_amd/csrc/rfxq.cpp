@@ -37,6 +37,7 @@
 extern "C" const unsigned char rfxq_code_object[];
 extern "C" const unsigned char rfxq_code_object_end[];
 extern "C" const unsigned char rfxq_half_code_object[];
+extern "C" const unsigned char rfxq_f8_code_object[];
 
 namespace {
 
@@ -154,6 +155,14 @@ struct HalfKernels {
     hipFunction_t lora_down[5][2] = {}, lora_up[5][3] = {};  // [16, 32 rows, 16 rows of any rank and columns]
 };
 
+// kernels of the third code object (f8_host.hpp); [F32, F16, BF16]
+struct F8Kernels {
+    hipFunction_t quantize[3] = {}, silu[3] = {};
+    hipFunction_t norm[3][3] = {};  // [type][1 piece, 4 pieces, any length]
+    hipFunction_t any[2][2] = {};   // [half results, f32][one matrix, grouped]
+    hipFunction_t few[2] = {};
+};
+
 struct Ctx {
     int device = -1;
     int cus = 256;
@@ -174,6 +183,8 @@ struct Ctx {
     hipFunction_t moe_dec_gu[3][4] = {}, moe_dec_dn[3][4] = {};
     hipModule_t half_mod = nullptr;  // half.hip: grouped rows, half-typed stacks, adapters
     HalfKernels half;
+    hipModule_t f8_mod = nullptr;  // f8.hip: 8-bit floating point
+    F8Kernels f8;
     void* ws = nullptr;
     uint64_t ws_bytes = 0;
     void* scratch = nullptr;  // this device's fixed scratch array (rfxq_gemm_no_alloc)
@@ -244,6 +255,29 @@ int load_half(hipModule_t mod, HalfKernels* h) {
             if (e != hipSuccess)
                 return fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name, hipGetErrorString(e));
         }
+    return RFXQ_OK;
+}
+
+int load_f8(hipModule_t mod, F8Kernels* h) {
+    const auto get = [&](hipFunction_t* f, const std::string& name) {
+        hipError_t e = hipModuleGetFunction(f, mod, name.c_str());
+        return e == hipSuccess ? RFXQ_OK
+                               : fail(RFXQ_ERR_GPU, "hipModuleGetFunction(%s): %s", name.c_str(), hipGetErrorString(e));
+    };
+    static const char* const kType[3] = {"f32", "f16", "bf16"};
+    static const char* const kNorm[3] = {"_1", "_4", "_any"};
+    for (int t = 0; t < 3; t++) {
+        if (int rc = get(&h->quantize[t], std::string("rfxq_f8_quantize_") + kType[t])) return rc;
+        if (int rc = get(&h->silu[t], std::string("rfxq_f8_silu_") + kType[t])) return rc;
+        for (int f = 0; f < 3; f++)
+            if (int rc = get(&h->norm[t][f], std::string("rfxq_f8_norm_") + kType[t] + kNorm[f])) return rc;
+    }
+    for (int g = 0; g < 2; g++) {
+        const std::string end = g ? "_grouped" : "";
+        if (int rc = get(&h->any[0][g], "rfxq_f8_any_half" + end)) return rc;
+        if (int rc = get(&h->any[1][g], "rfxq_f8_any_f32" + end)) return rc;
+        if (int rc = get(&h->few[g], "rfxq_f8_few_1_1_8" + end)) return rc;
+    }
     return RFXQ_OK;
 }
 
@@ -334,6 +368,8 @@ int load_ctx(int device, Ctx** out) {
             }
     HIPCHK(hipModuleLoadData(&c->half_mod, rfxq_half_code_object), "hipModuleLoadData(embedded gfx950 code object)");
     if (int rc = load_half(c->half_mod, &c->half)) return rc;
+    HIPCHK(hipModuleLoadData(&c->f8_mod, rfxq_f8_code_object), "hipModuleLoadData(embedded gfx950 code object)");
+    if (int rc = load_f8(c->f8_mod, &c->f8)) return rc;
     // the fixed scratch of rfxq_gemm_no_alloc, resolved now (the device is
     // current); a failure disables only that entry point, which reports it
     c->scratch_err = rfxq_scratch::setup(device, &c->scratch);
@@ -3797,3 +3833,4 @@ int rfxq_gguf_upload(const rfxq_gguf* g, const uint64_t* indices, uint32_t count
 }  // extern "C"
 
 #include "half_host.hpp"
+#include "f8_host.hpp"

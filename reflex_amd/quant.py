@@ -16,7 +16,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from . import RfxqGemmPolicy, RfxqGemvItem, RfxqOptions, RfxqRows, RfxqWeight, lib
+from . import RfxqF8Rows, RfxqF8Weight, RfxqGemmPolicy, RfxqGemvItem, RfxqOptions, RfxqRows, RfxqWeight, lib
 
 __all__ = [
     "ReflexError", "GgmlError", "GpuError", "OutOfMemoryError", "InvalidInputError", "IoError", "GgufFile",
@@ -30,6 +30,7 @@ __all__ = [
     "act_q8_1_size", "quantize_act_q8_1", "rmsnorm_q8_1", "silu_and_mul_q8_1", "gemm_q8_1", "gemm_q8_1_batch",
     "gemm_gate_up_silu_q8_1",
     "RowGroups", "group_rows", "group_rows_workspace_size", "grouped_gemm", "lora_add", "lora_add_workspace_size",
+    "F8Rows", "F8Weight", "quantize_f8", "silu_and_mul_f8", "add_rmsnorm_f8", "gemm_f8", "grouped_gemm_f8",
     "get_options", "set_options", "options", "gemm_policy", "PATH_GEMV_ROWS", "PATH_MMQ_INT8", "PATH_MMQ_F16",
 ]
 
@@ -760,6 +761,165 @@ def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.
                                    _ints(groups.order, xr.rows, dev, "lora_add order"), yr, outr, space, size,
                                    _stream()))
     return out
+
+
+# ------------------------------------------------------------------ 8-bit floating point
+
+_F8_TYPES = (torch.float8_e4m3fn, torch.uint8)
+
+
+@dataclass
+class F8Rows:
+    """Rows in e4m3 with a scale for each 128 of a row (``rfxq_f8_rows``): value (r, c) is
+    ``codes[r, c] * scales[r, c // 128]``."""
+
+    codes: torch.Tensor   # float8_e4m3fn (or its bytes as uint8) [rows, columns]
+    scales: torch.Tensor  # f32 [rows, ceil(columns / 128)]
+
+    @classmethod
+    def empty(cls, rows: int, columns: int, device="cuda") -> "F8Rows":
+        return cls(torch.empty(rows, columns, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty(rows, (columns + 127) // 128, dtype=torch.float32, device=device))
+
+
+class F8Weight:
+    """A matrix [out, in] or a stack [count, out, in] in e4m3 with a scale for each block of 128 x 128
+    (``rfxq_f8_weight``), as checkpoints hold them; scales f32 [(count,) ceil(out / 128), ceil(in / 128)].
+    Both contiguous, on one GPU; no copy: the weight reads the tensors' memory."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype not in _F8_TYPES or codes.dim() not in (2, 3) or not codes.is_contiguous():
+            raise InvalidInputError(11, f"F8Weight: codes {codes.dtype} {list(codes.shape)} (contiguous float8_e4m3fn or "
+                                        "uint8 of 2 or 3 dimensions)")
+        want = list(codes.shape[:-2]) + [(v + 127) // 128 for v in codes.shape[-2:]]
+        if (scales.dtype is not torch.float32 or list(scales.shape) != want or not scales.is_contiguous()
+                or scales.device != codes.device):
+            raise InvalidInputError(11, f"F8Weight: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
+                                        f"(contiguous f32 {want} on {codes.device})")
+        self.codes, self.scales = codes, scales
+        self.count = _count(codes.shape[0], 1, "F8Weight: count") if codes.dim() == 3 else 0
+        self.out_features, self.in_features = (_count(v, 1, "F8Weight: shape") for v in codes.shape[-2:])
+        self._c = RfxqF8Weight(self.in_features, self.out_features, self.count, codes.data_ptr(), scales.data_ptr(),
+                               codes.numel(), 4 * scales.numel())
+
+
+def _steps(t: torch.Tensor, what: str) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are contiguous."""
+    (rows, columns), (step, one) = t.shape, t.stride()
+    if rows <= 1:
+        step = columns
+    if step < columns or (one != 1 and columns > 1):
+        raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
+    return step
+
+
+def _f8_rows(r: F8Rows, rows: int | None, columns: int, dev: int, what: str) -> RfxqF8Rows:
+    c, s = r.codes, r.scales
+    if (c.dtype not in _F8_TYPES or len(c.shape) != 2 or c.shape[1] != columns or c.get_device() != dev
+            or (rows is not None and c.shape[0] != rows)):
+        raise InvalidInputError(11, f"{what}: codes {c.dtype} {list(c.shape)} on {c.device} (float8_e4m3fn or uint8 "
+                                    f"[{'rows' if rows is None else rows}, {columns}] on cuda:{dev})")
+    if (s.dtype is not torch.float32 or len(s.shape) != 2 or s.shape[0] != c.shape[0]
+            or s.shape[1] != (columns + 127) // 128 or s.get_device() != dev):
+        raise InvalidInputError(11, f"{what}: scales {s.dtype} {list(s.shape)} on {s.device} "
+                                    f"(f32 [{c.shape[0]}, {(columns + 127) // 128}] on cuda:{dev})")
+    return RfxqF8Rows(c.data_ptr(), s.data_ptr(), _count(c.shape[0], 0, f"{what}: rows"), _steps(c, what), _steps(s, what))
+
+
+def _matrix(t: torch.Tensor, what: str) -> tuple[int, int]:
+    if t.dim() != 2:
+        raise InvalidInputError(11, f"{what}: {list(t.shape)} (two dimensions)")
+    return t.shape[0], _count(t.shape[1], 1, f"{what}: columns")
+
+
+def quantize_f8(x: torch.Tensor, out: F8Rows | None = None) -> F8Rows:
+    """f32, f16 or bf16 rows [rows, k] in e4m3 with a scale for each 128 of a row: the largest size / 448."""
+    dev = _on(x, "quantize_f8: x")
+    rows, k = _matrix(x, "quantize_f8 x")
+    xr = _rows(x, k, dev, "quantize_f8 x")
+    if out is None:
+        out = F8Rows.empty(rows, k, x.device)
+    with _dev(x):
+        _check(lib().rfxq_quantize_f8(xr, k, _f8_rows(out, rows, k, dev, "quantize_f8 out"), _stream()))
+    return out
+
+
+def silu_and_mul_f8(gate: torch.Tensor, up: torch.Tensor, out: F8Rows | None = None) -> F8Rows:
+    """``silu_and_mul`` with its result in e4m3 (``quantize_f8``); gate and up [rows, k] of one type may be columns of
+    one matrix."""
+    dev = _on(gate, "silu_and_mul_f8: gate")
+    rows, k = _matrix(gate, "silu_and_mul_f8 gate")
+    gr, ur = _rows(gate, k, dev, "silu_and_mul_f8 gate"), _rows(up, k, dev, "silu_and_mul_f8 up")
+    if out is None:
+        out = F8Rows.empty(rows, k, gate.device)
+    with _dev(gate):
+        _check(lib().rfxq_silu_and_mul_f8(gr, ur, k, _f8_rows(out, rows, k, dev, "silu_and_mul_f8 out"), _stream()))
+    return out
+
+
+def add_rmsnorm_f8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,
+                   sum_out: torch.Tensor | None = None, out: F8Rows | None = None, want_y: bool = False):
+    """The residual stream's addition, the RMS norm behind it and its result in e4m3 (``quantize_f8``): (out, sum, y).
+    ``sum = x + residual`` [rows, k] (None without a residual and ``sum_out``; ``sum_out`` may be x or residual itself),
+    ``y`` (``want_y``, else None) and out are ``sum / sqrt(mean(sum^2) + eps) * weight``, in f32 from the unrounded sum.
+    weight: k f32 values."""
+    dev = _on(x, "add_rmsnorm_f8: x")
+    rows, k = _matrix(x, "add_rmsnorm_f8 x")
+    xr = _rows(x, k, dev, "add_rmsnorm_f8 x")
+    rr = None if residual is None else _rows(residual, k, dev, "add_rmsnorm_f8 residual")
+    if (weight.dtype is not torch.float32 or weight.numel() != k or weight.get_device() != dev
+            or not weight.is_contiguous()):
+        raise InvalidInputError(11, f"add_rmsnorm_f8: weight {weight.dtype} {list(weight.shape)} on {weight.device} "
+                                    f"(f32, {k} contiguous values on cuda:{dev})")
+    if sum_out is None and residual is not None:
+        sum_out = torch.empty(rows, k, dtype=x.dtype, device=x.device)
+    sr = None if sum_out is None else _rows(sum_out, k, dev, "add_rmsnorm_f8 sum_out")
+    y = torch.empty(rows, k, dtype=x.dtype, device=x.device) if want_y else None
+    yr = None if y is None else _rows(y, k, dev, "add_rmsnorm_f8 y")
+    if out is None:
+        out = F8Rows.empty(rows, k, x.device)
+    with _dev(x):
+        _check(lib().rfxq_add_rmsnorm_f8(xr, rr, weight.data_ptr(), k, eps, sr,
+                                         _f8_rows(out, rows, k, dev, "add_rmsnorm_f8 out"), yr, _stream()))
+    return out, sum_out, y
+
+
+def _f8_weight(w: F8Weight, dev: int, what: str) -> RfxqF8Weight:
+    if w.codes.get_device() != dev:
+        raise InvalidInputError(11, f"{what}: weight on {w.codes.device}, rows on cuda:{dev}")
+    return w._c
+
+
+def gemm_f8(x: F8Rows, w: F8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``gemm`` of e4m3 rows with an e4m3 matrix, both with their scales: [rows, out] in ``out``'s type (f32, f16 or
+    bf16; without ``out`` a new tensor of ``dtype``)."""
+    dev = _on(x.codes, "gemm_f8: x")
+    c = _f8_weight(w, dev, "gemm_f8")
+    xr = _f8_rows(x, None, c.in_features, dev, "gemm_f8 x")
+    y = out if out is not None else torch.empty(xr.rows, c.out_features, dtype=dtype, device=x.codes.device)
+    yr = _rows(y, c.out_features, dev, "gemm_f8 out")
+    with _dev(x.codes):
+        _check(lib().rfxq_gemm_f8(xr, c, yr, _stream()))
+    return y
+
+
+def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
+                    x_div: int = 1, y_index: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``grouped_gemm`` of e4m3 rows with an e4m3 stack, both with their scales. Without ``out``, a new tensor of
+    ``dtype`` with ``rows`` rows, zero where no place of a group writes."""
+    dev = _on(x.codes, "grouped_gemm_f8: x")
+    c = _f8_weight(w, dev, "grouped_gemm_f8")
+    _count(rows, 0, "grouped_gemm_f8: rows")
+    _count(x_div, 1, "grouped_gemm_f8: x_div")
+    xr = _f8_rows(x, None, c.in_features, dev, "grouped_gemm_f8 x")
+    y = out if out is not None else torch.zeros(rows, c.out_features, dtype=dtype, device=x.codes.device)
+    yr = _rows(y, c.out_features, dev, "grouped_gemm_f8 out")
+    with _dev(x.codes):
+        _check(lib().rfxq_grouped_gemm_f8(xr, c, _ints(offsets, (c.expert_count or 1) + 1, dev, "grouped_gemm_f8 offsets"),
+                                          rows, _ints(x_index, rows, dev, "grouped_gemm_f8 x_index"), x_div,
+                                          _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), yr, _stream()))
+    return y
 
 
 # ------------------------------------------------------------------ GGUF files

@@ -1,0 +1,234 @@
+"""Refusals of the entry points in 8-bit floating point (rfxq_quantize_f8, rfxq_silu_and_mul_f8,
+rfxq_add_rmsnorm_f8, rfxq_gemm_f8, rfxq_grouped_gemm_f8): all of them are decided on the host, before
+any launch, so they run without a GPU (addresses that are never read)."""
+import ctypes
+
+import pytest
+import torch
+
+P = 1 << 20  # a plausible device address
+F32, F16, BF16, Q4K = 0, 1, 30, 12
+INF = float("inf")
+
+
+@pytest.fixture(scope="module")
+def L():
+    import reflex_amd
+
+    return reflex_amd.lib()
+
+
+def _rows(ty=F16, rows=8, stride=300, data=2 * P):
+    import reflex_amd as rq
+
+    return rq.RfxqRows(data, ty, rows, stride)
+
+
+def _f8(rows=8, stride=300, scale_stride=3, data=4 * P, scales=5 * P):
+    import reflex_amd as rq
+
+    return rq.RfxqF8Rows(data, scales, rows, stride, scale_stride)
+
+
+def _weight(k=300, n=200, e=0, data=6 * P, scales=7 * P, length=None, scales_len=None):
+    import reflex_amd as rq
+
+    c = max(e, 1)
+    return rq.RfxqF8Weight(k, n, e, data, scales, c * k * n if length is None else length,
+                           4 * c * ((k + 127) // 128) * ((n + 127) // 128) if scales_len is None else scales_len)
+
+
+def _ref(make, v):
+    return None if v is None else ctypes.byref(make(**v))
+
+
+def _expect(L, rc, code, text):
+    assert rc == code and text in L.rfxq_last_error().decode(), (rc, L.rfxq_last_error())
+
+
+ROWS = [
+    ({"x": None}, 11, "x is NULL"),
+    ({"x": {"ty": Q4K}}, 1, "of type 12"),
+    ({"x": {"data": None}}, 11, "x data is NULL"),
+    ({"x": {"data": 2 * P + 1}}, 12, "aligned"),
+    ({"x": {"stride": 299}}, 12, "stride=299"),
+    ({"x": {"rows": 7}}, 12, "7"),
+    ({"x": {"rows": 1 << 31}}, 12, "rows"),
+    ({"out": None}, 11, "out is NULL"),
+    ({"out": {"data": None}}, 11, "data or scales is NULL"),
+    ({"out": {"scales": None}}, 11, "data or scales is NULL"),
+    ({"out": {"scales": 5 * P + 2}}, 12, "4-byte aligned"),
+    ({"out": {"stride": 299}}, 12, "stride=299"),
+    ({"out": {"scale_stride": 2}}, 12, "scale_stride=2"),
+    ({"out": {"stride": 1 << 46}}, 12, "stride="),
+    ({"out": {"rows": 9}}, 12, "9"),
+    ({"out": {"data": 2 * P + 100}}, 11, "overlap"),
+    ({"out": {"scales": 2 * P + 100}}, 11, "overlap"),
+    ({"out": {"scales": 4 * P + 2000}}, 11, "overlap"),
+    ({"k": 0}, 12, "k=0"),
+    ({"k": 1 << 31}, 12, "k="),
+]
+
+
+@pytest.mark.parametrize("change,code,text", ROWS)
+def test_quantize_refusals(L, change, code, text):
+    a = {"x": {}, "out": {}, "k": 300, **change}
+    _expect(L, L.rfxq_quantize_f8(_ref(_rows, a["x"]), a["k"], _ref(_f8, a["out"]), None), code, text)
+
+
+@pytest.mark.parametrize("change,code,text", [(c, code, "gate is NULL" if text == "x is NULL" else
+                                               "gate data is NULL" if text == "x data is NULL" else text)
+                                              for c, code, text in ROWS] + [
+    ({"up": None}, 11, "up is NULL"),
+    ({"up": {"ty": F32}}, 11, "gate of type 1, up 0"),
+    ({"up": {"rows": 9}}, 12, "9 of up"),
+    ({"up": {"stride": 200}}, 12, "stride=200"),
+    ({"up": {"data": 4 * P}}, 11, "overlap"),
+])
+def test_silu_refusals(L, change, code, text):
+    a = {"x": {}, "up": {"data": 3 * P}, "out": {}, "k": 300, **change}
+    if a["up"] is not None:
+        a["up"] = {"data": 3 * P, **a["up"]}
+    _expect(L, L.rfxq_silu_and_mul_f8(_ref(_rows, a["x"]), _ref(_rows, a["up"]), a["k"], _ref(_f8, a["out"]), None), code,
+            text)
+
+
+@pytest.mark.parametrize("change,code,text", ROWS + [
+    ({"residual": {"ty": F32}}, 11, "types 1 and 0"),
+    ({"residual": {"rows": 5}}, 12, "8 and 5 rows"),
+    ({"residual": {"data": 4 * P}}, 11, "overlap"),
+    ({"sum": {"ty": BF16}}, 11, "types 1 and 30"),
+    ({"sum": {"stride": 1}}, 12, "stride=1"),
+    ({"sum": {"data": 2 * P + 64}}, 11, "x and sum overlap"),
+    ({"sum": {"data": 2 * P, "stride": 400}}, 11, "x and sum overlap"),
+    ({"sum": {"data": 3 * P + 2}}, 11, "residual and sum overlap"),
+    ({"sum": {"data": 4 * P}}, 11, "out and sum overlap"),
+    ({"sum": {"data": 10 * P}}, 11, "weight and sum overlap"),
+    ({"y": {"data": 2 * P}}, 11, "x and y overlap"),
+    ({"y": {"data": 9 * P}}, 11, "sum and y overlap"),
+    ({"y": {"ty": F32}}, 11, "types 1 and 0"),
+    ({"weight": None}, 11, "weight is NULL"),
+    ({"weight": 10 * P + 2}, 11, "weight is NULL or not 4-byte aligned"),
+    ({"eps": -1e-6}, 11, "eps="),
+    ({"eps": INF}, 11, "eps="),
+    ({"eps": float("nan")}, 11, "eps="),
+])
+def test_norm_refusals(L, change, code, text):
+    a = {"x": {}, "residual": {}, "sum": {}, "y": None, "out": {}, "k": 300, "weight": 10 * P, "eps": 1e-6, **change}
+    a["residual"] = {"data": 3 * P, **a["residual"]}
+    a["sum"] = {"data": 9 * P, **a["sum"]}
+    _expect(L, L.rfxq_add_rmsnorm_f8(_ref(_rows, a["x"]), _ref(_rows, a["residual"]), a["weight"], a["k"], a["eps"],
+                                     _ref(_rows, a["sum"]), _ref(_f8, a["out"]), _ref(_rows, a["y"]), None), code, text)
+
+
+PRODUCT = [
+    ({"w": None}, 11, "weight is NULL"),
+    ({"w": {"k": 0}}, 12, "shape"),
+    ({"w": {"n": 0}}, 12, "shape"),
+    ({"w": {"n": 1 << 31, "length": 1 << 62}}, 12, "shape"),
+    ({"w": {"length": 300 * 200 - 1}}, 12, "needs"),
+    ({"w": {"scales_len": 4 * 6 - 1}}, 12, "needs"),
+    ({"w": {"data": None}}, 11, "data or scales is NULL"),
+    ({"w": {"scales": None}}, 11, "data or scales is NULL"),
+    ({"w": {"scales": 7 * P + 1}}, 12, "aligned"),
+    ({"w": {"e": 1025}}, 12, "expert_count=1025"),
+    ({"x": None}, 11, "x is NULL"),
+    ({"x": {"data": None}}, 11, "NULL"),
+    ({"x": {"scales": None}}, 11, "NULL"),
+    ({"x": {"stride": 299}}, 12, "stride=299"),
+    ({"x": {"scale_stride": 2}}, 12, "scale_stride=2"),
+    ({"x": {"scales": 5 * P + 1}}, 12, "aligned"),
+    ({"y": None}, 11, "y is NULL"),
+    ({"y": {"ty": Q4K}}, 1, "of type 12"),
+    ({"y": {"stride": 199}}, 12, "stride=199"),
+    ({"y": {"data": 2 * P + 1}}, 12, "aligned"),
+    ({"y": {"data": 4 * P + 128}}, 11, "x and y overlap"),
+    ({"y": {"data": 5 * P + 8}}, 11, "x's scales and y overlap"),
+]
+
+
+@pytest.mark.parametrize("change,code,text", PRODUCT + [
+    ({"w": {"e": 2}}, 12, "stack of 2"),
+    ({"y": {"rows": 9}}, 12, "8 rows of x, 9 of y"),
+])
+def test_gemm_refusals(L, change, code, text):
+    a = {"x": {}, "w": {}, "y": {}, **change}
+    _expect(L, L.rfxq_gemm_f8(_ref(_f8, a["x"]), _ref(_weight, a["w"]), _ref(_rows, a["y"]), None), code, text)
+
+
+def _grouped(L, x={}, w={}, offsets=8 * P, rows=8, x_index=None, x_div=1, y_index=None, y={}):
+    return L.rfxq_grouped_gemm_f8(_ref(_f8, x), _ref(_weight, w), offsets, rows, x_index, x_div, y_index, _ref(_rows, y), None)
+
+
+@pytest.mark.parametrize("change,code,text", PRODUCT + [
+    ({"rows": 1 << 31}, 12, "rows="),
+    ({"x_div": 0}, 11, "x_div=0"),
+    ({"x_div": 2}, 11, "x_div=2 without x_index"),
+    ({"offsets": None}, 11, "offsets is NULL"),
+])
+def test_grouped_refusals(L, change, code, text):
+    if isinstance(change.get("w"), dict) and "e" not in change["w"] and change["w"].get("length") is None:
+        change = {**change, "w": {"e": 1, **change["w"]}}
+    _expect(L, _grouped(L, **change), code, text)
+
+
+@pytest.mark.parametrize("empty", [{"rows": 0}, {"x": {"rows": 0, "data": None, "scales": None}},
+                                   {"y": {"rows": 0, "data": None}}])
+def test_products_of_nothing(L, empty):
+    assert _grouped(L, **empty) == 0
+    if "rows" not in empty:
+        both = {"x": {"rows": 0, "data": None}, "y": {"rows": 0, "data": None}}
+        assert L.rfxq_gemm_f8(_ref(_f8, both["x"]), _ref(_weight, {}), _ref(_rows, both["y"]), None) == 0
+
+
+def test_rows_of_nothing(L):
+    x, out = _ref(_rows, {"rows": 0, "data": None}), _ref(_f8, {"rows": 0, "data": None})
+    assert L.rfxq_quantize_f8(x, 300, out, None) == 0
+    assert L.rfxq_silu_and_mul_f8(x, x, 300, out, None) == 0
+    assert L.rfxq_add_rmsnorm_f8(x, None, None, 300, 1e-6, None, out, None, None) == 0
+
+
+def test_policy_refusals(L):
+    import reflex_amd as rq
+
+    p = rq.RfxqF8Policy()
+    x, w = _ref(_f8, {}), _ref(_weight, {})
+    _expect(L, L.rfxq_gemm_f8_policy(x, w, 8, 0, None), 11, "NULL output")
+    _expect(L, L.rfxq_gemm_f8_policy(x, None, 8, 0, ctypes.byref(p)), 11, "weight is NULL")
+    _expect(L, L.rfxq_gemm_f8_policy(None, w, 8, 0, ctypes.byref(p)), 11, "x is NULL")
+    _expect(L, L.rfxq_gemm_f8_policy(x, w, 0, 0, ctypes.byref(p)), 11, "rows=0")
+    assert L.rfxq_gemm_f8_policy(x, w, 8, 1, ctypes.byref(p)) == 0
+
+
+def test_python_checks():
+    import reflex_amd as rq
+
+    f8 = torch.float8_e4m3fn
+    codes, scales = torch.zeros(4, 300, dtype=f8), torch.zeros(4, 3)
+    bad = rq.InvalidInputError
+    with pytest.raises(bad, match="codes"):
+        rq.F8Weight(torch.zeros(4, 300), scales)
+    with pytest.raises(bad, match="codes"):
+        rq.F8Weight(codes[:, ::2], scales)
+    with pytest.raises(bad, match="codes"):
+        rq.F8Weight(codes[0], scales)
+    with pytest.raises(bad, match="scales"):
+        rq.F8Weight(codes, scales)
+    with pytest.raises(bad, match="scales"):
+        rq.F8Weight(codes, torch.zeros(1, 3, dtype=torch.float16))
+    with pytest.raises(bad, match="shape=0"):
+        rq.F8Weight(torch.zeros(0, 300, dtype=f8), torch.zeros(0, 3))
+    with pytest.raises(bad, match="count=0"):
+        rq.F8Weight(torch.zeros(0, 4, 300, dtype=f8), torch.zeros(0, 1, 3))
+    w = rq.F8Weight(codes, torch.zeros(1, 3))
+    assert (w.in_features, w.out_features, w.count) == (300, 4, 0)
+    assert rq.F8Weight(torch.zeros(2, 4, 300, dtype=torch.uint8), torch.zeros(2, 1, 3)).count == 2
+    # rows on the CPU
+    for call in (lambda: rq.quantize_f8(torch.zeros(4, 300)), lambda: rq.silu_and_mul_f8(torch.zeros(4, 3), torch.zeros(4, 3)),
+                 lambda: rq.add_rmsnorm_f8(torch.zeros(4, 3), None, torch.zeros(3), 1e-6),
+                 lambda: rq.gemm_f8(rq.F8Rows(codes, scales), w),
+                 lambda: rq.grouped_gemm_f8(rq.F8Rows(codes, scales), w, torch.zeros(2, dtype=torch.int32), 4)):
+        with pytest.raises(bad, match="on cpu"):
+            call()
+    empty = rq.F8Rows.empty(3, 129, "cpu")
+    assert empty.codes.shape == (3, 129) and empty.scales.shape == (3, 2)
