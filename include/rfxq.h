@@ -540,8 +540,8 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
  * results have exact products summed in f32; for f16 and bf16 ones the matrix
  * instructions may cut each product to a multiple of 2^-13 of the largest of the eight
  * neighbours that are added first (by the exponents of their codes, subnormal codes
- * and zeros counted as 2^-6), which costs 1.5e-5 of a result for normal values. NaN codes and scales give NaN in the results that they
- * belong to. Any sizes, strides and alignment of whole elements (scales and
+ * and zeros counted as 2^-6), which costs 1.5e-5 of a result for normal values. NaN codes give NaN, and scales that are not finite
+ * results that are not finite, where they belong, and nowhere else. Any sizes, strides and alignment of whole elements (scales and
  * y); rows of x and w that start at multiples of 16 bytes are faster. y must not overlap x. One
  * launch, no workspace, no host synchronisation: it can be captured. The order of a sum depends
  * on the call's sizes and alignment, not on anything else: equal calls give equal bits. */
@@ -557,14 +557,18 @@ int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const i
 
 /* Test hook: the kernel and tile that rfxq_gemm_f8 (grouped = 0) or
  * rfxq_grouped_gemm_f8 runs on the current device (256 compute units before
- * rfxq_init) for `rows` rows or places of x and w; no memory is read. */
-#define RFXQ_F8_ANY 0 /* 64 x 128 tiles through registers, any alignment */
-#define RFXQ_F8_FEW 1 /* weights straight from memory, K among a workgroup's waves */
+ * rfxq_init) for `rows` rows or places of x and w and results of a type; no memory is read. */
+#define RFXQ_F8_ANY 0    /* 64 x 128 tiles through registers, any alignment */
+#define RFXQ_F8_FEW 1    /* 16 x 16, straight from memory, any alignment */
+#define RFXQ_F8_STREAM 2 /* few rows: K among a workgroup's waves, each with copies of its own */
+#define RFXQ_F8_COPIED 3 /* 64 or 128 x 128 tiles, asynchronous copies */
+#define RFXQ_F8_LARGE 4  /* 128 or 256 x 256 tiles, asynchronous copies, f16 and bf16 results */
 typedef struct rfxq_f8_policy {
     uint32_t kernel; /* RFXQ_F8_* */
     uint32_t tile_m, tile_n;
 } rfxq_f8_policy;
-int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, rfxq_f8_policy* out);
+int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
+                        rfxq_f8_policy* out);
 
 /* ---- GGUF files (the on-disk path) ---------------------------------------- */
 

@@ -5,3 +5,5 @@
 #include "tiles.hpp"
 #include "f8_rows.hpp"
 #include "f8_gemm.hpp"
+#include "f8_tile.hpp"
+#include "f8_few.hpp"

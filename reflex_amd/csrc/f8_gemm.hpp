@@ -81,14 +81,33 @@ RFXQ_DEV f4v_t multiply(const Operand<true>& a, const Operand<true>& b) {
 
 // 16 codes at any byte
 RFXQ_DEV u4_t ld_codes(const uint8_t* p) { return *(const RFXQ_GLOBAL u4a1_t*)p; }
-// the first `have` of them, one by one, then zeros
-RFXQ_DEV u4_t ld_codes(const uint8_t* p, uint32_t have) {
-    if (have >= 16u) return ld_codes(p);
+// The first `have` (< 16) of the 16 codes that end where a row of k codes ends, zeros behind
+// them: the row's last 16, moved down by whole dwords and then by bytes (a row
+// of fewer than 16: one by one).
+RFXQ_DEV u4_t ld_tail(const uint8_t* row, uint32_t k, uint32_t have) {
     u4_t r = {0, 0, 0, 0};
+    if (k >= 16u) {
+        const uint32_t by = 16u - have;
+        u4_t v = ld_codes(row + k - 16u);
+        if (by & 8u) v = u4_t{v.z, v.w, 0, 0};
+        if (by & 4u) v = u4_t{v.y, v.z, v.w, 0};
+        r = u4_t{alignbyte(v.y, v.x, by & 3u), alignbyte(v.z, v.y, by & 3u), alignbyte(v.w, v.z, by & 3u),
+                 alignbyte(0, v.w, by & 3u)};
+        if (have == 0) r = u4_t{0, 0, 0, 0};
+    } else {
+#pragma unroll 1
+        for (uint32_t i = 0; i < have; i++) {
+            const uint32_t c = (uint32_t)((const RFXQ_GLOBAL uint8_t*)row)[i] << (8u * (i & 3u));
 #pragma unroll
-    for (uint32_t i = 0; i < 16u; i++)
-        if (i < have) r[i >> 2] |= (uint32_t)((const RFXQ_GLOBAL uint8_t*)p)[i] << (8u * (i & 3u));
+            for (uint32_t d = 0; d < 4u; d++) r[d] |= i >> 2 == d ? c : 0u;
+        }
+    }
     return r;
+}
+// 16 codes of a row of k from its code `at` on, of which all, some or none are there
+RFXQ_DEV u4_t ld_codes(const uint8_t* row, uint32_t k, uint32_t at) {
+    if (at + 16u <= k) return ld_codes(row + at);
+    return ld_tail(row, k, at < k ? k - at : 0u);
 }
 
 // The rows of a tile: a search among the groups, or counted.
@@ -142,20 +161,23 @@ RFXQ_DEV void f8_out(const F8Args& a, int64_t row, uint32_t n, const f4v_t (&v)[
 
 // ---------------------------------------------------------------- any alignment
 
-// 64 x 128 tiles (one block of weights' scales a step), 4 waves of 32 x 64, operands
-// through registers to LDS, the next block's loads in flight during the products. Rows and
-// columns past the tile read others, whose results are not stored; the last,
-// partial block is loaded byte by byte with zeros behind the end of both operands.
-template <bool EXACT, bool GROUPED>
+// 64 x 128 tiles (one block of weights' scales a step), operands through registers to
+// LDS, the next step's loads in flight during the products. KG groups of four waves of
+// 32 x 64 results take a block of K each of a step's KG, and add their parts in LDS. Rows
+// and columns past the tile read others, whose results are not stored; the last,
+// partial block has zeros behind the end of both operands, a block past it no
+// weights and the scale 0.
+template <uint32_t KG, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_any(const F8Args& a) {
-    constexpr uint32_t BM = 64, BN = 128, NX = BM * 8u / 256u, NW = BN * 8u / 256u;
-    __shared__ u4_t xs[BM * 8u], ws[BN * 8u];
+    constexpr uint32_t BM = 64, BN = 128, ROWS = 32, NX = BM / ROWS, NW = BN / ROWS;
+    __shared__ u4_t xs[KG][BM * 8u], ws[KG][BN * 8u];
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
     const RowTile t = f8_tile<GROUPED>(a, BM, tm);
     if (!t.any) return;
-    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63u, l = lane & 15u, q = lane >> 4;
-    const uint32_t n0 = tn * BN, c = tid & 7u, row0 = (wave >> 1) * 32u, col0 = (wave & 1u) * 64u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), kg = wave >> 2;
+    const uint32_t tid = threadIdx.x & 255u, lane = tid & 63u, l = lane & 15u, q = lane >> 4;
+    const uint32_t n0 = tn * BN, c = tid & 7u, row0 = (wave >> 1 & 1u) * 32u, col0 = (wave & 1u) * 64u;
     const uint32_t full = a.k / kBlock, tail = a.k % kBlock, blocks = full + (tail ? 1u : 0u);
     const uint8_t* w = a.w + (uint64_t)t.group * a.w_stride;
     const float* sw = a.ws + (uint64_t)t.group * a.ws_stride + (uint64_t)tn * blocks;
@@ -163,8 +185,8 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     const float* sx[2];
 #pragma unroll
     for (uint32_t i = 0; i < NX; i++) {
-        const int64_t s = f8_src<GROUPED>(a, min(t.beg + (tid >> 3) + 32u * i, t.end - 1u));
-        xp[i] = a.x + (s < 0 ? 0 : (uint64_t)s * a.ldx) + 16u * c;
+        const int64_t s = f8_src<GROUPED>(a, min(t.beg + (tid >> 3) + ROWS * i, t.end - 1u));
+        xp[i] = a.x + (s < 0 ? 0 : (uint64_t)s * a.ldx);
     }
 #pragma unroll
     for (uint32_t m = 0; m < 2u; m++) {
@@ -173,55 +195,74 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     }
 #pragma unroll
     for (uint32_t i = 0; i < NW; i++)
-        wp[i] = w + (uint64_t)min(n0 + col_of((tid >> 3) + 32u * i), a.n - 1u) * a.k + 16u * c;
+        wp[i] = w + (uint64_t)min(n0 + col_of((tid >> 3) + ROWS * i), a.n - 1u) * a.k;
     f4v_t acc[2][4] = {};
-    u4_t xv[NX], wv[NW];
-    float xsc[2], wsc;
+    struct Block {
+        u4_t x[NX], w[NW];
+        float sx[2], sw;
+    } r;
     const auto load = [&](uint32_t b) {
-        const uint32_t k = b * kBlock;
+        const uint32_t k = b * kBlock + 16u * c;
         if (b < full) {
 #pragma unroll
-            for (uint32_t i = 0; i < NW; i++) wv[i] = ld_codes(wp[i] + k);
+            for (uint32_t i = 0; i < NW; i++) r.w[i] = ld_codes(wp[i] + k);
 #pragma unroll
-            for (uint32_t i = 0; i < NX; i++) xv[i] = ld_codes(xp[i] + k);
+            for (uint32_t i = 0; i < NX; i++) r.x[i] = ld_codes(xp[i] + k);
         } else if (b < blocks) {
-            const uint32_t have = tail > 16u * c ? tail - 16u * c : 0u;
 #pragma unroll
-            for (uint32_t i = 0; i < NW; i++) wv[i] = ld_codes(wp[i] + k, have);
+            for (uint32_t i = 0; i < NW; i++) r.w[i] = ld_codes(wp[i], a.k, k);
 #pragma unroll
-            for (uint32_t i = 0; i < NX; i++) xv[i] = ld_codes(xp[i] + k, have);
+            for (uint32_t i = 0; i < NX; i++) r.x[i] = ld_codes(xp[i], a.k, k);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < NW; i++) r.w[i] = u4_t{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < NX; i++) r.x[i] = u4_t{0, 0, 0, 0};
         }
         const uint32_t at = min(b, blocks - 1u);
-        wsc = ((const RFXQ_GLOBAL float*)sw)[at];
+        r.sw = b < blocks ? ((const RFXQ_GLOBAL float*)sw)[at] : 0.0f;
 #pragma unroll
-        for (uint32_t m = 0; m < 2u; m++) xsc[m] = ((const RFXQ_GLOBAL float*)sx[m])[at];
+        for (uint32_t m = 0; m < 2u; m++) r.sx[m] = b < blocks ? ((const RFXQ_GLOBAL float*)sx[m])[at] : 0.0f;
     };
-    load(0);
-    for (uint32_t b = 0; b < blocks; b++) {
-        __syncthreads();
+    load(kg);
+    for (uint32_t b = 0; b < blocks; b += KG) {
+        lds_barrier();
 #pragma unroll
-        for (uint32_t i = 0; i < NX; i++) xs[lds_piece((tid >> 3) + 32u * i, c)] = xv[i];
+        for (uint32_t i = 0; i < NX; i++) xs[kg][lds_piece((tid >> 3) + ROWS * i, c)] = r.x[i];
 #pragma unroll
-        for (uint32_t i = 0; i < NW; i++) ws[lds_piece((tid >> 3) + 32u * i, c)] = wv[i];
-        __syncthreads();
+        for (uint32_t i = 0; i < NW; i++) ws[kg][lds_piece((tid >> 3) + ROWS * i, c)] = r.w[i];
+        lds_barrier();
         float scale[2];
 #pragma unroll
-        for (uint32_t m = 0; m < 2u; m++) scale[m] = xsc[m] * wsc;
-        load(b + 1u);
+        for (uint32_t m = 0; m < 2u; m++) scale[m] = r.sx[m] * r.sw;
+        if (b + KG < blocks) load(b + KG + kg);
         Operand<EXACT> wf[4];
 #pragma unroll
         for (uint32_t f = 0; f < 4u; f++)
-            wf[f].take(ws[lds_piece(col0 + 16u * f + l, q)], ws[lds_piece(col0 + 16u * f + l, 4u + q)]);
+            wf[f].take(ws[kg][lds_piece(col0 + 16u * f + l, q)], ws[kg][lds_piece(col0 + 16u * f + l, 4u + q)]);
 #pragma unroll
         for (uint32_t m = 0; m < 2u; m++) {
             Operand<EXACT> xf;
-            xf.take(xs[lds_piece(row0 + 16u * m + l, q)], xs[lds_piece(row0 + 16u * m + l, 4u + q)]);
+            xf.take(xs[kg][lds_piece(row0 + 16u * m + l, q)], xs[kg][lds_piece(row0 + 16u * m + l, 4u + q)]);
             f4v_t d[4];
 #pragma unroll
             for (uint32_t f = 0; f < 4u; f++) d[f] = multiply(wf[f], xf);
 #pragma unroll
             for (uint32_t f = 0; f < 4u; f++) acc[m][f] += d[f] * scale[m];
         }
+    }
+    if constexpr (KG > 1) {
+        static_assert(KG == 2 && sizeof ws >= 4u * 8u * 64u * sizeof(f4v_t));
+        __syncthreads();
+        f4v_t* part = reinterpret_cast<f4v_t*>(ws) + (wave & 3u) * 8u * 64u + lane;
+        if (kg) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; i++) part[64u * i] = acc[i >> 2][i & 3u];
+        }
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) acc[i >> 2][i & 3u] += part[64u * i];
     }
 #pragma unroll
     for (uint32_t m = 0; m < 2u; m++) {
@@ -232,82 +273,65 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     }
 }
 
-#define RFXQ_F8_ANY(name, EXACT)                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, 3) void rfxq_f8_any_##name(F8Args a) { f8_any<EXACT, false>(a); }          \
-    extern "C" __global__ __launch_bounds__(256, 3) void rfxq_f8_any_##name##_grouped(F8Args a) { f8_any<EXACT, true>(a); }
-RFXQ_F8_ANY(half, false)
-RFXQ_F8_ANY(f32, true)
+#define RFXQ_F8_ANY(KG, WAVES, name, EXACT)                                                                                  \
+    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##KG##_##name(F8Args a) {                       \
+        f8_any<KG, EXACT, false>(a);                                                                                         \
+    }                                                                                                                        \
+    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##KG##_##name##_grouped(F8Args a) {             \
+        f8_any<KG, EXACT, true>(a);                                                                                          \
+    }
+RFXQ_F8_ANY(1, 3, half, false)
+RFXQ_F8_ANY(2, 2, half, false)
+RFXQ_F8_ANY(2, 2, f32, true)
 
-// ---------------------------------------------------------------- few rows
+// ---------------------------------------------------------------- few rows, any alignment
 
-// Up to 16 MT rows of a tile: what the weights weigh is all that counts, so they go
-// from memory straight into registers, each once, as the matrix instructions' 16-row
-// operands. A workgroup's WK waves take every WKth block of K each (neighbouring
-// blocks are on their way together) for all of its 16 MT x 16 NT results and add
-// their parts in LDS. Two blocks are multiplied while the next two are on their way.
-template <uint32_t MT, uint32_t NT, uint32_t WK, bool GROUPED>
+// 16 x 16 results a workgroup: both operands from memory straight into registers, a block
+// of K in every 8th for each of its 8 waves, which add their parts in LDS. Two blocks are
+// multiplied while the next two are on their way. A matrix instruction's operand has
+// 16 rows' pieces side by side, which memory pipes take at 16 bytes a cycle (whole lines: 63):
+// f8_few.hpp is for rows that start at 16 bytes.
+template <bool GROUPED>
 RFXQ_DEV void f8_few(const F8Args& a) {
-    constexpr uint32_t D = 2;
-    __shared__ f4v_t part[WK][MT * NT][64];
+    constexpr uint32_t D = 2, WK = 8;
+    __shared__ f4v_t part[WK][64];
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
-    const RowTile t = f8_tile<GROUPED>(a, 16u * MT, tm);
+    const RowTile t = f8_tile<GROUPED>(a, 16, tm);
     if (!t.any) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4, n0 = tn * 16u * NT;
+    const uint32_t lane = threadIdx.x & 63u, l = lane & 15u, q = lane >> 4, n0 = tn * 16u;
     const uint32_t full = a.k / kBlock, tail = a.k % kBlock, blocks = full + (tail ? 1u : 0u);
     const float* sw = a.ws + (uint64_t)t.group * a.ws_stride + (uint64_t)(n0 / kBlock) * blocks;
-    const uint8_t *w[NT], *x[MT];
-    const float* sx[MT];
-#pragma unroll
-    for (uint32_t f = 0; f < NT; f++)  // columns past the last read it again; their results are not stored
-        w[f] = a.w + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + 16u * f + l, a.n - 1u) * a.k + 16u * q;
+    // columns past the last read it again; their results are not stored
+    const uint8_t* w = a.w + (uint64_t)t.group * a.w_stride + (uint64_t)min(n0 + l, a.n - 1u) * a.k;
     struct Block {
-        u4_t w[NT][2], x[MT][2];
-        float sx[MT], sw;
+        u4_t w[2], x[2];
+        float sx, sw;
     } s[2][D];
     const auto load_w = [&](Block& r, uint32_t b) {
-#pragma unroll
-        for (uint32_t f = 0; f < NT; f++) {
-            r.w[f][0] = ld_codes(w[f] + (uint64_t)b * kBlock);
-            r.w[f][1] = ld_codes(w[f] + (uint64_t)b * kBlock + 64u);
-        }
+        r.w[0] = ld_codes(w + (uint64_t)b * kBlock + 16u * q);
+        r.w[1] = ld_codes(w + (uint64_t)b * kBlock + 64u + 16u * q);
         r.sw = ((const RFXQ_GLOBAL float*)sw)[b];
-    };
-    const auto load_x = [&](Block& r, uint32_t b) {
-#pragma unroll
-        for (uint32_t m = 0; m < MT; m++) {
-            r.x[m][0] = ld_codes(x[m] + (uint64_t)b * kBlock);
-            r.x[m][1] = ld_codes(x[m] + (uint64_t)b * kBlock + 64u);
-            r.sx[m] = ((const RFXQ_GLOBAL float*)sx[m])[b];
-        }
-    };
-    f4v_t acc[MT][NT] = {};
-    const auto products = [&](const Block& r) {
-        Operand<true> wf[NT];
-#pragma unroll
-        for (uint32_t f = 0; f < NT; f++) wf[f].take(r.w[f][0], r.w[f][1]);
-#pragma unroll
-        for (uint32_t m = 0; m < MT; m++) {
-            Operand<true> xf;
-            xf.take(r.x[m][0], r.x[m][1]);
-            const float scale = r.sx[m] * r.sw;
-            f4v_t d[NT];
-#pragma unroll
-            for (uint32_t f = 0; f < NT; f++) d[f] = multiply(wf[f], xf);
-#pragma unroll
-            for (uint32_t f = 0; f < NT; f++) acc[m][f] += d[f] * scale;
-        }
     };
 #pragma unroll
     for (uint32_t i = 0; i < D; i++)  // on their way while the rows are looked up
         if (wave + WK * i < full) load_w(s[0][i], wave + WK * i);
-#pragma unroll
-    for (uint32_t m = 0; m < MT; m++) {
-        const int64_t src = f8_src<GROUPED>(a, min(t.beg + 16u * m + l, t.end - 1u));
-        x[m] = a.x + (src < 0 ? 0 : (uint64_t)src * a.ldx) + 16u * q;
-        sx[m] = a.xs + (src < 0 ? 0 : (uint64_t)src * a.ldxs);
-    }
+    const int64_t src = f8_src<GROUPED>(a, min(t.beg + l, t.end - 1u));
+    const uint8_t* x = a.x + (src < 0 ? 0 : (uint64_t)src * a.ldx);
+    const float* sx = a.xs + (src < 0 ? 0 : (uint64_t)src * a.ldxs);
+    const auto load_x = [&](Block& r, uint32_t b) {
+        r.x[0] = ld_codes(x + (uint64_t)b * kBlock + 16u * q);
+        r.x[1] = ld_codes(x + (uint64_t)b * kBlock + 64u + 16u * q);
+        r.sx = ((const RFXQ_GLOBAL float*)sx)[b];
+    };
+    f4v_t acc = {0, 0, 0, 0};
+    const auto products = [&](const Block& r) {
+        Operand<true> wf, xf;
+        wf.take(r.w[0], r.w[1]);
+        xf.take(r.x[0], r.x[1]);
+        acc += multiply(wf, xf) * (r.sx * r.sw);
+    };
 #pragma unroll
     for (uint32_t i = 0; i < D; i++)
         if (wave + WK * i < full) load_x(s[0][i], wave + WK * i);
@@ -332,38 +356,24 @@ RFXQ_DEV void f8_few(const F8Args& a) {
         Block& r = s[0][0];
 #pragma unroll
         for (uint32_t h = 0; h < 2u; h++) {
-            const uint32_t k = 64u * h + 16u * q, have = tail > k ? tail - k : 0u;
-#pragma unroll
-            for (uint32_t f = 0; f < NT; f++) r.w[f][h] = ld_codes(w[f] + (uint64_t)full * kBlock + 64u * h, have);
-#pragma unroll
-            for (uint32_t m = 0; m < MT; m++) r.x[m][h] = ld_codes(x[m] + (uint64_t)full * kBlock + 64u * h, have);
+            r.w[h] = ld_codes(w, a.k, full * kBlock + 64u * h + 16u * q);
+            r.x[h] = ld_codes(x, a.k, full * kBlock + 64u * h + 16u * q);
         }
         r.sw = sw[full];
-#pragma unroll
-        for (uint32_t m = 0; m < MT; m++) r.sx[m] = sx[m][full];
+        r.sx = sx[full];
         products(r);
     }
-#pragma unroll
-    for (uint32_t m = 0; m < MT; m++)
-#pragma unroll
-        for (uint32_t f = 0; f < NT; f++) part[wave][m * NT + f][lane] = acc[m][f];
+    part[wave][lane] = acc;
     __syncthreads();
-    for (uint32_t i = wave; i < MT * NT; i += WK) {
-        f4v_t sum[1] = {part[0][i][lane]};
+    if (wave) return;
+    f4v_t sum[1] = {part[0][lane]};
 #pragma unroll
-        for (uint32_t v = 1; v < WK; v++) sum[0] += part[v][i][lane];
-        const uint32_t p = t.beg + 16u * (i / NT) + l;
-        if (p >= t.end) continue;
-        const int64_t src = f8_src<GROUPED>(a, p), dst = f8_dst<GROUPED>(a, p);
-        if (src >= 0 && dst >= 0) f8_out(a, dst, n0 + 16u * (i % NT) + 4u * q, sum);
-    }
+    for (uint32_t v = 1; v < WK; v++) sum[0] += part[v][lane];
+    const uint32_t p = t.beg + l;
+    if (p >= t.end || src < 0) return;
+    const int64_t dst = f8_dst<GROUPED>(a, p);
+    if (dst >= 0) f8_out(a, dst, n0 + 4u * q, sum);
 }
 
-#define RFXQ_F8_FEW(MT, NT, WK)                                                                                             \
-    extern "C" __global__ __launch_bounds__(64 * WK) void rfxq_f8_few_##MT##_##NT##_##WK(F8Args a) {                        \
-        f8_few<MT, NT, WK, false>(a);                                                                                       \
-    }                                                                                                                       \
-    extern "C" __global__ __launch_bounds__(64 * WK) void rfxq_f8_few_##MT##_##NT##_##WK##_grouped(F8Args a) {              \
-        f8_few<MT, NT, WK, true>(a);                                                                                        \
-    }
-RFXQ_F8_FEW(1, 1, 8)
+extern "C" __global__ __launch_bounds__(512) void rfxq_f8_few(F8Args a) { f8_few<false>(a); }
+extern "C" __global__ __launch_bounds__(512) void rfxq_f8_few_grouped(F8Args a) { f8_few<true>(a); }

@@ -123,20 +123,79 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
     return launch(fns[float_index(x->type)], (uint32_t)grid, 0, stream, &a, sizeof a, what);
 }
 
-// The kernel and tile of a product.
+// The kernels of a product: place in kF8ProductNames, its tile, and what it takes (us), measured
+// over rows of 1..8192, N and K of 768..14336: `start` once, and for every round of tiles over
+// the CUs `tile` and `block` for each 128 of K. Kernels whose workgroups share a CU take rounds as they
+// come, those that fill it (`whole`) whole ones. Rows that start at 16 bytes:
+//   stream 16 x 16  64 tiles: 4.3 (1 x 4096 x 1024), 256: 6.3 (1 x 4096 x 4096), 11.9 (1 x 14336 x 4096)
+//   stream 16 x 32  1 x 4096 x 14336: 11.5 (16 x 16: 15), 32 x 4096 x 4096: 6.4 (32 x 32: 7.5)
+//   stream 32 x 32  64 x 4096 x 4096: 7.6 (16 x 32: 8.7, 64 x 128: 13), 128 rows: 11.0 (64 x 128: 13)
+//   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 31.5 (16 x 32: 56, 64 x 128: 46)
+//   64 x 128        256 x 4096 x 4096: 13 (32 x 32: 19), 512 x 14336 x 4096: 39 (128 x 128: 65); f32 results 68
+//   128 x 128       1000 x 4096 x 4096: 23 (64 x 128: 26, 128 x 256: 28); f32 38 (64 x 128: 47)
+//   128 x 256       2048 x 4096 x 4096: 36 (128 x 128: 46, 256 x 256: 46)
+//   256 x 256       4096 x 4096 x 14336: 229 (128 x 256: 244)
+// and rows at any byte:
+//   few 16 x 16     1 x 4099 x 4099: 11.8 (64 x 128: 34), 32 x 4099 x 4099: 33 (38), 16 x 4099 x 14336: 79 (36)
+//   any             half results, 4000 x 4099 x 4099: 218 with 4 waves, 309 with 8; 333 x 4099 x 4099: 44, 39
 struct F8Variant {
-    uint32_t kernel;  // RFXQ_F8_*
+    uint32_t product, kernel;  // kernel: RFXQ_F8_*
     uint32_t bm, bn, threads;
+    float start, tile, block;
+    bool whole;
 };
-F8Variant f8_variant(uint64_t cus, uint32_t rows, uint32_t groups, uint32_t k, uint32_t n, bool aligned) {
-    const uint32_t used = std::min(rows, groups), mean = rows / used;
-    if (mean <= 16u) return {RFXQ_F8_FEW, 16, 16, 512};
-    return {RFXQ_F8_ANY, 64, 128, 256};
-}
+constexpr F8Variant kF8Any1 = {0, RFXQ_F8_ANY, 64, 128, 256, 0, 0, 0, false};
+constexpr F8Variant kF8Any2[2] = {{1, RFXQ_F8_ANY, 64, 128, 512, 0, 0, 0, false}, {2, RFXQ_F8_ANY, 64, 128, 512, 0, 0, 0, false}};
+constexpr F8Variant kF8Few = {3, RFXQ_F8_FEW, 16, 16, 512, 0, 0, 0, false};
+constexpr F8Variant kF8Stream[] = {{4, RFXQ_F8_STREAM, 16, 16, 512, 2.8f, 1.3f, 0.069f, false},
+                                   {5, RFXQ_F8_STREAM, 16, 32, 512, 2.8f, 0.9f, 0.085f, false},
+                                   {6, RFXQ_F8_STREAM, 32, 32, 512, 2.8f, 1.0f, 0.1175f, false},
+                                   {7, RFXQ_F8_STREAM, 16, 64, 256, 2.8f, 0.6f, 0.2f, false}};
+constexpr F8Variant kF8Half[] = {{8, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
+                                 {10, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.59f, true},
+                                 {12, RFXQ_F8_LARGE, 128, 256, 512, 0, 4.5f, 0.95f, true},
+                                 {13, RFXQ_F8_LARGE, 256, 256, 512, 0, 6.0f, 1.6f, true}};
+constexpr F8Variant kF8F32[] = {{9, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
+                                {11, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.95f, true}};
 
+// `copies`: rows start at 16 bytes and offsets fit 32 bits
+F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32, bool copies) {
+    const uint32_t used = std::min(rows, groups);
+    const double mean = (double)rows / used;
+    const auto tiles = [&](uint32_t bm, uint32_t bn) {  // grouped rows end inside a tile, half a tile on average
+        const double tm = grouped ? used * std::max(1.0, mean / bm + 0.5) : std::ceil((double)rows / bm);
+        return tm * std::ceil((double)n / bn);
+    };
+    if (!copies) {
+        if (tiles(16, 16) <= 2.0 * cus) return kF8Few;
+        return !f32 && tiles(64, 128) > cus ? kF8Any1 : kF8Any2[f32];
+    }
+    const F8Variant* best = nullptr;
+    double least = 0;
+    const auto look = [&](const F8Variant& v) {
+        double rounds = tiles(v.bm, v.bn) / cus;
+        rounds = v.whole ? std::ceil(rounds) : std::max(rounds, 1.0);
+        if (v.product == 7 && rounds < 2.0) return;  // four waves: measured where they are many
+        const double t = v.start + rounds * (v.tile + (double)f8_groups(k) * v.block);
+        if (!best || t < least) {
+            best = &v;
+            least = t;
+        }
+    };
+    for (const F8Variant& v : kF8Stream) look(v);
+    if (f32)
+        for (const F8Variant& v : kF8F32) look(v);
+    else
+        for (const F8Variant& v : kF8Half) look(v);
+    return *best;
+}
 // the kernel for `rows` (> 0) places of checked x and w
-F8Variant f8_variant(uint64_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped) {
-    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, w->in_features, w->out_features, false);
+F8Variant f8_variant(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped, bool f32) {
+    const uint32_t k = w->in_features, n = w->out_features;
+    const bool copies = aligned16(x->data) && x->stride % 16u == 0 && aligned16(w->data) && k % 16u == 0 &&
+                        codes_of(x, k, "").bytes < kMaxOffset && scales_of(x, k, "").bytes < kMaxOffset &&
+                        (uint64_t)k * n < kMaxOffset;
+    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, grouped, k, n, f32, copies);
 }
 
 int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows, const int32_t* x_index,
@@ -167,7 +226,7 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     a.n = n;
     a.groups = groups;
     a.y_type = float_index(y->type);
-    const F8Variant v = f8_variant((uint64_t)c->cus, x, w, rows, offsets != nullptr);
+    const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, a.y_type == 0);
     a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks as rfxq_grouped_gemm's
@@ -179,9 +238,7 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
         return fail(RFXQ_ERR_OTHER, "%s: %u rows x %u columns need %llu workgroups", what, rows, n, (unsigned long long)grid);
-    const uint32_t g = offsets ? 1u : 0u;
-    const hipFunction_t f = v.kernel == RFXQ_F8_FEW ? c->f8.few[g] : c->f8.any[a.y_type == 0 ? 1u : 0u][g];
-    return launch(f, (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_f8 product launch",
+    return launch(c->f8.product[v.product][offsets ? 1 : 0], (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_f8 product launch",
                   v.threads);
 }
 
@@ -332,14 +389,16 @@ int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const i
     return ok();
 }
 
-int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, rfxq_f8_policy* out) {
+int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
+                        rfxq_f8_policy* out) {
     if (!out) return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: NULL output");
     if (int rc = check_f8_weight(w, "gemm_f8_policy")) return rc;
     if (int rc = check_f8_rows(x, w->in_features, "gemm_f8_policy", "x")) return rc;
     if (rows == 0 || rows > 0x7FFFFFFFu || x->rows == 0)
         return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: rows=%u of %u", rows, x->rows);
+    if (!float_type(y_type)) return fail(RFXQ_ERR_GGUF, "gemm_f8_policy: y of type %u (F32, F16 or BF16)", y_type);
     const Ctx* c = loaded_ctx();
-    const F8Variant v = f8_variant(c ? (uint64_t)c->cus : 256u, x, w, rows, grouped != 0);
+    const F8Variant v = f8_variant(c ? (uint32_t)c->cus : 256u, x, w, rows, grouped != 0, y_type == RFXQ_TYPE_F32);
     *out = {v.kernel, v.bm, v.bn};
     return ok();
 }

@@ -155,12 +155,15 @@ struct HalfKernels {
     hipFunction_t lora_down[5][2] = {}, lora_up[5][3] = {};  // [16, 32 rows, 16 rows of any rank and columns]
 };
 
-// kernels of the third code object (f8_host.hpp); [F32, F16, BF16]
+// kernels of the third code object (f8_host.hpp); types: [F32, F16, BF16]
+constexpr uint32_t kF8Products = 14;
+const char* const kF8ProductNames[kF8Products] = {"any1_half", "any2_half",  "any2_f32",   "few",      "stream_1_1_2_8",
+                                                  "stream_1_2_1_8", "stream_2_2_1_8", "stream_1_4_1_4", "64_half", "64_f32",
+                                                  "128_half",  "128_f32",    "128_wide", "256_wide"};
 struct F8Kernels {
     hipFunction_t quantize[3] = {}, silu[3] = {};
     hipFunction_t norm[3][3] = {};  // [type][1 piece, 4 pieces, any length]
-    hipFunction_t any[2][2] = {};   // [half results, f32][one matrix, grouped]
-    hipFunction_t few[2] = {};
+    hipFunction_t product[kF8Products][2] = {};  // [f8_host.hpp's list][one matrix, grouped]
 };
 
 struct Ctx {
@@ -272,12 +275,9 @@ int load_f8(hipModule_t mod, F8Kernels* h) {
         for (int f = 0; f < 3; f++)
             if (int rc = get(&h->norm[t][f], std::string("rfxq_f8_norm_") + kType[t] + kNorm[f])) return rc;
     }
-    for (int g = 0; g < 2; g++) {
-        const std::string end = g ? "_grouped" : "";
-        if (int rc = get(&h->any[0][g], "rfxq_f8_any_half" + end)) return rc;
-        if (int rc = get(&h->any[1][g], "rfxq_f8_any_f32" + end)) return rc;
-        if (int rc = get(&h->few[g], "rfxq_f8_few_1_1_8" + end)) return rc;
-    }
+    for (uint32_t p = 0; p < kF8Products; p++)
+        for (int g = 0; g < 2; g++)
+            if (int rc = get(&h->product[p][g], std::string("rfxq_f8_") + kF8ProductNames[p] + (g ? "_grouped" : ""))) return rc;
     return RFXQ_OK;
 }
 

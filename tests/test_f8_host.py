@@ -193,11 +193,43 @@ def test_policy_refusals(L):
 
     p = rq.RfxqF8Policy()
     x, w = _ref(_f8, {}), _ref(_weight, {})
-    _expect(L, L.rfxq_gemm_f8_policy(x, w, 8, 0, None), 11, "NULL output")
-    _expect(L, L.rfxq_gemm_f8_policy(x, None, 8, 0, ctypes.byref(p)), 11, "weight is NULL")
-    _expect(L, L.rfxq_gemm_f8_policy(None, w, 8, 0, ctypes.byref(p)), 11, "x is NULL")
-    _expect(L, L.rfxq_gemm_f8_policy(x, w, 0, 0, ctypes.byref(p)), 11, "rows=0")
-    assert L.rfxq_gemm_f8_policy(x, w, 8, 1, ctypes.byref(p)) == 0
+    _expect(L, L.rfxq_gemm_f8_policy(x, w, 8, 0, F32, None), 11, "NULL output")
+    _expect(L, L.rfxq_gemm_f8_policy(x, None, 8, 0, F32, ctypes.byref(p)), 11, "weight is NULL")
+    _expect(L, L.rfxq_gemm_f8_policy(None, w, 8, 0, F32, ctypes.byref(p)), 11, "x is NULL")
+    _expect(L, L.rfxq_gemm_f8_policy(x, w, 0, 0, F32, ctypes.byref(p)), 11, "rows=0")
+    _expect(L, L.rfxq_gemm_f8_policy(x, w, 8, 0, Q4K, ctypes.byref(p)), 1, "of type 12")
+    assert L.rfxq_gemm_f8_policy(x, w, 8, 1, F16, ctypes.byref(p)) == 0
+
+
+ANY, FEW, STREAM, COPIED, LARGE = range(5)
+
+
+@pytest.mark.parametrize("rows,experts,k,n,ty,shift,kernel", [
+    (1, 0, 4096, 1024, F32, 0, (STREAM, 16, 16)),
+    (1, 0, 4096, 14336, BF16, 0, (STREAM, 16, 32)),
+    (32, 0, 4096, 4096, F32, 0, (STREAM, 16, 32)),
+    (64, 0, 14336, 4096, F16, 0, (STREAM, 32, 32)),
+    (256, 128, 768, 2048, F32, 0, (STREAM, 16, 64)),
+    (512, 0, 14336, 4096, BF16, 0, (COPIED, 64, 128)),
+    (512, 0, 14336, 4096, F32, 0, (COPIED, 64, 128)),
+    (1000, 0, 4096, 4096, F16, 0, (COPIED, 128, 128)),
+    (4096, 0, 4096, 14336, F32, 0, (COPIED, 128, 128)),
+    (2048, 0, 4096, 4096, BF16, 0, (LARGE, 128, 256)),
+    (4096, 0, 4096, 14336, BF16, 0, (LARGE, 256, 256)),
+    (4096, 0, 4096, 14336, BF16, 8, (ANY, 64, 128)),      # rows at 8 bytes
+    (4096, 0, 4104, 14336, F32, 0, (ANY, 64, 128)),       # K not a multiple of 16
+    (16, 0, 4096, 4096, F32, 1, (FEW, 16, 16)),
+    (1, 0, 65536, 65536, BF16, 0, (ANY, 64, 128)),        # a matrix of 4 GiB
+    (1, 0, 65520, 65552, BF16, 0, (STREAM, 16, 32)),      # a little less
+])
+def test_product_kernel(L, rows, experts, k, n, ty, shift, kernel):
+    import reflex_amd as rq
+
+    x = rq.RfxqF8Rows(4 * P + shift, 64 * P, rows, (k + 15) // 16 * 16, (k + 127) // 128)
+    w = _weight(k, n, experts, data=1 << 30, scales=1 << 40)
+    p = rq.RfxqF8Policy()
+    assert L.rfxq_gemm_f8_policy(ctypes.byref(x), ctypes.byref(w), rows, 1 if experts else 0, ty, ctypes.byref(p)) == 0
+    assert (p.kernel, p.tile_m, p.tile_n) == kernel
 
 
 def test_python_checks():
