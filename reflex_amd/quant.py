@@ -661,7 +661,9 @@ def _rows(t: torch.Tensor, columns: int, dev: int, what: str) -> RfxqRows:
         step = columns
     if step < columns or (one != 1 and columns > 1):
         raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
-    return RfxqRows(t.data_ptr(), ty, _count(rows, 0, f"{what}: rows"), step)
+    if rows > 0x7FFFFFFF:
+        raise InvalidInputError(11, f"{what}: rows={rows}")
+    return RfxqRows(t.data_ptr(), ty, rows, step)
 
 
 def _space(t: torch.Tensor | None, dev: int, what: str) -> tuple[int | None, int]:
@@ -768,13 +770,46 @@ def lora_add(x: torch.Tensor, a: Weight, b: Weight, groups: RowGroups, y: torch.
 _F8_TYPES = (torch.float8_e4m3fn, torch.uint8)
 
 
-@dataclass
+def _steps(t: torch.Tensor, what: str) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are contiguous."""
+    (rows, columns), (step, one) = t.shape, t.stride()
+    if rows <= 1:
+        step = columns
+    if step < columns or (one != 1 and columns > 1):
+        raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
+    return step
+
+
 class F8Rows:
     """Rows in e4m3 with a scale for each 128 of a row (``rfxq_f8_rows``): value (r, c) is
-    ``codes[r, c] * scales[r, c // 128]``."""
+    ``codes[r, c] * scales[r, c // 128]``. codes float8_e4m3fn (or its bytes as uint8) [rows, columns], scales f32
+    [rows, ceil(columns / 128)], rows contiguous and any distance apart; no copy: calls read and write the
+    tensors' memory."""
 
-    codes: torch.Tensor   # float8_e4m3fn (or its bytes as uint8) [rows, columns]
-    scales: torch.Tensor  # f32 [rows, ceil(columns / 128)]
+    __slots__ = ("_codes", "_scales", "_c", "_rows", "_columns", "_dev")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype not in _F8_TYPES or codes.dim() != 2 or codes.shape[1] < 1:
+            raise InvalidInputError(11, f"F8Rows: codes {codes.dtype} {list(codes.shape)} (float8_e4m3fn or uint8, "
+                                        "[rows, columns])")
+        rows, columns = codes.shape
+        want = [rows, (columns + 127) // 128]
+        if scales.dtype is not torch.float32 or list(scales.shape) != want or scales.device != codes.device:
+            raise InvalidInputError(11, f"F8Rows: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
+                                        f"(f32 {want} on {codes.device})")
+        self._codes, self._scales = codes, scales
+        self._rows, self._columns = _count(rows, 0, "F8Rows: rows"), _count(columns, 1, "F8Rows: columns")
+        self._dev = codes.get_device()
+        self._c = RfxqF8Rows(codes.data_ptr(), scales.data_ptr(), rows, _steps(codes, "F8Rows codes"),
+                             _steps(scales, "F8Rows scales"))
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @classmethod
     def empty(cls, rows: int, columns: int, device="cuda") -> "F8Rows":
@@ -796,40 +831,42 @@ class F8Weight:
                 or scales.device != codes.device):
             raise InvalidInputError(11, f"F8Weight: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
                                         f"(contiguous f32 {want} on {codes.device})")
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales, self._dev = codes, scales, codes.get_device()
         self.count = _count(codes.shape[0], 1, "F8Weight: count") if codes.dim() == 3 else 0
         self.out_features, self.in_features = (_count(v, 1, "F8Weight: shape") for v in codes.shape[-2:])
         self._c = RfxqF8Weight(self.in_features, self.out_features, self.count, codes.data_ptr(), scales.data_ptr(),
                                codes.numel(), 4 * scales.numel())
 
 
-def _steps(t: torch.Tensor, what: str) -> int:
-    """Elements between the rows of a 2-D tensor whose rows are contiguous."""
-    (rows, columns), (step, one) = t.shape, t.stride()
-    if rows <= 1:
-        step = columns
-    if step < columns or (one != 1 and columns > 1):
-        raise InvalidInputError(11, f"{what}: strides {t.stride()} (rows of contiguous values that do not overlap)")
-    return step
+# Launches of a few microseconds: the checks compare plain integers that F8Rows and F8Weight keep.
+
+def _f8_rows(r: F8Rows, rows: int, columns: int, dev: int, what: str) -> RfxqF8Rows:
+    if r._rows != rows or r._columns != columns or r._dev != dev:
+        raise InvalidInputError(11, f"{what}: [{r._rows}, {r._columns}] on {r._codes.device} ([{rows}, {columns}] on "
+                                    f"cuda:{dev})")
+    return r._c
 
 
-def _f8_rows(r: F8Rows, rows: int | None, columns: int, dev: int, what: str) -> RfxqF8Rows:
-    c, s = r.codes, r.scales
-    if (c.dtype not in _F8_TYPES or len(c.shape) != 2 or c.shape[1] != columns or c.get_device() != dev
-            or (rows is not None and c.shape[0] != rows)):
-        raise InvalidInputError(11, f"{what}: codes {c.dtype} {list(c.shape)} on {c.device} (float8_e4m3fn or uint8 "
-                                    f"[{'rows' if rows is None else rows}, {columns}] on cuda:{dev})")
-    if (s.dtype is not torch.float32 or len(s.shape) != 2 or s.shape[0] != c.shape[0]
-            or s.shape[1] != (columns + 127) // 128 or s.get_device() != dev):
-        raise InvalidInputError(11, f"{what}: scales {s.dtype} {list(s.shape)} on {s.device} "
-                                    f"(f32 [{c.shape[0]}, {(columns + 127) // 128}] on cuda:{dev})")
-    return RfxqF8Rows(c.data_ptr(), s.data_ptr(), _count(c.shape[0], 0, f"{what}: rows"), _steps(c, what), _steps(s, what))
+def _f8_call(fn, dev: int, *args) -> None:
+    if _raw_stream is not None and _get_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream())
+    if rc:
+        _check(rc)
+
+
+def _f8_dev(dev: int, t: torch.Tensor, what: str) -> int:
+    if dev < 0:
+        raise InvalidInputError(11, f"{what} on {t.device}")
+    return dev
 
 
 def _matrix(t: torch.Tensor, what: str) -> tuple[int, int]:
     if t.dim() != 2:
         raise InvalidInputError(11, f"{what}: {list(t.shape)} (two dimensions)")
-    return t.shape[0], _count(t.shape[1], 1, f"{what}: columns")
+    return t.shape
 
 
 def quantize_f8(x: torch.Tensor, out: F8Rows | None = None) -> F8Rows:
@@ -839,8 +876,7 @@ def quantize_f8(x: torch.Tensor, out: F8Rows | None = None) -> F8Rows:
     xr = _rows(x, k, dev, "quantize_f8 x")
     if out is None:
         out = F8Rows.empty(rows, k, x.device)
-    with _dev(x):
-        _check(lib().rfxq_quantize_f8(xr, k, _f8_rows(out, rows, k, dev, "quantize_f8 out"), _stream()))
+    _f8_call(lib().rfxq_quantize_f8, dev, xr, k, _f8_rows(out, rows, k, dev, "quantize_f8 out"))
     return out
 
 
@@ -852,8 +888,7 @@ def silu_and_mul_f8(gate: torch.Tensor, up: torch.Tensor, out: F8Rows | None = N
     gr, ur = _rows(gate, k, dev, "silu_and_mul_f8 gate"), _rows(up, k, dev, "silu_and_mul_f8 up")
     if out is None:
         out = F8Rows.empty(rows, k, gate.device)
-    with _dev(gate):
-        _check(lib().rfxq_silu_and_mul_f8(gr, ur, k, _f8_rows(out, rows, k, dev, "silu_and_mul_f8 out"), _stream()))
+    _f8_call(lib().rfxq_silu_and_mul_f8, dev, gr, ur, k, _f8_rows(out, rows, k, dev, "silu_and_mul_f8 out"))
     return out
 
 
@@ -878,14 +913,13 @@ def add_rmsnorm_f8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch
     yr = None if y is None else _rows(y, k, dev, "add_rmsnorm_f8 y")
     if out is None:
         out = F8Rows.empty(rows, k, x.device)
-    with _dev(x):
-        _check(lib().rfxq_add_rmsnorm_f8(xr, rr, weight.data_ptr(), k, eps, sr,
-                                         _f8_rows(out, rows, k, dev, "add_rmsnorm_f8 out"), yr, _stream()))
+    _f8_call(lib().rfxq_add_rmsnorm_f8, dev, xr, rr, weight.data_ptr(), k, eps, sr,
+             _f8_rows(out, rows, k, dev, "add_rmsnorm_f8 out"), yr)
     return out, sum_out, y
 
 
 def _f8_weight(w: F8Weight, dev: int, what: str) -> RfxqF8Weight:
-    if w.codes.get_device() != dev:
+    if w._dev != dev:
         raise InvalidInputError(11, f"{what}: weight on {w.codes.device}, rows on cuda:{dev}")
     return w._c
 
@@ -893,14 +927,13 @@ def _f8_weight(w: F8Weight, dev: int, what: str) -> RfxqF8Weight:
 def gemm_f8(x: F8Rows, w: F8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``gemm`` of e4m3 rows with an e4m3 matrix, both with their scales: [rows, out] in ``out``'s type (f32, f16 or
     bf16; without ``out`` a new tensor of ``dtype``)."""
-    dev = _on(x.codes, "gemm_f8: x")
+    dev = _f8_dev(x._dev, x._codes, "gemm_f8: x")
     c = _f8_weight(w, dev, "gemm_f8")
-    xr = _f8_rows(x, None, c.in_features, dev, "gemm_f8 x")
-    y = out if out is not None else torch.empty(xr.rows, c.out_features, dtype=dtype, device=x.codes.device)
-    yr = _rows(y, c.out_features, dev, "gemm_f8 out")
-    with _dev(x.codes):
-        _check(lib().rfxq_gemm_f8(xr, c, yr, _stream()))
-    return y
+    xr = _f8_rows(x, x._rows, w.in_features, dev, "gemm_f8 x")
+    if out is None:
+        out = torch.empty(x._rows, w.out_features, dtype=dtype, device=x._codes.device)
+    _f8_call(lib().rfxq_gemm_f8, dev, xr, c, _rows(out, w.out_features, dev, "gemm_f8 out"))
+    return out
 
 
 def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
@@ -908,18 +941,18 @@ def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_
                     dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``grouped_gemm`` of e4m3 rows with an e4m3 stack, both with their scales. Without ``out``, a new tensor of
     ``dtype`` with ``rows`` rows, zero where no place of a group writes."""
-    dev = _on(x.codes, "grouped_gemm_f8: x")
+    dev = _f8_dev(x._dev, x._codes, "grouped_gemm_f8: x")
     c = _f8_weight(w, dev, "grouped_gemm_f8")
     _count(rows, 0, "grouped_gemm_f8: rows")
     _count(x_div, 1, "grouped_gemm_f8: x_div")
-    xr = _f8_rows(x, None, c.in_features, dev, "grouped_gemm_f8 x")
-    y = out if out is not None else torch.zeros(rows, c.out_features, dtype=dtype, device=x.codes.device)
-    yr = _rows(y, c.out_features, dev, "grouped_gemm_f8 out")
-    with _dev(x.codes):
-        _check(lib().rfxq_grouped_gemm_f8(xr, c, _ints(offsets, (c.expert_count or 1) + 1, dev, "grouped_gemm_f8 offsets"),
-                                          rows, _ints(x_index, rows, dev, "grouped_gemm_f8 x_index"), x_div,
-                                          _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), yr, _stream()))
-    return y
+    xr = _f8_rows(x, x._rows, w.in_features, dev, "grouped_gemm_f8 x")
+    if out is None:
+        out = torch.zeros(rows, w.out_features, dtype=dtype, device=x._codes.device)
+    _f8_call(lib().rfxq_grouped_gemm_f8, dev, xr, c,
+             _ints(offsets, (w.count or 1) + 1, dev, "grouped_gemm_f8 offsets"), rows,
+             _ints(x_index, rows, dev, "grouped_gemm_f8 x_index"), x_div,
+             _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), _rows(out, w.out_features, dev, "grouped_gemm_f8 out"))
+    return out
 
 
 # ------------------------------------------------------------------ GGUF files

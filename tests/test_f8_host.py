@@ -262,5 +262,84 @@ def test_python_checks():
                  lambda: rq.grouped_gemm_f8(rq.F8Rows(codes, scales), w, torch.zeros(2, dtype=torch.int32), 4)):
         with pytest.raises(bad, match="on cpu"):
             call()
+    for args, text in (((torch.zeros(4, 300), scales), "codes"), ((codes[0], scales), "codes"), ((codes[:, :0], scales), "codes"),
+                       ((codes, scales[:3]), "scales"), ((codes, scales.double()), "scales"), ((codes, scales[:, :2]), "scales"),
+                       ((codes.t(), torch.zeros(300, 1)), "strides"), ((codes[:1].expand(4, 300), scales), "strides")):
+        with pytest.raises(bad, match=text):
+            rq.F8Rows(*args)
+    rows = rq.F8Rows(codes, scales)
+    with pytest.raises(AttributeError):
+        rows.codes = codes
     empty = rq.F8Rows.empty(3, 129, "cpu")
     assert empty.codes.shape == (3, 129) and empty.scales.shape == (3, 2)
+
+
+def test_matrix_results_are_not_read_too_early(tmp_path):
+    """The kernels' listing: on no path is a matrix instruction's result read before the wait states that the
+    compiler itself keeps in straight code (12 behind the 16x16x128 ones on e4m3, 8 behind the 16x16x32 ones). It
+    has left them out where the reading instruction is the first behind a branch."""
+    import os
+    import re
+    import subprocess
+
+    from reflex_amd import build
+
+    listing = tmp_path / "f8.s"
+    flags = [f for f in build.DEVICE_FLAGS if f != "--no-gpu-bundle-output"]
+    subprocess.run([os.path.join(build.ROCM, "bin", "hipcc"), *flags, "-S", os.path.join(build.CSRC, "f8.hip"), "-o",
+                    str(listing)], check=True, capture_output=True)
+    code, labels, kernel = [], {}, None
+    for line in listing.read_text().split("\n"):
+        m = re.match(r"^([\w.$]+):", line)
+        if m:
+            labels[m.group(1)] = len(code)
+            kernel = m.group(1) if m.group(1).startswith("rfxq") else kernel
+            continue
+        text = line.split(";")[0].strip()
+        if text and not text.startswith("."):
+            code.append((text, kernel))
+
+    def registers(operand):
+        found = set()
+        for m in re.finditer(r"\b([av])(?:\[(\d+):(\d+)\]|(\d+)\b)", operand):
+            lo, hi = (m.group(2), m.group(3)) if m.group(2) else (m.group(4), m.group(4))
+            found |= {(m.group(1), i) for i in range(int(lo), int(hi) + 1)}
+        return found
+
+    early, products = [], {"f8f6f4": 0, "32_f16": 0}
+    for i, (text, kernel) in enumerate(code):
+        if not text.startswith("v_mfma"):
+            continue
+        kind = "f8f6f4" if "16x16x128_f8f6f4" in text else "32_f16" if "16x16x32_f16" in text else None
+        assert kind, text
+        products[kind] += 1
+        need = 12 if kind == "f8f6f4" else 8
+        paths, seen = [(i + 1, 0, frozenset(registers(text.split(None, 1)[1].split(", ")[0])))], set()
+        while paths:
+            at, waited, live = state = paths.pop()
+            if waited >= need or not live or at >= len(code) or state in seen:
+                continue
+            seen.add(state)
+            name, _, rest = code[at][0].partition(" ")
+            operands = rest.split(", ")
+            if name == "s_endpgm":
+                continue
+            if name == "s_nop":
+                paths.append((at + 1, waited + int(rest, 0) + 1, live))
+                continue
+            if name.startswith(("s_branch", "s_cbranch")):
+                paths.append((labels[rest.strip()], waited + 1, live))
+                if name == "s_branch":
+                    continue
+            elif name.startswith(("v_", "ds_", "global_", "buffer_", "flat_", "scratch_")):
+                writes = set() if "store" in name or "ds_write" in name else registers(operands[0])
+                reads = set().union(*map(registers, operands[1:] if writes else operands))
+                if name.startswith("v_mfma"):  # the next product may add to the same result
+                    reads = registers(operands[1]) | registers(operands[2])
+                if reads & live:
+                    early.append((kernel, text, code[at][0], waited))
+                live = frozenset(live - writes)
+            paths.append((at + 1, waited + 1, live))
+    assert products["f8f6f4"] > 500 and products["32_f16"] > 200 and not early, (products, early[:5])
+    # copies that the compiler does not count: nothing that it does count may be spilled beside them
+    assert "Folded" not in listing.read_text()

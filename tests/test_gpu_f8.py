@@ -288,12 +288,12 @@ def _slack(x, xs, w, ws, y_type):
 
 
 def _check_product(x, xs, w, ws, y):
-    """y [rows, n] on the GPU against x @ w.T of both with their scales (on the CPU)."""
+    """y [rows, n] on the GPU against x @ w.T of both with their scales (where x is)."""
     xd, wd = _wide(x, xs), _wide_weight(w, ws)
     want, size = xd @ wd.t(), xd.abs() @ wd.abs().t()
     bound = size * (_blocks(x.shape[1]) + 32) * 2.0 ** -23 + want.abs() * torch.finfo(y.dtype).eps / 2 + TINY[y.dtype]
     bound = bound + _slack(x, xs, w, ws, y.dtype) * (1 + torch.finfo(y.dtype).eps)
-    got = y.cpu().double()
+    got = y.to(x.device).double()
     bad = ~((got - want).abs() <= bound)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:5].tolist(), float((got - want).abs().max()))
 
@@ -411,6 +411,72 @@ def test_gemm_matrix_past_4_gib(rq):
         assert not y[:, rest.to(DEV)].any()
 
 
+ANY, FEW, STREAM, COPIED, LARGE = range(5)
+
+
+def _kernel(rq, x, w, rows, grouped, y_type):
+    import ctypes
+
+    p = rq.RfxqF8Policy()
+    ty = {F32: 0, F16: 1, BF16: 30}[y_type]
+    assert rq.lib().rfxq_gemm_f8_policy(x._c, w._c, rows, grouped, ty, ctypes.byref(p)) == 0
+    return p.kernel, p.tile_m, p.tile_n
+
+
+# each kernel over short and long K: whole and odd numbers of blocks, a last block of one piece, more blocks than
+# a kernel's buffers, places or staged scales hold; tiles that end inside one
+EACH = [
+    (3, 9360, 48, F32, (STREAM, 16, 16)), (16, 16, 1000, BF16, (STREAM, 16, 32)), (7, 3856, 1040, F16, (STREAM, 16, 16)),
+    (5, 8448, 4992, BF16, (STREAM, 16, 32)), (30, 8208, 4100, F32, (STREAM, 16, 32)), (60, 8304, 4090, BF16, (STREAM, 32, 32)),
+    (130, 8304, 3600, F32, (STREAM, 32, 32)), (300, 4368, 2048, F16, (COPIED, 64, 128)), (512, 784, 3100, BF16, (COPIED, 64, 128)),
+    (400, 4368, 3100, F32, (COPIED, 64, 128)), (390, 784, 2050, F32, (COPIED, 64, 128)), (600, 4368, 4090, BF16, (COPIED, 128, 128)),
+    (1000, 2176, 4000, F16, (COPIED, 128, 128)), (700, 1040, 3600, F32, (COPIED, 128, 128)), (1000, 4368, 4000, F32, (COPIED, 128, 128)),
+    (1024, 1664, 7000, BF16, (LARGE, 128, 256)), (2040, 128, 4090, F16, (LARGE, 128, 256)), (2048, 1168, 4000, BF16, (LARGE, 128, 256)),
+    (4095, 656, 4090, BF16, (LARGE, 256, 256)), (4090, 128, 4096, F16, (LARGE, 256, 256)), (4096, 16, 4096, BF16, (LARGE, 256, 256)),
+    (4090, 1040, 4088, F16, (LARGE, 256, 256)),
+]
+
+
+@pytest.mark.parametrize("rows,k,n,y_type,kernel", EACH)
+def test_gemm_each_kernel(rq, rows, k, n, y_type, kernel):
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, k, n, rows + k))
+    xr, weight = rq.F8Rows(x, xs), rq.F8Weight(w, ws)
+    _say("each", rows, k, n, y_type, kernel)
+    assert _kernel(rq, xr, weight, rows, 0, y_type) == kernel
+    y = torch.full((rows + 2, n + 3), 7.0, dtype=y_type, device=DEV)
+    rq.gemm_f8(xr, weight, out=y[1:rows + 1, :n])
+    _check_product(x, xs, w, ws, y[1:rows + 1, :n])
+    y[1:rows + 1, :n] = 7.0
+    assert (y == 7.0).all()
+
+
+@pytest.mark.parametrize("extra", [0, 16, 112, 128, 129, 240])
+@pytest.mark.parametrize("blocks", range(1, 15))
+@pytest.mark.parametrize("rows,n,y_type", [(2, 40, F32), (40, 300, BF16), (200, 2100, F32), (300, 2050, BF16), (2048, 2050, BF16),
+                                           (1100, 2050, F32)])
+def test_gemm_every_number_of_blocks(rq, rows, n, y_type, blocks, extra):
+    """Few rows of ones and a last row that counts blocks: what each block gives is a power of two of its own."""
+    k = 128 * (blocks - 1) + (extra or 128)
+    g = _gen(blocks + extra)
+    x = torch.where(torch.rand(rows, k, generator=g) < 0.5, 1.0, -1.0).to(F8).to(DEV)
+    xs = torch.exp2(torch.arange(_blocks(k)).float()).repeat(rows, 1).to(DEV)
+    w = torch.where(torch.rand(n, k, generator=g) < 0.5, 1.0, 0.5).to(F8).to(DEV)
+    ws = torch.ones(_blocks(n), _blocks(k), device=DEV)
+    y = rq.gemm_f8(rq.F8Rows(x, xs), rq.F8Weight(w, ws), dtype=y_type)
+    want = _wide(x, xs) @ _wide_weight(w, ws).t()
+    # sums of halves below 2^24 are exact in f32
+    half = 0.0 if y_type == F32 else torch.finfo(y_type).eps / 2
+    assert ((y.double() - want).abs() <= want.abs() * half).all()
+
+
+def test_gemm_rows_that_repeat(rq):
+    """A matrix of one row repeated (stride 0 is refused; equal rows are not): equal rows give equal bits in every kernel."""
+    for rows, n in ((13, 64), (100, 1024), (400, 3100), (2048, 4000)):
+        x, xs, w, ws = (t.to(DEV) for t in _case(1, 1168, n, rows))
+        y = rq.gemm_f8(rq.F8Rows(x.repeat(rows, 1), xs.repeat(rows, 1)), rq.F8Weight(w, ws), dtype=BF16)
+        assert (y == y[:1]).all()
+
+
 # ------------------------------------------------------------------ grouped products
 
 def _run_grouped(rq, x, xs, w, ws, ids, top_k, side, y_type, spare=3):
@@ -456,6 +522,57 @@ def test_grouped(rq, tokens, count, top_k, k, n, side, y_type):
     ids = torch.from_numpy(r.integers(-1, count + 1, pairs).astype(np.int32))  # some in no group
     y, g = _run_grouped(rq, x, xs, w, ws, ids, top_k, side, y_type)
     _check_grouped(x, xs, w, ws, ids, top_k, side, y, g)
+
+
+GROUPED_EACH = [
+    (100, 3, 8320, 48, F32, (STREAM, 16, 16)), (260, 60, 8320, 1040, BF16, (STREAM, 16, 32)), (300, 7, 768, 520, BF16, (STREAM, 32, 32)),
+    (260, 120, 1040, 1040, F32, (STREAM, 16, 64)), (260, 120, 784, 2050, F16, (STREAM, 16, 64)), (3000, 6, 4240, 520, F32, (COPIED, 64, 128)),
+    (1800, 7, 400, 1100, BF16, (COPIED, 128, 128)), (3000, 6, 656, 1030, F32, (COPIED, 128, 128)),
+    (6000, 6, 400, 1030, F16, (LARGE, 128, 256)), (8000, 5, 1040, 1100, BF16, (LARGE, 256, 256)),
+]
+
+
+@pytest.mark.parametrize("side", ["gate", "down"])
+@pytest.mark.parametrize("pairs,count,k,n,y_type,kernel", GROUPED_EACH)
+def test_grouped_each_kernel(rq, pairs, count, k, n, y_type, kernel, side):
+    top_k = 2
+    x, xs, w, ws = _case(pairs // top_k if side == "gate" else pairs, k, n, pairs + k, count)
+    _say("grouped each", pairs, count, k, n, y_type, kernel, side)
+    r = np.random.default_rng(pairs + n)
+    ids = torch.from_numpy(r.integers(-1, count + 1, pairs).astype(np.int32))
+    x, xs, w, ws = (t.to(DEV) for t in (x, xs, w, ws))
+    assert _kernel(rq, rq.F8Rows(x, xs), rq.F8Weight(w, ws), pairs, 1, y_type) == kernel
+    y, g = _run_grouped(rq, x, xs, w, ws, ids, top_k, side, y_type)
+    offsets, order = g.offsets.cpu().long(), g.order.long()
+    for e in range(count):
+        at = torch.arange(int(offsets[e]), int(offsets[e + 1]), device=DEV)
+        if at.numel():
+            src, dst = (order[at] // top_k, at) if side == "gate" else (at, order[at])
+            _check_product(x[src], xs[src], w[e], ws[e], y[dst])
+    none = torch.arange(int(offsets[-1]), pairs, device=DEV)
+    left = torch.cat([none if side == "gate" else order[none], torch.arange(pairs, y.shape[0], device=DEV)])
+    assert (y[left] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows", [20, 300, 3000])
+def test_grouped_a_row_twice(rq, rows):
+    """A source that many places name; a destination that two places name holds one of their results."""
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, 256, 140, rows, 2))
+    offsets = torch.tensor([0, rows // 2, rows], dtype=torch.int32, device=DEV)
+    xr, weight = rq.F8Rows(x, xs), rq.F8Weight(w, ws)
+    same = torch.full((rows,), 3, dtype=torch.int32, device=DEV)
+    y = rq.grouped_gemm_f8(xr, weight, offsets, rows, x_index=same)
+    for e in range(2):
+        at = torch.arange(int(offsets[e]), int(offsets[e + 1]), device=DEV)
+        _check_product(x[3:4].repeat(at.numel(), 1), xs[3:4].repeat(at.numel(), 1), w[e], ws[e], y[at])
+    twice = torch.arange(rows, dtype=torch.int32, device=DEV) // 2
+    z = torch.full((rows, 140), 7.0, device=DEV)
+    rq.grouped_gemm_f8(xr, weight, offsets, rows, y_index=twice, out=z)
+    each = rq.grouped_gemm_f8(xr, weight, offsets, rows)
+    for d in range((rows + 1) // 2):
+        named = each[2 * d:2 * d + 2]
+        assert any(torch.equal(z[d], r) for r in named) or all(((z[d] == r) | (z[d] == named[0])).all() for r in named)
+    assert (z[(rows + 1) // 2:] == 7.0).all()
 
 
 @pytest.mark.parametrize("how", ["one", "first", "none"])
