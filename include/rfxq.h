@@ -558,7 +558,7 @@ int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const i
 /* Test hook: the kernel and tile that rfxq_gemm_f8 (grouped = 0) or
  * rfxq_grouped_gemm_f8 runs on the current device (256 compute units before
  * rfxq_init) for `rows` rows or places of x and w and results of a type; no memory is read. */
-#define RFXQ_F8_ANY 0    /* 64 x 128 tiles through registers, any alignment */
+#define RFXQ_F8_ANY 0    /* 32 x 64 or 64 x 128 tiles through registers, any alignment */
 #define RFXQ_F8_FEW 1    /* 16 x 16, straight from memory, any alignment */
 #define RFXQ_F8_STREAM 2 /* few rows: K among a workgroup's waves, each with copies of its own */
 #define RFXQ_F8_COPIED 3 /* 64 or 128 x 128 tiles, asynchronous copies */

@@ -161,15 +161,15 @@ RFXQ_DEV void f8_out(const F8Args& a, int64_t row, uint32_t n, const f4v_t (&v)[
 
 // ---------------------------------------------------------------- any alignment
 
-// 64 x 128 tiles (one block of weights' scales a step), operands through registers to
-// LDS, the next step's loads in flight during the products. KG groups of four waves of
-// 32 x 64 results take a block of K each of a step's KG, and add their parts in LDS. Rows
+// 32 MF x 32 NF tiles (in one block of columns: a scale of the weights' a step), operands through
+// registers to LDS, the next step's loads in flight during the products. KG groups of four waves
+// of 16 MF x 16 NF results take a block of K each of a step's KG, and add their parts in LDS. Rows
 // and columns past the tile read others, whose results are not stored; the last,
 // partial block has zeros behind the end of both operands, a block past it no
 // weights and the scale 0.
-template <uint32_t KG, bool EXACT, bool GROUPED>
+template <uint32_t MF, uint32_t NF, uint32_t KG, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_any(const F8Args& a) {
-    constexpr uint32_t BM = 64, BN = 128, ROWS = 32, NX = BM / ROWS, NW = BN / ROWS;
+    constexpr uint32_t BM = 32u * MF, BN = 32u * NF, ROWS = 32, NX = BM / ROWS, NW = BN / ROWS;
     __shared__ u4_t xs[KG][BM * 8u], ws[KG][BN * 8u];
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
@@ -177,29 +177,29 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     if (!t.any) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), kg = wave >> 2;
     const uint32_t tid = threadIdx.x & 255u, lane = tid & 63u, l = lane & 15u, q = lane >> 4;
-    const uint32_t n0 = tn * BN, c = tid & 7u, row0 = (wave >> 1 & 1u) * 32u, col0 = (wave & 1u) * 64u;
+    const uint32_t n0 = tn * BN, c = tid & 7u, row0 = (wave >> 1 & 1u) * 16u * MF, col0 = (wave & 1u) * 16u * NF;
     const uint32_t full = a.k / kBlock, tail = a.k % kBlock, blocks = full + (tail ? 1u : 0u);
     const uint8_t* w = a.w + (uint64_t)t.group * a.w_stride;
-    const float* sw = a.ws + (uint64_t)t.group * a.ws_stride + (uint64_t)tn * blocks;
+    const float* sw = a.ws + (uint64_t)t.group * a.ws_stride + (uint64_t)(n0 / kBlock) * blocks;
     const uint8_t *xp[NX], *wp[NW];
-    const float* sx[2];
+    const float* sx[MF];
 #pragma unroll
     for (uint32_t i = 0; i < NX; i++) {
         const int64_t s = f8_src<GROUPED>(a, min(t.beg + (tid >> 3) + ROWS * i, t.end - 1u));
         xp[i] = a.x + (s < 0 ? 0 : (uint64_t)s * a.ldx);
     }
 #pragma unroll
-    for (uint32_t m = 0; m < 2u; m++) {
+    for (uint32_t m = 0; m < MF; m++) {
         const int64_t s = f8_src<GROUPED>(a, min(t.beg + row0 + 16u * m + l, t.end - 1u));
         sx[m] = a.xs + (s < 0 ? 0 : (uint64_t)s * a.ldxs);
     }
 #pragma unroll
     for (uint32_t i = 0; i < NW; i++)
-        wp[i] = w + (uint64_t)min(n0 + col_of((tid >> 3) + ROWS * i), a.n - 1u) * a.k;
-    f4v_t acc[2][4] = {};
+        wp[i] = w + (uint64_t)min(n0 + col_of<NF>((tid >> 3) + ROWS * i), a.n - 1u) * a.k;
+    f4v_t acc[MF][NF] = {};
     struct Block {
         u4_t x[NX], w[NW];
-        float sx[2], sw;
+        float sx[MF], sw;
     } r;
     const auto load = [&](uint32_t b) {
         const uint32_t k = b * kBlock + 16u * c;
@@ -222,7 +222,7 @@ RFXQ_DEV void f8_any(const F8Args& a) {
         const uint32_t at = min(b, blocks - 1u);
         r.sw = b < blocks ? ((const RFXQ_GLOBAL float*)sw)[at] : 0.0f;
 #pragma unroll
-        for (uint32_t m = 0; m < 2u; m++) r.sx[m] = b < blocks ? ((const RFXQ_GLOBAL float*)sx[m])[at] : 0.0f;
+        for (uint32_t m = 0; m < MF; m++) r.sx[m] = b < blocks ? ((const RFXQ_GLOBAL float*)sx[m])[at] : 0.0f;
     };
     load(kg);
     for (uint32_t b = 0; b < blocks; b += KG) {
@@ -232,57 +232,59 @@ RFXQ_DEV void f8_any(const F8Args& a) {
 #pragma unroll
         for (uint32_t i = 0; i < NW; i++) ws[kg][lds_piece((tid >> 3) + ROWS * i, c)] = r.w[i];
         lds_barrier();
-        float scale[2];
+        float scale[MF];
 #pragma unroll
-        for (uint32_t m = 0; m < 2u; m++) scale[m] = r.sx[m] * r.sw;
+        for (uint32_t m = 0; m < MF; m++) scale[m] = r.sx[m] * r.sw;
         if (b + KG < blocks) load(b + KG + kg);
-        Operand<EXACT> wf[4];
+        Operand<EXACT> wf[NF];
 #pragma unroll
-        for (uint32_t f = 0; f < 4u; f++)
+        for (uint32_t f = 0; f < NF; f++)
             wf[f].take(ws[kg][lds_piece(col0 + 16u * f + l, q)], ws[kg][lds_piece(col0 + 16u * f + l, 4u + q)]);
 #pragma unroll
-        for (uint32_t m = 0; m < 2u; m++) {
+        for (uint32_t m = 0; m < MF; m++) {
             Operand<EXACT> xf;
             xf.take(xs[kg][lds_piece(row0 + 16u * m + l, q)], xs[kg][lds_piece(row0 + 16u * m + l, 4u + q)]);
-            f4v_t d[4];
+            f4v_t d[NF];
 #pragma unroll
-            for (uint32_t f = 0; f < 4u; f++) d[f] = multiply(wf[f], xf);
+            for (uint32_t f = 0; f < NF; f++) d[f] = multiply(wf[f], xf);
 #pragma unroll
-            for (uint32_t f = 0; f < 4u; f++) acc[m][f] += d[f] * scale[m];
+            for (uint32_t f = 0; f < NF; f++) acc[m][f] += d[f] * scale[m];
         }
     }
     if constexpr (KG > 1) {
-        static_assert(KG == 2 && sizeof ws >= 4u * 8u * 64u * sizeof(f4v_t));
+        static_assert(KG == 2 && sizeof ws >= 4u * MF * NF * 64u * sizeof(f4v_t));
         __syncthreads();
-        f4v_t* part = reinterpret_cast<f4v_t*>(ws) + (wave & 3u) * 8u * 64u + lane;
+        f4v_t* part = reinterpret_cast<f4v_t*>(ws) + (wave & 3u) * MF * NF * 64u + lane;
         if (kg) {
 #pragma unroll
-            for (uint32_t i = 0; i < 8u; i++) part[64u * i] = acc[i >> 2][i & 3u];
+            for (uint32_t i = 0; i < MF * NF; i++) part[64u * i] = acc[i / NF][i % NF];
         }
         __syncthreads();
         if (kg) return;
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) acc[i >> 2][i & 3u] += part[64u * i];
+        for (uint32_t i = 0; i < MF * NF; i++) acc[i / NF][i % NF] += part[64u * i];
     }
 #pragma unroll
-    for (uint32_t m = 0; m < 2u; m++) {
+    for (uint32_t m = 0; m < MF; m++) {
         const uint32_t p = t.beg + row0 + 16u * m + l;
         if (p >= t.end) continue;
         const int64_t src = f8_src<GROUPED>(a, p), dst = f8_dst<GROUPED>(a, p);
-        if (src >= 0 && dst >= 0) f8_out(a, dst, n0 + col0 + 16u * q, acc[m]);
+        if (src >= 0 && dst >= 0) f8_out(a, dst, n0 + col0 + 4u * NF * q, acc[m]);
     }
 }
 
-#define RFXQ_F8_ANY(KG, WAVES, name, EXACT)                                                                                  \
-    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##KG##_##name(F8Args a) {                       \
-        f8_any<KG, EXACT, false>(a);                                                                                         \
+#define RFXQ_F8_ANY(MF, NF, KG, WAVES, name, EXACT)                                                                          \
+    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##MF##_##KG##_##name(F8Args a) {                \
+        f8_any<MF, NF, KG, EXACT, false>(a);                                                                                 \
     }                                                                                                                        \
-    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##KG##_##name##_grouped(F8Args a) {             \
-        f8_any<KG, EXACT, true>(a);                                                                                          \
+    extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##MF##_##KG##_##name##_grouped(F8Args a) {      \
+        f8_any<MF, NF, KG, EXACT, true>(a);                                                                                  \
     }
-RFXQ_F8_ANY(1, 3, half, false)
-RFXQ_F8_ANY(2, 2, half, false)
-RFXQ_F8_ANY(2, 2, f32, true)
+RFXQ_F8_ANY(1, 2, 2, 4, half, false)
+RFXQ_F8_ANY(1, 2, 2, 4, f32, true)
+RFXQ_F8_ANY(2, 4, 1, 3, half, false)
+RFXQ_F8_ANY(2, 4, 2, 2, half, false)
+RFXQ_F8_ANY(2, 4, 2, 2, f32, true)
 
 // ---------------------------------------------------------------- few rows, any alignment
 

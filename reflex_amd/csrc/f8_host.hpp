@@ -136,57 +136,65 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   128 x 256       2048 x 4096 x 4096: 36 (128 x 128: 46, 256 x 256: 46)
 //   256 x 256       4096 x 4096 x 14336: 229 (128 x 256: 244)
 // and rows at any byte:
-//   few 16 x 16     1 x 4099 x 4099: 11.8 (64 x 128: 34), 32 x 4099 x 4099: 33 (38), 16 x 4099 x 14336: 79 (36)
-//   any             half results, 4000 x 4099 x 4099: 218 with 4 waves, 309 with 8; 333 x 4099 x 4099: 44, 39
+//   few 16 x 16     1 x 4099 x 4099: 11.8 (32 x 64: 22), 16 rows: 22 (22), 40 x 1235 x 1531: 7.0 (7.8)
+//   32 x 64         333 x 1235 x 1531: 10.5 (64 x 128: 15.9), 16 x 4099 x 14336: 23 (37; few: 79)
+//   64 x 128        1000 x 4099 x 4099, half results: 83 with 4 waves, 107 with 8 (32 x 64: 109); 333 rows: 43, 39 (49);
+//                   f32, 8 waves: 333 rows 41 (32 x 64: 53)
 struct F8Variant {
     uint32_t product, kernel;  // kernel: RFXQ_F8_*
     uint32_t bm, bn, threads;
     float start, tile, block;
     bool whole;
 };
-constexpr F8Variant kF8Any1 = {0, RFXQ_F8_ANY, 64, 128, 256, 0, 0, 0, false};
-constexpr F8Variant kF8Any2[2] = {{1, RFXQ_F8_ANY, 64, 128, 512, 0, 0, 0, false}, {2, RFXQ_F8_ANY, 64, 128, 512, 0, 0, 0, false}};
-constexpr F8Variant kF8Few = {3, RFXQ_F8_FEW, 16, 16, 512, 0, 0, 0, false};
-constexpr F8Variant kF8Stream[] = {{4, RFXQ_F8_STREAM, 16, 16, 512, 2.8f, 1.3f, 0.069f, false},
-                                   {5, RFXQ_F8_STREAM, 16, 32, 512, 2.8f, 0.9f, 0.085f, false},
-                                   {6, RFXQ_F8_STREAM, 32, 32, 512, 2.8f, 1.0f, 0.1175f, false},
-                                   {7, RFXQ_F8_STREAM, 16, 64, 256, 2.8f, 0.6f, 0.2f, false}};
-constexpr F8Variant kF8Half[] = {{8, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
-                                 {10, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.59f, true},
-                                 {12, RFXQ_F8_LARGE, 128, 256, 512, 0, 4.5f, 0.95f, true},
-                                 {13, RFXQ_F8_LARGE, 256, 256, 512, 0, 6.0f, 1.6f, true}};
-constexpr F8Variant kF8F32[] = {{9, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
-                                {11, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.95f, true}};
+constexpr F8Variant kF8Stream[] = {{6, RFXQ_F8_STREAM, 16, 16, 512, 2.8f, 1.3f, 0.069f, false},
+                                   {7, RFXQ_F8_STREAM, 16, 32, 512, 2.8f, 0.9f, 0.085f, false},
+                                   {8, RFXQ_F8_STREAM, 32, 32, 512, 2.8f, 1.0f, 0.1175f, false},
+                                   {9, RFXQ_F8_STREAM, 16, 64, 256, 2.8f, 0.6f, 0.2f, false}};
+constexpr F8Variant kF8Half[] = {{10, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
+                                 {12, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.59f, true},
+                                 {14, RFXQ_F8_LARGE, 128, 256, 512, 0, 4.5f, 0.95f, true},
+                                 {15, RFXQ_F8_LARGE, 256, 256, 512, 0, 6.0f, 1.6f, true}};
+constexpr F8Variant kF8F32[] = {{11, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
+                                {13, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.95f, true}};
+// one row's operand has one line where 16 have 16
+constexpr F8Variant kF8Few[2] = {{5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.27f, false}, {5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.55f, false}};
+constexpr F8Variant kF8AnyHalf[] = {{0, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.51f, false},
+                                    {2, RFXQ_F8_ANY, 64, 128, 256, 2.0f, 2.0f, 1.2f, false},
+                                    {3, RFXQ_F8_ANY, 64, 128, 512, 0, 5.0f, 1.0f, true}};
+constexpr F8Variant kF8AnyF32[] = {{1, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.51f, false},
+                                   {4, RFXQ_F8_ANY, 64, 128, 512, 0, 7.1f, 1.02f, true}};
 
 // `copies`: rows start at 16 bytes and offsets fit 32 bits
 F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32, bool copies) {
     const uint32_t used = std::min(rows, groups);
     const double mean = (double)rows / used;
-    const auto tiles = [&](uint32_t bm, uint32_t bn) {  // grouped rows end inside a tile, half a tile on average
-        const double tm = grouped ? used * std::max(1.0, mean / bm + 0.5) : std::ceil((double)rows / bm);
-        return tm * std::ceil((double)n / bn);
-    };
-    if (!copies) {
-        if (tiles(16, 16) <= 2.0 * cus) return kF8Few;
-        return !f32 && tiles(64, 128) > cus ? kF8Any1 : kF8Any2[f32];
-    }
     const F8Variant* best = nullptr;
     double least = 0;
     const auto look = [&](const F8Variant& v) {
-        double rounds = tiles(v.bm, v.bn) / cus;
+        // grouped rows end inside a tile, half a tile on average
+        const double tm = grouped ? used * std::max(1.0, mean / v.bm + 0.5) : std::ceil((double)rows / v.bm);
+        double rounds = tm * std::ceil((double)n / v.bn) / cus;
         rounds = v.whole ? std::ceil(rounds) : std::max(rounds, 1.0);
-        if (v.product == 7 && rounds < 2.0) return;  // four waves: measured where they are many
+        if (v.bm == 16u && v.bn == 64u && rounds < 2.0) return;  // four waves: measured where they are many
         const double t = v.start + rounds * (v.tile + (double)f8_groups(k) * v.block);
         if (!best || t < least) {
             best = &v;
             least = t;
         }
     };
-    for (const F8Variant& v : kF8Stream) look(v);
-    if (f32)
-        for (const F8Variant& v : kF8F32) look(v);
-    else
-        for (const F8Variant& v : kF8Half) look(v);
+    if (copies) {
+        for (const F8Variant& v : kF8Stream) look(v);
+        if (f32)
+            for (const F8Variant& v : kF8F32) look(v);
+        else
+            for (const F8Variant& v : kF8Half) look(v);
+    } else {
+        look(kF8Few[mean > 1.0 ? 1 : 0]);
+        if (f32)
+            for (const F8Variant& v : kF8AnyF32) look(v);
+        else
+            for (const F8Variant& v : kF8AnyHalf) look(v);
+    }
     return *best;
 }
 // the kernel for `rows` (> 0) places of checked x and w

@@ -88,7 +88,7 @@ struct F8Tile {
         }
 #pragma unroll
         for (uint32_t j = 0; j < NW / DEPTH; j++) {
-            const uint32_t n = n0 + col_of((wave * (NW / DEPTH) + j) * 8u + (lane >> 3));
+            const uint32_t n = n0 + col_of<>((wave * (NW / DEPTH) + j) * 8u + (lane >> 3));
             wo[j] = n < a.n ? n * k + 16u * piece : PAST;
         }
         return true;

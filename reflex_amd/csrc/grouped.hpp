@@ -241,7 +241,7 @@ RFXQ_DEV void grouped_any(const GroupedArgs& a) {
     }
 #pragma unroll
     for (uint32_t i = 0; i < NW; i++)
-        wp[i] = w + (uint64_t)min(n0 + col_of((tid >> 3) + 32u * i), a.n - 1u) * a.k + 8u * c;
+        wp[i] = w + (uint64_t)min(n0 + col_of<>((tid >> 3) + 32u * i), a.n - 1u) * a.k + 8u * c;
     f4v_t acc[2][4] = {};
     const uint32_t full = a.k / 64u, tail = a.k % 64u, steps = full + (tail ? 1u : 0u);
     const uint32_t row0 = (wave >> 1) * 32u, col0 = (wave & 1u) * 64u;
@@ -367,7 +367,7 @@ struct GroupedTile {
         }
 #pragma unroll
         for (uint32_t i = 0; i < NW; i++) {
-            const uint32_t n = n0 + col_of((wave * NW + i) * 8u + (lane >> 3));
+            const uint32_t n = n0 + col_of<>((wave * NW + i) * 8u + (lane >> 3));
             wo[i] = n < a.n ? n * a.k * 2u + 16u * piece : PAST;
         }
         steps = (a.k + 63u) / 64u;

@@ -191,5 +191,8 @@ RFXQ_DEV uint32_t lds_piece(uint32_t r, uint32_t c) { return r * 8u + (c ^ (r & 
 
 // The column of a tile that LDS row j of the weights holds. A lane's results
 // are rows 4q..4q+3 of each 16-row operand (q = lane / 16): with this order the
-// four operands of a wave's 64 columns give it 16 neighbouring ones.
-RFXQ_DEV uint32_t col_of(uint32_t j) { return (j & ~63u) + ((j >> 2) & 3u) * 16u + ((j >> 4) & 3u) * 4u + (j & 3u); }
+// F operands of a wave's 16 F columns give it 4 F neighbouring ones.
+template <uint32_t F = 4>
+RFXQ_DEV uint32_t col_of(uint32_t j) {
+    return (j & ~(16u * F - 1u)) + ((j >> 2) & 3u) * 4u * F + ((j >> 4) & (F - 1u)) * 4u + (j & 3u);
+}

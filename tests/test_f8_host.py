@@ -218,8 +218,13 @@ ANY, FEW, STREAM, COPIED, LARGE = range(5)
     (4096, 0, 4096, 14336, BF16, 0, (LARGE, 256, 256)),
     (4096, 0, 4096, 14336, BF16, 8, (ANY, 64, 128)),      # rows at 8 bytes
     (4096, 0, 4104, 14336, F32, 0, (ANY, 64, 128)),       # K not a multiple of 16
-    (16, 0, 4096, 4096, F32, 1, (FEW, 16, 16)),
-    (1, 0, 65536, 65536, BF16, 0, (ANY, 64, 128)),        # a matrix of 4 GiB
+    (1, 0, 4096, 4096, F32, 1, (FEW, 16, 16)),
+    (333, 0, 1235, 1531, F32, 0, (ANY, 32, 64)),
+    (333, 0, 4099, 4099, F32, 0, (ANY, 64, 128)),
+    (16, 0, 4099, 14336, BF16, 0, (ANY, 32, 64)),
+    (1200, 128, 200, 512, F16, 0, (ANY, 64, 128)),
+    (128, 128, 1235, 1000, F32, 0, (ANY, 32, 64)),
+    (4, 0, 65536, 65536, BF16, 0, (ANY, 64, 128)),        # a matrix of 4 GiB
     (1, 0, 65520, 65552, BF16, 0, (STREAM, 16, 32)),      # a little less
 ])
 def test_product_kernel(L, rows, experts, k, n, ty, shift, kernel):
