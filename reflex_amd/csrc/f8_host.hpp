@@ -237,11 +237,23 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, a.y_type == 0);
     a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
     a.tiles_n = (n + v.bn - 1u) / v.bn;
-    // XCD blocks as rfxq_grouped_gemm's
+    // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of workgroups that fill
+    // a CU, rounds of them. Of those, dense ones of four rows of tiles (4096 x 4096 x 14336: 214 us, of two 221,
+    // of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64 us, four
+    // 83); a group's rows are few tiles, most often at most three (4096 tokens over 8 of 128 experts, 2048 x 768:
+    // 91 us, of four 104, of one 100). The others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531:
+    // 10.8, 10.7, 11.8).
     const uint32_t across = (a.tiles_n + 3u) / 4u;
-    const uint64_t each = (uint64_t)a.tiles_m * across / 64u;
-    a.sm = each >= 4u ? 4u : each >= 2u ? 2u : 1u;
     a.sn = (a.tiles_n + across - 1u) / across;
+    uint64_t least = ~0ull;
+    for (uint32_t s = std::min(a.tiles_m, !v.whole ? 2u : offsets ? 3u : 4u); s; s--) {
+        const uint64_t each = ((uint64_t)((a.tiles_m + s - 1u) / s) * across + 7u) / 8u * s * a.sn;
+        const uint64_t take = v.whole ? (each * 8u + (uint32_t)c->cus - 1u) / (uint32_t)c->cus : each;
+        if (take < least) {
+            least = take;
+            a.sm = s;
+        }
+    }
     const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
     const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads

@@ -96,7 +96,7 @@ struct F8Tile {
 
     // Scales of the tile's rows for blocks [b0, b0 + COUNT), [block][row], with those of
     // its columns where they are one block's (BN = 128). Blocks past the last
-    // (which are zeros) repeat it.
+    // have zeros: an infinite scale would make NaN of their products.
     template <uint32_t COUNT>
     __device__ __forceinline__ void stage_scales(const F8Args& a, float* ss, uint32_t b0) {
         constexpr uint32_t PER = COUNT / 4u;
@@ -111,6 +111,7 @@ struct F8Tile {
                 const uint32_t at_block = min(b0 + b + e, blocks - 1u);
                 v[e] = ((const RFXQ_GLOBAL float*)p)[at_block];
                 if constexpr (BN == kBlock) v[e] *= ((const RFXQ_GLOBAL float*)sw)[at_block];
+                if (b0 + b + e >= blocks) v[e] = 0.0f;
             }
 #pragma unroll
             for (uint32_t e = 0; e < 4u; e++) ss[(b + e) * BM + r] = v[e];

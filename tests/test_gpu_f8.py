@@ -10,6 +10,8 @@ row, each within 2^-23 of the sum of the products' sizes (scales included); the 
 value. Where the result is f16 or bf16 the matrix instructions may add eight neighbouring products cut to multiples of
 2^-13 2^e, e the largest sum of two codes' exponents there (at least -6 each): eight products, 2^-10 2^e, and e is at
 most the sum of the largest exponents of either side."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -387,6 +389,21 @@ def test_gemm_not_finite(rq, rows, k, n, y_type):
         w[n // 3] = 0.0
         y[:, n // 3] = 0.0
         _check_product(x[row], xs[row], w[:full], ws[:-1], y[row][:, :full])
+
+
+@pytest.mark.parametrize("y_type", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(1, 40), (40, 300), (300, 2050), (900, 2100), (2040, 4090), (4090, 4090)])
+@pytest.mark.parametrize("k", [128, 300, 336, 640, 645])
+def test_gemm_infinite_scale(rq, rows, n, k, y_type):
+    """Positive values and a scale that is infinite in the last block of K: infinity there, not NaN of blocks behind it."""
+    x, w = (torch.full((r, k), 1.0).to(F8).to(DEV) for r in (rows, n))
+    xs, ws = torch.ones(rows, _blocks(k), device=DEV), torch.ones(_blocks(n), _blocks(k), device=DEV)
+    xs[rows // 2, -1] = math.inf
+    _say("infinite scale", rows, n, k, y_type)
+    y = rq.gemm_f8(rq.F8Rows(x, xs), rq.F8Weight(w, ws), dtype=y_type)
+    assert (y[rows // 2] == math.inf).all()
+    y[rows // 2] = float(k)  # exact in f32; bf16 rounds it
+    assert (y == torch.tensor(float(k)).to(y_type)).all()
 
 
 def test_gemm_matrix_past_4_gib(rq):
