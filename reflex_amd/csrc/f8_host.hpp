@@ -71,9 +71,9 @@ int check_f8_weight(const rfxq_f8_weight* w, const char* what) {
     const unsigned __int128 need = (unsigned __int128)count * k * n;
     const unsigned __int128 scales = (unsigned __int128)count * f8_groups(k) * f8_groups(n) * 4u;
     if (w->len < need || w->scales_len < scales)
-        return fail(RFXQ_ERR_OTHER, "%s: weight of %llu bytes and %llu of scales, shape [%u, %u, %u] needs %llu and %llu", what,
-                    (unsigned long long)w->len, (unsigned long long)w->scales_len, k, n, count, (unsigned long long)need,
-                    (unsigned long long)scales);
+        return fail(RFXQ_ERR_OTHER, "%s: weight of %llu bytes and %llu of scales, shape [%u, %u, %u] needs %llu and %llu",
+                    what, (unsigned long long)w->len, (unsigned long long)w->scales_len, k, n, count,
+                    (unsigned long long)need, (unsigned long long)scales);
     if (!w->data || !w->scales) return fail(RFXQ_ERR_INVALID_INPUT, "%s: weight data or scales is NULL", what);
     if (reinterpret_cast<uintptr_t>(w->scales) % 4u)
         return fail(RFXQ_ERR_OTHER, "%s: weight scales at %p are not 4-byte aligned", what, (const void*)w->scales);
@@ -138,8 +138,8 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 // and rows at any byte:
 //   few 16 x 16     1 x 4099 x 4099: 11.8 (32 x 64: 22), 16 rows: 22 (22), 40 x 1235 x 1531: 7.0 (7.8)
 //   32 x 64         333 x 1235 x 1531: 10.5 (64 x 128: 15.9), 16 x 4099 x 14336: 23 (37; few: 79)
-//   64 x 128        1000 x 4099 x 4099, half results: 83 with 4 waves, 107 with 8 (32 x 64: 109); 333 rows: 43, 39 (49);
-//                   f32, 8 waves: 333 rows 41 (32 x 64: 53)
+//   64 x 128        1000 x 4099 x 4099, half results: 83 with 4 waves, 107 with 8 (32 x 64: 109); 333 rows: 43,
+//                   39 (49); f32, 8 waves: 333 rows 41 (32 x 64: 53)
 struct F8Variant {
     uint32_t product, kernel;  // kernel: RFXQ_F8_*
     uint32_t bm, bn, threads;
@@ -157,7 +157,8 @@ constexpr F8Variant kF8Half[] = {{10, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.3
 constexpr F8Variant kF8F32[] = {{11, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
                                 {13, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.95f, true}};
 // one row's operand has one line where 16 have 16
-constexpr F8Variant kF8Few[2] = {{5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.27f, false}, {5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.55f, false}};
+constexpr F8Variant kF8Few[2] = {{5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.27f, false},
+                                 {5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.55f, false}};
 constexpr F8Variant kF8AnyHalf[] = {{0, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.51f, false},
                                     {2, RFXQ_F8_ANY, 64, 128, 256, 2.0f, 2.0f, 1.2f, false},
                                     {3, RFXQ_F8_ANY, 64, 128, 512, 0, 5.0f, 1.0f, true}};
@@ -165,7 +166,8 @@ constexpr F8Variant kF8AnyF32[] = {{1, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.5
                                    {4, RFXQ_F8_ANY, 64, 128, 512, 0, 7.1f, 1.02f, true}};
 
 // `copies`: rows start at 16 bytes and offsets fit 32 bits
-F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32, bool copies) {
+F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32,
+                     bool copies) {
     const uint32_t used = std::min(rows, groups);
     const double mean = (double)rows / used;
     const F8Variant* best = nullptr;
@@ -206,11 +208,17 @@ F8Variant f8_variant(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* 
     return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, grouped, k, n, f32, copies);
 }
 
-int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows, const int32_t* x_index,
-               uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, hipStream_t stream, const char* what) {
+int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
+               const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, hipStream_t stream,
+               const char* what) {
+    const uint32_t k = w->in_features, n = w->out_features, groups = std::max(w->expert_count, 1u);
+    const Span sy = span_of(y, n, "y");
+    const Span inputs[] = {codes_of(x, k, "x"), scales_of(x, k, "x's scales"), {w->data, (uint64_t)groups * k * n, "weight"},
+                           {w->scales, 4ull * groups * f8_groups(k) * f8_groups(n), "weight's scales"}};
+    for (const Span& in : inputs)
+        if (int rc = check_apart(in, sy, what)) return rc;
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
-    const uint32_t k = w->in_features, n = w->out_features, groups = std::max(w->expert_count, 1u);
     F8Args a;
     std::memset(&a, 0, sizeof a);
     a.x = static_cast<const uint8_t*>(x->data);
@@ -237,12 +245,12 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, a.y_type == 0);
     a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
     a.tiles_n = (n + v.bn - 1u) / v.bn;
-    // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of workgroups that fill
-    // a CU, rounds of them. Of those, dense ones of four rows of tiles (4096 x 4096 x 14336: 214 us, of two 221,
-    // of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64 us, four
-    // 83); a group's rows are few tiles, most often at most three (4096 tokens over 8 of 128 experts, 2048 x 768:
-    // 91 us, of four 104, of one 100). The others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531:
-    // 10.8, 10.7, 11.8).
+    // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
+    // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles
+    // (4096 x 4096 x 14336: 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x
+    // 14336: three 64 us, four 83); a group's rows are few tiles, most often at most three (4096 tokens
+    // over 8 of 128 experts, 2048 x 768: 91 us, of four 104, of one 100). The others two (64 x 4096 x
+    // 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531: 10.8, 10.7, 11.8).
     const uint32_t across = (a.tiles_n + 3u) / 4u;
     a.sn = (a.tiles_n + across - 1u) / across;
     uint64_t least = ~0ull;
@@ -258,8 +266,8 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
     if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
         return fail(RFXQ_ERR_OTHER, "%s: %u rows x %u columns need %llu workgroups", what, rows, n, (unsigned long long)grid);
-    return launch(c->f8.product[v.product][offsets ? 1 : 0], (uint32_t)grid, 0, stream, &a, sizeof a, "rfxq_f8 product launch",
-                  v.threads);
+    return launch(c->f8.product[v.product][offsets ? 1 : 0], (uint32_t)grid, 0, stream, &a, sizeof a,
+                  "rfxq_f8 product launch", v.threads);
 }
 
 }  // namespace
@@ -294,7 +302,8 @@ int rfxq_silu_and_mul_f8(const rfxq_rows* gate, const rfxq_rows* up, uint32_t k,
     if (gate->rows == 0) return ok();
     const Span sg = span_of(gate, k, "gate"), su = span_of(up, k, "up"), sc = codes_of(out, k, "out");
     const Span ss = scales_of(out, k, "out's scales");
-    for (auto& [a, b] : {std::pair{sg, sc}, std::pair{su, sc}, std::pair{sg, ss}, std::pair{su, ss}, std::pair{sc, ss}})
+    for (auto& [a, b] :
+         {std::pair{sg, sc}, std::pair{su, sc}, std::pair{sg, ss}, std::pair{su, ss}, std::pair{sc, ss}})
         if (int rc = check_apart(a, b, "silu_and_mul_f8")) return rc;
     Ctx* c;
     if (int rc = current_ctx(&c)) return rc;
@@ -327,9 +336,10 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
     if (!weight || reinterpret_cast<uintptr_t>(weight) % 4u)
         return fail(RFXQ_ERR_INVALID_INPUT, "add_rmsnorm_f8: weight is NULL or not 4-byte aligned");
     const Span none = {nullptr, 0, ""};
-    const Span in[] = {span_of(x, k, "x"), residual ? span_of(residual, k, "residual") : none, {weight, 4ull * k, "weight"}};
-    const Span results[] = {codes_of(out, k, "out"), scales_of(out, k, "out's scales"), sum ? span_of(sum, k, "sum") : none,
-                            y ? span_of(y, k, "y") : none};
+    const Span in[] = {span_of(x, k, "x"), residual ? span_of(residual, k, "residual") : none,
+                       {weight, 4ull * k, "weight"}};
+    const Span results[] = {codes_of(out, k, "out"), scales_of(out, k, "out's scales"),
+                            sum ? span_of(sum, k, "sum") : none, y ? span_of(y, k, "y") : none};
     for (size_t i = 0; i < 4; i++) {
         for (size_t j = 0; j < 3; j++) {
             const rfxq_rows* r = j == 0 ? x : j == 1 ? residual : nullptr;
@@ -383,9 +393,6 @@ int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows
     if (int rc = check_rows(y, n, "gemm_f8", "y")) return rc;
     if (x->rows != y->rows) return fail(RFXQ_ERR_OTHER, "gemm_f8: %u rows of x, %u of y", x->rows, y->rows);
     if (x->rows == 0) return ok();
-    const Span sy = span_of(y, n, "y");
-    if (int rc = check_apart(codes_of(x, k, "x"), sy, "gemm_f8")) return rc;
-    if (int rc = check_apart(scales_of(x, k, "x's scales"), sy, "gemm_f8")) return rc;
     if (int rc = f8_product(x, w, nullptr, x->rows, nullptr, 1, nullptr, y, stream, "gemm_f8")) return rc;
     return ok();
 }
@@ -402,9 +409,6 @@ int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const i
     if (!x_index && x_div != 1) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: x_div=%u without x_index", x_div);
     if (rows == 0 || x->rows == 0 || y->rows == 0) return ok();
     if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: offsets is NULL");
-    const Span sy = span_of(y, n, "y");
-    if (int rc = check_apart(codes_of(x, k, "x"), sy, "grouped_gemm_f8")) return rc;
-    if (int rc = check_apart(scales_of(x, k, "x's scales"), sy, "grouped_gemm_f8")) return rc;
     if (int rc = f8_product(x, w, offsets, rows, x_index, x_div, y_index, y, stream, "grouped_gemm_f8")) return rc;
     return ok();
 }

@@ -1,5 +1,12 @@
 // Tiles of rfxq_gemm_f8 and rfxq_grouped_gemm_f8 filled by asynchronous copies
 // (f8_gemm.hpp has the formula, and the kernels of the rest).
+//
+// What bounds them, a CU: the instruction of 16 x 16 x 128 takes 33 cycles, 35 with its four
+// multiply-adds beside it and two waves a SIMD (4.1 PFLOP/s in all at 2.1 GHz); LDS
+// gives 239 bytes a cycle to 8 waves (124 to 4), copies bring 63. A 256 x 256 tile takes 2240
+// cycles of instructions for a block of K, 800 of LDS (192 KB) and 1040 of copies (64 KB): large tiles are bound by
+// the instructions and by what holds their issue up, small ones by copies and
+// by the way from a copy's issue to its landing.
 #pragma once
 #include "f8_gemm.hpp"
 
@@ -131,7 +138,12 @@ struct F8Tile {
 
 // 8 waves: four of 16 MF x 64 results take the even blocks of K, four the odd ones,
 // and they add their parts in LDS. Buffers of two blocks, copies STAGES - 1 steps ahead, a
-// barrier a step.
+// barrier a step. 512 x 14336 x 4096, half results: 40 us in 64 x 128 tiles, one a CU (1.5 PFLOP/s, a
+// third of the instructions' rate; 33 bytes of copies a cycle and CU); 1000 x 4096 x 4096 in 128 x 128: 23 us. f32
+// results 64 and 38 us: their codes are widened, their instructions run at half the rate. Tried: operands
+// read from LDS a step ahead (no gain), 64 x 64 tiles of four blocks a step (256 x 4096 x 4096: 12.7 us, 64 x 128
+// 13.4; f32 16.7 and 22.4, but two rounds of them 28.6), weights straight to registers (4096 x 4096 x 14336:
+// 354 us).
 template <uint32_t MF, uint32_t STAGES, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_mid(const F8Args& a) {
     constexpr uint32_t BM = 32u * MF, BN = 128, D = 2, CHUNK = 32;  // CHUNK: blocks whose scales are in LDS
@@ -245,23 +257,27 @@ RFXQ_DEV void f8_mid(const F8Args& a) {
     if (half) add(Count<MF / 2u>{});
 }
 
-#define RFXQ_F8_MID(BM, STAGES, name, EXACT)                                                                                    \
-    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_##name(F8Args a) {                                         \
-        f8_mid<BM / 32, STAGES, EXACT, false>(a);                                                                               \
-    }                                                                                                                           \
-    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_##name##_grouped(F8Args a) {                               \
-        f8_mid<BM / 32, STAGES, EXACT, true>(a);                                                                                \
+#define RFXQ_F8_MID(BM, STAGES, name, EXACT)                                                                        \
+    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_##name(F8Args a) {                             \
+        f8_mid<BM / 32, STAGES, EXACT, false>(a);                                                                   \
+    }                                                                                                               \
+    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_##name##_grouped(F8Args a) {                   \
+        f8_mid<BM / 32, STAGES, EXACT, true>(a);                                                                    \
     }
 RFXQ_F8_MID(64, 3, half, false)
 RFXQ_F8_MID(64, 3, f32, true)
 RFXQ_F8_MID(128, 2, half, false)
 RFXQ_F8_MID(128, 2, f32, true)
 
-// ---------------------------------------------------------------- 256 x 256, half results
+// ---------------------------------------------------------------- 128 x 256 and 256 x 256, half results
 
-// 8 waves of 16 MF x 64. A step's weights are in registers from its start, its
+// 8 waves of 16 MF x 64. A step is a block of K: its weights are in registers from its start, its
 // activations come from LDS two 16-row operands ahead of their products; at MF - 2
-// of them all reads of the step are done and the next step's copies have landed (the one barrier).
+// of them all reads of the step are done and the next step's copies have landed (the one
+// barrier). 4096 x 4096 x 14336: 214..225 us, 2.1..2.2 PFLOP/s (128 x 256: 244; a library's product with one
+// scale a tensor: 200); instructions 59% busy at 8192^3, 3.5 rounds of tiles over the CUs done as 4.
+// 128 x 256 has three stages, for 256 x 256 two fill the LDS. Tried: two workgroups of 128 x 128 a CU
+// (283 us), operands that two waves take in turns (311), 192 x 256 tiles.
 template <uint32_t MF, uint32_t STAGES, bool GROUPED>
 RFXQ_DEV void f8_large(const F8Args& a) {
     constexpr uint32_t BM = 32u * MF, BN = 256;
@@ -275,7 +291,8 @@ RFXQ_DEV void f8_large(const F8Args& a) {
     const uint32_t row0 = (t.wave >> 2) * 16u * MF, col0 = (t.wave & 3u) * 64u;
     f4v_t acc[MF][4] = {};
     // columns past the last: any scale
-    const uint64_t first_w = reinterpret_cast<uint64_t>(t.sw + (t.n0 + col0 < a.n ? (uint64_t)(col0 / kBlock) * steps : 0u));
+    const uint64_t first_w =
+        reinterpret_cast<uint64_t>(t.sw + (t.n0 + col0 < a.n ? (uint64_t)(col0 / kBlock) * steps : 0u));
     const __attribute__((address_space(4))) float* s_w = (const __attribute__((address_space(4))) float*)(
         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)first_w) |
         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(first_w >> 32)) << 32);
@@ -299,7 +316,9 @@ RFXQ_DEV void f8_large(const F8Args& a) {
         so = src < 0 ? Tile::PAST : (uint32_t)((uint64_t)src * a.ldxs * 4u);
     }
     const auto copy_scales = [&](uint32_t c) {
-        if (t.wave < BM / 64u) copy16(sr, lds_addr(ss) + 16u * ((c & 1u) * BM + 64u * t.wave), 4u * c < steps ? so : Tile::PAST, 4u * c < steps ? 16u * c : 0u);
+        const bool there = 4u * c < steps;
+        if (t.wave < BM / 64u)
+            copy16(sr, lds_addr(ss) + 16u * ((c & 1u) * BM + 64u * t.wave), there ? so : Tile::PAST, there ? 16u * c : 0u);
     };
     const auto read_w = [&](const u4_t* ws, uint32_t f) { wf[f].take(ws[w0 + 128u * f], ws[w1 + 128u * f]); };
     const auto step = [&](uint32_t s, const u4_t* xs, const u4_t* xn, const u4_t* wn, const u4_t* xc, const u4_t* wc,
@@ -331,8 +350,10 @@ RFXQ_DEV void f8_large(const F8Args& a) {
             }
             // copies one by one: their issue holds a wave up
             if constexpr (STAGES == 3) {
-                if ((i & 1u) == 0 && i < 2u * Tile::NX) t.issue_x(lds_addr(xc), i / 2u, i / 2u + 1u);
-                if ((i & 1u) == 0 && i >= 2u * Tile::NX && i < 2u * COPIES) t.issue_w(lds_addr(wc), i / 2u - Tile::NX, i / 2u - Tile::NX + 1u);
+                constexpr uint32_t NX = Tile::NX;
+                if ((i & 1u) == 0 && i < 2u * NX) t.issue_x(lds_addr(xc), i / 2u, i / 2u + 1u);
+                if ((i & 1u) == 0 && i >= 2u * NX && i < 2u * COPIES)
+                    t.issue_w(lds_addr(wc), i / 2u - NX, i / 2u - NX + 1u);
                 if (i + 2u == 2u * COPIES) t.at += kBlock;
             } else {
                 if (i < 2u * Tile::NW && (i & 1u) == 0) {
@@ -390,8 +411,12 @@ RFXQ_DEV void f8_large(const F8Args& a) {
     for (uint32_t m = 0; m < MF; m++) t.out_row(a, row0 + 16u * m + l, t.n0 + col0 + 16u * q, acc[m]);
 }
 
-#define RFXQ_F8_LARGE(BM, STAGES)                                                                                          \
-    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_wide(F8Args a) { f8_large<BM / 32, STAGES, false>(a); }      \
-    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_wide_grouped(F8Args a) { f8_large<BM / 32, STAGES, true>(a); }
+#define RFXQ_F8_LARGE(BM, STAGES)                                                                                   \
+    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_wide(F8Args a) {                               \
+        f8_large<BM / 32, STAGES, false>(a);                                                                        \
+    }                                                                                                               \
+    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_##BM##_wide_grouped(F8Args a) {                       \
+        f8_large<BM / 32, STAGES, true>(a);                                                                         \
+    }
 RFXQ_F8_LARGE(256, 2)
 RFXQ_F8_LARGE(128, 3)

@@ -908,7 +908,8 @@ def add_rmsnorm_f8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch
                                     f"(f32, {k} contiguous values on cuda:{dev})")
     if sum_out is None and residual is not None:
         sum_out = torch.empty(rows, k, dtype=x.dtype, device=x.device)
-    sr = None if sum_out is None else _rows(sum_out, k, dev, "add_rmsnorm_f8 sum_out")
+    sr = (None if sum_out is None else xr if sum_out is x else rr if sum_out is residual
+          else _rows(sum_out, k, dev, "add_rmsnorm_f8 sum_out"))
     y = torch.empty(rows, k, dtype=x.dtype, device=x.device) if want_y else None
     yr = None if y is None else _rows(y, k, dev, "add_rmsnorm_f8 y")
     if out is None:

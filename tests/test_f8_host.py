@@ -144,6 +144,8 @@ PRODUCT = [
     ({"y": {"data": 2 * P + 1}}, 12, "aligned"),
     ({"y": {"data": 4 * P + 128}}, 11, "x and y overlap"),
     ({"y": {"data": 5 * P + 8}}, 11, "x's scales and y overlap"),
+    ({"y": {"data": 6 * P + 16}}, 11, "weight and y overlap"),
+    ({"y": {"data": 7 * P - 16}}, 11, "weight's scales and y overlap"),
 ]
 
 
