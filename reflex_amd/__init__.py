@@ -1,5 +1,6 @@
 """reflex_amd: MI355X-native GGUF quantized-matmul path (Q4_K / Q6_K / Q8_0), with products of
-grouped rows and half-typed stacks (F16 / BF16 experts) and low-rank adapters beside it.
+grouped rows and half-typed stacks (F16 / BF16 experts), low-rank adapters, and weights in 8-bit
+floating point with a scale a block beside it.
 
 The compute lives in ``librfxq.so`` (HIP C++ host code + an embedded gfx950
 code object, see ``build.py``); its C ABI is ``include/rfxq.h``. This package

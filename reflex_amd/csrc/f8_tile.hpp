@@ -143,7 +143,8 @@ struct F8Tile {
 // results 64 and 38 us: their codes are widened, their instructions run at half the rate. Tried: operands
 // read from LDS a step ahead (no gain), 64 x 64 tiles of four blocks a step (256 x 4096 x 4096: 12.7 us, 64 x 128
 // 13.4; f32 16.7 and 22.4, but two rounds of them 28.6), weights straight to registers (4096 x 4096 x 14336:
-// 354 us).
+// 354 us), a ring of six buffers of one block filled by four waves that only copy (45 us for 40: lines take
+// 400 cycles and are there in time; the operands' 64 KB of LDS reads a block, and a barrier for each, are not).
 template <uint32_t MF, uint32_t STAGES, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_mid(const F8Args& a) {
     constexpr uint32_t BM = 32u * MF, BN = 128, D = 2, CHUNK = 32;  // CHUNK: blocks whose scales are in LDS
