@@ -10,7 +10,8 @@
 // operands take 16. 1 x 4096 x 14336: 11.4 us, 5.2 TB/s of weights (a large copy: 4.87);
 // 1 x 4096 x 4096: 6.5; 32 tokens over 8 of 128 experts, 2048 x 768: 28 us, 7.2 TB/s of those that
 // stay in the memory-side cache. More columns a workgroup read x less often, fewer make more
-// workgroups; the host's table has what each measured.
+// workgroups; the host's table has what each measured. 32 x 64 and 64 x 64 tiles are for 33 to some 256 rows,
+// whose copies bound: 128 x 14336 x 4096 22..24 us, 256 rows 35..39 (f32 results; one workgroup a CU).
 template <uint32_t MT, uint32_t NT, uint32_t R, uint32_t WAVES, bool GROUPED>
 RFXQ_DEV void f8_stream(const F8Args& a) {
     constexpr uint32_t CHUNK = 64;  // blocks whose scales are in LDS
@@ -134,15 +135,20 @@ RFXQ_DEV void f8_stream(const F8Args& a) {
     }
 }
 
+// the last two for one matrix: grouped rows, of which tiles end early, took 1.1 to 1.7 times as long with them
 #define RFXQ_F8_STREAM(MT, NT, R, WAVES)                                                                            \
     extern "C" __global__ __launch_bounds__(64 * WAVES) void rfxq_f8_stream_##MT##_##NT##_##R##_##WAVES(F8Args a) {     \
         f8_stream<MT, NT, R, WAVES, false>(a);                                                                      \
-    }                                                                                                               \
+    }
+#define RFXQ_F8_STREAM_GROUPED(MT, NT, R, WAVES)                                                                    \
+    RFXQ_F8_STREAM(MT, NT, R, WAVES)                                                                                \
     extern "C" __global__                                                                                           \
         __launch_bounds__(64 * WAVES) void rfxq_f8_stream_##MT##_##NT##_##R##_##WAVES##_grouped(F8Args a) {         \
         f8_stream<MT, NT, R, WAVES, true>(a);                                                                       \
     }
-RFXQ_F8_STREAM(1, 1, 2, 8)
-RFXQ_F8_STREAM(1, 2, 1, 8)
-RFXQ_F8_STREAM(2, 2, 1, 8)
-RFXQ_F8_STREAM(1, 4, 1, 4)
+RFXQ_F8_STREAM_GROUPED(1, 1, 2, 8)
+RFXQ_F8_STREAM_GROUPED(1, 2, 1, 8)
+RFXQ_F8_STREAM_GROUPED(2, 2, 1, 8)
+RFXQ_F8_STREAM_GROUPED(1, 4, 1, 4)
+RFXQ_F8_STREAM(2, 4, 1, 8)
+RFXQ_F8_STREAM(4, 4, 1, 8)

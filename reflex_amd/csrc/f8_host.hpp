@@ -130,7 +130,12 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   stream 16 x 16  64 tiles: 4.3 (1 x 4096 x 1024), 256: 6.3 (1 x 4096 x 4096), 11.9 (1 x 14336 x 4096)
 //   stream 16 x 32  1 x 4096 x 14336: 11.5 (16 x 16: 15), 32 x 4096 x 4096: 6.4 (32 x 32: 7.5)
 //   stream 32 x 32  64 x 4096 x 4096: 7.6 (16 x 32: 8.7, 64 x 128: 13), 128 rows: 11.0 (64 x 128: 13)
-//   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 31.5 (16 x 32: 56, 64 x 128: 46)
+//   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 28 (16 x 32: 56, 64 x 128: 46);
+//                   32 x 4096 x 14336: 12.8 (16 x 32: 14.3)
+//   stream 32 x 64  128 x 4096 x 4096: 9.2 (32 x 32: 11.1), 128 x 14336 x 4096: 22.4 (28.1); 32 x 4096 x 14336: 17.3
+//                   (16 x 32: 14.3, 32 x 32: 18.8)
+//   stream 64 x 64  f32 results of 200 x 4096 x 4096: 13.2 (32 x 32: 18.3, 64 x 128: 22.2), 256 x 14336 x 4096: 35
+//                   (65; half results 34.8, 64 x 128: 36.8); 300 x 4096 x 4096: 23.8 (64 x 128: 22.8)
 //   64 x 128        256 x 4096 x 4096: 13 (32 x 32: 19), 512 x 14336 x 4096: 39 (128 x 128: 65); f32 results 68
 //   128 x 128       1000 x 4096 x 4096: 23 (64 x 128: 26, 128 x 256: 28); f32 38 (64 x 128: 47)
 //   128 x 256       2048 x 4096 x 4096: 36 (128 x 128: 46, 256 x 256: 46)
@@ -150,6 +155,8 @@ constexpr F8Variant kF8Stream[] = {{6, RFXQ_F8_STREAM, 16, 16, 512, 2.8f, 1.3f, 
                                    {7, RFXQ_F8_STREAM, 16, 32, 512, 2.8f, 0.9f, 0.085f, false},
                                    {8, RFXQ_F8_STREAM, 32, 32, 512, 2.8f, 1.0f, 0.1175f, false},
                                    {9, RFXQ_F8_STREAM, 16, 64, 256, 2.8f, 0.6f, 0.2f, false}};
+constexpr F8Variant kF8Stream1[] = {{16, RFXQ_F8_STREAM, 32, 64, 512, 2.3f, 1.5f, 0.166f, true},  // one matrix
+                                    {17, RFXQ_F8_STREAM, 64, 64, 512, 2.0f, 3.3f, 0.258f, true}};
 constexpr F8Variant kF8Half[] = {{10, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
                                  {12, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.59f, true},
                                  {14, RFXQ_F8_LARGE, 128, 256, 512, 0, 4.5f, 0.95f, true},
@@ -177,7 +184,9 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
         const double tm = grouped ? used * std::max(1.0, mean / v.bm + 0.5) : std::ceil((double)rows / v.bm);
         double rounds = tm * std::ceil((double)n / v.bn) / cus;
         rounds = v.whole ? std::ceil(rounds) : std::max(rounds, 1.0);
-        if (v.bm == 16u && v.bn == 64u && rounds < 2.0) return;  // four waves: measured where they are many
+        if (v.bm == 16u && v.bn == 64u && rounds < 1.5) return;  // four waves: measured where they are many
+        // the weights' bytes bound: tiles of 16 rows have more of them in flight
+        if (copies && !grouped && rows <= 32u && v.bm > 16u) return;
         const double t = v.start + rounds * (v.tile + (double)f8_groups(k) * v.block);
         if (!best || t < least) {
             best = &v;
@@ -186,6 +195,8 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     };
     if (copies) {
         for (const F8Variant& v : kF8Stream) look(v);
+        if (!grouped)
+            for (const F8Variant& v : kF8Stream1) look(v);
         if (f32)
             for (const F8Variant& v : kF8F32) look(v);
         else

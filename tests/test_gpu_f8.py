@@ -445,8 +445,10 @@ def _kernel(rq, x, w, rows, grouped, y_type):
 EACH = [
     (3, 9360, 48, F32, (STREAM, 16, 16)), (16, 16, 1000, BF16, (STREAM, 16, 32)), (7, 3856, 1040, F16, (STREAM, 16, 16)),
     (5, 8448, 4992, BF16, (STREAM, 16, 32)), (30, 8208, 4100, F32, (STREAM, 16, 32)), (60, 8304, 4090, BF16, (STREAM, 32, 32)),
-    (130, 8304, 3600, F32, (STREAM, 32, 32)), (300, 4368, 2048, F16, (COPIED, 64, 128)), (512, 784, 3100, BF16, (COPIED, 64, 128)),
-    (400, 4368, 3100, F32, (COPIED, 64, 128)), (390, 784, 2050, F32, (COPIED, 64, 128)), (600, 4368, 4090, BF16, (COPIED, 128, 128)),
+    (130, 8304, 3600, F32, (STREAM, 32, 32)), (300, 4368, 3600, F16, (COPIED, 64, 128)), (512, 784, 3100, BF16, (COPIED, 64, 128)),
+    (128, 8304, 4090, BF16, (STREAM, 32, 64)), (120, 9360, 3800, F32, (STREAM, 32, 64)), (250, 784, 2040, F16, (STREAM, 32, 64)),
+    (200, 8304, 4090, F32, (STREAM, 64, 64)), (250, 9360, 3900, BF16, (STREAM, 64, 64)), (250, 1040, 4050, F32, (STREAM, 64, 64)),
+    (400, 4368, 3100, F32, (COPIED, 64, 128)), (390, 784, 2600, F32, (COPIED, 64, 128)), (600, 4368, 4090, BF16, (COPIED, 128, 128)),
     (1000, 2176, 4000, F16, (COPIED, 128, 128)), (700, 1040, 3600, F32, (COPIED, 128, 128)), (1000, 4368, 4000, F32, (COPIED, 128, 128)),
     (1024, 1664, 7000, BF16, (LARGE, 128, 256)), (2040, 128, 4090, F16, (LARGE, 128, 256)), (2048, 1168, 4000, BF16, (LARGE, 128, 256)),
     (4095, 656, 4090, BF16, (LARGE, 256, 256)), (4090, 128, 4096, F16, (LARGE, 256, 256)), (4096, 16, 4096, BF16, (LARGE, 256, 256)),
