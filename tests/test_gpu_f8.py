@@ -428,6 +428,57 @@ def test_gemm_matrix_past_4_gib(rq):
         assert not y[:, rest.to(DEV)].any()
 
 
+@pytest.mark.parametrize("rows,gap", [(3, 1 << 31), (200, 1 << 25)])
+@pytest.mark.parametrize("what", ["codes", "scales"])
+def test_gemm_rows_past_4_gib(rq, rows, gap, what):
+    """Rows, or their scales, that lie further apart than 32 bits of bytes reach."""
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, 400, 300, rows))
+    far = x.view(torch.uint8) if what == "codes" else xs
+    step = gap // far.element_size()
+    buf = torch.empty((rows - 1) * step + far.shape[1], dtype=far.dtype, device=DEV)
+    view = buf.as_strided(far.shape, (step, 1))
+    view.copy_(far)
+    _say("past 4 GiB", rows, what)
+    rows_ = rq.F8Rows(view.view(F8), xs) if what == "codes" else rq.F8Rows(x, view)
+    weight = rq.F8Weight(w, ws)
+    for y_type in (F32, BF16):
+        _check_product(x, xs, w, ws, rq.gemm_f8(rows_, weight, dtype=y_type))
+    back = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device=DEV)
+    y = rq.grouped_gemm_f8(rows_, weight, torch.tensor([0, rows], dtype=torch.int32, device=DEV), rows, x_index=back)
+    _check_product(x.view(torch.uint8).flip(0).view(F8), xs.flip(0), w, ws, y)
+
+
+@pytest.mark.parametrize("k,n", [(16, 5), (17, 5), (128, 130)])
+def test_gemm_many_rows(rq, k, n):
+    rows = 2_000_003
+    g = torch.Generator(DEV).manual_seed(k)
+    x = torch.randint(-1, 2, (rows, k), generator=g, device=DEV).float().to(F8)
+    w = torch.randint(-1, 2, (n, k), generator=g, device=DEV).float().to(F8)
+    xs = torch.exp2(torch.randint(-3, 4, (rows, 1), generator=g, device=DEV).float())
+    _say("many rows", k, n)
+    y = rq.gemm_f8(rq.F8Rows(x, xs), rq.F8Weight(w, torch.ones(_blocks(n), 1, device=DEV)))
+    assert torch.equal(y, (x.float() @ w.float().t()) * xs)  # whole numbers times powers of two
+
+
+def test_more_groups_than_a_launch(rq):
+    """More rows than the largest launches have places for."""
+    rows = (1 << 24) + 77
+    x = torch.randn(rows, 1, generator=torch.Generator(DEV).manual_seed(1), device=DEV)
+    one = torch.ones_like(x)
+    for out, v in ((rq.quantize_f8(x), x), (rq.silu_and_mul_f8(x, one), torch.nn.functional.silu(x))):
+        _say("groups", rows)
+        # a group of one value: the largest code, but for 0, whose quotient by the least scale is 0
+        assert torch.equal(out.codes.float().abs(), torch.where(v == 0, 0.0, 448.0))
+        assert ((out.codes.float() * out.scales - v).abs() <= v.abs() * 2.0 ** -18).all()
+    rows = (1 << 20) + 37
+    x = torch.randn(rows, 8, generator=torch.Generator(DEV).manual_seed(2), device=DEV)
+    out, _, y = rq.add_rmsnorm_f8(x, None, torch.ones(8, device=DEV), 1e-6, want_y=True)
+    want = x.double() / (x.double().square().mean(1, keepdim=True) + 1e-6).sqrt()
+    assert ((y.double() - want).abs() <= want.abs() * 2.0 ** -20).all()
+    assert ((out.codes.double() * out.scales.double() - y.double()).abs()
+            <= torch.maximum(y.abs().double() * 2.0 ** -4, out.scales.double() * 2.0 ** -10) * (1 + 2.0 ** -18)).all()
+
+
 ANY, FEW, STREAM, COPIED, LARGE = range(5)
 
 
