@@ -81,33 +81,27 @@ RFXQ_DEV f4v_t multiply(const Operand<true>& a, const Operand<true>& b) {
 
 // 16 codes at any byte
 RFXQ_DEV u4_t ld_codes(const uint8_t* p) { return *(const RFXQ_GLOBAL u4a1_t*)p; }
-// The first `have` (< 16) of the 16 codes that end where a row of k codes ends, zeros behind
-// them: the row's last 16, moved down by whole dwords and then by bytes (a row
-// of fewer than 16: one by one).
-RFXQ_DEV u4_t ld_tail(const uint8_t* row, uint32_t k, uint32_t have) {
+// The last, partial block of a row of k >= 16 codes: 16 codes from `at` on are read from min(at, k - 16) on, so that no
+// load has a condition (those are waited for one by one), and moved down by as many bytes, zeros behind
+// them: by whole dwords, then by bytes.
+RFXQ_DEV u4_t cut_codes(u4_t v, uint32_t by) {
+    if (by & 8u) v = u4_t{v.z, v.w, 0, 0};
+    if (by & 4u) v = u4_t{v.y, v.z, v.w, 0};
+    const u4_t r = {alignbyte(v.y, v.x, by & 3u), alignbyte(v.z, v.y, by & 3u), alignbyte(v.w, v.z, by & 3u),
+                    alignbyte(0, v.w, by & 3u)};
+    return by < 16u ? r : u4_t{0, 0, 0, 0};
+}
+// A row of k < 16 codes: one by one.
+RFXQ_DEV u4_t ld_short(const uint8_t* row, uint32_t k, uint32_t at) {
     u4_t r = {0, 0, 0, 0};
-    if (k >= 16u) {
-        const uint32_t by = 16u - have;
-        u4_t v = ld_codes(row + k - 16u);
-        if (by & 8u) v = u4_t{v.z, v.w, 0, 0};
-        if (by & 4u) v = u4_t{v.y, v.z, v.w, 0};
-        r = u4_t{alignbyte(v.y, v.x, by & 3u), alignbyte(v.z, v.y, by & 3u), alignbyte(v.w, v.z, by & 3u),
-                 alignbyte(0, v.w, by & 3u)};
-        if (have == 0) r = u4_t{0, 0, 0, 0};
-    } else {
+    const uint32_t have = at ? 0u : k;
 #pragma unroll 1
-        for (uint32_t i = 0; i < have; i++) {
-            const uint32_t c = (uint32_t)((const RFXQ_GLOBAL uint8_t*)row)[i] << (8u * (i & 3u));
+    for (uint32_t i = 0; i < have; i++) {
+        const uint32_t c = (uint32_t)((const RFXQ_GLOBAL uint8_t*)row)[i] << (8u * (i & 3u));
 #pragma unroll
-            for (uint32_t d = 0; d < 4u; d++) r[d] |= i >> 2 == d ? c : 0u;
-        }
+        for (uint32_t d = 0; d < 4u; d++) r[d] |= i >> 2 == d ? c : 0u;
     }
     return r;
-}
-// 16 codes of a row of k from its code `at` on, of which all, some or none are there
-RFXQ_DEV u4_t ld_codes(const uint8_t* row, uint32_t k, uint32_t at) {
-    if (at + 16u <= k) return ld_codes(row + at);
-    return ld_tail(row, k, at < k ? k - at : 0u);
 }
 
 // The rows of a tile: a search among the groups, or counted.
@@ -162,17 +156,19 @@ RFXQ_DEV void f8_out(const F8Args& a, int64_t row, uint32_t n, const f4v_t (&v)[
 // ---------------------------------------------------------------- any alignment
 
 // 32 MF x 32 NF tiles (in one block of columns: a scale of the weights' a step), operands through
-// registers to LDS, the next step's loads in flight during the products. KG groups of four waves
-// of 16 MF x 16 NF results take a block of K each of a step's KG, and add their parts in LDS. Rows
-// and columns past the tile read others, whose results are not stored; the last,
-// partial block has zeros behind the end of both operands, a block past it no
-// weights and the scale 0. Loads of 16 bytes at any byte, of which each touches two lines: no copy to
-// LDS takes those. Bound by that and by the two barriers a step: 333 x 1235 x 1531 f32 10.8 us in 32 x 64 tiles
-// (264 of them), 1000 x 4099 x 4099 half results 82 us, 16 x 4099 x 14336 f32 23 us (2.6 TB/s).
-template <uint32_t MF, uint32_t NF, uint32_t KG, bool EXACT, bool GROUPED>
+// registers to one of two LDS buffers, a barrier a step, the loads of AHEAD steps in flight during the
+// products. KG groups of four waves of 16 MF x 16 NF results take a block of K each of a step's KG,
+// and add their parts in LDS. Rows and columns past the tile read others, whose results are not
+// stored; the last, partial block has zeros behind the end of both operands, a block past it
+// zeros and the scale 0. Bound by loads of 16 bytes at any byte (100 x K x 4099, f32: K = 4096 18 us, 4100 21, 4098
+// 25, 4099 28): 333 x 1235 x 1531 f32 9.4 us in 32 x 64 tiles (264 of them), 1000 x 4099 x 4099 half
+// results 83 us, 16 x 4099 x 14336 f32 24.5 us (2.4 TB/s). Two steps ahead pay for 64 x 128 tiles (333 x 4099 x
+// 4099 half: 34 us, one 37), not for 32 x 64 (11.4, one 9.4). Tried: whole dwords and the fifth that a lane needs by a load
+// of its own or from the next lane (10.5 and 11.1), four groups of waves (15).
+template <uint32_t MF, uint32_t NF, uint32_t KG, uint32_t AHEAD, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_any(const F8Args& a) {
     constexpr uint32_t BM = 32u * MF, BN = 32u * NF, ROWS = 32, NX = BM / ROWS, NW = BN / ROWS;
-    __shared__ u4_t xs[KG][BM * 8u], ws[KG][BN * 8u];
+    __shared__ u4_t xs[2][KG][BM * 8u], ws[2][KG][BN * 8u];
     uint32_t tm, tn;
     if (!tile_place(a, blockIdx.x, tm, tn)) return;
     const RowTile t = f8_tile<GROUPED>(a, BM, tm);
@@ -202,56 +198,70 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     struct Block {
         u4_t x[NX], w[NW];
         float sx[MF], sw;
-    } r;
-    const auto load = [&](uint32_t b) {
-        const uint32_t k = b * kBlock + 16u * c;
-        if (b < full) {
+    } r[AHEAD];
+    // no condition round loads: those under one are waited for at its end. Blocks past the last read its end.
+    const auto load = [&](Block& to, uint32_t b) {
+        const uint32_t k = min(b * kBlock + 16u * c, a.k - 16u), at = min(b, blocks - 1u);
 #pragma unroll
-            for (uint32_t i = 0; i < NW; i++) r.w[i] = ld_codes(wp[i] + k);
+        for (uint32_t i = 0; i < NW; i++) to.w[i] = ld_codes(wp[i] + k);
 #pragma unroll
-            for (uint32_t i = 0; i < NX; i++) r.x[i] = ld_codes(xp[i] + k);
-        } else if (b < blocks) {
+        for (uint32_t i = 0; i < NX; i++) to.x[i] = ld_codes(xp[i] + k);
+        to.sw = ((const RFXQ_GLOBAL float*)sw)[at];
 #pragma unroll
-            for (uint32_t i = 0; i < NW; i++) r.w[i] = ld_codes(wp[i], a.k, k);
-#pragma unroll
-            for (uint32_t i = 0; i < NX; i++) r.x[i] = ld_codes(xp[i], a.k, k);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < NW; i++) r.w[i] = u4_t{0, 0, 0, 0};
-#pragma unroll
-            for (uint32_t i = 0; i < NX; i++) r.x[i] = u4_t{0, 0, 0, 0};
-        }
-        const uint32_t at = min(b, blocks - 1u);
-        r.sw = b < blocks ? ((const RFXQ_GLOBAL float*)sw)[at] : 0.0f;
-#pragma unroll
-        for (uint32_t m = 0; m < MF; m++) r.sx[m] = b < blocks ? ((const RFXQ_GLOBAL float*)sx[m])[at] : 0.0f;
+        for (uint32_t m = 0; m < MF; m++) to.sx[m] = ((const RFXQ_GLOBAL float*)sx[m])[at];
     };
-    load(kg);
-    for (uint32_t b = 0; b < blocks; b += KG) {
-        lds_barrier();
+    const auto step = [&](uint32_t b, Block& now, uint32_t buffer, auto more) {
+        u4_t *xl = xs[buffer][kg], *wl = ws[buffer][kg];
+        if (b + kg >= full) {  // a partial block, or one behind it
+            const uint32_t k = (b + kg) * kBlock + 16u * c, by = k - min(k, a.k - 16u);
 #pragma unroll
-        for (uint32_t i = 0; i < NX; i++) xs[kg][lds_piece((tid >> 3) + ROWS * i, c)] = r.x[i];
+            for (uint32_t i = 0; i < NW; i++) now.w[i] = cut_codes(now.w[i], by);
 #pragma unroll
-        for (uint32_t i = 0; i < NW; i++) ws[kg][lds_piece((tid >> 3) + ROWS * i, c)] = r.w[i];
-        lds_barrier();
+            for (uint32_t i = 0; i < NX; i++) now.x[i] = cut_codes(now.x[i], by);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < NX; i++) xl[lds_piece((tid >> 3) + ROWS * i, c)] = now.x[i];
+#pragma unroll
+        for (uint32_t i = 0; i < NW; i++) wl[lds_piece((tid >> 3) + ROWS * i, c)] = now.w[i];
         float scale[MF];
 #pragma unroll
-        for (uint32_t m = 0; m < MF; m++) scale[m] = r.sx[m] * r.sw;
-        if (b + KG < blocks) load(b + KG + kg);
+        for (uint32_t m = 0; m < MF; m++) scale[m] = b + kg < blocks ? now.sx[m] * now.sw : 0.0f;
+        lds_barrier();
+        if constexpr (decltype(more)::value) load(now, b + AHEAD * KG + kg);
         Operand<EXACT> wf[NF];
 #pragma unroll
         for (uint32_t f = 0; f < NF; f++)
-            wf[f].take(ws[kg][lds_piece(col0 + 16u * f + l, q)], ws[kg][lds_piece(col0 + 16u * f + l, 4u + q)]);
+            wf[f].take(wl[lds_piece(col0 + 16u * f + l, q)], wl[lds_piece(col0 + 16u * f + l, 4u + q)]);
 #pragma unroll
         for (uint32_t m = 0; m < MF; m++) {
             Operand<EXACT> xf;
-            xf.take(xs[kg][lds_piece(row0 + 16u * m + l, q)], xs[kg][lds_piece(row0 + 16u * m + l, 4u + q)]);
+            xf.take(xl[lds_piece(row0 + 16u * m + l, q)], xl[lds_piece(row0 + 16u * m + l, 4u + q)]);
             f4v_t d[NF];
 #pragma unroll
             for (uint32_t f = 0; f < NF; f++) d[f] = multiply(wf[f], xf);
 #pragma unroll
             for (uint32_t f = 0; f < NF; f++) acc[m][f] += d[f] * scale[m];
         }
+    };
+    if (a.k >= 16u) {
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; i++) load(r[i], KG * i + kg);
+        for (uint32_t b = 0;; b += 2u * KG) {
+            step(b, r[0], 0, Count<1>{});
+            if (b + KG >= blocks) break;
+            step(b + KG, r[AHEAD - 1u], 1, Count<1>{});
+            if (b + 2u * KG >= blocks) break;
+        }
+    } else {
+        const uint32_t k = kg * kBlock + 16u * c;
+#pragma unroll
+        for (uint32_t i = 0; i < NW; i++) r[0].w[i] = ld_short(wp[i], a.k, k);
+#pragma unroll
+        for (uint32_t i = 0; i < NX; i++) r[0].x[i] = ld_short(xp[i], a.k, k);
+        r[0].sw = *(const RFXQ_GLOBAL float*)sw;
+#pragma unroll
+        for (uint32_t m = 0; m < MF; m++) r[0].sx[m] = *(const RFXQ_GLOBAL float*)sx[m];
+        step(0, r[0], 0, Count<0>{});
     }
     if constexpr (KG > 1) {
         static_assert(KG == 2 && sizeof ws >= 4u * MF * NF * 64u * sizeof(f4v_t));
@@ -275,18 +285,18 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     }
 }
 
-#define RFXQ_F8_ANY(MF, NF, KG, WAVES, name, EXACT)                                                                 \
+#define RFXQ_F8_ANY(MF, NF, KG, AHEAD, WAVES, name, EXACT)                                                          \
     extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##MF##_##KG##_##name(F8Args a) {       \
-        f8_any<MF, NF, KG, EXACT, false>(a);                                                                        \
+        f8_any<MF, NF, KG, AHEAD, EXACT, false>(a);                                                                 \
     }                                                                                                               \
     extern "C" __global__ __launch_bounds__(256 * KG, WAVES) void rfxq_f8_any##MF##_##KG##_##name##_grouped(F8Args a) { \
-        f8_any<MF, NF, KG, EXACT, true>(a);                                                                         \
+        f8_any<MF, NF, KG, AHEAD, EXACT, true>(a);                                                                  \
     }
-RFXQ_F8_ANY(1, 2, 2, 4, half, false)
-RFXQ_F8_ANY(1, 2, 2, 4, f32, true)
-RFXQ_F8_ANY(2, 4, 1, 3, half, false)
-RFXQ_F8_ANY(2, 4, 2, 2, half, false)
-RFXQ_F8_ANY(2, 4, 2, 2, f32, true)
+RFXQ_F8_ANY(1, 2, 2, 1, 4, half, false)
+RFXQ_F8_ANY(1, 2, 2, 1, 4, f32, true)
+RFXQ_F8_ANY(2, 4, 1, 1, 3, half, false)
+RFXQ_F8_ANY(2, 4, 2, 2, 2, half, false)
+RFXQ_F8_ANY(2, 4, 2, 2, 2, f32, true)
 
 // ---------------------------------------------------------------- few rows, any alignment
 
@@ -358,10 +368,25 @@ RFXQ_DEV void f8_few(const F8Args& a) {
     }
     if (tail && wave == full % WK) {
         Block& r = s[0][0];
+        const uint32_t k = full * kBlock + 16u * q;
+        if (a.k >= 16u) {
+            const uint32_t from[2] = {min(k, a.k - 16u), min(k + 64u, a.k - 16u)};
 #pragma unroll
-        for (uint32_t h = 0; h < 2u; h++) {
-            r.w[h] = ld_codes(w, a.k, full * kBlock + 64u * h + 16u * q);
-            r.x[h] = ld_codes(x, a.k, full * kBlock + 64u * h + 16u * q);
+            for (uint32_t h = 0; h < 2u; h++) {
+                r.w[h] = ld_codes(w + from[h]);
+                r.x[h] = ld_codes(x + from[h]);
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                r.w[h] = cut_codes(r.w[h], k + 64u * h - from[h]);
+                r.x[h] = cut_codes(r.x[h], k + 64u * h - from[h]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++) {
+                r.w[h] = ld_short(w, a.k, k + 64u * h);
+                r.x[h] = ld_short(x, a.k, k + 64u * h);
+            }
         }
         r.sw = sw[full];
         r.sx = sx[full];

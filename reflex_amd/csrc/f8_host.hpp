@@ -142,9 +142,9 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   256 x 256       4096 x 4096 x 14336: 229 (128 x 256: 244)
 // and rows at any byte:
 //   few 16 x 16     1 x 4099 x 4099: 11.8 (32 x 64: 22), 16 rows: 22 (22), 40 x 1235 x 1531: 7.0 (7.8)
-//   32 x 64         333 x 1235 x 1531: 10.5 (64 x 128: 15.9), 16 x 4099 x 14336: 23 (37; few: 79)
-//   64 x 128        1000 x 4099 x 4099, half results: 83 with 4 waves, 107 with 8 (32 x 64: 109); 333 rows: 43,
-//                   39 (49); f32, 8 waves: 333 rows 41 (32 x 64: 53)
+//   32 x 64         333 x 1235 x 1531: 9.4 (64 x 128: 15.2), 16 x 4099 x 14336: 24.5 (35; few: 80)
+//   64 x 128        1000 x 4099 x 4099, half results: 83 with 4 waves, 93 with 8 (32 x 64: 110); 333 rows: 43,
+//                   34 (48); f32, 8 waves: 333 rows 39 (32 x 64: 49)
 struct F8Variant {
     uint32_t product, kernel;  // kernel: RFXQ_F8_*
     uint32_t bm, bn, threads;
@@ -166,11 +166,11 @@ constexpr F8Variant kF8F32[] = {{11, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55
 // one row's operand has one line where 16 have 16
 constexpr F8Variant kF8Few[2] = {{5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.27f, false},
                                  {5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.55f, false}};
-constexpr F8Variant kF8AnyHalf[] = {{0, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.51f, false},
+constexpr F8Variant kF8AnyHalf[] = {{0, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.2f, 0.45f, false},
                                     {2, RFXQ_F8_ANY, 64, 128, 256, 2.0f, 2.0f, 1.2f, false},
-                                    {3, RFXQ_F8_ANY, 64, 128, 512, 0, 5.0f, 1.0f, true}};
-constexpr F8Variant kF8AnyF32[] = {{1, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.9f, 0.51f, false},
-                                   {4, RFXQ_F8_ANY, 64, 128, 512, 0, 7.1f, 1.02f, true}};
+                                    {3, RFXQ_F8_ANY, 64, 128, 512, 0, 5.0f, 0.87f, true}};
+constexpr F8Variant kF8AnyF32[] = {{1, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.2f, 0.45f, false},
+                                   {4, RFXQ_F8_ANY, 64, 128, 512, 0, 7.1f, 0.97f, true}};
 
 // `copies`: rows start at 16 bytes and offsets fit 32 bits
 F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32,

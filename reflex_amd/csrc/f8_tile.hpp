@@ -5,15 +5,16 @@
 // multiply-adds beside it and two waves a SIMD (4.1 PFLOP/s in all at 2.1 GHz); LDS
 // gives 239 bytes a cycle to 8 waves (124 to 4), copies bring 63. A 256 x 256 tile takes 2240
 // cycles of instructions for a block of K, 800 of LDS (192 KB) and 1040 of copies (64 KB): large tiles are bound by
-// the instructions and by what holds their issue up, small ones by copies and
-// by the way from a copy's issue to its landing.
+// the instructions and by what holds their issue up, small ones by their operands' LDS reads, by the copies' writes
+// there and by the barrier of a step.
 #pragma once
 #include "f8_gemm.hpp"
 
 // dma16 to LDS address `lds` with an offset that all lanes share, and unseen by the compiler's wait counting: it
 // takes LDS reads of one buffer to depend on copies into another and waits for
 // them. Whoever calls it waits with wait_copies, and has no other load from memory in
-// flight that the compiler would wait for.
+// flight that the compiler would wait for. The buffer's end is checked for each dword, the shared offset
+// included: dwords behind it are zeros.
 RFXQ_DEV void copy16(rsrc_t r, uint32_t lds, uint32_t off, uint32_t by) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :

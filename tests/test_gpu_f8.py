@@ -505,7 +505,8 @@ EACH = [
     (4095, 656, 4090, BF16, (LARGE, 256, 256)), (4090, 128, 4096, F16, (LARGE, 256, 256)), (4096, 16, 4096, BF16, (LARGE, 256, 256)),
     (4090, 1040, 4088, F16, (LARGE, 256, 256)),
     (1, 4099, 4099, F32, (FEW, 16, 16)), (16, 1237, 300, BF16, (FEW, 16, 16)), (333, 1235, 1531, F32, (ANY, 32, 64)),
-    (100, 4101, 1531, F16, (ANY, 32, 64)), (333, 4099, 4099, F32, (ANY, 64, 128)), (900, 13, 4099, F32, (ANY, 64, 128)),
+    (100, 4101, 1531, F16, (ANY, 32, 64)), (333, 4099, 4099, F32, (ANY, 64, 128)), (900, 13, 4099, F32, (ANY, 32, 64)),
+    (700, 1301, 2100, F32, (ANY, 64, 128)),
     (1000, 4099, 4099, BF16, (ANY, 64, 128)), (333, 2099, 4099, F16, (ANY, 64, 128)), (900, 7, 3100, BF16, (ANY, 64, 128)),
     (300, 3, 1700, F32, (ANY, 32, 64)), (5, 11, 100, BF16, (FEW, 16, 16)),
 ]
