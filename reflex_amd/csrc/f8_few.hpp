@@ -11,8 +11,10 @@
 // 1 x 4096 x 4096: 6.5; 32 tokens over 8 of 128 experts, 2048 x 768: 28 us, 7.2 TB/s of those that
 // stay in the memory-side cache. More columns a workgroup read x less often, fewer make more
 // workgroups; the host's table has what each measured. 32 x 64 and 64 x 64 tiles are for 33 to some 256 rows,
-// whose copies bound: 128 x 14336 x 4096 22..24 us, 256 rows 35..39 (f32 results; one workgroup a CU).
-template <uint32_t MT, uint32_t NT, uint32_t R, uint32_t WAVES, bool GROUPED>
+// whose copies and products bound: 128 x 14336 x 4096 21 us for half results and 23 for f32 ones, 256 rows 29 and 35. (The
+// smaller tiles gain less by the instruction of 128, 64 rows in 32 x 32 16.4 us for 17.0, and have
+// exact products for all results.)
+template <uint32_t MT, uint32_t NT, uint32_t R, uint32_t WAVES, bool EXACT, bool GROUPED>
 RFXQ_DEV void f8_stream(const F8Args& a) {
     constexpr uint32_t CHUNK = 64;  // blocks whose scales are in LDS
     constexpr uint32_t PER = MT + NT, COPIES = 2u * PER, PAST = 0xFFFFFFF0u;
@@ -88,12 +90,12 @@ RFXQ_DEV void f8_stream(const F8Args& a) {
         __builtin_amdgcn_sched_barrier(0);
         copy_w(at, b + WAVES * R);
         copy_x(at, b + WAVES * R);
-        Operand<true> wf[NT];
+        Operand<EXACT> wf[NT];
 #pragma unroll
         for (uint32_t f = 0; f < NT; f++) wf[f].take(raw[f][0], raw[f][1]);
 #pragma unroll
         for (uint32_t m = 0; m < MT; m++) {
-            Operand<true> xf;
+            Operand<EXACT> xf;
             xf.take(raw[NT + m][0], raw[NT + m][1]);
             f4v_t d[NT];
 #pragma unroll
@@ -135,20 +137,24 @@ RFXQ_DEV void f8_stream(const F8Args& a) {
     }
 }
 
-// the last two for one matrix: grouped rows, of which tiles end early, took 1.1 to 1.7 times as long with them
+// the last four for one matrix: grouped rows, of which tiles end early, took 1.1 to 1.7 times as long with them
 #define RFXQ_F8_STREAM(MT, NT, R, WAVES)                                                                            \
     extern "C" __global__ __launch_bounds__(64 * WAVES) void rfxq_f8_stream_##MT##_##NT##_##R##_##WAVES(F8Args a) {     \
-        f8_stream<MT, NT, R, WAVES, false>(a);                                                                      \
-    }
-#define RFXQ_F8_STREAM_GROUPED(MT, NT, R, WAVES)                                                                    \
-    RFXQ_F8_STREAM(MT, NT, R, WAVES)                                                                                \
+        f8_stream<MT, NT, R, WAVES, true, false>(a);                                                                \
+    }                                                                                                               \
     extern "C" __global__                                                                                           \
         __launch_bounds__(64 * WAVES) void rfxq_f8_stream_##MT##_##NT##_##R##_##WAVES##_grouped(F8Args a) {         \
-        f8_stream<MT, NT, R, WAVES, true>(a);                                                                       \
+        f8_stream<MT, NT, R, WAVES, true, true>(a);                                                                 \
     }
-RFXQ_F8_STREAM_GROUPED(1, 1, 2, 8)
-RFXQ_F8_STREAM_GROUPED(1, 2, 1, 8)
-RFXQ_F8_STREAM_GROUPED(2, 2, 1, 8)
-RFXQ_F8_STREAM_GROUPED(1, 4, 1, 4)
-RFXQ_F8_STREAM(2, 4, 1, 8)
-RFXQ_F8_STREAM(4, 4, 1, 8)
+#define RFXQ_F8_STREAM1(MT, NT, name, EXACT)                                                                        \
+    extern "C" __global__ __launch_bounds__(512) void rfxq_f8_stream_##MT##_##NT##_##name(F8Args a) {               \
+        f8_stream<MT, NT, 1, 8, EXACT, false>(a);                                                                   \
+    }
+RFXQ_F8_STREAM(1, 1, 2, 8)
+RFXQ_F8_STREAM(1, 2, 1, 8)
+RFXQ_F8_STREAM(2, 2, 1, 8)
+RFXQ_F8_STREAM(1, 4, 1, 4)
+RFXQ_F8_STREAM1(2, 4, half, false)
+RFXQ_F8_STREAM1(2, 4, f32, true)
+RFXQ_F8_STREAM1(4, 4, half, false)
+RFXQ_F8_STREAM1(4, 4, f32, true)

@@ -132,10 +132,11 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   stream 32 x 32  64 x 4096 x 4096: 7.6 (16 x 32: 8.7, 64 x 128: 13), 128 rows: 11.0 (64 x 128: 13)
 //   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 28 (16 x 32: 56, 64 x 128: 46);
 //                   32 x 4096 x 14336: 12.8 (16 x 32: 14.3)
-//   stream 32 x 64  128 x 4096 x 4096: 9.2 (32 x 32: 11.1), 128 x 14336 x 4096: 22.4 (28.1); 32 x 4096 x 14336: 17.3
-//                   (16 x 32: 14.3, 32 x 32: 18.8)
-//   stream 64 x 64  f32 results of 200 x 4096 x 4096: 13.2 (32 x 32: 18.3, 64 x 128: 22.2), 256 x 14336 x 4096: 35
-//                   (65; half results 34.8, 64 x 128: 36.8); 300 x 4096 x 4096: 23.8 (64 x 128: 22.8)
+//   stream 32 x 64  128 x 4096 x 4096: 8.7, f32 results 9.2 (32 x 32: 11.1), 128 x 14336 x 4096: 20.9, 22.4 (28.1);
+//                   32 x 4096 x 14336: 17.3 (16 x 32: 14.3, 32 x 32: 18.8)
+//   stream 64 x 64  256 x 4096 x 4096: 12.0 (64 x 128: 13.3), 256 x 14336 x 4096: 29.0 (36.7), 64 x 4096 x 14336: 16.3
+//                   (14.9); f32 results of 200 x 4096 x 4096: 13.2 (32 x 32: 18.3, 64 x 128: 22.2), 256 x
+//                   14336 x 4096: 35 (65); 300 x 4096 x 4096: 23.8 (64 x 128: 22.8)
 //   64 x 128        256 x 4096 x 4096: 13 (32 x 32: 19), 512 x 14336 x 4096: 39 (128 x 128: 65); f32 results 68
 //   128 x 128       1000 x 4096 x 4096: 23 (64 x 128: 26, 128 x 256: 28); f32 38 (64 x 128: 47)
 //   128 x 256       2048 x 4096 x 4096: 36 (128 x 128: 46, 256 x 256: 46)
@@ -155,13 +156,16 @@ constexpr F8Variant kF8Stream[] = {{6, RFXQ_F8_STREAM, 16, 16, 512, 2.8f, 1.3f, 
                                    {7, RFXQ_F8_STREAM, 16, 32, 512, 2.8f, 0.9f, 0.085f, false},
                                    {8, RFXQ_F8_STREAM, 32, 32, 512, 2.8f, 1.0f, 0.1175f, false},
                                    {9, RFXQ_F8_STREAM, 16, 64, 256, 2.8f, 0.6f, 0.2f, false}};
-constexpr F8Variant kF8Stream1[] = {{16, RFXQ_F8_STREAM, 32, 64, 512, 2.3f, 1.5f, 0.166f, true},  // one matrix
-                                    {17, RFXQ_F8_STREAM, 64, 64, 512, 2.0f, 3.3f, 0.258f, true}};
-constexpr F8Variant kF8Half[] = {{10, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
+// the first two of each: one matrix
+constexpr F8Variant kF8Half[] = {{16, RFXQ_F8_STREAM, 32, 64, 512, 2.3f, 1.5f, 0.153f, true},
+                                 {18, RFXQ_F8_STREAM, 64, 64, 512, 2.0f, 2.9f, 0.2125f, true},
+                                 {10, RFXQ_F8_COPIED, 64, 128, 512, 0, 3.5f, 0.31f, true},
                                  {12, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.59f, true},
                                  {14, RFXQ_F8_LARGE, 128, 256, 512, 0, 4.5f, 0.95f, true},
                                  {15, RFXQ_F8_LARGE, 256, 256, 512, 0, 6.0f, 1.6f, true}};
-constexpr F8Variant kF8F32[] = {{11, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
+constexpr F8Variant kF8F32[] = {{17, RFXQ_F8_STREAM, 32, 64, 512, 2.3f, 1.5f, 0.166f, true},
+                                {19, RFXQ_F8_STREAM, 64, 64, 512, 2.0f, 3.3f, 0.258f, true},
+                                {11, RFXQ_F8_COPIED, 64, 128, 512, 0, 4.0f, 0.55f, true},
                                 {13, RFXQ_F8_COPIED, 128, 128, 512, 0, 4.0f, 0.95f, true}};
 // one row's operand has one line where 16 have 16
 constexpr F8Variant kF8Few[2] = {{5, RFXQ_F8_FEW, 16, 16, 512, 3.0f, 0, 0.27f, false},
@@ -180,6 +184,8 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     const F8Variant* best = nullptr;
     double least = 0;
     const auto look = [&](const F8Variant& v) {
+        const bool one = v.kernel == RFXQ_F8_STREAM && v.whole;  // for one matrix
+        if (one && grouped) return;
         // grouped rows end inside a tile, half a tile on average
         const double tm = grouped ? used * std::max(1.0, mean / v.bm + 0.5) : std::ceil((double)rows / v.bm);
         double rounds = tm * std::ceil((double)n / v.bn) / cus;
@@ -187,7 +193,8 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
         if (v.bm == 16u && v.bn == 64u && rounds < 1.5) return;  // four waves: measured where they are many
         // the weights' bytes bound: tiles of 16 rows have more of them in flight
         if (copies && !grouped && rows <= 32u && v.bm > 16u) return;
-        const double t = v.start + rounds * (v.tile + (double)f8_groups(k) * v.block);
+        double t = v.start + rounds * (v.tile + (double)f8_groups(k) * v.block);
+        if (one) t = std::max(t, (double)k * n / 3.6e6);  // weights at 3.6 TB/s (64 x 4096 x 14336: 16.3)
         if (!best || t < least) {
             best = &v;
             least = t;
@@ -195,8 +202,6 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     };
     if (copies) {
         for (const F8Variant& v : kF8Stream) look(v);
-        if (!grouped)
-            for (const F8Variant& v : kF8Stream1) look(v);
         if (f32)
             for (const F8Variant& v : kF8F32) look(v);
         else

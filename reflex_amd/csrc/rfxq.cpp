@@ -156,11 +156,11 @@ struct HalfKernels {
 };
 
 // kernels of the third code object (f8_host.hpp); types: [F32, F16, BF16]
-constexpr uint32_t kF8Products = 18, kF8Grouped = 16;  // the last two: one matrix only
+constexpr uint32_t kF8Products = 20, kF8Grouped = 16;  // the last four: one matrix only
 const char* const kF8ProductNames[kF8Products] = {
-    "any1_2_half",    "any1_2_f32",     "any2_1_half",    "any2_2_half",    "any2_2_f32",     "few",
-    "stream_1_1_2_8", "stream_1_2_1_8", "stream_2_2_1_8", "stream_1_4_1_4", "64_half",        "64_f32",
-    "128_half",       "128_f32",        "128_wide",       "256_wide",       "stream_2_4_1_8", "stream_4_4_1_8"};
+    "any1_2_half",    "any1_2_f32",     "any2_1_half",     "any2_2_half",    "any2_2_f32",      "few",      "stream_1_1_2_8",
+    "stream_1_2_1_8", "stream_2_2_1_8", "stream_1_4_1_4",  "64_half",        "64_f32",          "128_half", "128_f32",
+    "128_wide",       "256_wide",       "stream_2_4_half", "stream_2_4_f32", "stream_4_4_half", "stream_4_4_f32"};
 struct F8Kernels {
     hipFunction_t quantize[3] = {}, silu[3] = {};
     hipFunction_t norm[3][3] = {};  // [type][1 piece, 4 pieces, any length]

@@ -784,7 +784,7 @@ class F8Rows:
     """Rows in e4m3 with a scale for each 128 of a row (``rfxq_f8_rows``): value (r, c) is
     ``codes[r, c] * scales[r, c // 128]``. codes float8_e4m3fn (or its bytes as uint8) [rows, columns], scales f32
     [rows, ceil(columns / 128)], rows contiguous and any distance apart; no copy: calls read and write the
-    tensors' memory."""
+    memory that the tensors have now (which may not be resized or set anew)."""
 
     __slots__ = ("_codes", "_scales", "_c", "_rows", "_columns", "_dev")
 
@@ -820,7 +820,8 @@ class F8Rows:
 class F8Weight:
     """A matrix [out, in] or a stack [count, out, in] in e4m3 with a scale for each block of 128 x 128
     (``rfxq_f8_weight``), as checkpoints hold them; scales f32 [(count,) ceil(out / 128), ceil(in / 128)].
-    Both contiguous, on one GPU; no copy: the weight reads the tensors' memory."""
+    Both contiguous, on one GPU; no copy: calls read the memory that the tensors have now (which may not be resized or
+    set anew)."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype not in _F8_TYPES or codes.dim() not in (2, 3) or not codes.is_contiguous():
