@@ -176,19 +176,21 @@ constexpr F8Variant kF8AnyHalf[] = {{0, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.2f, 0.
 constexpr F8Variant kF8AnyF32[] = {{1, RFXQ_F8_ANY, 32, 64, 512, 3.5f, 1.2f, 0.45f, false},
                                    {4, RFXQ_F8_ANY, 64, 128, 512, 0, 7.1f, 0.97f, true}};
 
+// rows of tiles: grouped rows end inside a tile, half a tile on average
+double f8_tile_rows(uint32_t rows, uint32_t groups, bool grouped, uint32_t bm) {
+    const double used = std::min(rows, groups);
+    return grouped ? used * std::max(1.0, rows / used / bm + 0.5) : std::ceil((double)rows / bm);
+}
+
 // `copies`: rows start at 16 bytes and offsets fit 32 bits
 F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32,
                      bool copies) {
-    const uint32_t used = std::min(rows, groups);
-    const double mean = (double)rows / used;
     const F8Variant* best = nullptr;
     double least = 0;
     const auto look = [&](const F8Variant& v) {
         const bool one = v.kernel == RFXQ_F8_STREAM && v.whole;  // for one matrix
         if (one && grouped) return;
-        // grouped rows end inside a tile, half a tile on average
-        const double tm = grouped ? used * std::max(1.0, mean / v.bm + 0.5) : std::ceil((double)rows / v.bm);
-        double rounds = tm * std::ceil((double)n / v.bn) / cus;
+        double rounds = f8_tile_rows(rows, groups, grouped, v.bm) * std::ceil((double)n / v.bn) / cus;
         rounds = v.whole ? std::ceil(rounds) : std::max(rounds, 1.0);
         if (v.bm == 16u && v.bn == 64u && rounds < 1.5) return;  // four waves: measured where they are many
         // the weights' bytes bound: tiles of 16 rows have more of them in flight
@@ -207,7 +209,7 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
         else
             for (const F8Variant& v : kF8Half) look(v);
     } else {
-        look(kF8Few[mean > 1.0 ? 1 : 0]);
+        look(kF8Few[rows > std::min(rows, groups) ? 1 : 0]);
         if (f32)
             for (const F8Variant& v : kF8AnyF32) look(v);
         else
@@ -262,15 +264,17 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
-    // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles
-    // (4096 x 4096 x 14336: 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x
-    // 14336: three 64 us, four 83); a group's rows are few tiles, most often at most three (4096 tokens
-    // over 8 of 128 experts, 2048 x 768: 91 us, of four 104, of one 100). The others two (64 x 4096 x
-    // 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531: 10.8, 10.7, 11.8).
+    // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles (4096 x 4096 x 14336:
+    // 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64
+    // us, four 83); grouped ones of as many as a group has, up to three (4096 tokens over 8 of 128 experts, 2048 x 768:
+    // 91 us, of four 104, of one 100; 128 tokens over 2 of 8, 4096 x 4096, f32 results: of one 42, of three 53). The
+    // others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531 the same).
     const uint32_t across = (a.tiles_n + 3u) / 4u;
     a.sn = (a.tiles_n + across - 1u) / across;
+    const double tiles = f8_tile_rows(rows, groups, offsets != nullptr, v.bm) / std::min(rows, groups);
+    const uint32_t most = std::min(!v.whole ? 2u : offsets ? 3u : 4u, offsets ? (uint32_t)std::min(std::ceil(tiles), 3.0) : 4u);
     uint64_t least = ~0ull;
-    for (uint32_t s = std::min(a.tiles_m, !v.whole ? 2u : offsets ? 3u : 4u); s; s--) {
+    for (uint32_t s = std::min(most, a.tiles_m); s; s--) {
         const uint64_t each = ((uint64_t)((a.tiles_m + s - 1u) / s) * across + 7u) / 8u * s * a.sn;
         const uint64_t take = v.whole ? (each * 8u + (uint32_t)c->cus - 1u) / (uint32_t)c->cus : each;
         if (take < least) {
