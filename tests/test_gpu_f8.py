@@ -851,6 +851,37 @@ def test_two_streams_at_once(rq):
         assert all(torch.equal(t, want[i]) for t in got[i])
 
 
+def test_threads(rq):
+    """Calls of four host threads at once, a stream each."""
+    import threading
+
+    sizes = [(1, 1024, 640), (40, 2048, 512), (130, 1536, 1024), (300, 645, 333)]
+    cases = [tuple(t.to(DEV) for t in _case(rows, k, n, rows)) for rows, k, n in sizes]
+    values = [torch.randn(rows, k, generator=_gen(rows)).to(DEV) for rows, k, _ in sizes]
+    want = [(rq.gemm_f8(rq.F8Rows(x, xs), rq.F8Weight(w, ws)), rq.quantize_f8(v)) for (x, xs, w, ws), v in zip(cases, values)]
+    torch.cuda.synchronize()
+    right = []
+
+    def work(i):
+        (x, xs, w, ws), (y, q) = cases[i], want[i]
+        rows, weight = rq.F8Rows(x, xs), rq.F8Weight(w, ws)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got, codes = rq.gemm_f8(rows, weight), rq.quantize_f8(values[i])
+                torch.cuda.current_stream().synchronize()
+                if (torch.equal(got, y) and torch.equal(codes.codes.view(torch.uint8), q.codes.view(torch.uint8))
+                        and torch.equal(codes.scales, q.scales)):
+                    right.append(i)
+
+    _say("threads")
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(right) == 20 * len(sizes)
+
+
 @pytest.mark.parametrize("rows,k,n", [(1, 4096, 4096), (30, 2048, 1024), (100, 4096, 512), (700, 1024, 1024), (1500, 2048, 2048)])
 def test_same_results_every_time(rq, rows, k, n):
     x, xs, w, ws = _case(rows, k, n, 2)
