@@ -3,6 +3,7 @@
 // produces them: plain rows, SiLU(gate) * up, and the RMS norm with the residual's
 // addition. Of a group's 128 values v
 //   amax = max |v|,  scale = max(amax, 448 * 2^-120) / 448,  code = RN_e4m3(v / scale)
+// with both quotients rounded to f32 (SiLU's second one within 2^-22).
 // A group with a value that is not finite has NaN for its scale. The smallest scale
 // keeps 1 / scale an f32 value; groups of zeros have it.
 //
@@ -10,7 +11,7 @@
 // group's codes one 128-byte line. All three kernels are bound by memory: each input
 // is read once, each output written once (a large copy runs at 4.87 TB/s, reads and writes
 // together; few rows cost what a launch does: an empty one 1.7 us in a graph).
-//   quantize  4096 x 4096 bf16    10.2 us, 5.0 TB/s;  1 x 4096: 1.8 us
+//   quantize  4096 x 4096 bf16    10.3 us, 4.9 TB/s;  1 x 4096: 1.8 us
 //   SiLU      4096 x 14336 bf16   51.6 us, 5.7 TB/s;  256 x 768: 2.2 us
 //   norm      4096 x 4096 bf16    20.1 us, 5.9 TB/s;  1 x 4096: 2.5 us, 32 x 4096 f32: 2.9 us
 #pragma once
@@ -35,25 +36,59 @@ struct F8RowsArgs {
     uint32_t by_rows, by_groups;  // the launch's groups, in rows and groups (quantize, SiLU)
 };
 
+// v / s rounded once, for 8 values and the group's scale s, as f32 division has it, where that changes a code
+// (SiLU's v are within 2^-20 themselves and do with a reciprocal). Two operations a value, where division takes
+// eleven and another reciprocal (4096 x 4096 bf16 10.3 us, by division 13.0, by one reciprocal 9.95; the norm 25.1, 26.4,
+// 25.1; SiLU of 4096 x 14336 bf16 would take 60 and 69 for 55):
+//   near + rest is 1 / s to 2^-44 of it, near below it so that rest >= 0 keeps the sign of zeros;
+//   RN(v near + v rest) is RN(v / s), unless a midpoint of two f32 values lies within 2^-44 of v / s.
+// A code depends on that only where RN may or may not give a midpoint m of two codes: at m + h / 2 and m - h / 2, with h f32's
+// step there (below a power of two m - h / 4). m has 5 bits, so that v and m s are multiples of h s0 / 16, s0 the power of two
+// below s, and v comes that near to (m +- h / 2) s only if 8 s / s0 is next to a whole number: less than 26 of its steps away,
+// and not on it, since a quotient is no midpoint. Such scales take the division itself, and so do large ones, whose
+// `rest` has no bits left. Groups that are not `fine` have zeros, and NaN of what is not finite (s is NaN or finite there).
+RFXQ_DEV void over_scale(const float (&v)[8], float s, bool fine, float (&q)[8]) {
+    const uint32_t off = __builtin_bit_cast(uint32_t, s) & 0xFFFFFu;
+    if (min(off - 1u, 0x100000u - off) < 64u || s > 0x1p96f) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) q[i] = v[i] / s;
+    } else {
+        const float r = __builtin_amdgcn_rcpf(s), up = __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r);
+        const float below = as_f32(__builtin_bit_cast(uint32_t, up) - 1u), e = __builtin_fmaf(-s, below, 1.0f);
+        const float near = fine ? below : 0.0f, rest = fine ? below * __builtin_fmaf(e, e, e) : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) q[i] = __builtin_fmaf(v[i], near, v[i] * rest);
+    }
+}
+
 // 8 values starting at v of the group that the 16 lanes of this DPP row hold, as codes
 // and the group's scale.
+template <bool EXACT>
 RFXQ_DEV u2_t to_f8(const float (&v)[8], float& scale) {
     uint32_t top = 0;
 #pragma unroll
     for (uint32_t i = 0; i < 8u; i++) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
     top = top_over_8(top);
     top = max(top, RFXQ_DPP_U32(top, 0x140));
-    scale = fmaxf(as_f32(top) * (1.0f / kF8Top), kF8Least);
-    float inv = __builtin_amdgcn_rcpf(scale);
-    if (top >= kInfBits) {
-        scale = __builtin_nanf("");
-        inv = 0.0f;
+    // amax / 448 rounded once: a product, and over 448 what it left. A quotient by 7 lies a fourteenth of a step or
+    // more from any midpoint, the error before the last rounding is far less.
+    const bool fine = top < kInfBits;
+    const float amax = fmaxf(as_f32(top), kF8Top * kF8Least), s0 = amax * (1.0f / kF8Top);
+    const float s = __builtin_fmaf(__builtin_fmaf(-kF8Top, s0, amax), 1.0f / kF8Top, s0);
+    scale = fine ? s : __builtin_nanf("");
+    float q[8];
+    if constexpr (EXACT) {
+        over_scale(v, s, fine, q);
+    } else {
+        const float r = fine ? __builtin_amdgcn_rcpf(s) : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) q[i] = v[i] * r;
     }
     u2_t codes;
 #pragma unroll
     for (uint32_t i = 0; i < 2u; i++) {
-        int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, 0, false);
-        codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, c, true);
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+        codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], c, true);
     }
     return codes;
 }
@@ -121,7 +156,7 @@ RFXQ_DEV void f8_rows(const F8RowsArgs& a) {
 #pragma unroll
             for (uint32_t j = 0; j < 8u; j++) v[j] = x.at(j);
         }
-        const u2_t codes = to_f8(v, scale);
+        const u2_t codes = to_f8<!SILU>(v, scale);
         st_codes(a.out + (uint64_t)row * a.ldo + k, codes, have);
         if (c == 0) stf(a.scales + (uint64_t)row * a.lds + group, scale);
         group += a.by_groups;
@@ -192,7 +227,7 @@ RFXQ_DEV void f8_norm(const F8RowsArgs& a) {
 #pragma unroll
             for (uint32_t j = 0; j < 8u; j++) y[j] = v[j] * rinv * w.at(j);
             if (a.y) st_eight(static_cast<T*>(a.y) + (uint64_t)row * a.ldy + k, y, have);
-            const u2_t codes = to_f8(y, scale);
+            const u2_t codes = to_f8<true>(y, scale);
             st_codes(a.out + (uint64_t)row * a.ldo + k, codes, have);
             if ((tid & 15u) == 0 && have) stf(a.scales + (uint64_t)row * a.lds + k / kF8Block, scale);
         };

@@ -214,6 +214,65 @@ def test_groups_of_every_size(rq):
     assert (got.codes[:3].cpu().float() == 0).all()
 
 
+def _quantized(x):
+    """Codes and scales of [rows, k] values by f32 divisions, on the CPU; scale NaN where a group is not finite."""
+    rows, k = x.shape
+    v = torch.nn.functional.pad(x.float(), (0, _blocks(k) * 128 - k)).view(rows, _blocks(k), 128).numpy()
+    with np.errstate(invalid="ignore"):
+        scales = np.maximum(np.abs(v).max(2), np.float32(448 * LEAST)) / np.float32(448)
+        codes = torch.from_numpy(v / scales[:, :, None]).to(F8).view(torch.uint8).view(rows, -1)[:, :k]
+    return codes, torch.from_numpy(np.where(np.isfinite(scales), scales, np.float32("nan")))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k", [(1, 4096), (777, 1235), (400, 2048), (3, 129)])
+def test_quantize_by_division(rq, rows, k, dtype):
+    """Scales and codes are those of f32 divisions to the last bit, ties included (8-bit values meet many)."""
+    _say("by division", rows, k, dtype)
+    g = _gen(rows + k)
+    whole = torch.randint(-448, 449, (rows, k), generator=g).float() * torch.exp2(torch.randint(-5, 3, (rows, 1), generator=g))
+    for x in (_values(rows, k, dtype, rows, 1.0), whole.to(dtype)):
+        codes, scales = _quantized(x)
+        got = rq.quantize_f8(x.to(DEV))
+        assert torch.equal(got.scales.cpu(), scales)
+        assert torch.equal(got.codes.view(torch.uint8).cpu(), codes)
+
+
+@pytest.mark.parametrize("exponent", [-120, -119, -70, 0, 60, 95, 96, 97, 110])
+def test_quantize_next_to_ties(rq, exponent):
+    """Values within some steps of a midpoint of two codes, scales within some steps of eighths of a power of two and
+    anywhere: the codes of f32 quotients, rounded twice as those are."""
+    _say("ties", exponent)
+    r = np.random.default_rng(exponent + 200)
+    groups = 12000
+    near = 0x100000 * r.integers(0, 8, groups) + r.integers(-130, 131, groups)
+    s = np.where(r.random(groups) < 0.8, near % (1 << 23), r.integers(0, 1 << 23, groups)).astype(np.uint32)
+    s = (s + np.uint32((127 + exponent) << 23)).view(np.float32)
+    x = np.empty((groups, 128), np.float32)
+    x[:, 0] = (s.astype(np.float64) * 448).astype(np.float32)
+    s = x[:, 0] / np.float32(448)
+    tie = r.integers(16, 32, (groups, 127)) * np.exp2(r.integers(-10, 5, (groups, 127)))  # 1/64 .. 496
+    tie = np.where(r.random(tie.shape) < 0.1, r.integers(0, 17, tie.shape) * 2.0 ** -10, np.minimum(tie, 432))
+    v = (tie * s[:, None].astype(np.float64)).astype(np.float32)
+    v = (v.view(np.int32) + np.where(v > 0, r.integers(-3, 4, v.shape), 0).astype(np.int32)).view(np.float32)
+    x[:, 1:] = np.where(r.random(v.shape) < 0.5, v, -v)
+    x = torch.from_numpy(x)
+    codes, scales = _quantized(x)
+    got = rq.quantize_f8(x.to(DEV))
+    assert torch.equal(got.scales.cpu(), scales)
+    wrong = got.codes.view(torch.uint8).cpu() != codes
+    assert not wrong.any(), (int(wrong.sum()), wrong.nonzero()[:5].tolist())
+
+
+@pytest.mark.parametrize("k", [128, 1000, 9000, 33001])
+def test_norm_is_quantized_like_rows(rq, k):
+    """The norm's codes and scales are those of its f32 result."""
+    x = _values(20, k, F32, k, 1.0)
+    out, _, y = rq.add_rmsnorm_f8(x.to(DEV), None, torch.rand(k, generator=_gen(1)).to(DEV), 1e-6, want_y=True)
+    codes, scales = _quantized(y.cpu())
+    assert torch.equal(out.scales.cpu(), scales) and torch.equal(out.codes.view(torch.uint8).cpu(), codes)
+
+
 def test_silu_at_the_ends(rq):
     """Gates from -inf to inf; below -87 the result is 0."""
     gate = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 20.0, -20.0, 80.0, -80.0, -86.0, 1e4, 3e38, 1.0, -1.0, 0.5, -40.0, 60.0])
