@@ -163,7 +163,9 @@ SIGNATURES = {
     "rfxq_silu_and_mul_f8": (_I, [_RP, _RP, _U32, _F8R, _P]),
     "rfxq_add_rmsnorm_f8": (_I, [_RP, _RP, _P, _U32, ctypes.c_float, _RP, _F8R, _RP, _P]),
     "rfxq_gemm_f8": (_I, [_F8R, _F8W, _RP, _P]),
+    "rfxq_gemm_f8_exact": (_I, [_F8R, _F8W, _RP, _P]),
     "rfxq_grouped_gemm_f8": (_I, [_F8R, _F8W, _P, _U32, _P, _U32, _P, _RP, _P]),
+    "rfxq_grouped_gemm_f8_exact": (_I, [_F8R, _F8W, _P, _U32, _P, _U32, _P, _RP, _P]),
     "rfxq_gemm_f8_policy": (_I, [_F8R, _F8W, _U32, _I, _U32, ctypes.POINTER(RfxqF8Policy)]),
 }
 

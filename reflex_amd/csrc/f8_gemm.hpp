@@ -14,7 +14,7 @@
 //                 normal values, under either.
 //   f32 results   the codes are widened to f16, which holds all of them, and multiplied by
 //                 v_mfma_f32_16x16x32_f16: products exact, sums f32, at half the rate.
-// Kernels that memory bounds (few rows) use the second for all.
+// Kernels that memory bounds (few rows) use the second for all, and the exact entry points only it.
 //
 // Both operands lie in memory with K along their rows. Which of the 128 values a lane
 // brings does not matter as long as both operands agree: a lane takes 16 bytes of

@@ -182,8 +182,8 @@ double f8_tile_rows(uint32_t rows, uint32_t groups, bool grouped, uint32_t bm) {
     return grouped ? used * std::max(1.0, rows / used / bm + 0.5) : std::ceil((double)rows / bm);
 }
 
-// `copies`: rows start at 16 bytes and offsets fit 32 bits
-F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool f32,
+// `exact`: exact products (f32 results have them); `copies`: rows start at 16 bytes and offsets fit 32 bits
+F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped, uint32_t k, uint32_t n, bool exact,
                      bool copies) {
     const F8Variant* best = nullptr;
     double least = 0;
@@ -204,13 +204,13 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     };
     if (copies) {
         for (const F8Variant& v : kF8Stream) look(v);
-        if (f32)
+        if (exact)
             for (const F8Variant& v : kF8F32) look(v);
         else
             for (const F8Variant& v : kF8Half) look(v);
     } else {
         look(kF8Few[rows > std::min(rows, groups) ? 1 : 0]);
-        if (f32)
+        if (exact)
             for (const F8Variant& v : kF8AnyF32) look(v);
         else
             for (const F8Variant& v : kF8AnyHalf) look(v);
@@ -218,17 +218,17 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     return *best;
 }
 // the kernel for `rows` (> 0) places of checked x and w
-F8Variant f8_variant(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped, bool f32) {
+F8Variant f8_variant(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped, bool exact) {
     const uint32_t k = w->in_features, n = w->out_features;
     const bool copies = aligned16(x->data) && x->stride % 16u == 0 && aligned16(w->data) && k % 16u == 0 &&
                         codes_of(x, k, "").bytes < kMaxOffset && scales_of(x, k, "").bytes < kMaxOffset &&
                         (uint64_t)k * n < kMaxOffset;
-    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, grouped, k, n, f32, copies);
+    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, grouped, k, n, exact, copies);
 }
 
 int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
-               const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, hipStream_t stream,
-               const char* what) {
+               const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, bool exact,
+               hipStream_t stream, const char* what) {
     const uint32_t k = w->in_features, n = w->out_features, groups = std::max(w->expert_count, 1u);
     const Span sy = span_of(y, n, "y");
     const Span inputs[] = {codes_of(x, k, "x"), scales_of(x, k, "x's scales"), {w->data, (uint64_t)groups * k * n, "weight"},
@@ -260,7 +260,7 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     a.n = n;
     a.groups = groups;
     a.y_type = float_index(y->type);
-    const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, a.y_type == 0);
+    const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, exact || a.y_type == 0);
     a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
     a.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
@@ -288,6 +288,34 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
         return fail(RFXQ_ERR_OTHER, "%s: %u rows x %u columns need %llu workgroups", what, rows, n, (unsigned long long)grid);
     return launch(c->f8.product[v.product][offsets ? 1 : 0], (uint32_t)grid, 0, stream, &a, sizeof a,
                   "rfxq_f8 product launch", v.threads);
+}
+
+int f8_gemm(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, bool exact, hipStream_t stream,
+            const char* what) {
+    if (int rc = check_f8_weight(w, what)) return rc;
+    if (w->expert_count > 1u)
+        return fail(RFXQ_ERR_OTHER, "%s: a stack of %u matrices (rfxq_grouped_gemm_f8 takes stacks)", what, w->expert_count);
+    if (int rc = check_f8_rows(x, w->in_features, what, "x")) return rc;
+    if (int rc = check_rows(y, w->out_features, what, "y")) return rc;
+    if (x->rows != y->rows) return fail(RFXQ_ERR_OTHER, "%s: %u rows of x, %u of y", what, x->rows, y->rows);
+    if (x->rows == 0) return ok();
+    if (int rc = f8_product(x, w, nullptr, x->rows, nullptr, 1, nullptr, y, exact, stream, what)) return rc;
+    return ok();
+}
+
+int f8_grouped(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
+               const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y, bool exact,
+               hipStream_t stream, const char* what) {
+    if (int rc = check_f8_weight(w, what)) return rc;
+    if (int rc = check_f8_rows(x, w->in_features, what, "x")) return rc;
+    if (int rc = check_rows(y, w->out_features, what, "y")) return rc;
+    if (rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "%s: rows=%u", what, rows);
+    if (x_div == 0) return fail(RFXQ_ERR_INVALID_INPUT, "%s: x_div=0", what);
+    if (!x_index && x_div != 1) return fail(RFXQ_ERR_INVALID_INPUT, "%s: x_div=%u without x_index", what, x_div);
+    if (rows == 0 || x->rows == 0 || y->rows == 0) return ok();
+    if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "%s: offsets is NULL", what);
+    if (int rc = f8_product(x, w, offsets, rows, x_index, x_div, y_index, y, exact, stream, what)) return rc;
+    return ok();
 }
 
 }  // namespace
@@ -405,32 +433,23 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
 }
 
 int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream) {
-    if (int rc = check_f8_weight(w, "gemm_f8")) return rc;
-    if (w->expert_count > 1u)
-        return fail(RFXQ_ERR_OTHER, "gemm_f8: a stack of %u matrices (rfxq_grouped_gemm_f8 takes stacks)", w->expert_count);
-    const uint32_t k = w->in_features, n = w->out_features;
-    if (int rc = check_f8_rows(x, k, "gemm_f8", "x")) return rc;
-    if (int rc = check_rows(y, n, "gemm_f8", "y")) return rc;
-    if (x->rows != y->rows) return fail(RFXQ_ERR_OTHER, "gemm_f8: %u rows of x, %u of y", x->rows, y->rows);
-    if (x->rows == 0) return ok();
-    if (int rc = f8_product(x, w, nullptr, x->rows, nullptr, 1, nullptr, y, stream, "gemm_f8")) return rc;
-    return ok();
+    return f8_gemm(x, w, y, false, stream, "gemm_f8");
+}
+
+int rfxq_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream) {
+    return f8_gemm(x, w, y, true, stream, "gemm_f8_exact");
 }
 
 int rfxq_grouped_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
                          const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
                          hipStream_t stream) {
-    if (int rc = check_f8_weight(w, "grouped_gemm_f8")) return rc;
-    const uint32_t k = w->in_features, n = w->out_features;
-    if (int rc = check_f8_rows(x, k, "grouped_gemm_f8", "x")) return rc;
-    if (int rc = check_rows(y, n, "grouped_gemm_f8", "y")) return rc;
-    if (rows > 0x7FFFFFFFu) return fail(RFXQ_ERR_OTHER, "grouped_gemm_f8: rows=%u", rows);
-    if (x_div == 0) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: x_div=0");
-    if (!x_index && x_div != 1) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: x_div=%u without x_index", x_div);
-    if (rows == 0 || x->rows == 0 || y->rows == 0) return ok();
-    if (!offsets) return fail(RFXQ_ERR_INVALID_INPUT, "grouped_gemm_f8: offsets is NULL");
-    if (int rc = f8_product(x, w, offsets, rows, x_index, x_div, y_index, y, stream, "grouped_gemm_f8")) return rc;
-    return ok();
+    return f8_grouped(x, w, offsets, rows, x_index, x_div, y_index, y, false, stream, "grouped_gemm_f8");
+}
+
+int rfxq_grouped_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
+                               const int32_t* x_index, uint32_t x_div, const int32_t* y_index, const rfxq_rows* y,
+                               hipStream_t stream) {
+    return f8_grouped(x, w, offsets, rows, x_index, x_div, y_index, y, true, stream, "grouped_gemm_f8_exact");
 }
 
 int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,

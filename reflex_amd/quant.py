@@ -926,23 +926,26 @@ def _f8_weight(w: F8Weight, dev: int, what: str) -> RfxqF8Weight:
     return w._c
 
 
-def gemm_f8(x: F8Rows, w: F8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+def gemm_f8(x: F8Rows, w: F8Weight, out: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
+            exact: bool = False) -> torch.Tensor:
     """``gemm`` of e4m3 rows with an e4m3 matrix, both with their scales: [rows, out] in ``out``'s type (f32, f16 or
-    bf16; without ``out`` a new tensor of ``dtype``)."""
+    bf16; without ``out`` a new tensor of ``dtype``). f16 and bf16 results may have products cut to 2^-13 of the largest of
+    eight neighbours (1.5e-5 of a result); ``exact``: they are f32 results rounded once, many rows at up to twice the time."""
     dev = _f8_dev(x._dev, x._codes, "gemm_f8: x")
     c = _f8_weight(w, dev, "gemm_f8")
     xr = _f8_rows(x, x._rows, w.in_features, dev, "gemm_f8 x")
     if out is None:
         out = torch.empty(x._rows, w.out_features, dtype=dtype, device=x._codes.device)
-    _f8_call(lib().rfxq_gemm_f8, dev, xr, c, _rows(out, w.out_features, dev, "gemm_f8 out"))
+    fn = lib().rfxq_gemm_f8_exact if exact else lib().rfxq_gemm_f8
+    _f8_call(fn, dev, xr, c, _rows(out, w.out_features, dev, "gemm_f8 out"))
     return out
 
 
 def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_index: torch.Tensor | None = None,
                     x_div: int = 1, y_index: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                    dtype: torch.dtype = torch.float32) -> torch.Tensor:
+                    dtype: torch.dtype = torch.float32, exact: bool = False) -> torch.Tensor:
     """``grouped_gemm`` of e4m3 rows with an e4m3 stack, both with their scales. Without ``out``, a new tensor of
-    ``dtype`` with ``rows`` rows, zero where no place of a group writes."""
+    ``dtype`` with ``rows`` rows, zero where no place of a group writes. ``exact``: as ``gemm_f8`` has it."""
     dev = _f8_dev(x._dev, x._codes, "grouped_gemm_f8: x")
     c = _f8_weight(w, dev, "grouped_gemm_f8")
     _count(rows, 0, "grouped_gemm_f8: rows")
@@ -950,7 +953,8 @@ def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_
     xr = _f8_rows(x, x._rows, w.in_features, dev, "grouped_gemm_f8 x")
     if out is None:
         out = torch.zeros(rows, w.out_features, dtype=dtype, device=x._codes.device)
-    _f8_call(lib().rfxq_grouped_gemm_f8, dev, xr, c,
+    fn = lib().rfxq_grouped_gemm_f8_exact if exact else lib().rfxq_grouped_gemm_f8
+    _f8_call(fn, dev, xr, c,
              _ints(offsets, (w.count or 1) + 1, dev, "grouped_gemm_f8 offsets"), rows,
              _ints(x_index, rows, dev, "grouped_gemm_f8 x_index"), x_div,
              _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), _rows(out, w.out_features, dev, "grouped_gemm_f8 out"))

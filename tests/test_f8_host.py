@@ -174,6 +174,19 @@ def test_grouped_refusals(L, change, code, text):
     _expect(L, _grouped(L, **change), code, text)
 
 
+@pytest.mark.parametrize("change,code,text", PRODUCT + [({"w": {"e": 2}}, 12, "stack of 2"), ({"y": {"rows": 9}}, 12, "9 of y")])
+def test_exact_refusals(L, change, code, text):
+    """The exact forms refuse what the others do."""
+    a = {"x": {}, "w": {}, "y": {}, **change}
+    _expect(L, L.rfxq_gemm_f8_exact(_ref(_f8, a["x"]), _ref(_weight, a["w"]), _ref(_rows, a["y"]), None), code, text)
+    assert L.rfxq_last_error().decode().startswith("gemm_f8_exact: ")
+    if "e" in (a["w"] or {}) or "rows" in (a["y"] or {}):
+        return
+    rc = L.rfxq_grouped_gemm_f8_exact(_ref(_f8, a["x"]), _ref(_weight, a["w"]), 8 * P, 8, None, 1, None, _ref(_rows, a["y"]), None)
+    _expect(L, rc, code, text)
+    assert L.rfxq_last_error().decode().startswith("grouped_gemm_f8_exact: ")
+
+
 @pytest.mark.parametrize("empty", [{"rows": 0}, {"x": {"rows": 0, "data": None, "scales": None}},
                                    {"y": {"rows": 0, "data": None}}])
 def test_products_of_nothing(L, empty):

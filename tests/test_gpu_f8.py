@@ -584,6 +584,39 @@ def test_gemm_each_kernel(rq, rows, k, n, y_type, kernel):
     assert (y == 7.0).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows,k,n,kernel", [(r, k, n, p) for r, k, n, t, p in EACH if t == F32] + [
+    (30, 700, 900, None), (300, 333, 500, None), (60, 8304, 4090, (STREAM, 32, 32)), (2048, 4096, 4096, (COPIED, 128, 128))])
+def test_gemm_exact(rq, rows, k, n, kernel, dtype):
+    """exact: half results are f32 results rounded once, to the last bit, in every kernel that has them."""
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, k, n, rows + k))
+    xr, weight = rq.F8Rows(x, xs), rq.F8Weight(w, ws)
+    _say("exact", rows, k, n, kernel, dtype)
+    assert kernel is None or _kernel(rq, xr, weight, rows, 0, F32) == kernel
+    want = rq.gemm_f8(xr, weight)
+    assert torch.equal(rq.gemm_f8(xr, weight, dtype=dtype, exact=True), want.to(dtype))
+    assert torch.equal(rq.gemm_f8(xr, weight, exact=True), want)
+    y = torch.full((rows + 2, n + 3), 7.0, dtype=dtype, device=DEV)
+    assert rq.gemm_f8(xr, weight, out=y[1:rows + 1, :n], exact=True).data_ptr() == y[1:].data_ptr()
+    assert torch.equal(y[1:rows + 1, :n], want.to(dtype))
+    y[1:rows + 1, :n] = 7.0
+    assert (y == 7.0).all()
+
+
+def test_gemm_exact_keeps_small_products(rq):
+    """Products below 2^-13 of their neighbours add up: 7 of them in each eight, in each kernel of many rows."""
+    for rows, n in ((100, 1024), (200, 4090), (400, 3100), (1000, 4000), (2048, 4000)):
+        k = 1024
+        x = torch.full((rows, k), 0.5)
+        x[:, ::8] = 256.0
+        w = torch.full((n, k), 2.0 ** -6)
+        w[:, ::8] = 1.0
+        w[:, 8::16] = -1.0  # the large ones cancel
+        one, two = torch.ones(rows, _blocks(k), device=DEV), torch.ones(_blocks(n), _blocks(k), device=DEV)
+        y = rq.gemm_f8(rq.F8Rows(x.to(F8).to(DEV), one), rq.F8Weight(w.to(F8).to(DEV), two), dtype=F16, exact=True)
+        assert (y == 7 * 128 * 2.0 ** -7).all()
+
+
 @pytest.mark.parametrize("extra", [0, 16, 112, 128, 129, 240])
 @pytest.mark.parametrize("blocks", range(1, 15))
 @pytest.mark.parametrize("rows,n,y_type", [(2, 40, F32), (40, 300, BF16), (200, 2100, F32), (300, 2050, BF16), (2048, 2050, BF16),
@@ -686,6 +719,19 @@ def test_grouped_each_kernel(rq, pairs, count, k, n, y_type, kernel, side):
     none = torch.arange(int(offsets[-1]), pairs, device=DEV)
     left = torch.cat([none if side == "gate" else order[none], torch.arange(pairs, y.shape[0], device=DEV)])
     assert (y[left] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("pairs,count,k,n", [(100, 3, 384, 520), (300, 7, 768, 520), (3000, 6, 656, 1030), (500, 11, 1235, 531)])
+def test_grouped_exact(rq, pairs, count, k, n, dtype):
+    x, xs, w, ws = (t.to(DEV) for t in _case(pairs, k, n, pairs + k, count))
+    ids = torch.from_numpy(np.random.default_rng(pairs).integers(-1, count + 1, pairs).astype(np.int32))
+    g = rq.group_rows(ids.to(DEV), count)
+    _say("grouped exact", pairs, count, k, n, dtype)
+    args = rq.F8Rows(x, xs), rq.F8Weight(w, ws), g.offsets, pairs
+    want = rq.grouped_gemm_f8(*args, y_index=g.order)
+    got = rq.grouped_gemm_f8(*args, y_index=g.order, dtype=dtype, exact=True)
+    assert got.dtype == dtype and torch.equal(got, want.to(dtype))
 
 
 @pytest.mark.parametrize("rows", [20, 300, 3000])
