@@ -519,8 +519,9 @@ typedef struct rfxq_f8_weight {
 /* out = x [rows][k]. */
 int rfxq_quantize_f8(const rfxq_rows* x, uint32_t k, const rfxq_f8_rows* out, hipStream_t stream);
 
-/* out = gate / (1 + exp(-gate)) * up: Model::silu_and_mul (silu_and_mul.cu:7-23). gate
- * and up may be columns of one matrix. */
+/* out = gate / (1 + exp(-gate)) * up: Model::silu_and_mul (silu_and_mul.cu:7-23), within
+ * 2^-20 over f32's whole range of results: also where exp(-gate) by itself would not be an
+ * f32 value (gates below -88 beside large ups). gate and up may be columns of one matrix. */
 int rfxq_silu_and_mul_f8(const rfxq_rows* gate, const rfxq_rows* up, uint32_t k, const rfxq_f8_rows* out,
                          hipStream_t stream);
 

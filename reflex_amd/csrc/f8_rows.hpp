@@ -126,14 +126,23 @@ RFXQ_DEV void st_eight(T* p, const float (&v)[8], uint32_t have) {
     }
 }
 
-// g / (1 + exp(-g)) * u, by p = exp(-|g|): 1 / (1 + p) or p / (1 + p), which do not overflow.
-// exp by 2^(t + r) with t = RN(-|g| log2 e) and r what the rounding and log2 e's own bits
-// left, so that far values keep f32's bits (below -87 p is under f32's normal range: 0).
+// g / (1 + exp(-g)) * u. exp by 2^(t + r) with t = RN(-g log2 e) and r what the rounding and log2 e's
+// own bits left, so that far values keep f32's bits; no product of it overflows within its bounds, beyond which
+// it is 0 beside 1, or the gate far.
+constexpr float kLog2e = 1.44269504088896340736f, kLog2eRest = 1.92596299112661746887e-8f, kSiluFar = -87.0f;
 RFXQ_DEV float silu_mul(float g, float u) {
-    constexpr float kLog2e = 1.44269504088896340736f, kLog2eRest = 1.92596299112661746887e-8f;
-    const float n = fmaxf(-__builtin_fabsf(g), -128.0f), t = n * kLog2e, r = __builtin_fmaf(n, kLog2e, -t) + n * kLog2eRest;
-    const float e = __builtin_amdgcn_exp2f(t), p = __builtin_fmaf(e, r * 0.69314718055994530942f, e);
-    return g * ((g < 0.0f ? p : 1.0f) * __builtin_amdgcn_rcpf(1.0f + p)) * u;
+    const float n = __builtin_amdgcn_fmed3f(-g, -128.0f, 128.0f), t = n * kLog2e;
+    const float r = __builtin_fmaf(n, kLog2e, -t) + n * kLog2eRest, e = __builtin_amdgcn_exp2f(t);
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e, r * 0.69314718055994530942f, e)) * u;
+}
+// The same for g below kSiluFar, where it is g exp(g) u and exp(g), or exp(-g), may leave f32's range: an ordinary value
+// beside a large u down to g = -197. exp(g) is f 2^i with f near 1, and half of i goes to g, half to the product, so that
+// what counts of neither leaves it (below -256 all of it is 0; 0 g makes NaN of an infinite g).
+RFXQ_DEV float silu_mul_far(float g, float u) {
+    const float n = fmaxf(g, -256.0f), whole = rintf(n * kLog2e);
+    const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(n, kLog2eRest, __builtin_fmaf(n, kLog2e, -whole)));
+    const int i = (int)whole, half = i / 2;
+    return __builtin_fmaf(0.0f, g, ldexpf(ldexpf(n * f, half) * u, i - half));
 }
 
 // Plain rows, and SiLU(gate) * up: a group is 16 lanes' work, whichever row it is of, so that
@@ -152,6 +161,14 @@ RFXQ_DEV void f8_rows(const F8RowsArgs& a) {
             const Eight<T> up = ld_eight(static_cast<const T*>(a.x2) + (uint64_t)row * a.ldx2 + k, have);
 #pragma unroll
             for (uint32_t j = 0; j < 8u; j++) v[j] = silu_mul(x.at(j), up.at(j));
+            float least = x.at(0);
+#pragma unroll
+            for (uint32_t j = 1; j < 8u; j++) least = fminf(least, x.at(j));
+            if (least < kSiluFar) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; j++)
+                    if (x.at(j) < kSiluFar) v[j] = silu_mul_far(x.at(j), up.at(j));
+            }
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < 8u; j++) v[j] = x.at(j);

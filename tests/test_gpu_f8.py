@@ -289,6 +289,40 @@ def test_silu_at_the_ends(rq):
         assert torch.isnan(got.scales).all()
 
 
+def test_silu_of_far_gates(rq):
+    """Gates whose exp(gate) is below f32's normal range, beside large ups: gate exp(gate) up is an ordinary value down
+    to gates of -197 and is kept, each in a group of its own and all in one row."""
+    gate = torch.cat([torch.linspace(-86.5, -88.9, 97), torch.linspace(-89, -200, 223), torch.tensor([-256.0, -257.0, -3e4, -3e38])])
+    for top in (1.0, 1e20, -3e38, 2.0 ** -140):
+        up = torch.full_like(gate, top)
+        v = gate.double() * torch.exp(gate.double()) / (1 + torch.exp(gate.double())) * up.double()
+        v = torch.where(gate < -300, torch.zeros_like(v), v)
+        got = rq.silu_and_mul_f8(gate.view(-1, 1).to(DEV), up.view(-1, 1).to(DEV))
+        codes, scales = got.codes.cpu().float().double()[:, 0], got.scales.cpu().double()[:, 0]
+        # a group of one value: the scale is its size / 448 (2^-22 and SiLU's 2^-20; below 2^-126 a step of 2^-149 more, as
+        # the product and its last factor each round there)
+        size = v.abs().clamp(min=448 * LEAST) / 448
+        assert ((scales - size).abs() <= size * (2.0 ** -22 + 2.0 ** -20)).all()
+        sure = v.abs() >= 448 * LEAST
+        assert (codes[sure] == torch.sign(v[sure]) * 448).all()
+        half = torch.clamp(v.abs() / scales * 2.0 ** -4, min=2.0 ** -10)
+        assert ((codes - v / scales).abs() <= half * (1 + 2.0 ** -10) + v.abs() / scales * 2.0 ** -19).all()
+        _check_codes(*(lambda o: (o.codes, o.scales))(rq.silu_and_mul_f8(gate.view(1, -1).to(DEV), up.view(1, -1).to(DEV))),
+                     v.view(1, -1), 2.0 ** -20)
+    for dtype in (F16, BF16):
+        g, u = gate[:300].to(dtype), torch.full((300,), 6e4).to(dtype)
+        v = g.double() * torch.exp(g.double()) / (1 + torch.exp(g.double())) * u.double()
+        got = rq.silu_and_mul_f8(g.view(1, -1).to(DEV), u.view(1, -1).to(DEV))
+        _check_codes(got.codes, got.scales, v.view(1, -1), 2.0 ** -20)
+    mixed = torch.randn(40, 700, generator=_gen(8)) * 60  # near and far ones side by side
+    ups = torch.randn(40, 700, generator=_gen(9)) * 1e30
+    got = rq.silu_and_mul_f8(mixed.to(DEV), ups.to(DEV))
+    m = mixed.double()
+    _check_codes(got.codes, got.scales, m * torch.sigmoid(m) * ups.double(), 2.0 ** -20)
+    got = rq.silu_and_mul_f8(torch.tensor([[-200.0, -math.inf]], device=DEV), torch.ones(1, 2, device=DEV))
+    assert torch.isnan(got.scales).all()
+
+
 @pytest.mark.parametrize("k", [128, 4096, 40000])
 def test_norm_of_odd_rows(rq, k):
     """Rows of zeros, of huge and of tiny values, a row that is not finite: the others keep their results."""
