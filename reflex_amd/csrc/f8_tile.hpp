@@ -19,7 +19,7 @@ RFXQ_DEV void copy16(rsrc_t r, uint32_t lds, uint32_t off, uint32_t by) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(r), "s"(by)
-                 : "memory");
+                 : "memory", "m0");
 }
 // all of the wave's copies but the last N have landed
 template <uint32_t N>

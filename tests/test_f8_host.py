@@ -363,3 +363,21 @@ def test_matrix_results_are_not_read_too_early(tmp_path):
     assert products["f8f6f4"] > 500 and products["32_f16"] > 200 and not early, (products, early[:5])
     # copies that the compiler does not count: nothing that it does count may be spilled beside them
     assert "Folded" not in listing.read_text()
+
+
+def test_registers_that_inline_assembly_writes_are_declared():
+    """The compiler may keep a copy's LDS address in m0 across inline assembly that does not say that it writes there."""
+    import glob
+    import os
+    import re
+
+    from reflex_amd import build
+
+    found = 0
+    for path in sorted(glob.glob(os.path.join(build.CSRC, "*.h*"))):
+        for text in re.findall(r"asm volatile\((.*?)\);", open(path).read(), re.S):
+            if re.search(r"s_mov_b32 (m0|vcc|exec)", text):
+                found += 1
+                register = re.search(r"s_mov_b32 (m0|vcc|exec)", text).group(1)
+                assert f'"{register}"' in text.rsplit(":", 1)[1], (path, text)
+    assert found
