@@ -549,8 +549,8 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
  * codes give NaN, and scales that are not finite results that are not finite, where
  * they belong, and nowhere else. Any sizes, strides and alignment of whole elements
  * (scales and y); rows of x and w that start at multiples of 16 bytes are faster. y must
- * not overlap x or w. One launch, no workspace, no host synchronisation: it can be
- * captured. The order of a sum depends on the call's sizes and alignment, not on
+ * not overlap x or w. One launch (more where it would have 2^32 threads: narrow products of
+ * 100 million rows), no workspace, no host synchronisation: it can be captured. The order of a sum depends on the call's sizes and alignment, not on
  * anything else: equal calls give equal bits. */
 int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream);
 
@@ -584,6 +584,8 @@ int rfxq_grouped_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, c
 typedef struct rfxq_f8_policy {
     uint32_t kernel; /* RFXQ_F8_* */
     uint32_t tile_m, tile_n;
+    uint32_t threads;  /* of a workgroup */
+    uint32_t launches; /* each of fewer than 2^32 threads */
 } rfxq_f8_policy;
 int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
                         rfxq_f8_policy* out);

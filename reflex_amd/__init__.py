@@ -67,7 +67,8 @@ class RfxqF8Weight(ctypes.Structure):
 class RfxqF8Policy(ctypes.Structure):
     """``rfxq_f8_policy`` (include/rfxq.h)."""
 
-    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32)]
+    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32),
+                ("threads", ctypes.c_uint32), ("launches", ctypes.c_uint32)]
 
 
 class RfxqOptions(ctypes.Structure):

@@ -22,7 +22,7 @@ RFXQ_DEV void f8_stream(const F8Args& a) {
     __shared__ float ss[CHUNK][16 * MT];
     static_assert(sizeof ring >= WAVES * MT * NT * 64u * sizeof(f4v_t));
     uint32_t tm, tn;
-    if (!tile_place(a, blockIdx.x, tm, tn)) return;
+    if (!f8_place(a, tm, tn)) return;
     const RowTile t = f8_tile<GROUPED>(a, 16u * MT, tm);
     if (!t.any) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));

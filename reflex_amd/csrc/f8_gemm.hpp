@@ -39,6 +39,7 @@ struct F8Args {
     uint32_t rows, x_rows, y_rows, x_div;
     uint32_t k, n, groups, y_type;  // y_type: 0 f32, 1 f16, 2 bf16
     uint32_t tiles_m, tiles_n, sm, sn;
+    uint32_t first_m, first_n;  // the launch's first tile
 };
 
 constexpr uint32_t kBlock = 128;
@@ -104,6 +105,13 @@ RFXQ_DEV u4_t ld_short(const uint8_t* row, uint32_t k, uint32_t at) {
     return r;
 }
 
+// The tile of this workgroup; false: there is none.
+RFXQ_DEV bool f8_place(const F8Args& a, uint32_t& tm, uint32_t& tn) {
+    const bool there = tile_place(a, blockIdx.x, tm, tn);
+    tm += a.first_m;
+    tn += a.first_n;
+    return there;
+}
 // The rows of a tile: a search among the groups, or counted.
 template <bool GROUPED>
 RFXQ_DEV RowTile f8_tile(const F8Args& a, uint32_t bm, uint32_t tm) {
@@ -170,7 +178,7 @@ RFXQ_DEV void f8_any(const F8Args& a) {
     constexpr uint32_t BM = 32u * MF, BN = 32u * NF, ROWS = 32, NX = BM / ROWS, NW = BN / ROWS;
     __shared__ u4_t xs[2][KG][BM * 8u], ws[2][KG][BN * 8u];
     uint32_t tm, tn;
-    if (!tile_place(a, blockIdx.x, tm, tn)) return;
+    if (!f8_place(a, tm, tn)) return;
     const RowTile t = f8_tile<GROUPED>(a, BM, tm);
     if (!t.any) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), kg = wave >> 2;
@@ -310,7 +318,7 @@ RFXQ_DEV void f8_few(const F8Args& a) {
     constexpr uint32_t D = 2, WK = 8;
     __shared__ f4v_t part[WK][64];
     uint32_t tm, tn;
-    if (!tile_place(a, blockIdx.x, tm, tn)) return;
+    if (!f8_place(a, tm, tn)) return;
     const RowTile t = f8_tile<GROUPED>(a, 16, tm);
     if (!t.any) return;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));

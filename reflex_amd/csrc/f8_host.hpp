@@ -37,8 +37,9 @@ struct F8Args {
     uint32_t rows, x_rows, y_rows, x_div;
     uint32_t k, n, groups, y_type;
     uint32_t tiles_m, tiles_n, sm, sn;
+    uint32_t first_m, first_n;
 };
-static_assert(sizeof(F8Args) == 152, "F8Args layout");
+static_assert(sizeof(F8Args) == 160, "F8Args layout");
 
 uint32_t f8_groups(uint32_t k) { return (k + kF8Block - 1u) / kF8Block; }
 uint32_t float_index(uint32_t ty) { return ty == RFXQ_TYPE_F32 ? 0u : ty == RFXQ_TYPE_F16 ? 1u : 2u; }
@@ -217,13 +218,52 @@ F8Variant f8_variant(uint32_t cus, uint32_t rows, uint32_t groups, bool grouped,
     }
     return *best;
 }
-// the kernel for `rows` (> 0) places of checked x and w
-F8Variant f8_variant(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped, bool exact) {
-    const uint32_t k = w->in_features, n = w->out_features;
+// How a product of `rows` (> 0) places of checked x and w runs: its kernel, its tiles, their blocks for an XCD, and the
+// tiles of a launch.
+struct F8Plan {
+    F8Variant v;
+    uint32_t tiles_m, tiles_n, sm, sn;
+    uint32_t most_m, most_n;
+    uint64_t grid(uint32_t m, uint32_t n) const {  // workgroups for m x n tiles
+        return ((uint64_t)((m + sm - 1u) / sm) * ((n + sn - 1u) / sn) + 7u) / 8u * 8u * sm * sn;
+    }
+};
+F8Plan f8_plan(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, bool grouped, bool exact) {
+    const uint32_t k = w->in_features, n = w->out_features, groups = grouped ? std::max(w->expert_count, 1u) : 1u;
     const bool copies = aligned16(x->data) && x->stride % 16u == 0 && aligned16(w->data) && k % 16u == 0 &&
                         codes_of(x, k, "").bytes < kMaxOffset && scales_of(x, k, "").bytes < kMaxOffset &&
                         (uint64_t)k * n < kMaxOffset;
-    return f8_variant(cus, rows, grouped ? std::max(w->expert_count, 1u) : 1u, grouped, k, n, exact, copies);
+    F8Plan p;
+    const F8Variant v = p.v = f8_variant(cus, rows, groups, grouped, k, n, exact, copies);
+    p.tiles_m = grouped ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
+    p.tiles_n = (n + v.bn - 1u) / v.bn;
+    // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
+    // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles (4096 x 4096 x 14336:
+    // 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64
+    // us, four 83); grouped ones of as many as a group has, up to three (4096 tokens over 8 of 128 experts, 2048 x 768:
+    // 91 us, of four 104, of one 100; 128 tokens over 2 of 8, 4096 x 4096, f32 results: of one 42, of three 53). The
+    // others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531 the same).
+    const uint32_t across = (p.tiles_n + 3u) / 4u;
+    p.sn = (p.tiles_n + across - 1u) / across;
+    const double tiles = f8_tile_rows(rows, groups, grouped, v.bm) / std::min(rows, groups);
+    const uint32_t most = std::min(!v.whole ? 2u : grouped ? 3u : 4u, grouped ? (uint32_t)std::min(std::ceil(tiles), 3.0) : 4u);
+    uint64_t least = ~0ull;
+    for (uint32_t s = std::min(most, p.tiles_m); s; s--) {
+        const uint64_t each = ((uint64_t)((p.tiles_m + s - 1u) / s) * across + 7u) / 8u * s * p.sn;
+        const uint64_t take = v.whole ? (each * 8u + cus - 1u) / cus : each;
+        if (take < least) {
+            least = take;
+            p.sm = s;
+        }
+    }
+    // a launch has fewer than 2^32 threads: 134 million rows of 16 x 16 tiles are two
+    p.most_m = p.tiles_m;
+    p.most_n = p.tiles_n;
+    while (p.grid(p.most_m, p.most_n) * v.threads > 0xFFFFFFFFull) {
+        uint32_t& longer = p.most_m > p.most_n ? p.most_m : p.most_n;
+        longer = (longer + 1u) / 2u;
+    }
+    return p;
 }
 
 int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* offsets, uint32_t rows,
@@ -260,34 +300,19 @@ int f8_product(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     a.n = n;
     a.groups = groups;
     a.y_type = float_index(y->type);
-    const F8Variant v = f8_variant((uint32_t)c->cus, x, w, rows, offsets != nullptr, exact || a.y_type == 0);
-    a.tiles_m = offsets ? max_tiles(rows, groups, v.bm) : (rows + v.bm - 1u) / v.bm;
-    a.tiles_n = (n + v.bn - 1u) / v.bn;
-    // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
-    // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles (4096 x 4096 x 14336:
-    // 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64
-    // us, four 83); grouped ones of as many as a group has, up to three (4096 tokens over 8 of 128 experts, 2048 x 768:
-    // 91 us, of four 104, of one 100; 128 tokens over 2 of 8, 4096 x 4096, f32 results: of one 42, of three 53). The
-    // others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531 the same).
-    const uint32_t across = (a.tiles_n + 3u) / 4u;
-    a.sn = (a.tiles_n + across - 1u) / across;
-    const double tiles = f8_tile_rows(rows, groups, offsets != nullptr, v.bm) / std::min(rows, groups);
-    const uint32_t most = std::min(!v.whole ? 2u : offsets ? 3u : 4u, offsets ? (uint32_t)std::min(std::ceil(tiles), 3.0) : 4u);
-    uint64_t least = ~0ull;
-    for (uint32_t s = std::min(most, a.tiles_m); s; s--) {
-        const uint64_t each = ((uint64_t)((a.tiles_m + s - 1u) / s) * across + 7u) / 8u * s * a.sn;
-        const uint64_t take = v.whole ? (each * 8u + (uint32_t)c->cus - 1u) / (uint32_t)c->cus : each;
-        if (take < least) {
-            least = take;
-            a.sm = s;
+    const F8Plan p = f8_plan((uint32_t)c->cus, x, w, rows, offsets != nullptr, exact || a.y_type == 0);
+    a.sm = p.sm;
+    a.sn = p.sn;
+    for (a.first_m = 0; a.first_m < p.tiles_m; a.first_m += a.tiles_m) {
+        a.tiles_m = std::min(p.most_m, p.tiles_m - a.first_m);
+        for (a.first_n = 0; a.first_n < p.tiles_n; a.first_n += a.tiles_n) {
+            a.tiles_n = std::min(p.most_n, p.tiles_n - a.first_n);
+            if (int rc = launch(c->f8.product[p.v.product][offsets ? 1 : 0], (uint32_t)p.grid(a.tiles_m, a.tiles_n), 0, stream, &a,
+                                sizeof a, "rfxq_f8 product launch", p.v.threads))
+                return rc;
         }
     }
-    const uint64_t blocks = (uint64_t)((a.tiles_m + a.sm - 1u) / a.sm) * ((a.tiles_n + a.sn - 1u) / a.sn);
-    const uint64_t grid = (blocks + 7u) / 8u * 8u * a.sm * a.sn;
-    if (grid * v.threads > 0xFFFFFFFFull)  // a launch's threads
-        return fail(RFXQ_ERR_OTHER, "%s: %u rows x %u columns need %llu workgroups", what, rows, n, (unsigned long long)grid);
-    return launch(c->f8.product[v.product][offsets ? 1 : 0], (uint32_t)grid, 0, stream, &a, sizeof a,
-                  "rfxq_f8 product launch", v.threads);
+    return RFXQ_OK;
 }
 
 int f8_gemm(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, bool exact, hipStream_t stream,
@@ -461,8 +486,9 @@ int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t
         return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: rows=%u of %u", rows, x->rows);
     if (!float_type(y_type)) return fail(RFXQ_ERR_GGUF, "gemm_f8_policy: y of type %u (F32, F16 or BF16)", y_type);
     const Ctx* c = loaded_ctx();
-    const F8Variant v = f8_variant(c ? (uint32_t)c->cus : 256u, x, w, rows, grouped != 0, y_type == RFXQ_TYPE_F32);
-    *out = {v.kernel, v.bm, v.bn};
+    const F8Plan p = f8_plan(c ? (uint32_t)c->cus : 256u, x, w, rows, grouped != 0, y_type == RFXQ_TYPE_F32);
+    const auto times = [](uint32_t all, uint32_t most) { return (all + most - 1u) / most; };
+    *out = {p.v.kernel, p.v.bm, p.v.bn, p.v.threads, times(p.tiles_m, p.most_m) * times(p.tiles_n, p.most_n)};
     return ok();
 }
 

@@ -76,7 +76,7 @@ struct F8Tile {
     // the tile, and where its rows are; false: there is none
     __device__ __forceinline__ bool begin(const F8Args& a) {
         uint32_t tm;
-        if (!tile_place(a, blockIdx.x, tm, tn)) return false;
+        if (!f8_place(a, tm, tn)) return false;
         t = f8_tile<GROUPED>(a, BM, tm);
         if (!t.any) return false;
         lane = threadIdx.x & 63u;

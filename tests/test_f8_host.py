@@ -252,6 +252,26 @@ def test_product_kernel(L, rows, experts, k, n, ty, shift, kernel):
     assert (p.kernel, p.tile_m, p.tile_n) == kernel
 
 
+@pytest.mark.parametrize("rows,experts,k,n,ty", [
+    (4096, 0, 4096, 14336, BF16), (32768, 128, 2048, 768, BF16), (1 << 26, 0, 17, 5, F32), ((1 << 27) + 12345, 0, 17, 5, F16),
+    (1 << 28, 0, 16, 16, F32), ((1 << 31) - 1, 0, 1, 1, F32), (1, 0, 17, (1 << 27) + 77, F32), (1, 0, 1, (1 << 31) - 1, BF16),
+    ((1 << 27) + 999, 3, 17, 5, F16), (1 << 26, 0, 16, 1 << 20, BF16), (1 << 30, 1000, 3, 1 << 20, F32)])
+def test_launches_have_fewer_than_2_32_threads(L, rows, experts, k, n, ty):
+    """Products of any sizes are as many launches as that takes: one where it can be, few more than the threads need
+    (each launch at least a quarter full, tiles of 8 XCDs' blocks left empty at the ends)."""
+    import reflex_amd as rq
+
+    x = rq.RfxqF8Rows(1 << 44, 1 << 45, rows, k, -(-k // 128))
+    w = _weight(k, n, experts, data=1 << 43, scales=1 << 42)
+    p = rq.RfxqF8Policy()
+    assert L.rfxq_gemm_f8_policy(ctypes.byref(x), ctypes.byref(w), rows, 1 if experts else 0, ty, ctypes.byref(p)) == 0
+    assert p.threads in (256, 512)
+    threads = -(-rows // p.tile_m) * -(-n // p.tile_n) * p.threads
+    if threads < 1 << 31:
+        assert p.launches == 1
+    assert threads / ((1 << 32) - 1) <= p.launches <= max(1, threads / (1 << 29))
+
+
 def test_python_checks():
     import reflex_amd as rq
 

@@ -553,6 +553,79 @@ def test_gemm_many_rows(rq, k, n):
     assert torch.equal(y, (x.float() @ w.float().t()) * xs)  # whole numbers times powers of two
 
 
+def _whole(rows, k, seed):
+    """Codes of -1, 0 and 1."""
+    return torch.randint(-1, 2, (rows, k), generator=torch.Generator(DEV).manual_seed(seed), device=DEV).float().to(F8)
+
+
+def _launches(rq, x, w, rows, grouped, y_type):
+    import ctypes
+
+    p = rq.RfxqF8Policy()
+    ty = {F32: 0, F16: 1, BF16: 30}[y_type]
+    assert rq.lib().rfxq_gemm_f8_policy(x._c, w._c, rows, grouped, ty, ctypes.byref(p)) == 0
+    return p.launches
+
+
+PERIOD = (1 << 20) + 77
+
+
+def test_gemm_more_rows_than_a_launch(rq):
+    """A narrow product of more workgroups than a launch takes: every row, the gaps between rows left as they were."""
+    rows, k, n = (1 << 27) + 12345, 17, 5
+    few, w = _whole(PERIOD, k, 1), _whole(n, k, 2)
+    few_scales = torch.exp2(torch.randint(-3, 4, (PERIOD, 1), generator=torch.Generator(DEV).manual_seed(3), device=DEV).float())
+    times = -(-rows // PERIOD)
+    x = rq.F8Rows(few.view(torch.uint8).repeat(times, 1)[:rows].view(F8), few_scales.repeat(times, 1)[:rows])
+    weight = rq.F8Weight(w, torch.ones(1, 1, device=DEV))
+    _say("rows", rows, _launches(rq, x, weight, rows, 0, F16))
+    assert _launches(rq, x, weight, rows, 0, F16) > 1
+    buf = torch.full((rows + 1, n + 1), 7.0, dtype=F16, device=DEV)
+    rq.gemm_f8(x, weight, out=buf[:rows, :n])
+    want = ((few.float() @ w.float().t()) * few_scales).to(F16)  # whole numbers times powers of two
+    for at in range(0, rows, PERIOD):
+        part = buf[at:min(at + PERIOD, rows)]
+        assert torch.equal(part[:, :n], want[:part.shape[0]]), at
+    assert (buf[:, n] == 7.0).all() and (buf[rows] == 7.0).all()
+
+
+def test_gemm_more_columns_than_a_launch(rq):
+    rows, k, n = 1, 17, (1 << 27) + 77
+    x, few = _whole(rows, k, 1), _whole(PERIOD, k, 2)
+    times = -(-n // PERIOD)
+    scales = torch.exp2((torch.arange(_blocks(n), device=DEV) % 7 - 3).float())
+    weight = rq.F8Weight(few.view(torch.uint8).repeat(times, 1)[:n].view(F8), scales.view(-1, 1))
+    xr = rq.F8Rows(x, torch.ones(rows, 1, device=DEV))
+    _say("columns", n, _launches(rq, xr, weight, rows, 0, F32))
+    assert _launches(rq, xr, weight, rows, 0, F32) > 1
+    y = rq.gemm_f8(xr, weight)[0]
+    want = (few.float() @ x[0].float()).repeat(times)[:n] * scales.repeat_interleave(128)[:n]
+    assert torch.equal(y, want)
+
+
+def test_grouped_more_places_than_a_launch(rq):
+    """Places of three groups that name few rows of x, some none."""
+    rows, k, n = (1 << 27) + 999, 17, 5
+    x, w = _whole(PERIOD, k, 1), torch.stack([_whole(n, k, 2 + e) for e in range(3)])
+    offsets = [3, 1000, (1 << 26) + 5, rows - 2]
+    index = torch.arange(rows, dtype=torch.int32, device=DEV) % (PERIOD + 1) - 1  # -1: no row
+    xr, weight = rq.F8Rows(x, torch.ones(PERIOD, 1, device=DEV)), rq.F8Weight(w, torch.ones(3, 1, 1, device=DEV))
+    _say("places", rows, _launches(rq, xr, weight, rows, 1, F16))
+    assert _launches(rq, xr, weight, rows, 1, F16) > 1
+    y = torch.full((rows, n), 7.0, dtype=F16, device=DEV)
+    rq.grouped_gemm_f8(xr, weight, torch.tensor(offsets, dtype=torch.int32, device=DEV), rows, x_index=index, out=y)
+    each = [torch.cat([torch.full((1, n), 7.0, device=DEV), x.float() @ w[e].float().t()]).to(F16) for e in range(3)]
+    step = 1 << 22
+    for at in range(0, rows, step):
+        end = min(at + step, rows)
+        want = torch.full((end - at, n), 7.0, dtype=F16, device=DEV)
+        for e in range(3):
+            lo, hi = max(offsets[e], at), min(offsets[e + 1], end)
+            if lo < hi:
+                want[lo - at:hi - at] = each[e][index[lo:hi].long() + 1]
+        assert torch.equal(y[at:end], want), at
+
+
 def test_more_groups_than_a_launch(rq):
     """More rows than the largest launches have places for."""
     rows = (1 << 24) + 77
