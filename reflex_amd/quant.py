@@ -821,7 +821,9 @@ class F8Weight:
     """A matrix [out, in] or a stack [count, out, in] in e4m3 with a scale for each block of 128 x 128
     (``rfxq_f8_weight``), as checkpoints hold them; scales f32 [(count,) ceil(out / 128), ceil(in / 128)].
     Both contiguous, on one GPU; no copy: calls read the memory that the tensors have now (which may not be resized or
-    set anew)."""
+    set anew; other weights are another F8Weight)."""
+
+    __slots__ = ("_codes", "_scales", "_c", "_dev", "_count", "_out", "_in", "__weakref__")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype not in _F8_TYPES or codes.dim() not in (2, 3) or not codes.is_contiguous():
@@ -832,11 +834,32 @@ class F8Weight:
                 or scales.device != codes.device):
             raise InvalidInputError(11, f"F8Weight: scales {scales.dtype} {list(scales.shape)} on {scales.device} "
                                         f"(contiguous f32 {want} on {codes.device})")
-        self.codes, self.scales, self._dev = codes, scales, codes.get_device()
-        self.count = _count(codes.shape[0], 1, "F8Weight: count") if codes.dim() == 3 else 0
-        self.out_features, self.in_features = (_count(v, 1, "F8Weight: shape") for v in codes.shape[-2:])
-        self._c = RfxqF8Weight(self.in_features, self.out_features, self.count, codes.data_ptr(), scales.data_ptr(),
+        self._codes, self._scales, self._dev = codes, scales, codes.get_device()
+        self._count = _count(codes.shape[0], 1, "F8Weight: count") if codes.dim() == 3 else 0
+        self._out, self._in = (_count(v, 1, "F8Weight: shape") for v in codes.shape[-2:])
+        self._c = RfxqF8Weight(self._in, self._out, self._count, codes.data_ptr(), scales.data_ptr(),
                                codes.numel(), 4 * scales.numel())
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    @property
+    def count(self) -> int:
+        """Matrices of a stack; 0 for one matrix."""
+        return self._count
+
+    @property
+    def out_features(self) -> int:
+        return self._out
+
+    @property
+    def in_features(self) -> int:
+        return self._in
 
 
 # Launches of a few microseconds: the checks compare plain integers that F8Rows and F8Weight keep.
@@ -922,7 +945,7 @@ def add_rmsnorm_f8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch
 
 def _f8_weight(w: F8Weight, dev: int, what: str) -> RfxqF8Weight:
     if w._dev != dev:
-        raise InvalidInputError(11, f"{what}: weight on {w.codes.device}, rows on cuda:{dev}")
+        raise InvalidInputError(11, f"{what}: weight on {w._codes.device}, rows on cuda:{dev}")
     return w._c
 
 
@@ -933,11 +956,11 @@ def gemm_f8(x: F8Rows, w: F8Weight, out: torch.Tensor | None = None, dtype: torc
     eight neighbours (1.5e-5 of a result); ``exact``: they are f32 results rounded once, many rows at up to twice the time."""
     dev = _f8_dev(x._dev, x._codes, "gemm_f8: x")
     c = _f8_weight(w, dev, "gemm_f8")
-    xr = _f8_rows(x, x._rows, w.in_features, dev, "gemm_f8 x")
+    xr = _f8_rows(x, x._rows, w._in, dev, "gemm_f8 x")
     if out is None:
-        out = torch.empty(x._rows, w.out_features, dtype=dtype, device=x._codes.device)
+        out = torch.empty(x._rows, w._out, dtype=dtype, device=x._codes.device)
     fn = lib().rfxq_gemm_f8_exact if exact else lib().rfxq_gemm_f8
-    _f8_call(fn, dev, xr, c, _rows(out, w.out_features, dev, "gemm_f8 out"))
+    _f8_call(fn, dev, xr, c, _rows(out, w._out, dev, "gemm_f8 out"))
     return out
 
 
@@ -950,14 +973,14 @@ def grouped_gemm_f8(x: F8Rows, w: F8Weight, offsets: torch.Tensor, rows: int, x_
     c = _f8_weight(w, dev, "grouped_gemm_f8")
     _count(rows, 0, "grouped_gemm_f8: rows")
     _count(x_div, 1, "grouped_gemm_f8: x_div")
-    xr = _f8_rows(x, x._rows, w.in_features, dev, "grouped_gemm_f8 x")
+    xr = _f8_rows(x, x._rows, w._in, dev, "grouped_gemm_f8 x")
     if out is None:
-        out = torch.zeros(rows, w.out_features, dtype=dtype, device=x._codes.device)
+        out = torch.zeros(rows, w._out, dtype=dtype, device=x._codes.device)
     fn = lib().rfxq_grouped_gemm_f8_exact if exact else lib().rfxq_grouped_gemm_f8
     _f8_call(fn, dev, xr, c,
-             _ints(offsets, (w.count or 1) + 1, dev, "grouped_gemm_f8 offsets"), rows,
+             _ints(offsets, (w._count or 1) + 1, dev, "grouped_gemm_f8 offsets"), rows,
              _ints(x_index, rows, dev, "grouped_gemm_f8 x_index"), x_div,
-             _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), _rows(out, w.out_features, dev, "grouped_gemm_f8 out"))
+             _ints(y_index, rows, dev, "grouped_gemm_f8 y_index"), _rows(out, w._out, dev, "grouped_gemm_f8 out"))
     return out
 
 

@@ -314,6 +314,21 @@ def test_python_checks():
     assert empty.codes.shape == (3, 129) and empty.scales.shape == (3, 2)
 
 
+def test_weights_keep_what_they_were_made_of():
+    """Calls read the memory that a weight was made with: another tensor put in its place would not be read."""
+    import reflex_amd as rq
+
+    codes, scales = torch.zeros(2, 4, 300, dtype=torch.uint8), torch.zeros(2, 1, 3)
+    w = rq.F8Weight(codes, scales)
+    assert w.codes is codes and w.scales is scales
+    for name, value in (("codes", codes.clone()), ("scales", scales.clone()), ("count", 1), ("out_features", 2),
+                        ("in_features", 2), ("anything", 0)):
+        with pytest.raises(AttributeError):
+            setattr(w, name, value)
+    assert (w._c.data, w._c.scales) == (codes.data_ptr(), scales.data_ptr())
+    assert (w.count, w.out_features, w.in_features) == (2, 4, 300)
+
+
 def test_matrix_results_are_not_read_too_early(tmp_path):
     """The kernels' listing: on no path is a matrix instruction's result read before the wait states that the
     compiler itself keeps in straight code (12 behind the 16x16x128 ones on e4m3, 8 behind the 16x16x32 ones). It
