@@ -828,6 +828,88 @@ def test_grouped_each_kernel(rq, pairs, count, k, n, y_type, kernel, side):
     assert (y[left] == 7.0).all()
 
 
+def _threads(rq, x, w, rows, grouped, y_type):
+    """The policy's kernel, tile and threads: two kernels of rows at any byte have one tile."""
+    import ctypes
+
+    p = rq.RfxqF8Policy()
+    ty = {F32: 0, F16: 1, BF16: 30}[y_type]
+    assert rq.lib().rfxq_gemm_f8_policy(x._c, w._c, rows, grouped, ty, ctypes.byref(p)) == 0
+    return p.kernel, p.tile_m, p.tile_n, p.threads
+
+
+# each kernel of rows at any byte: K below 16, of less than a block, of whole blocks and a short one, of many
+GROUPED_ANY = [
+    (40, 8, 11, 531, F32, (FEW, 16, 16, 512)), (16, 30, 1235, 531, F16, (FEW, 16, 16, 512)), (100, 30, 645, 100, BF16, (FEW, 16, 16, 512)),
+    (500, 120, 129, 20, F32, (FEW, 16, 16, 512)),
+    (2500, 8, 3, 100, F32, (ANY, 32, 64, 512)), (600, 3, 2099, 531, F32, (ANY, 32, 64, 512)), (4000, 3, 129, 1100, F32, (ANY, 32, 64, 512)),
+    (4000, 1, 13, 100, F16, (ANY, 32, 64, 512)), (600, 30, 300, 531, BF16, (ANY, 32, 64, 512)), (260, 1, 1235, 2100, F16, (ANY, 32, 64, 512)),
+    (1200, 120, 3, 531, BF16, (ANY, 64, 128, 256)), (2500, 8, 645, 2100, F16, (ANY, 64, 128, 256)), (4000, 3, 11, 531, BF16, (ANY, 64, 128, 256)),
+    (2500, 3, 3, 531, F32, (ANY, 64, 128, 512)), (1200, 8, 1235, 2100, F32, (ANY, 64, 128, 512)), (2500, 8, 2099, 531, F32, (ANY, 64, 128, 512)),
+    (600, 1, 645, 2100, F16, (ANY, 64, 128, 512)), (2500, 8, 645, 531, BF16, (ANY, 64, 128, 512)), (1200, 8, 1235, 1100, F16, (ANY, 64, 128, 512)),
+]
+
+
+@pytest.mark.parametrize("side", ["gate", "down"])
+@pytest.mark.parametrize("pairs,count,k,n,y_type,kernel", GROUPED_ANY)
+def test_grouped_each_kernel_of_any_byte(rq, pairs, count, k, n, y_type, kernel, side):
+    """Rows and matrices at odd bytes, NaN between the rows and in front of the stack; some places in no group."""
+    top_k = 2 if pairs % 2 == 0 else 1
+    x, xs, w, ws = _case(pairs // top_k if side == "gate" else pairs, k, n, pairs + k, count)
+    _say("grouped any", pairs, count, k, n, y_type, kernel, side)
+    ids = torch.from_numpy(np.random.default_rng(pairs + n).integers(-1, count + 1, pairs).astype(np.int32))
+    xd, _ = _strided(x.view(torch.uint8), k + 3, 1, 0x7F)
+    xsd, _ = _strided(xs, _blocks(k) + 1, 1, 0xFF)
+    wd, _ = _strided(w.view(torch.uint8).reshape(1, -1), w.numel(), 3, 0x7F)
+    xr, weight = rq.F8Rows(xd, xsd), rq.F8Weight(wd.view(count, n, k), ws.to(DEV))
+    assert _threads(rq, xr, weight, pairs, 1, y_type) == kernel
+    g = rq.group_rows(ids.to(DEV), count)
+    y, buf = _strided(torch.full((pairs, n), 7.0, dtype=y_type), n + 5, 3, 0xA5)
+    before = buf.clone()
+    more = {"x_index": g.order, "x_div": top_k} if side == "gate" else {"y_index": g.order}
+    rq.grouped_gemm_f8(xr, weight, g.offsets, pairs, out=y, **more)
+    offsets, order = g.offsets.cpu().long(), g.order.long()
+    x, xs, w, ws = (t.to(DEV) for t in (x, xs, w, ws))
+    for e in range(count):
+        at = torch.arange(int(offsets[e]), int(offsets[e + 1]), device=DEV)
+        if at.numel():
+            src, dst = (order[at] // top_k, at) if side == "gate" else (at, order[at])
+            _check_product(x[src], xs[src], w[e], ws[e], y[dst])
+            y[dst] = 7.0
+    assert torch.equal(buf.view(torch.uint8), before.view(torch.uint8))  # and nothing else was written
+
+
+@pytest.mark.parametrize("pairs,k,n,y_type,kernel", [
+    (30, 13, 211, F32, (FEW, 16, 16, 512)), (30, 301, 211, BF16, (FEW, 16, 16, 512)), (600, 1235, 531, F32, (ANY, 32, 64, 512)),
+    (600, 301, 1100, F16, (ANY, 32, 64, 512)), (2500, 333, 1100, BF16, (ANY, 64, 128, 256)), (2500, 1235, 1100, F32, (ANY, 64, 128, 512)),
+    (2500, 1235, 531, F16, (ANY, 64, 128, 512)), (2500, 7, 531, F32, (ANY, 64, 128, 512)),
+    (30, 256, 211, BF16, (STREAM, 16, 32, 512)), (2000, 656, 1030, F32, (COPIED, 128, 128, 512)), (2500, 400, 1030, BF16, (COPIED, 128, 128, 512)),
+    (4000, 400, 1030, F16, (LARGE, 128, 256, 512)), (8000, 1040, 1100, BF16, (LARGE, 256, 256, 512))])
+def test_grouped_indexes_out_of_range_in_each_kernel(rq, pairs, k, n, y_type, kernel):
+    """Places whose index names no row, in three groups of which one is short and one ends inside a tile."""
+    x, xs, w, ws = (t.to(DEV) for t in _case(pairs, k, n, pairs + k, 3))
+    weight, xr = rq.F8Weight(w, ws), rq.F8Rows(x, xs)
+    _say("out of range", pairs, k, n, y_type, kernel)
+    assert _threads(rq, xr, weight, pairs, 1, y_type) == kernel
+    offsets = [0, 5, 5 + (pairs - 5) * 2 // 3, pairs]
+    index = torch.arange(pairs - 1, -1, -1, dtype=torch.int32, device=DEV)
+    for bad, at in ((-1, 0), (pairs, 1), (-(1 << 31), 3), ((1 << 31) - 1, 8)):
+        index[at::11] = bad
+    index[offsets[2]:offsets[2] + 40] = -1  # whole operands of a tile
+    good = (index >= 0) & (index < pairs)
+    for kind in ("x_index", "y_index"):
+        y = torch.full((pairs + 2, n), 7.0, dtype=y_type, device=DEV)
+        rq.grouped_gemm_f8(xr, weight, torch.tensor(offsets, dtype=torch.int32, device=DEV), pairs, out=y[:pairs], **{kind: index})
+        for e in range(3):
+            at = torch.arange(offsets[e], offsets[e + 1], device=DEV)
+            at = at[good[at]]
+            src, dst = (index[at].long(), at) if kind == "x_index" else (at, index[at].long())
+            if at.numel():
+                _check_product(x[src], xs[src], w[e], ws[e], y[dst])
+                y[dst] = 7.0
+        assert (y == 7.0).all()
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("pairs,count,k,n", [(100, 3, 384, 520), (300, 7, 768, 520), (3000, 6, 656, 1030), (500, 11, 1235, 531)])
 def test_grouped_exact(rq, pairs, count, k, n, dtype):
