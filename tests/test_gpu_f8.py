@@ -724,6 +724,43 @@ def test_gemm_exact_keeps_small_products(rq):
         assert (y == 7 * 128 * 2.0 ** -7).all()
 
 
+# a size of each kernel that cuts products, over short and long K, and of kernels that do not
+RMS = [(120, 1280, 3800, (STREAM, 32, 64)), (128, 8304, 4090, (STREAM, 32, 64)), (200, 2048, 4050, (STREAM, 64, 64)),
+       (250, 9360, 3900, (STREAM, 64, 64)), (512, 784, 3100, (COPIED, 64, 128)), (300, 4368, 3600, (COPIED, 64, 128)),
+       (1000, 512, 4000, (COPIED, 128, 128)), (600, 4368, 4090, (COPIED, 128, 128)), (2040, 256, 4090, (LARGE, 128, 256)),
+       (1024, 8192, 7000, (LARGE, 128, 256)), (4090, 256, 4096, (LARGE, 256, 256)), (4096, 4096, 4096, (LARGE, 256, 256)),
+       (100, 1101, 1531, (ANY, 32, 64)), (100, 4101, 1531, (ANY, 32, 64)), (333, 2099, 4099, (ANY, 64, 128)),
+       (1000, 4099, 4099, (ANY, 64, 128)), (64, 4096, 4096, (STREAM, 32, 32)), (16, 1237, 1100, (FEW, 16, 16))]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k,n,kernel", RMS)
+def test_gemm_error_of_normal_values(rq, rows, k, n, kernel, dtype):
+    """What results are off by as a whole, where the bound of each by itself has to allow for the worst.
+
+    A product of codes has 8 bits: cut to multiples of 2^-13 2^e (e the largest sum of two codes' exponents among eight) it
+    loses something only if its own exponents sum to e - 8 or less, so that it is below 2^-6 2^e. For normal values these are 5%
+    of the products and 2^e is 1.1 of a product's deviation; each losing anything up to 2^-13 2^e, evenly spread, they
+    are sqrt(0.05 / 3) 1.1 2^-13 = 1.7e-5 of a result (the cut itself, carried out on such codes: 1.5e-5): 2e-5. Sums: 2^-23 an
+    addition, K / 128 + 32 of them in a row, by chance: sqrt(105) 2^-23 = 1.2e-6 at K = 9360. Beyond that a result is
+    rounded once: as much as the 64-bit value's rounding, give or take 2% for the few of 16000 and more that round to the
+    other side."""
+    cut = 0.0 if dtype == F32 or kernel in ((STREAM, 32, 32), (FEW, 16, 16)) else 2e-5
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, k, n, rows + k + n))
+    xr, weight = rq.F8Rows(x, xs), rq.F8Weight(w, ws)
+    _say("rms", rows, k, n, dtype, _kernel(rq, xr, weight, rows, 0, dtype))
+    assert dtype == F32 or _kernel(rq, xr, weight, rows, 0, dtype) == kernel
+    want = _wide(x, xs) @ _wide_weight(w, ws).t()
+    for exact in (False, True):
+        y = rq.gemm_f8(xr, weight, dtype=dtype, exact=exact).double()
+        # rows have scales of their own: each by its own size
+        size = want.square().mean(1, keepdim=True).sqrt()
+        off = ((y - want) / size).square().mean().sqrt()
+        rounded = ((want.to(dtype).double() - want) / size).square().mean().sqrt()
+        _say("off by", float(off), "rounding", float(rounded))
+        assert off <= 1.02 * rounded + (0.0 if exact else cut) + 1.5e-6
+
+
 @pytest.mark.parametrize("extra", [0, 16, 112, 128, 129, 240])
 @pytest.mark.parametrize("blocks", range(1, 15))
 @pytest.mark.parametrize("rows,n,y_type", [(2, 40, F32), (40, 300, BF16), (200, 2100, F32), (300, 2050, BF16), (2048, 2050, BF16),
