@@ -504,9 +504,9 @@ typedef struct rfxq_f8_weight {
 } rfxq_f8_weight;
 
 /* What writes such rows. Of a group's values v (of 128, in f32)
- *   scale = max(amax, 448 * 2^-120) / 448, amax = max |v|;  code = e4m3(v / scale)
- * rounded to nearest even. Both quotients are f32 divisions' (of rfxq_silu_and_mul_f8
- * the second within its last bits, as its values are); a group
+ *   scale = max(amax * (1 / 448), 2^-120), amax = max |v|;  code = e4m3(v / scale)
+ * rounded to nearest even, 1 / 448 and the quotient f32 values (of rfxq_silu_and_mul_f8
+ * the quotient within its last bits, as its values are); a group
  * with a value that is not finite has NaN for its scale. Rows of x, gate, up, residual,
  * sum and y are f32, f16 or bf16, all of one call of one type and count, any
  * alignment of whole elements; out's codes and scales, sum and y must not overlap

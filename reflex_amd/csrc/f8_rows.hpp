@@ -2,8 +2,10 @@
 // infinities, largest 448) with an f32 scale for each 128 of a row, written by what
 // produces them: plain rows, SiLU(gate) * up, and the RMS norm with the residual's
 // addition. Of a group's 128 values v
-//   amax = max |v|,  scale = max(amax, 448 * 2^-120) / 448,  code = RN_e4m3(v / scale)
-// with both quotients rounded to f32 (SiLU's second one within 2^-22).
+//   amax = max |v|,  scale = max(amax / 448, 2^-120),  code = RN_e4m3(v / scale)
+// with amax / 448 a product by f32's 1 / 448, as tensor libraries divide by a number (a step of f32 off the quotient
+// at most; the quotient itself would make one code in 100000 of f16 rows another than theirs, next to ties, and those
+// are what rows are compared with), and v / scale an f32 quotient (SiLU's within 2^-22).
 // A group with a value that is not finite has NaN for its scale. The smallest scale
 // keeps 1 / scale an f32 value; groups of zeros have it.
 //
@@ -46,7 +48,7 @@ struct F8RowsArgs {
 // step there (below a power of two m - h / 4). m has 5 bits, so that v and m s are multiples of h s0 / 16, s0 the power of two
 // below s, and v comes that near to (m +- h / 2) s only if 8 s / s0 is next to a whole number: less than 26 of its steps away,
 // and not on it, since a quotient is no midpoint. Such scales take the division itself, and so do large ones, whose
-// `rest` has no bits left. Groups that are not `fine` have zeros, and NaN of what is not finite (s is NaN or finite there).
+// `rest` has no bits left. Groups that are not `fine` have zeros, and NaN of what is not finite (infinite s: the division's).
 RFXQ_DEV void over_scale(const float (&v)[8], float s, bool fine, float (&q)[8]) {
     const uint32_t off = __builtin_bit_cast(uint32_t, s) & 0xFFFFFu;
     if (min(off - 1u, 0x100000u - off) < 64u || s > 0x1p96f) {
@@ -70,11 +72,8 @@ RFXQ_DEV u2_t to_f8(const float (&v)[8], float& scale) {
     for (uint32_t i = 0; i < 8u; i++) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
     top = top_over_8(top);
     top = max(top, RFXQ_DPP_U32(top, 0x140));
-    // amax / 448 rounded once: a product, and over 448 what it left. A quotient by 7 lies a fourteenth of a step or
-    // more from any midpoint, the error before the last rounding is far less.
     const bool fine = top < kInfBits;
-    const float amax = fmaxf(as_f32(top), kF8Top * kF8Least), s0 = amax * (1.0f / kF8Top);
-    const float s = __builtin_fmaf(__builtin_fmaf(-kF8Top, s0, amax), 1.0f / kF8Top, s0);
+    const float s = fmaxf(as_f32(top) * (1.0f / kF8Top), kF8Least);
     scale = fine ? s : __builtin_nanf("");
     float q[8];
     if constexpr (EXACT) {

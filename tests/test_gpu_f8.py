@@ -215,11 +215,12 @@ def test_groups_of_every_size(rq):
 
 
 def _quantized(x):
-    """Codes and scales of [rows, k] values by f32 divisions, on the CPU; scale NaN where a group is not finite."""
+    """Codes and scales of [rows, k] values by f32's 1 / 448 and f32 divisions, on the CPU; scale NaN where a group is not
+    finite."""
     rows, k = x.shape
     v = torch.nn.functional.pad(x.float(), (0, _blocks(k) * 128 - k)).view(rows, _blocks(k), 128).numpy()
     with np.errstate(invalid="ignore"):
-        scales = np.maximum(np.abs(v).max(2), np.float32(448 * LEAST)) / np.float32(448)
+        scales = np.maximum(np.abs(v).max(2) * (np.float32(1) / np.float32(448)), np.float32(LEAST))
         codes = torch.from_numpy(v / scales[:, :, None]).to(F8).view(torch.uint8).view(rows, -1)[:, :k]
     return codes, torch.from_numpy(np.where(np.isfinite(scales), scales, np.float32("nan")))
 
@@ -227,7 +228,7 @@ def _quantized(x):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("rows,k", [(1, 4096), (777, 1235), (400, 2048), (3, 129)])
 def test_quantize_by_division(rq, rows, k, dtype):
-    """Scales and codes are those of f32 divisions to the last bit, ties included (8-bit values meet many)."""
+    """Scales and codes to the last bit, ties included (8-bit values meet many): what torch makes of the same formula."""
     _say("by division", rows, k, dtype)
     g = _gen(rows + k)
     whole = torch.randint(-448, 449, (rows, k), generator=g).float() * torch.exp2(torch.randint(-5, 3, (rows, 1), generator=g))
@@ -236,12 +237,16 @@ def test_quantize_by_division(rq, rows, k, dtype):
         got = rq.quantize_f8(x.to(DEV))
         assert torch.equal(got.scales.cpu(), scales)
         assert torch.equal(got.codes.view(torch.uint8).cpu(), codes)
+        v = torch.nn.functional.pad(x.to(DEV).float(), (0, _blocks(k) * 128 - k)).view(rows, -1, 128)
+        scales = v.abs().amax(2).clamp(min=448.0 * LEAST) / 448.0
+        assert torch.equal(got.scales, scales)
+        assert torch.equal(got.codes.float(), (v / scales.unsqueeze(2)).to(F8).float().view(rows, -1)[:, :k])
 
 
 @pytest.mark.parametrize("exponent", [-120, -119, -70, 0, 60, 95, 96, 97, 110])
 def test_quantize_next_to_ties(rq, exponent):
     """Values within some steps of a midpoint of two codes, scales within some steps of eighths of a power of two and
-    anywhere: the codes of f32 quotients, rounded twice as those are."""
+    anywhere: the codes of f32 quotients, which are rounded twice."""
     _say("ties", exponent)
     r = np.random.default_rng(exponent + 200)
     groups = 12000
@@ -250,7 +255,7 @@ def test_quantize_next_to_ties(rq, exponent):
     s = (s + np.uint32((127 + exponent) << 23)).view(np.float32)
     x = np.empty((groups, 128), np.float32)
     x[:, 0] = (s.astype(np.float64) * 448).astype(np.float32)
-    s = x[:, 0] / np.float32(448)
+    s = x[:, 0] * (np.float32(1) / np.float32(448))
     tie = r.integers(16, 32, (groups, 127)) * np.exp2(r.integers(-10, 5, (groups, 127)))  # 1/64 .. 496
     tie = np.where(r.random(tie.shape) < 0.1, r.integers(0, 17, tie.shape) * 2.0 ** -10, np.minimum(tie, 432))
     v = (tie * s[:, None].astype(np.float64)).astype(np.float32)
