@@ -13,7 +13,7 @@
 // group's codes one 128-byte line. All three kernels are bound by memory: each input
 // is read once, each output written once (a large copy runs at 4.87 TB/s, reads and writes
 // together; few rows cost what a launch does: an empty one 1.7 us in a graph).
-//   quantize  4096 x 4096 bf16    10.3 us, 4.9 TB/s;  1 x 4096: 1.8 us
+//   quantize  4096 x 4096 bf16    10.4 us, 4.9 TB/s;  1 x 4096: 1.8 us
 //   SiLU      4096 x 14336 bf16   51.6 us, 5.7 TB/s;  256 x 768: 2.2 us
 //   norm      4096 x 4096 bf16    20.1 us, 5.9 TB/s;  1 x 4096: 2.5 us, 32 x 4096 f32: 2.9 us
 #pragma once
@@ -40,7 +40,7 @@ struct F8RowsArgs {
 
 // v / s rounded once, for 8 values and the group's scale s, as f32 division has it, where that changes a code
 // (SiLU's v are within 2^-20 themselves and do with a reciprocal). Two operations a value, where division takes
-// eleven and another reciprocal (4096 x 4096 bf16 10.3 us, by division 13.0, by one reciprocal 9.95; the norm 25.1, 26.4,
+// eleven and another reciprocal (4096 x 4096 bf16 10.4 us, by division 13.0, by one reciprocal 9.95; the norm 25.1, 26.4,
 // 25.1; SiLU of 4096 x 14336 bf16 would take 60 and 69 for 55):
 //   near + rest is 1 / s to 2^-44 of it, near below it so that rest >= 0 keeps the sign of zeros;
 //   RN(v near + v rest) is RN(v / s), unless a midpoint of two f32 values lies within 2^-44 of v / s.
@@ -48,10 +48,14 @@ struct F8RowsArgs {
 // step there (below a power of two m - h / 4). m has 5 bits, so that v and m s are multiples of h s0 / 16, s0 the power of two
 // below s, and v comes that near to (m +- h / 2) s only if 8 s / s0 is next to a whole number: less than 26 of its steps away,
 // and not on it, since a quotient is no midpoint. Such scales take the division itself, and so do large ones, whose
-// `rest` has no bits left. Groups that are not `fine` have zeros, and NaN of what is not finite (infinite s: the division's).
+// `rest` has no bits left. Rows of at most 11 bits (HALF: f16 and bf16 as they are) meet such scales often, where amax is a
+// multiple of 7, but no such v: with v and m N of so few bits, N the whole number, v would have to be m N s0 / 8, and lies 16
+// or more sixteenths of a step from m s then, for a half step's 8 to 15. Groups that are not `fine` have zeros, and NaN
+// of what is not finite (infinite s: the division's).
+template <bool HALF>
 RFXQ_DEV void over_scale(const float (&v)[8], float s, bool fine, float (&q)[8]) {
     const uint32_t off = __builtin_bit_cast(uint32_t, s) & 0xFFFFFu;
-    if (min(off - 1u, 0x100000u - off) < 64u || s > 0x1p96f) {
+    if (!HALF && min(off - 1u, 0x100000u - off) < 64u || s > 0x1p96f) {
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) q[i] = v[i] / s;
     } else {
@@ -65,7 +69,7 @@ RFXQ_DEV void over_scale(const float (&v)[8], float s, bool fine, float (&q)[8])
 
 // 8 values starting at v of the group that the 16 lanes of this DPP row hold, as codes
 // and the group's scale.
-template <bool EXACT>
+template <bool EXACT, bool HALF = false>
 RFXQ_DEV u2_t to_f8(const float (&v)[8], float& scale) {
     uint32_t top = 0;
 #pragma unroll
@@ -77,7 +81,7 @@ RFXQ_DEV u2_t to_f8(const float (&v)[8], float& scale) {
     scale = fine ? s : __builtin_nanf("");
     float q[8];
     if constexpr (EXACT) {
-        over_scale(v, s, fine, q);
+        over_scale<HALF>(v, s, fine, q);
     } else {
         const float r = fine ? __builtin_amdgcn_rcpf(s) : 0.0f;
 #pragma unroll
@@ -172,7 +176,7 @@ RFXQ_DEV void f8_rows(const F8RowsArgs& a) {
 #pragma unroll
             for (uint32_t j = 0; j < 8u; j++) v[j] = x.at(j);
         }
-        const u2_t codes = to_f8<!SILU>(v, scale);
+        const u2_t codes = to_f8<!SILU, !__is_same(T, float)>(v, scale);
         st_codes(a.out + (uint64_t)row * a.ldo + k, codes, have);
         if (c == 0) stf(a.scales + (uint64_t)row * a.lds + group, scale);
         group += a.by_groups;

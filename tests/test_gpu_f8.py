@@ -243,6 +243,25 @@ def test_quantize_by_division(rq, rows, k, dtype):
         assert torch.equal(got.codes.float(), (v / scales.unsqueeze(2)).to(F8).float().view(rows, -1)[:, :k])
 
 
+@pytest.mark.parametrize("dtype,bits,exponent", [(BF16, 7, -60), (BF16, 7, 0), (BF16, 7, 104), (BF16, 7, 127), (F16, 10, 0), (F16, 10, 13)])
+def test_quantize_every_half_value(rq, dtype, bits, exponent):
+    """Every pair of a largest value's fraction and another's, down to where codes are 0, to the last bit."""
+    _say("every", dtype, exponent)
+    low = max(exponent - 19, -14 if dtype == F16 else -126)
+    step = 2.0 ** -bits
+    fractions = 1 + torch.arange(1 << bits, dtype=torch.float64) * step
+    others = torch.cat([fractions * 2.0 ** e for e in range(low, exponent + 1)])
+    others = torch.nn.functional.pad(others, (0, -len(others) % 127)).view(-1, 127)
+    for part in fractions.split(128):
+        top = (part * 2.0 ** exponent).view(-1, 1, 1).expand(-1, others.shape[0], 1)
+        x = torch.cat([top, torch.minimum(others.expand(len(part), -1, -1), top)], 2).reshape(-1, 128).to(dtype).to(DEV)
+        x = torch.where(torch.arange(128, device=DEV) % 3 == 0, -x, x)
+        got = rq.quantize_f8(x)
+        scales = x.float().abs().amax(1, keepdim=True).clamp(min=448.0 * LEAST) / 448.0
+        assert torch.equal(got.scales, scales)
+        assert torch.equal(got.codes.view(torch.uint8), (x.float() / scales).to(F8).view(torch.uint8))
+
+
 @pytest.mark.parametrize("exponent", [-120, -119, -70, 0, 60, 95, 96, 97, 110])
 def test_quantize_next_to_ties(rq, exponent):
     """Values within some steps of a midpoint of two codes, scales within some steps of eighths of a power of two and
