@@ -8,8 +8,8 @@
 // Each wave copies its own operands into its own R places in LDS, R blocks ahead, and waits
 // for nobody. Whole lines by copies: 63 bytes a cycle and CU, where loads in the order of an instruction's
 // operands take 16. 1 x 4096 x 14336: 11.4 us, 5.2 TB/s of weights (a large copy: 4.87);
-// 1 x 4096 x 4096: 6.5; 32 tokens over 8 of 128 experts, 2048 x 768: 28 us, 7.2 TB/s of those that
-// stay in the memory-side cache. More columns a workgroup read x less often, fewer make more
+// 1 x 4096 x 4096: 6.3; 32 tokens over 8 of 128 experts, 2048 x 768: 31 us for the 118 MB of the 75 experts
+// that have rows, 3.8 TB/s (26 where a call finds part of them in the memory-side cache). More columns a workgroup read x less often, fewer make more
 // workgroups; the host's table has what each measured. 32 x 64 and 64 x 64 tiles are for 33 to some 256 rows,
 // whose copies and products bound: 128 x 14336 x 4096 21 us for half results and 23 for f32 ones, 256 rows 29 and 35. (The
 // smaller tiles gain less by the instruction of 128, 64 rows in 32 x 32 16.4 us for 17.0, and have

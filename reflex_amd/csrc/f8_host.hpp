@@ -131,7 +131,7 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   stream 16 x 16  64 tiles: 4.3 (1 x 4096 x 1024), 256: 6.3 (1 x 4096 x 4096), 11.9 (1 x 14336 x 4096)
 //   stream 16 x 32  1 x 4096 x 14336: 11.5 (16 x 16: 15), 32 x 4096 x 4096: 6.4 (32 x 32: 7.5)
 //   stream 32 x 32  64 x 4096 x 4096: 7.6 (16 x 32: 8.7, 64 x 128: 13), 128 rows: 11.0 (64 x 128: 13)
-//   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 28 (16 x 32: 56, 64 x 128: 46);
+//   stream 16 x 64  32 tokens over 8 of 128 experts, 2048 x 768: 31 (16 x 32: 56, 64 x 128: 44);
 //                   32 x 4096 x 14336: 12.8 (16 x 32: 14.3)
 //   stream 32 x 64  128 x 4096 x 4096: 8.7, f32 results 9.2 (32 x 32: 11.1), 128 x 14336 x 4096: 20.9, 22.4 (28.1);
 //                   32 x 4096 x 14336: 17.3 (16 x 32: 14.3, 32 x 32: 18.8)
@@ -141,7 +141,7 @@ int f8_rows_launch(const hipFunction_t* fns, const rfxq_rows* x, const rfxq_rows
 //   64 x 128        256 x 4096 x 4096: 13 (32 x 32: 19), 512 x 14336 x 4096: 39 (128 x 128: 65); f32 results 68
 //   128 x 128       1000 x 4096 x 4096: 23 (64 x 128: 26, 128 x 256: 28); f32 38 (64 x 128: 47)
 //   128 x 256       2048 x 4096 x 4096: 36 (128 x 128: 46, 256 x 256: 46)
-//   256 x 256       4096 x 4096 x 14336: 229 (128 x 256: 244)
+//   256 x 256       4096 x 4096 x 14336: 217 (128 x 256: 237)
 // and rows at any byte:
 //   few 16 x 16     1 x 4099 x 4099: 11.8 (32 x 64: 22), 16 rows: 22 (22), 40 x 1235 x 1531: 7.0 (7.8)
 //   32 x 64         333 x 1235 x 1531: 9.4 (64 x 128: 15.2), 16 x 4099 x 14336: 24.5 (35; few: 80)
@@ -239,9 +239,9 @@ F8Plan f8_plan(uint32_t cus, const rfxq_f8_rows* x, const rfxq_f8_weight* w, uin
     p.tiles_n = (n + v.bn - 1u) / v.bn;
     // XCD blocks of sm x sn tiles: the tallest of those whose fullest XCD has the fewest tiles, or, of
     // workgroups that fill a CU, rounds of them. Of those, dense ones of up to four rows of tiles (4096 x 4096 x 14336:
-    // 214 us, of two 221, of one 232), fewer where four leave blocks half empty (700 x 4096 x 14336: three 64
-    // us, four 83); grouped ones of as many as a group has, up to three (4096 tokens over 8 of 128 experts, 2048 x 768:
-    // 91 us, of four 104, of one 100; 128 tokens over 2 of 8, 4096 x 4096, f32 results: of one 42, of three 53). The
+    // 217 us, of two 230, of one 243), fewer where four leave blocks half empty (700 x 4096 x 14336, f32 results: three 100
+    // us, four 127); grouped ones of as many as a group has, up to three (4096 tokens over 8 of 128 experts, 2048 x 768:
+    // 91 us, of four 102, of one 101; 128 tokens over 2 of 8, 4096 x 4096, f32 results: of one 42, of three 52). The
     // others two (64 x 4096 x 14336: 19 us, of one 22, of four 30; 333 x 1235 x 1531 the same).
     const uint32_t across = (p.tiles_n + 3u) / 4u;
     p.sn = (p.tiles_n + across - 1u) / across;

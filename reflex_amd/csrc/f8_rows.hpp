@@ -12,10 +12,11 @@
 // 16 lanes (a DPP row) hold a group, 8 values each: amax is four lane moves, and the
 // group's codes one 128-byte line. All three kernels are bound by memory: each input
 // is read once, each output written once (a large copy runs at 4.87 TB/s, reads and writes
-// together; few rows cost what a launch does: an empty one 1.7 us in a graph).
-//   quantize  4096 x 4096 bf16    10.4 us, 4.9 TB/s;  1 x 4096: 1.8 us
-//   SiLU      4096 x 14336 bf16   51.6 us, 5.7 TB/s;  256 x 768: 2.2 us
-//   norm      4096 x 4096 bf16    20.1 us, 5.9 TB/s;  1 x 4096: 2.5 us, 32 x 4096 f32: 2.9 us
+// together; few rows cost what a launch does: an empty one 1.7 us in a graph). In a graph, on three sets of
+// operands in turn:
+//   quantize  4096 x 4096 bf16    10.4 us, 4.9 TB/s;  1 x 4096: 2.1 us
+//   SiLU      4096 x 14336 bf16   55 us, 5.4 TB/s;    256 x 768 f32: 2.3 us
+//   norm      4096 x 4096 bf16    25.2 us, 4.7 TB/s;  1 x 4096 f32: 2.9 us, 32 x 4096: 3.1 us
 #pragma once
 #include "common.hpp"
 #include "tiles.hpp"

@@ -276,7 +276,7 @@ RFXQ_F8_MID(128, 2, f32, true)
 // 8 waves of 16 MF x 64. A step is a block of K: its weights are in registers from its start, its
 // activations come from LDS two 16-row operands ahead of their products; at MF - 2
 // of them all reads of the step are done and the next step's copies have landed (the one
-// barrier). 4096 x 4096 x 14336: 214..225 us, 2.1..2.2 PFLOP/s (128 x 256: 244; a library's product with one
+// barrier). 4096 x 4096 x 14336: 217 us, 2.2 PFLOP/s (128 x 256: 237; a library's product with one
 // scale a tensor: 200); instructions 59% busy at 8192^3, 3.5 rounds of tiles over the CUs done as 4.
 // 128 x 256 has three stages, for 256 x 256 two fill the LDS. Tried: two workgroups of 128 x 128 a CU
 // (283 us), operands that two waves take in turns (311), 192 x 256 tiles.
