@@ -51,8 +51,9 @@ struct F8RowsArgs {
 // and not on it, since a quotient is no midpoint. Such scales take the division itself, and so do large ones, whose
 // `rest` has no bits left. Rows of at most 11 bits (HALF: f16 and bf16 as they are) meet such scales often, where amax is a
 // multiple of 7, but no such v: with v and m N of so few bits, N the whole number, v would have to be m N s0 / 8, and lies 16
-// or more sixteenths of a step from m s then, for a half step's 8 to 15. Groups that are not `fine` have zeros, and NaN
-// of what is not finite (infinite s: the division's).
+// or more sixteenths of a step from m s then, for a half step's 8 to 15 (16 would be a scale just below a power of
+// two, but 448 times one has that for its scale). Groups that are not `fine` have zeros, and NaN of what is not finite
+// (infinite s: the division's).
 template <bool HALF>
 RFXQ_DEV void over_scale(const float (&v)[8], float s, bool fine, float (&q)[8]) {
     const uint32_t off = __builtin_bit_cast(uint32_t, s) & 0xFFFFFu;

@@ -1171,6 +1171,36 @@ def test_captured_and_replayed(rq, rows):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("rows,k,n,dtype", [(1, 4099, 500, BF16), (300, 645, 531, F16), (333, 2099, 4099, BF16), (130, 4096, 700, F16),
+                                            (250, 1040, 3900, BF16), (500, 784, 3100, F16), (2048, 640, 4000, BF16)])
+def test_products_captured(rq, rows, k, n, dtype, exact):
+    """Products in a graph, dense and grouped, aligned and not: replays follow new inputs, with eager work between them."""
+    x, xs, w, ws = (t.to(DEV) for t in _case(rows, k, n, rows + k, 2))
+    xr, weight, stack = rq.F8Rows(x, xs), rq.F8Weight(w[0], ws[0]), rq.F8Weight(w, ws)
+    offsets = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device=DEV)
+
+    def step():
+        return (rq.gemm_f8(xr, weight, dtype=dtype, exact=exact),
+                rq.grouped_gemm_f8(xr, stack, offsets, rows, dtype=dtype, exact=exact))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (1, 2, 3, 1):
+        other = _case(rows, k, 1, seed)
+        x.copy_(other[0].to(DEV))
+        xs.copy_(other[1].to(DEV))
+        offsets[1] = seed * rows // 7
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+
+
 def test_other_stream(rq):
     """Work goes on the caller's current stream."""
     x, xs, w, ws = _case(300, 1024, 512, 1)
