@@ -584,11 +584,16 @@ int rfxq_grouped_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, c
 typedef struct rfxq_f8_policy {
     uint32_t kernel; /* RFXQ_F8_* */
     uint32_t tile_m, tile_n;
-    uint32_t threads;  /* of a workgroup */
-    uint32_t launches; /* each of fewer than 2^32 threads */
 } rfxq_f8_policy;
 int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
                         rfxq_f8_policy* out);
+/* Test hook: how that kernel is launched. */
+typedef struct rfxq_f8_launch {
+    uint32_t threads;  /* of a workgroup */
+    uint32_t launches; /* each of fewer than 2^32 threads */
+} rfxq_f8_launch;
+int rfxq_gemm_f8_launch(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
+                        rfxq_f8_launch* out);
 
 /* ---- GGUF files (the on-disk path) ---------------------------------------- */
 

@@ -67,8 +67,13 @@ class RfxqF8Weight(ctypes.Structure):
 class RfxqF8Policy(ctypes.Structure):
     """``rfxq_f8_policy`` (include/rfxq.h)."""
 
-    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32),
-                ("threads", ctypes.c_uint32), ("launches", ctypes.c_uint32)]
+    _fields_ = [("kernel", ctypes.c_uint32), ("tile_m", ctypes.c_uint32), ("tile_n", ctypes.c_uint32)]
+
+
+class RfxqF8Launch(ctypes.Structure):
+    """``rfxq_f8_launch`` (include/rfxq.h)."""
+
+    _fields_ = [("threads", ctypes.c_uint32), ("launches", ctypes.c_uint32)]
 
 
 class RfxqOptions(ctypes.Structure):
@@ -168,6 +173,7 @@ SIGNATURES = {
     "rfxq_grouped_gemm_f8": (_I, [_F8R, _F8W, _P, _U32, _P, _U32, _P, _RP, _P]),
     "rfxq_grouped_gemm_f8_exact": (_I, [_F8R, _F8W, _P, _U32, _P, _U32, _P, _RP, _P]),
     "rfxq_gemm_f8_policy": (_I, [_F8R, _F8W, _U32, _I, _U32, ctypes.POINTER(RfxqF8Policy)]),
+    "rfxq_gemm_f8_launch": (_I, [_F8R, _F8W, _U32, _I, _U32, ctypes.POINTER(RfxqF8Launch)]),
 }
 
 

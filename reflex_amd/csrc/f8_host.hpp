@@ -343,6 +343,19 @@ int f8_grouped(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const int32_t* of
     return ok();
 }
 
+// what the test hooks report of
+int f8_plan_for(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type, const char* what,
+                F8Plan* p) {
+    if (int rc = check_f8_weight(w, what)) return rc;
+    if (int rc = check_f8_rows(x, w->in_features, what, "x")) return rc;
+    if (rows == 0 || rows > 0x7FFFFFFFu || x->rows == 0)
+        return fail(RFXQ_ERR_INVALID_INPUT, "%s: rows=%u of %u", what, rows, x->rows);
+    if (!float_type(y_type)) return fail(RFXQ_ERR_GGUF, "%s: y of type %u (F32, F16 or BF16)", what, y_type);
+    const Ctx* c = loaded_ctx();
+    *p = f8_plan(c ? (uint32_t)c->cus : 256u, x, w, rows, grouped != 0, y_type == RFXQ_TYPE_F32);
+    return RFXQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -480,15 +493,19 @@ int rfxq_grouped_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, c
 int rfxq_gemm_f8_policy(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
                         rfxq_f8_policy* out) {
     if (!out) return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: NULL output");
-    if (int rc = check_f8_weight(w, "gemm_f8_policy")) return rc;
-    if (int rc = check_f8_rows(x, w->in_features, "gemm_f8_policy", "x")) return rc;
-    if (rows == 0 || rows > 0x7FFFFFFFu || x->rows == 0)
-        return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_policy: rows=%u of %u", rows, x->rows);
-    if (!float_type(y_type)) return fail(RFXQ_ERR_GGUF, "gemm_f8_policy: y of type %u (F32, F16 or BF16)", y_type);
-    const Ctx* c = loaded_ctx();
-    const F8Plan p = f8_plan(c ? (uint32_t)c->cus : 256u, x, w, rows, grouped != 0, y_type == RFXQ_TYPE_F32);
+    F8Plan p;
+    if (int rc = f8_plan_for(x, w, rows, grouped, y_type, "gemm_f8_policy", &p)) return rc;
+    *out = {p.v.kernel, p.v.bm, p.v.bn};
+    return ok();
+}
+
+int rfxq_gemm_f8_launch(const rfxq_f8_rows* x, const rfxq_f8_weight* w, uint32_t rows, int grouped, uint32_t y_type,
+                        rfxq_f8_launch* out) {
+    if (!out) return fail(RFXQ_ERR_INVALID_INPUT, "gemm_f8_launch: NULL output");
+    F8Plan p;
+    if (int rc = f8_plan_for(x, w, rows, grouped, y_type, "gemm_f8_launch", &p)) return rc;
     const auto times = [](uint32_t all, uint32_t most) { return (all + most - 1u) / most; };
-    *out = {p.v.kernel, p.v.bm, p.v.bn, p.v.threads, times(p.tiles_m, p.most_m) * times(p.tiles_n, p.most_n)};
+    *out = {p.v.threads, times(p.tiles_m, p.most_m) * times(p.tiles_n, p.most_n)};
     return ok();
 }
 

@@ -263,13 +263,16 @@ def test_launches_have_fewer_than_2_32_threads(L, rows, experts, k, n, ty):
 
     x = rq.RfxqF8Rows(1 << 44, 1 << 45, rows, k, -(-k // 128))
     w = _weight(k, n, experts, data=1 << 43, scales=1 << 42)
-    p = rq.RfxqF8Policy()
-    assert L.rfxq_gemm_f8_policy(ctypes.byref(x), ctypes.byref(w), rows, 1 if experts else 0, ty, ctypes.byref(p)) == 0
-    assert p.threads in (256, 512)
-    threads = -(-rows // p.tile_m) * -(-n // p.tile_n) * p.threads
+    p, how = rq.RfxqF8Policy(), rq.RfxqF8Launch()
+    args = ctypes.byref(x), ctypes.byref(w), rows, 1 if experts else 0, ty
+    assert L.rfxq_gemm_f8_policy(*args, ctypes.byref(p)) == 0 and L.rfxq_gemm_f8_launch(*args, ctypes.byref(how)) == 0
+    assert how.threads in (256, 512)
+    threads = -(-rows // p.tile_m) * -(-n // p.tile_n) * how.threads
     if threads < 1 << 31:
-        assert p.launches == 1
-    assert threads / ((1 << 32) - 1) <= p.launches <= max(1, threads / (1 << 29))
+        assert how.launches == 1
+    assert threads / ((1 << 32) - 1) <= how.launches <= max(1, threads / (1 << 29))
+    _expect(L, L.rfxq_gemm_f8_launch(*args, None), 11, "NULL output")
+    _expect(L, L.rfxq_gemm_f8_launch(args[0], args[1], 0, args[3], ty, ctypes.byref(how)), 11, "rows=0")
 
 
 def test_python_checks():

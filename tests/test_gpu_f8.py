@@ -585,10 +585,10 @@ def _whole(rows, k, seed):
 def _launches(rq, x, w, rows, grouped, y_type):
     import ctypes
 
-    p = rq.RfxqF8Policy()
+    how = rq.RfxqF8Launch()
     ty = {F32: 0, F16: 1, BF16: 30}[y_type]
-    assert rq.lib().rfxq_gemm_f8_policy(x._c, w._c, rows, grouped, ty, ctypes.byref(p)) == 0
-    return p.launches
+    assert rq.lib().rfxq_gemm_f8_launch(x._c, w._c, rows, grouped, ty, ctypes.byref(how)) == 0
+    return how.launches
 
 
 PERIOD = (1 << 20) + 77
@@ -890,13 +890,13 @@ def test_grouped_each_kernel(rq, pairs, count, k, n, y_type, kernel, side):
 
 
 def _threads(rq, x, w, rows, grouped, y_type):
-    """The policy's kernel, tile and threads: two kernels of rows at any byte have one tile."""
+    """The kernel, its tile and threads: two kernels of rows at any byte have one tile."""
     import ctypes
 
-    p = rq.RfxqF8Policy()
+    how = rq.RfxqF8Launch()
     ty = {F32: 0, F16: 1, BF16: 30}[y_type]
-    assert rq.lib().rfxq_gemm_f8_policy(x._c, w._c, rows, grouped, ty, ctypes.byref(p)) == 0
-    return p.kernel, p.tile_m, p.tile_n, p.threads
+    assert rq.lib().rfxq_gemm_f8_launch(x._c, w._c, rows, grouped, ty, ctypes.byref(how)) == 0
+    return _kernel(rq, x, w, rows, grouped, y_type) + (how.threads,)
 
 
 # each kernel of rows at any byte: K below 16, of less than a block, of whole blocks and a short one, of many
