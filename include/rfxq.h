@@ -519,9 +519,10 @@ typedef struct rfxq_f8_weight {
 /* out = x [rows][k]. */
 int rfxq_quantize_f8(const rfxq_rows* x, uint32_t k, const rfxq_f8_rows* out, hipStream_t stream);
 
-/* out = gate / (1 + exp(-gate)) * up: Model::silu_and_mul (silu_and_mul.cu:7-23), within
- * 2^-20 over f32's whole range of results: also where exp(-gate) by itself would not be an
- * f32 value (gates below -88 beside large ups). gate and up may be columns of one matrix. */
+/* out = gate / (1 + exp(-gate)) * up: Model::silu_and_mul (silu_and_mul.cu:7-23), normal
+ * f32 results within 2^-20 (of gates of 2^-125 and more in size), also where exp(-gate) by
+ * itself is no f32 value: gates below -88 beside large ups. gate and up may be columns of
+ * one matrix. */
 int rfxq_silu_and_mul_f8(const rfxq_rows* gate, const rfxq_rows* up, uint32_t k, const rfxq_f8_rows* out,
                          hipStream_t stream);
 
@@ -545,13 +546,13 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
  * and zeros counted as 2^-6), which costs 1.5e-5 of a result for normal values. Kernels
  * of few rows (tiles of 16 x 16 to 32 x 32 and 16 x 64) have exact products for them too,
  * so that a row's products may be cut in one batch and exact in another:
- * rfxq_gemm_f8_exact never cuts. NaN
- * codes give NaN, and scales that are not finite results that are not finite, where
+ * rfxq_gemm_f8_exact never cuts. NaN codes give NaN, and scales that are not finite results that are not finite, where
  * they belong, and nowhere else. Any sizes, strides and alignment of whole elements
  * (scales and y); rows of x and w that start at multiples of 16 bytes are faster. y must
- * not overlap x or w. One launch (more where it would have 2^32 threads: narrow products of
- * 100 million rows), no workspace, no host synchronisation: it can be captured. The order of a sum depends on the call's sizes and alignment, not on
- * anything else: equal calls give equal bits. */
+ * not overlap x or w. One launch (more where it would have 2^32 threads: narrow products
+ * of 100 million rows), no workspace, no host synchronisation: it can be captured. The
+ * order of a sum depends on the call's sizes and alignment, not on anything else: equal
+ * calls give equal bits. */
 int rfxq_gemm_f8(const rfxq_f8_rows* x, const rfxq_f8_weight* w, const rfxq_rows* y, hipStream_t stream);
 
 /* rfxq_gemm_f8 with exact products whatever y's type, by the kernels of f32 results:
@@ -575,7 +576,8 @@ int rfxq_grouped_gemm_f8_exact(const rfxq_f8_rows* x, const rfxq_f8_weight* w, c
 
 /* Test hook: the kernel and tile that rfxq_gemm_f8 (grouped = 0) or
  * rfxq_grouped_gemm_f8 runs on the current device (256 compute units before
- * rfxq_init) for `rows` rows or places of x and w and results of a type (f32: the exact ones' for all); no memory is read. */
+ * rfxq_init) for `rows` rows or places of x and w and results of a type (f32: what the
+ * exact forms run for all types); no memory is read. */
 #define RFXQ_F8_ANY 0    /* 32 x 64 or 64 x 128 tiles through registers, any alignment */
 #define RFXQ_F8_FEW 1    /* 16 x 16, straight from memory, any alignment */
 #define RFXQ_F8_STREAM 2 /* few rows: K among a workgroup's waves, each with copies of its own */
