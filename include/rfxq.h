@@ -546,8 +546,8 @@ int rfxq_add_rmsnorm_f8(const rfxq_rows* x, const rfxq_rows* residual, const flo
  * and zeros counted as 2^-6), which costs 1.5e-5 of a result for normal values. Kernels
  * of few rows (tiles of 16 x 16 to 32 x 32 and 16 x 64) have exact products for them too,
  * so that a row's products may be cut in one batch and exact in another:
- * rfxq_gemm_f8_exact never cuts. NaN codes give NaN, and scales that are not finite results that are not finite, where
- * they belong, and nowhere else. Any sizes, strides and alignment of whole elements
+ * rfxq_gemm_f8_exact never cuts. NaN codes give NaN, and scales that are not finite
+ * results that are not finite, where they belong, and nowhere else. Any sizes, strides and alignment of whole elements
  * (scales and y); rows of x and w that start at multiples of 16 bytes are faster. y must
  * not overlap x or w. One launch (more where it would have 2^32 threads: narrow products
  * of 100 million rows), no workspace, no host synchronisation: it can be captured. The
